@@ -318,6 +318,114 @@ WELVET_API welvet_status welvet_hip_swiglu_forward_device(welvet_hip_swiglu *s, 
                                                           void *stream);
 WELVET_API void welvet_hip_swiglu_release(welvet_hip_swiglu *s);
 
+/* ---- token ends of a network and adapters beside its layers (extensions) --
+ * What a language model built on this library's Dense layers needs around
+ * them.  All pointers named d_ are device memory; every call is enqueued on
+ * `stream` (a hipStream_t; NULL = the HIP null stream), returns once enqueued,
+ * allocates nothing and may be captured into a HIP graph.  Calls that take a
+ * workspace (d_ws, at least the bytes the _bytes call names, 16-byte aligned;
+ * NULL where that is 0) own it until the stream has passed them: calls that
+ * may overlap need one each.  Strides count elements between rows.  Types are
+ * dtype ids: 1 Float32, 2 Float16, 3 BFloat16 (code 2 for others).  Sizes,
+ * null or misaligned pointers, strides below a row and short workspaces
+ * answer code 1 before anything is enqueued.  Outputs must not overlap
+ * inputs except where a call says so. */
+
+/* Embedding: out[t] = scale * table[tokens[t]], t < n, rows of dim f32 values
+ * from a [vocab][dim] table.  A token outside [0, vocab) is padding: a row of
+ * zeros. */
+WELVET_API welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t dim,
+                                                      const void *d_table, int64_t table_stride,
+                                                      const int32_t *d_tokens, int32_t n,
+                                                      float scale, float *d_out,
+                                                      int64_t out_stride, void *stream);
+/* The same from a mounted layer's store [out][in], any dtype, decoded as the
+ * layer decodes it: an output layer's weights shared with the embedding. */
+WELVET_API welvet_status welvet_hip_embedding_store_forward(welvet_dense_session *s,
+                                                            const int32_t *d_tokens, int32_t n,
+                                                            float scale, float *d_out,
+                                                            int64_t out_stride, void *stream);
+/* Its gradient: dtable[v] = scale * sum of dout[t] over tokens[t] = v, with
+ * zeros in the rows no token names; with accumulate = 1, added to the rows
+ * that tokens name, the others left as they are (scale = -rate: an SGD step
+ * on a Float32 table in place).  Padding's rows of dout are not read.  A
+ * token's rows are added in f32 in their own order: the same bits on every
+ * run. */
+WELVET_API welvet_status welvet_hip_embedding_backward_bytes(int32_t vocab, int32_t dim,
+                                                             int32_t n, size_t *bytes);
+WELVET_API welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t dim,
+                                                       const int32_t *d_tokens, int32_t n,
+                                                       float scale, const float *d_dout,
+                                                       int64_t dout_stride, int32_t accumulate,
+                                                       float *d_dtable, int64_t dtable_stride,
+                                                       void *d_ws, size_t ws_bytes, void *stream);
+
+/* Low-rank adapters of many requests beside one projection in -> out.  The
+ * stack: `count` adapters of at most `rank` (<= 256), down factors
+ * [count][rank][in] and up factors [count][rank][out] of `dtype`, contiguous
+ * device arrays; adapter a uses its first d_ranks[a] rank rows (NULL: all;
+ * the rest is not read) and the factor d_scales[a] (NULL: 1).  Row t of n
+ * takes adapter ids[t], none where that lies outside [0, count).
+ * count <= 65535. */
+typedef struct welvet_hip_adapters {
+  int32_t dtype, count, rank, in, out;
+  const void *d_down, *d_up;
+  const int32_t *d_ranks;
+  const float *d_scales;
+} welvet_hip_adapters;
+/* The workspace either direction needs for n rows. */
+WELVET_API welvet_status welvet_hip_adapters_bytes(const welvet_hip_adapters *desc, int32_t n,
+                                                   size_t *bytes);
+/* h = x . down^T, y = base + scale * h . up; d_base (NULL: zeros) is the
+ * projection's own output, e.g. a Linear Dense layer's, and may be d_y.  d_h
+ * (nullable) [n][rank] receives h, which the backward takes: zeros past a
+ * row's rank and in rows without an adapter, whose y is their base. */
+WELVET_API welvet_status welvet_hip_adapters_forward(const welvet_hip_adapters *desc,
+                                                     const float *d_x, int64_t x_stride,
+                                                     const int32_t *d_ids, int32_t n,
+                                                     const float *d_base, int64_t base_stride,
+                                                     float *d_y, int64_t y_stride, float *d_h,
+                                                     void *d_ws, size_t ws_bytes, void *stream);
+/* g = dy . up^T, dx = dx_base + scale * g . down (d_dx_base NULL: zeros; it
+ * may be d_dx); ddown [count][rank][in] = scale * sum g x and dup
+ * [count][rank][out] = scale * sum h dy over each adapter's rows, f32, zeros
+ * for adapters without rows and past an adapter's rank; with accumulate = 1
+ * added to what d_ddown and d_dup hold.  Any of d_dx, d_ddown and d_dup may
+ * be NULL, not all three; d_x is read for ddown only, d_h for dup only.  The
+ * sums' order is fixed: the same bits on every run. */
+WELVET_API welvet_status welvet_hip_adapters_backward(
+    const welvet_hip_adapters *desc, const float *d_x, int64_t x_stride, const int32_t *d_ids,
+    int32_t n, const float *d_h, const float *d_dy, int64_t dy_stride, const float *d_dx_base,
+    int64_t dx_base_stride, float *d_dx, int64_t dx_stride, int32_t accumulate, float *d_ddown,
+    float *d_dup, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Distillation from a teacher's top logits.  Row t < n holds logits z over
+ * the vocabulary (Float32, Float16 or BFloat16; row stride `stride`), and the
+ * teacher's k entries (k <= 1024) index[t][k], teacher[t][k] (f32 logits).
+ * With temperature T (0 < T, finite): q = softmax of the row's teacher / T,
+ * or, where d_teacher_lse [n] is given, exp(teacher / T - teacher_lse[t])
+ * (the log-sum of the teacher's whole row at T: q then sums to what its top
+ * entries hold); p = softmax(z / T) over the vocabulary;
+ *   loss[t] = w T^2 sum_i q_i (log q_i - log p_index(i))
+ *   dlogits[t][v] = w T (p_v sum_i q_i - sum of q_i over index(i) = v)
+ * with w = weight[t] (d_weight NULL = 1): dlogits is the gradient of the
+ * losses' sum, in the logits' type, rounded to nearest even.  An entry whose
+ * index lies outside [0, vocab) or whose logit is -inf is absent; a row
+ * without entries, or of weight 0, has loss 0 and gradient 0 whatever its
+ * logits.  A logit of -inf has p = 0 (and an infinite loss where an entry
+ * names it); a row without a finite logit has p = 0.  d_loss [n] or
+ * d_dlogits may be NULL, not both; d_dlogits may be d_logits (the same
+ * stride): the gradient then takes the logits' place. */
+WELVET_API welvet_status welvet_hip_distill_bytes(int32_t dtype, int32_t n, int32_t vocab,
+                                                  int32_t k, size_t *bytes);
+WELVET_API welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab,
+                                            const void *d_logits, int64_t stride, int32_t k,
+                                            const int32_t *d_index, const float *d_teacher,
+                                            const float *d_teacher_lse, const float *d_weight,
+                                            float temperature, float *d_loss, void *d_dlogits,
+                                            int64_t dstride, void *d_ws, size_t ws_bytes,
+                                            void *stream);
+
 /* Kernel route of the forward: 0 auto, 1 GEMV, 2 MFMA GEMM, 3 element-wise. */
 WELVET_API void welvet_hip_set_forward_path(int32_t path);
 /* Route switch `key` := value, returns the previous value (-1 = unknown key,

@@ -1,0 +1,53 @@
+"""Host side of the token-side operators: their argument checks come before
+any device work, and their workspaces cover what the calls ask for."""
+import ctypes as C
+
+import pytest
+
+import pywelvet
+
+
+def test_refused_before_the_device():
+    L = pywelvet.lib()
+    assert pywelvet.embedding_forward(9, 4, 4, 16, 16, 1, 16, status=True).code == 2
+    assert pywelvet.embedding_forward(1, 0, 4, 16, 16, 1, 16, status=True).code == 1
+    assert L.welvet_hip_embedding_store_forward(None, 16, 1, 1.0, 16, 4, None).code == 1
+    assert pywelvet.embedding_backward(4, 4, 16, 1, None, 16, status=True).code == 1
+    st = pywelvet.embedding_backward(4, 4, 16, 300, 16, 16, status=True)
+    assert st.code == 1 and b"workspace" in st.message
+    a = pywelvet.Adapters(1, 1, 4, 8, 8, 16, 16)
+    st = a.forward(16, 16, 3, 16, 16, status=True)
+    assert st.code == 1 and b"workspace" in st.message
+    assert a.backward(16, 16, 3, 16, 16, status=True).code == 1
+    assert L.welvet_hip_adapters_forward(None, 16, 8, 16, 1, None, 0, 16, 8, None, None, 0, None).code == 1
+    assert pywelvet.distill(1, 1, 8, 16, 1, 16, 16, d_loss=16, temperature=0.0, status=True).code == 1
+    assert pywelvet.distill(7, 1, 8, 16, 1, 16, 16, d_loss=16, status=True).code == 2
+
+
+def test_no_device_is_unsupported():
+    if pywelvet.available():
+        pytest.skip("a GPU is present")
+    assert pywelvet.embedding_forward(1, 4, 4, 16, 16, 1, 16, status=True).code == 2
+    assert pywelvet.distill(1, 1, 8, 16, 1, 16, 16, d_loss=16, status=True).code == 2
+
+
+def test_sizes_past_a_launch_are_refused():
+    b = C.c_size_t()
+    L = pywelvet.lib()
+    assert L.welvet_hip_embedding_backward_bytes(2**31 - 1, 64, 1, C.byref(b)).code == 1
+    assert L.welvet_hip_embedding_backward_bytes(2**31 - 2, 8192, 1, C.byref(b)).code == 1
+    assert L.welvet_hip_embedding_backward_bytes(10, 10, 1, None).code == 1
+    assert L.welvet_hip_distill_bytes(1, 1, 2**31 - 1, 1, C.byref(b)).code == 1
+    a = pywelvet.Adapters(1, 1, 4, 8, 8, 16, 16)
+    assert L.welvet_hip_adapters_bytes(a._ref, 2**24 + 1, C.byref(b)).code == 1
+
+
+@pytest.mark.parametrize("n", [0, 1, 256, 257, 4096, 4097, 100000])
+def test_embedding_workspace(n):
+    """Nothing up to 256 tokens; above, the order (twice that past 4096 tokens)
+    and two partial rows for every 32 tokens."""
+    got = pywelvet.embedding_backward_bytes(5000, 100, n)
+    if n <= 256:
+        assert got == 0
+    else:
+        assert got >= n * 4 * (4 if n > 4096 else 2) + -(-n // 32) * 2 * 100 * 4

@@ -1,0 +1,417 @@
+// distill.hip — the loss of a student's logits against a teacher's top ones,
+// and the logits' gradient.  For a row of logits z over the vocabulary and
+// the teacher's k entries (index i, logit l_i) at temperature T:
+//   q_i = exp(l_i / T - L), L the log-sum of the row's entries, or the
+//         teacher's own over its whole vocabulary where that is given
+//   p   = softmax(z / T)
+//   loss = w T^2 sum_i q_i (log q_i - log p_i)
+//   dz_v = w T (p_v sum_i q_i - sum of the q_i of index v)
+// An entry with an index outside the vocabulary or a logit of -inf is absent;
+// a row without one, or of weight 0, has loss 0 and gradient 0.
+//
+// A row's maximum and sum of exponentials are one pass over it (each thread a
+// running pair, joined across the block), the gradient a second: bound by
+// HBM, which reads each logit once where a row's block still holds it and
+// writes the gradient once.  Exponentials are taken as 2^(z c - m c) with
+// c = log2(e) / T in one fma: its rounding of m c is common to the row and
+// leaves p as it is; the loss takes the same c and m c in f64.  Where m c
+// overflows (a row masked with the type's lowest value throughout) they are
+// 2^((z - m) c).
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "tokens.hpp"
+
+namespace wh {
+namespace {
+
+using namespace tok;
+
+constexpr int kMaxEntries = 1024;
+
+struct Args {
+  const void *logits;
+  int64_t stride;
+  int vocab, k;
+  const int32_t *index;
+  const float *teacher, *teacher_lse, *weight;
+  float temperature, c;  // c = log2(e) / T
+  float *loss;
+  void *grad;
+  int64_t gstride;
+};
+
+// Running maximum of z and sum of 2^(z c - mc), mc = m c as rounded.
+struct Stat {
+  float m, s;
+};
+// The exponent's offset; huge: m c overflows (m itself may be +inf).
+struct Shift {
+  float m, mc;
+  bool huge;
+  __device__ Shift(float m_, float c) : m(m_), mc(m_ == -INFINITY ? 0.0f : m_ * c) { huge = fabsf(mc) == INFINITY; }
+};
+__device__ inline float term(float z, float c, const Shift &h) {
+  return __builtin_amdgcn_exp2f(h.huge ? (z - h.m) * c : fmaf(z, c, -h.mc));
+}
+// The factor from a sum at maximum m to one at h's: between the offsets as
+// rounded, so 1 where they are equal.  An empty sum's (0) must not be NaN.
+__device__ inline float rescale(float m, float c, const Shift &h) {
+  if (m == -INFINITY) return 1.0f;
+  return __builtin_amdgcn_exp2f(h.huge ? (m - h.m) * c : m * c - h.mc);
+}
+__device__ inline Stat join(Stat a, Stat b, float c) {
+  const Shift h(fmaxf(a.m, b.m), c);
+  return {h.m, a.s * rescale(a.m, c, h) + b.s * rescale(b.m, c, h)};
+}
+template <int N>
+__device__ inline void take(Stat &a, const float (&z)[N], float c) {
+  float m = z[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
+  if (m > a.m) {
+    const Shift h(m, c);
+    a.s *= rescale(a.m, c, h);
+    a.m = m;
+  }
+  const Shift h(a.m, c);
+  if (__builtin_expect(h.huge, 0)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.s += __builtin_amdgcn_exp2f((z[i] - h.m) * c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.s += __builtin_amdgcn_exp2f(fmaf(z[i], c, -h.mc));
+  }
+}
+
+// The block's pair, on every thread.
+template <int WAVES>
+__device__ inline Stat block_join(Stat a, float c, Stat *lds) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) a = join(a, {__shfl_xor(a.m, off), __shfl_xor(a.s, off)}, c);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) a = join(a, lds[w], c);
+  return a;
+}
+template <int WAVES>
+__device__ inline float block_sum(float v, float *lds) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) v += lds[w];
+  return v;
+}
+
+// n values at p: `head` ones up to a 16-byte boundary, whole 16-byte words,
+// `tail` ones.
+template <class T>
+struct Span {
+  const typename T::raw *p;
+  int n, head, words, tail;
+  __device__ Span(const typename T::raw *p_, int n_) : p(p_), n(n_) {
+    const int off = (int)(((uintptr_t)p & 15) / sizeof(typename T::raw));
+    head = min(n, off ? T::kPer16 - off : 0);
+    words = (n - head) / T::kPer16;
+    tail = n - head - words * T::kPer16;
+  }
+  __device__ const uint4 *word(int i) const { return (const uint4 *)(p + head) + i; }
+  // the place of edge value i < head + tail
+  __device__ int edge(int i) const { return i < head ? i : n - tail + (i - head); }
+};
+
+// The teacher's entries of a row, in LDS.
+struct Entries {
+  int index[kMaxEntries];
+  float q[kMaxEntries];  // log q
+  float z[kMaxEntries];  // the student's logit, read before its gradient may take its place
+  float wave[16];
+  int some;
+};
+template <class T>
+__device__ inline float logit(const Args &a, int row, int v) {
+  return T::get(((const typename T::raw *)a.logits + (int64_t)row * a.stride)[v]);
+}
+// Fills e, *mass = the sum of q; false where the row has no entry.  zs: the
+// entries' logits of this row, or null for reading them.
+template <class T, int WAVES>
+__device__ inline bool read_teacher(const Args &a, int row, const float *zs, Entries &e, float *mass) {
+  const double inv = 1.0 / (double)a.temperature;
+  if (threadIdx.x == 0) e.some = 0;
+  __syncthreads();
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
+    const int v = a.index[(int64_t)row * a.k + i];
+    const float l = a.teacher[(int64_t)row * a.k + i];
+    const bool live = v >= 0 && v < a.vocab && l != -INFINITY;
+    e.index[i] = live ? v : -1;
+    e.q[i] = l;
+    e.z[i] = !live ? 0.0f : zs ? zs[i] : logit<T>(a, row, v);
+    if (live) top = fmaxf(top, l), e.some = 1;
+  }
+  __syncthreads();
+  if (!e.some) return false;
+  double most;
+  if (a.teacher_lse == nullptr) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if ((threadIdx.x & 63) == 0) e.wave[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = e.wave[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, e.wave[w]);
+    __syncthreads();
+    most = (double)top * inv;
+  } else {
+    most = (double)a.teacher_lse[row];
+  }
+  float sum = 0.0f;
+  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
+    e.q[i] = (float)((double)e.q[i] * inv - most);
+    if (e.index[i] >= 0) sum += expf(e.q[i]);
+  }
+  sum = block_sum<WAVES>(sum, e.wave);
+  if (a.teacher_lse == nullptr) {
+    const float log_sum = logf(sum);
+    for (int i = threadIdx.x; i < a.k; i += WAVES * 64) e.q[i] -= log_sum;
+    sum = 1.0f;
+  }
+  *mass = sum;
+  __syncthreads();
+  return true;
+}
+
+// loss of a row from the pair of its logits; every thread calls it.
+template <int WAVES>
+__device__ inline void write_loss(const Args &a, int row, const Entries &e, Stat st, float weight) {
+  const Shift h(st.m, a.c);
+  const double c = (double)a.c, mc = h.huge ? (double)h.m * c : (double)h.mc, log2s = log2((double)st.s);
+  double loss = 0.0;
+  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
+    if (e.index[i] < 0) continue;
+    // no finite logit: p = 0 everywhere
+    const double logp = st.s == 0.0f ? -INFINITY : 0.6931471805599453 * ((double)e.z[i] * c - mc - log2s);
+    const double q = exp((double)e.q[i]);
+    if (q != 0.0) loss += q * ((double)e.q[i] - logp);  // 0 log 0 = 0, also under p = 0
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) loss += __shfl_xor(loss, off);
+  __shared__ double lds[WAVES];
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int w = 0; w < WAVES; ++w) loss += lds[w];
+    a.loss[row] = (float)(loss * (double)a.temperature * (double)a.temperature * (double)weight);
+  }
+}
+
+// The entries' own gradients over the part [begin, begin + n) of the row,
+// once every thread's dense values are written: index v's first entry stands
+// for all of v's.
+template <class T, int WAVES>
+__device__ inline void write_entries(const Args &a, int row, const Entries &e, int begin, int n, const Shift &h,
+                                     float g, float wt) {
+  typename T::raw *out = (typename T::raw *)a.grad + (int64_t)row * a.gstride;
+  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
+    const int v = e.index[i];
+    if (v < begin || v >= begin + n) continue;
+    float q = 0.0f;
+    bool first = true;
+    for (int j = 0; j < a.k; ++j) {
+      if (e.index[j] != v) continue;
+      if (j < i) first = false;
+      q += expf(e.q[j]);
+    }
+    if (first) out[v] = T::put(fmaf(term(e.z[i], a.c, h), g, -q * wt));
+  }
+}
+
+// Dense values of n logits at z: term * g.
+template <class T>
+__device__ inline uint4 grad_word(const uint4 &word, float c, const Shift &h, float g) {
+  float f[T::kPer16];
+  unpack16<T>(word, f);
+#pragma unroll
+  for (int i = 0; i < T::kPer16; ++i) f[i] = term(f[i], c, h) * g;
+  return pack16<T>(f);
+}
+template <class T, int THREADS>
+__device__ inline void zero_grad(typename T::raw *out, int n) {
+  const Span<T> span(out, n);
+  for (int i = threadIdx.x; i < span.words; i += THREADS) *(uint4 *)span.word(i) = make_uint4(0, 0, 0, 0);
+  if ((int)threadIdx.x < span.head + span.tail) out[span.edge(threadIdx.x)] = 0;
+}
+
+// A block's part of a row.
+//   STATS  the part's pair into pairs[row][part], and by part 0 the entries'
+//          logits into zs[row][k]
+//   else   the part's gradient, and by part 0 the loss: the row's pair from
+//          `pairs`, or from the part itself where that is null (one part)
+template <class T, int WAVES, bool STATS>
+__global__ void __launch_bounds__(WAVES * 64) distill_kernel(Args a, int parts, int len, Stat *pairs, float *zs) {
+  constexpr int kThreads = WAVES * 64;
+  __shared__ Stat lds[WAVES];
+  const int row = blockIdx.x / parts, part = blockIdx.x % parts, begin = part * len;
+  const int n = min(len, a.vocab - begin);
+  const float weight = a.weight ? a.weight[row] : 1.0f;
+  const Span<T> in((const typename T::raw *)a.logits + (int64_t)row * a.stride + begin, n);
+  Stat st{-INFINITY, 0.0f};
+  const auto stats = [&] {
+    int i = threadIdx.x;
+    for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
+      uint4 w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float f[T::kPer16];
+        unpack16<T>(w[k], f);
+        take(st, f, a.c);
+      }
+    }
+    for (; i < in.words; i += kThreads) {
+      float f[T::kPer16];
+      unpack16<T>(*in.word(i), f);
+      take(st, f, a.c);
+    }
+    if ((int)threadIdx.x < in.head + in.tail) {
+      const float f[1] = {T::get(in.p[in.edge(threadIdx.x)])};
+      take(st, f, a.c);
+    }
+    st = block_join<WAVES>(st, a.c, lds);
+  };
+  if constexpr (STATS) {
+    if (weight == 0.0f) return;
+    if (part == 0)
+      for (int i = threadIdx.x; i < a.k; i += kThreads) {
+        const int v = a.index[(int64_t)row * a.k + i];
+        if (v >= 0 && v < a.vocab) zs[(int64_t)row * a.k + i] = logit<T>(a, row, v);
+      }
+    stats();
+    if (threadIdx.x == 0) pairs[(int64_t)row * parts + part] = st;
+  } else {
+    __shared__ Entries e;
+    typename T::raw *out = a.grad ? (typename T::raw *)a.grad + (int64_t)row * a.gstride + begin : nullptr;
+    float mass = 0.0f;
+    if (weight == 0.0f || !read_teacher<T, WAVES>(a, row, zs ? zs + (int64_t)row * a.k : nullptr, e, &mass)) {
+      if (threadIdx.x == 0 && part == 0 && a.loss) a.loss[row] = 0.0f;
+      if (out) zero_grad<T, kThreads>(out, n);
+      return;
+    }
+    if (pairs == nullptr) {
+      stats();
+    } else {
+      for (int i = threadIdx.x; i < parts; i += kThreads) st = join(st, pairs[(int64_t)row * parts + i], a.c);
+      st = block_join<WAVES>(st, a.c, lds);
+    }
+    if (part == 0 && a.loss) write_loss<WAVES>(a, row, e, st, weight);
+    if (!out) return;
+    const Shift h(st.m, a.c);
+    const float c = a.c, wt = weight * a.temperature;
+    const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
+    if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
+      uint4 *to = (uint4 *)(out + in.head);
+      int i = threadIdx.x;
+      for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to[i + k * kThreads] = grad_word<T>(w[k], c, h, g);
+      }
+      for (; i < in.words; i += kThreads) to[i] = grad_word<T>(*in.word(i), c, h, g);
+      if ((int)threadIdx.x < in.head + in.tail) {
+        const int at = in.edge(threadIdx.x);
+        out[at] = T::put(term(T::get(in.p[at]), c, h) * g);
+      }
+    } else {
+      for (int i = threadIdx.x; i < n; i += kThreads) out[i] = T::put(term(T::get(in.p[i]), c, h) * g);
+    }
+    __syncthreads();
+    write_entries<T, WAVES>(a, row, e, begin, n, h, g, wt);
+  }
+}
+
+// Parts of a row: one where there are rows for every CU, else as many as give
+// each CU two blocks of at least 4096 values.
+int parts_of(int n, int vocab) {
+  if (n == 0 || n >= 256) return 1;
+  return std::max(1, std::min((512 + n - 1) / n, vocab / 4096));
+}
+int part_len(int vocab, int parts) { return ((vocab + parts - 1) / parts + 63) / 64 * 64; }
+size_t pairs_bytes(int n, int vocab) { return pad256((size_t)n * parts_of(n, vocab) * sizeof(Stat)); }
+size_t workspace_bytes(int n, int vocab, int k) {
+  return parts_of(n, vocab) == 1 ? 0 : pairs_bytes(n, vocab) + pad256((size_t)n * k * sizeof(float));
+}
+
+template <class T>
+hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
+  const int most = parts_of(n, a.vocab);
+  if (most == 1) {
+    distill_kernel<T, 16, false><<<n, 1024, 0, s>>>(a, 1, a.vocab, nullptr, nullptr);
+    return hipGetLastError();
+  }
+  const int len = part_len(a.vocab, most), parts = (a.vocab + len - 1) / len;
+  Stat *pairs = (Stat *)ws;
+  float *zs = (float *)((char *)ws + pairs_bytes(n, a.vocab));
+  distill_kernel<T, 4, true><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  distill_kernel<T, 4, false><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
+  return hipGetLastError();
+}
+
+bool sizes_ok(int32_t dtype, int32_t n, int32_t vocab, int32_t k) {
+  return n >= 0 && n <= (1 << 28) && vocab > 0 && vocab <= INT32_MAX - 64 && k > 0 && k <= kMaxEntries;
+}
+
+}  // namespace
+}  // namespace wh
+
+using namespace wh;
+using namespace wh::rt;
+
+extern "C" {
+
+welvet_status welvet_hip_distill_bytes(int32_t dtype, int32_t n, int32_t vocab, int32_t k, size_t *bytes) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
+  if (!sizes_ok(dtype, n, vocab, k) || !bytes) return make_status(kInvalid, "distill: invalid argument");
+  *bytes = workspace_bytes(n, vocab, k);
+  return ok();
+}
+
+welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab, const void *d_logits, int64_t stride,
+                                 int32_t k, const int32_t *d_index, const float *d_teacher,
+                                 const float *d_teacher_lse, const float *d_weight, float temperature, float *d_loss,
+                                 void *d_dlogits, int64_t dstride, void *d_ws, size_t ws_bytes, void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
+  if (!sizes_ok(dtype, n, vocab, k) || (n > 0 && (!d_logits || !d_index || !d_teacher)) || (!d_loss && !d_dlogits))
+    return make_status(kInvalid, "distill: invalid argument");
+  if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+    return make_status(kInvalid, "distill: temperature must be positive and finite");
+  if (stride < vocab || (d_dlogits && dstride < vocab))
+    return make_status(kInvalid, "distill: row stride below vocab %d", vocab);
+  const int size = tok::float_size(dtype);
+  if (!tok::aligned(d_logits, size) || !tok::aligned(d_dlogits, size) || !tok::aligned(d_index, 4) ||
+      !tok::aligned(d_teacher, 4) || !tok::aligned(d_teacher_lse, 4) || !tok::aligned(d_weight, 4) ||
+      !tok::aligned(d_loss, 4))
+    return make_status(kInvalid, "distill: device pointers must be aligned to their elements");
+  const size_t need = workspace_bytes(n, vocab, k);
+  if (need > 0 && (!d_ws || ws_bytes < need || !tok::aligned(d_ws, 16)))
+    return make_status(kInvalid, "distill: %zu bytes of 16-byte aligned workspace are needed", need);
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  const Args a{d_logits, stride,   vocab, k,      d_index,   d_teacher, d_teacher_lse, d_weight, temperature,
+               (float)(1.4426950408889634 / (double)temperature), d_loss, d_dlogits, dstride};
+  WH_HIP(tok::with_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, d_ws, (hipStream_t)stream); }));
+  return ok();
+}
+
+}  // extern "C"

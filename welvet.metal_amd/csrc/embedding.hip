@@ -1,0 +1,440 @@
+// embedding.hip — rows of a table by token, scaled, and the table's gradient.
+//   forward   out[t] = scale * table[token[t]]
+//   gradient  dtable[v] = scale * sum of dout[t] over the t with token[t] = v
+// A token outside [0, vocab) is padding: its output row is zero and its
+// gradient row is left out.  The forward only moves bytes; the gradient adds
+// one f32 per value of dout and writes the table's rows, so both are bound by
+// HBM and every value is read and written once.
+#include <hip/hip_runtime.h>
+
+#include "codec.hpp"
+#include "tokens.hpp"
+
+namespace wh {
+namespace {
+
+using namespace tok;
+
+// A thread's columns of a block's column tile: four neighbours as one 16-byte
+// word (VEC: dim, strides and pointers allow it), or four blockDim apart.
+template <bool VEC>
+struct Cols {
+  int c0;  // first column
+  int step, dim;
+  __device__ Cols(int tile, int dim_) : dim(dim_) {
+    const int width = 4 * blockDim.x;
+    c0 = VEC ? tile * width + 4 * threadIdx.x : tile * width + threadIdx.x;
+    step = VEC ? 1 : blockDim.x;
+  }
+  __device__ bool any() const { return c0 < dim; }
+  __device__ float4 load(const float *row) const {
+    if constexpr (VEC) return *(const float4 *)(row + c0);
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c0 + i * step < dim ? row[c0 + i * step] : 0.0f;
+    return make_float4(v[0], v[1], v[2], v[3]);
+  }
+  __device__ void store(float *row, float4 v) const {
+    if constexpr (VEC) {
+      *(float4 *)(row + c0) = v;
+    } else {
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i * step < dim) row[c0 + i * step] = f[i];
+    }
+  }
+};
+
+__device__ inline float4 add4(float4 a, float4 b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+__device__ inline float4 mul4(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
+
+// ---------------------------------------------------------------- forward
+// A block takes ROWS tokens and a column tile; a thread four columns of each
+// row, all rows' loads in flight before the first store.
+template <class T, bool VEC, int ROWS>
+__global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__restrict__ table, int64_t tstride,
+                                                     uint32_t vocab, int dim, const int32_t *__restrict__ tokens,
+                                                     int n, float scale, float *__restrict__ out, int64_t ostride,
+                                                     int tiles) {
+  const int group = blockIdx.x / tiles;
+  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  if (!cols.any()) return;
+  float4 v[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int t = group * ROWS + r;
+    const uint32_t id = t < n ? (uint32_t)tokens[t] : vocab;
+    v[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (id >= vocab) continue;
+    const typename T::raw *row = table + (int64_t)id * tstride;
+    if constexpr (VEC && sizeof(typename T::raw) == 4) {
+      v[r] = *(const float4 *)(row + cols.c0);
+    } else if constexpr (VEC) {
+      const ushort4 u = *(const ushort4 *)(row + cols.c0);
+      v[r] = make_float4(T::get(u.x), T::get(u.y), T::get(u.z), T::get(u.w));
+    } else {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = cols.c0 + i * cols.step < dim ? T::get(row[cols.c0 + i * cols.step]) : 0.0f;
+      v[r] = make_float4(f[0], f[1], f[2], f[3]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int t = group * ROWS + r;
+    if (t >= n) break;
+    // padding stays +0 also under a negative scale
+    const bool pad = (uint32_t)tokens[t] >= vocab;
+    cols.store(out + (int64_t)t * ostride, pad ? v[r] : mul4(v[r], scale));
+  }
+}
+
+// The same from a packed store: any of the 34 formats, one element at a time
+// (a lookup reads a few rows; what the formats cost is their bit offsets).
+template <int DT>
+__global__ void __launch_bounds__(256) store_lookup_kernel(const uint8_t *__restrict__ body, float wscale,
+                                                           float minv, uint32_t vocab, int dim,
+                                                           const int32_t *__restrict__ tokens, float scale,
+                                                           float *__restrict__ out, int64_t ostride, int tiles) {
+  const int t = blockIdx.x / tiles;
+  const uint32_t id = (uint32_t)tokens[t];
+  const int c0 = blockIdx.x % tiles * 1024 + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + 256 * i;
+    if (c >= dim) break;
+    float v = 0.0f;
+    if (id < vocab) v = dec_code<DT>(load_code<DT>(body, (int64_t)id * dim + c), wscale, minv) * scale;
+    out[(int64_t)t * ostride + c] = v;
+  }
+}
+
+template <int DT = 0>
+hipError_t launch_store_lookup(const DevStore &w, const int32_t *tokens, int n, float scale, float *out,
+                               int64_t ostride, hipStream_t s) {
+  if constexpr (DT < kNumDTypes) {
+    if (w.dtype != DT) return launch_store_lookup<DT + 1>(w, tokens, n, scale, out, ostride, s);
+    const int tiles = (w.cols + 1023) / 1024;
+    store_lookup_kernel<DT><<<(uint32_t)((int64_t)n * tiles), 256, 0, s>>>(
+        w.body, w.scale, w.minv, (uint32_t)w.rows, w.cols, tokens, scale, out, ostride, tiles);
+    return hipGetLastError();
+  } else {
+    return hipErrorInvalidValue;
+  }
+}
+
+// --------------------------------------------------------------- gradient
+// Few tokens: a block takes one of them and a column tile, and where it is
+// the first of its token adds up that token's rows.
+constexpr int kDirect = 256;
+// More: rows in the tokens' order, kRun of them a block and column tile.  A
+// token whose rows end inside the block's is written from registers; one that
+// reaches into a neighbour's leaves a partial row (slot 0: began earlier,
+// slot 1: goes on), and join_kernel adds those up, in order.
+constexpr int kRun = 32;
+constexpr int kZeroRows = 8;  // table rows of a zeroing block
+
+template <bool VEC, bool ACC>
+__device__ inline void put_row(const Cols<VEC> &cols, float *row, float4 sum, float scale) {
+  float4 v = mul4(sum, scale);
+  if constexpr (ACC) v = add4(cols.load(row), v);
+  cols.store(row, v);
+}
+
+template <bool VEC>
+__device__ inline void zero_row(float *row, int dim) {
+  if constexpr (VEC) {
+    for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) *(float4 *)(row + c) = make_float4(0, 0, 0, 0);
+  } else {
+    for (int c = threadIdx.x; c < dim; c += blockDim.x) row[c] = 0.0f;
+  }
+}
+
+template <bool VEC, bool ACC>
+__global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__ tokens, int n, uint32_t vocab,
+                                                     int dim, const float *__restrict__ dout, int64_t dstride,
+                                                     float scale, float *__restrict__ dtable, int64_t tstride,
+                                                     int tiles) {
+  __shared__ int32_t tok_s[kDirect];
+  __shared__ int rows_s[kDirect];
+  __shared__ int count_s;
+  for (int j = threadIdx.x; j < n; j += blockDim.x) tok_s[j] = tokens[j];
+  const int adders = n * tiles;
+  if ((int)blockIdx.x >= adders) {  // rows without a token
+    __shared__ int named[kZeroRows];
+    if (threadIdx.x < kZeroRows) named[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)adders) * kZeroRows;
+    for (int j = threadIdx.x; j < n; j += blockDim.x) {
+      const uint32_t d = (uint32_t)tok_s[j] - v0;
+      if (d < kZeroRows) named[d] = 1;
+    }
+    __syncthreads();
+    for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
+      if (!named[r]) zero_row<VEC>(dtable + (int64_t)(v0 + r) * tstride, dim);
+    return;
+  }
+  if (threadIdx.x == 0) count_s = 0;
+  __syncthreads();
+  const int i = blockIdx.x / tiles;
+  const int32_t mine = tok_s[i];
+  if ((uint32_t)mine >= vocab) return;
+  if (threadIdx.x < 64) {  // this token's rows, in order
+    int count = 0;
+    bool first = true;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+      const int j = j0 + threadIdx.x;
+      const uint64_t same = __ballot(j < n && tok_s[j] == mine);
+      const uint64_t below = threadIdx.x ? ~0ull >> (64 - threadIdx.x) : 0ull;
+      if (j < n && tok_s[j] == mine) rows_s[count + __popcll(same & below)] = j;
+      if (count == 0 && same) first = j0 + __ffsll((long long)same) - 1 == i;
+      count += __popcll(same);
+    }
+    if (threadIdx.x == 0) count_s = first ? count : 0;
+  }
+  __syncthreads();
+  const int count = count_s;
+  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  if (count == 0 || !cols.any()) return;
+  float4 sum = make_float4(0, 0, 0, 0);
+  int r = 0;
+  for (; r + 4 <= count; r += 4) {
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = cols.load(dout + (int64_t)rows_s[r + k] * dstride);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
+  }
+  for (; r < count; ++r) sum = add4(sum, cols.load(dout + (int64_t)rows_s[r] * dstride));
+  put_row<VEC, ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+}
+
+// The first place of the sorted keys whose key is >= v.
+__device__ inline int first_at_least(const int32_t *__restrict__ skey, int n, uint32_t v) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((uint32_t)skey[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <bool VEC, bool ACC>
+__global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ skey,
+                                                   const int32_t *__restrict__ order, int n, uint32_t vocab, int dim,
+                                                   const float *__restrict__ dout, int64_t dstride, float scale,
+                                                   float *__restrict__ dtable, int64_t tstride,
+                                                   float *__restrict__ part, int tiles, int adders) {
+  if ((int)blockIdx.x >= adders) {
+    __shared__ int named[kZeroRows];
+    const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)adders) * kZeroRows;
+    if (threadIdx.x < kZeroRows) {
+      const int at = first_at_least(skey, n, v0 + threadIdx.x);
+      named[threadIdx.x] = at < n && (uint32_t)skey[at] == v0 + threadIdx.x;
+    }
+    __syncthreads();
+    for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
+      if (!named[r]) zero_row<VEC>(dtable + (int64_t)(v0 + r) * tstride, dim);
+    return;
+  }
+  __shared__ int32_t key_s[kRun + 2];  // with the neighbours' nearest
+  __shared__ int32_t row_s[kRun];
+  const int chunk = blockIdx.x / tiles, p0 = chunk * kRun;
+  if (threadIdx.x < kRun + 2) {
+    const int p = p0 - 1 + (int)threadIdx.x;
+    key_s[threadIdx.x] = p >= 0 && p < n ? skey[p] : -1;
+  }
+  if (threadIdx.x < kRun) row_s[threadIdx.x] = p0 + (int)threadIdx.x < n ? order[p0 + threadIdx.x] : 0;
+  __syncthreads();
+  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  if (!cols.any()) return;
+  const int32_t before = key_s[0], after = key_s[kRun + 1];
+  int32_t cur = key_s[1];
+  bool began = cur != before;
+  float4 sum = make_float4(0, 0, 0, 0);
+  const auto done = [&](bool goes_on) {
+    if ((uint32_t)cur >= vocab) return;  // padding, or past the last row
+    if (!began) cols.store(part + (int64_t)(2 * chunk) * dim, sum);
+    else if (goes_on) cols.store(part + (int64_t)(2 * chunk + 1) * dim, sum);
+    else put_row<VEC, ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale);
+  };
+#pragma unroll 1
+  for (int r0 = 0; r0 < kRun; r0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = make_float4(0, 0, 0, 0);
+      if ((uint32_t)key_s[1 + r0 + k] < vocab) v[k] = cols.load(dout + (int64_t)row_s[r0 + k] * dstride);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int32_t next = key_s[1 + r0 + k];
+      if (next != cur) {
+        done(false);
+        cur = next;
+        began = true;
+        sum = make_float4(0, 0, 0, 0);
+      }
+      sum = add4(sum, v[k]);
+    }
+  }
+  done(cur == after);
+}
+
+// Tokens whose rows fill more than one block's: the block where one begins
+// adds its later blocks' slot 0 to its own slot 1, in order.
+template <bool VEC, bool ACC>
+__global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ skey, int n, uint32_t vocab, int dim,
+                                                   const float *__restrict__ part, float scale,
+                                                   float *__restrict__ dtable, int64_t tstride, int tiles) {
+  const int chunk = blockIdx.x / tiles, p0 = chunk * kRun, p1 = p0 + kRun;
+  if (p1 >= n) return;
+  const int32_t mine = skey[p1 - 1];
+  if ((uint32_t)mine >= vocab || skey[p1] != mine) return;
+  if (p0 > 0 && skey[p0 - 1] == mine) return;  // began earlier
+  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  if (!cols.any()) return;
+  const int last = (first_at_least(skey, n, (uint32_t)mine + 1) - 1) / kRun;
+  float4 sum = cols.load(part + (int64_t)(2 * chunk + 1) * dim);
+  int c = chunk + 1;
+  for (; c + 4 <= last + 1; c += 4) {
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = cols.load(part + (int64_t)(2 * (c + k)) * dim);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
+  }
+  for (; c <= last; ++c) sum = add4(sum, cols.load(part + (int64_t)(2 * c) * dim));
+  put_row<VEC, ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+}
+
+int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
+
+size_t gradient_bytes(int dim, int n) {
+  if (n <= kDirect) return 0;
+  const size_t chunks = ((size_t)n + kRun - 1) / kRun;
+  return order_bytes(n) + pad256(chunks * 2 * (size_t)dim * sizeof(float));
+}
+
+template <bool VEC, bool ACC>
+hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, float scale, const float *dout,
+                           int64_t dstride, float *dtable, int64_t tstride, void *ws, hipStream_t s) {
+  const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
+  const int64_t zeros = ACC ? 0 : ((int64_t)vocab + kZeroRows - 1) / kZeroRows;
+  if (n <= kDirect) {
+    if (n == 0 && ACC) return hipSuccess;
+    direct_kernel<VEC, ACC><<<(uint32_t)((int64_t)n * tiles + zeros), threads, 0, s>>>(
+        tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles);
+    return hipGetLastError();
+  }
+  Order o;
+  hipError_t e = launch_order(tokens, n, vocab, ws, &o, s);
+  if (e != hipSuccess) return e;
+  float *part = (float *)((char *)ws + order_bytes(n));
+  const int64_t chunks = ((int64_t)n + kRun - 1) / kRun, adders = chunks * tiles;
+  sums_kernel<VEC, ACC><<<(uint32_t)(adders + zeros), threads, 0, s>>>(
+      o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, part, tiles, (int)adders);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  join_kernel<VEC, ACC><<<(uint32_t)adders, threads, 0, s>>>(o.skey, n, (uint32_t)vocab, dim, part, scale, dtable,
+                                                            tstride, tiles);
+  return hipGetLastError();
+}
+
+// A launch's blocks and the kernels' int counters: (n + vocab / 8) * tiles.
+bool sizes_ok(int32_t vocab, int32_t dim, int32_t n) {
+  return vocab > 0 && vocab < INT32_MAX && dim > 0 && n >= 0 &&
+         ((int64_t)n + vocab) * ((dim + 1023) / 1024 + 1) < INT32_MAX;
+}
+
+}  // namespace
+}  // namespace wh
+
+using namespace wh;
+using namespace wh::rt;
+
+extern "C" {
+
+welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t dim, const void *d_table,
+                                           int64_t table_stride, const int32_t *d_tokens, int32_t n, float scale,
+                                           float *d_out, int64_t out_stride, void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "embedding: unsupported dtype %d", dtype);
+  if (!sizes_ok(vocab, dim, n) || !d_table || (n > 0 && (!d_tokens || !d_out)))
+    return make_status(kInvalid, "embedding: invalid argument");
+  if (table_stride < dim || out_stride < dim) return make_status(kInvalid, "embedding: row stride below dim %d", dim);
+  const int size = tok::float_size(dtype);
+  if (!tok::aligned(d_table, size) || !tok::aligned(d_tokens, 4) || !tok::aligned(d_out, 4))
+    return make_status(kInvalid, "embedding: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  const bool vec = dim % 4 == 0 && table_stride % 4 == 0 && out_stride % 4 == 0 && tok::aligned(d_table, 4 * size) &&
+                   tok::aligned(d_out, 16);
+  const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
+  // four rows a block where there are blocks enough for every CU several times over
+  const int rows = (int64_t)n * tiles >= 8192 ? 4 : 1;
+  const uint32_t blocks = (uint32_t)(((int64_t)n + rows - 1) / rows * tiles);
+  tok::with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto go = [&](auto kernel) {
+      kernel<<<blocks, threads, 0, (hipStream_t)stream>>>((const typename T::raw *)d_table, table_stride,
+                                                          (uint32_t)vocab, dim, d_tokens, n, scale, d_out, out_stride,
+                                                          tiles);
+    };
+    if (vec) rows == 4 ? go(lookup_kernel<T, true, 4>) : go(lookup_kernel<T, true, 1>);
+    else rows == 4 ? go(lookup_kernel<T, false, 4>) : go(lookup_kernel<T, false, 1>);
+  });
+  WH_HIP(hipGetLastError());
+  return ok();
+}
+
+welvet_status welvet_hip_embedding_store_forward(welvet_dense_session *s, const int32_t *d_tokens, int32_t n,
+                                                 float scale, float *d_out, int64_t out_stride, void *stream) {
+  if (!s || n < 0 || (n > 0 && (!d_tokens || !d_out))) return make_status(kInvalid, "embedding: invalid argument");
+  std::unique_lock<std::mutex> lock;
+  const DevStore w = session_store(s, &lock);
+  if ((int64_t)n * ((w.cols + 1023) / 1024) > INT32_MAX) return make_status(kInvalid, "embedding: invalid argument");
+  if (out_stride < w.cols) return make_status(kInvalid, "embedding: row stride below dim %d", w.cols);
+  if (!tok::aligned(d_tokens, 4) || !tok::aligned(d_out, 4))
+    return make_status(kInvalid, "embedding: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  WH_HIP(launch_store_lookup(w, d_tokens, n, scale, d_out, out_stride, (hipStream_t)stream));
+  return ok();
+}
+
+welvet_status welvet_hip_embedding_backward_bytes(int32_t vocab, int32_t dim, int32_t n, size_t *bytes) {
+  if (!sizes_ok(vocab, dim, n) || !bytes) return make_status(kInvalid, "embedding backward: invalid argument");
+  *bytes = gradient_bytes(dim, n);
+  return ok();
+}
+
+welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t dim, const int32_t *d_tokens, int32_t n,
+                                            float scale, const float *d_dout, int64_t dout_stride, int32_t accumulate,
+                                            float *d_dtable, int64_t dtable_stride, void *d_ws, size_t ws_bytes,
+                                            void *stream) {
+  if (!sizes_ok(vocab, dim, n) || !d_dtable || (n > 0 && (!d_tokens || !d_dout)))
+    return make_status(kInvalid, "embedding backward: invalid argument");
+  if (dout_stride < dim || dtable_stride < dim)
+    return make_status(kInvalid, "embedding backward: row stride below dim %d", dim);
+  if (!tok::aligned(d_tokens, 4) || !tok::aligned(d_dout, 4) || !tok::aligned(d_dtable, 4))
+    return make_status(kInvalid, "embedding backward: device pointers must be aligned to their elements");
+  const size_t need = gradient_bytes(dim, n);
+  if (need > 0 && (!d_ws || ws_bytes < need || !tok::aligned(d_ws, 16)))
+    return make_status(kInvalid, "embedding backward: %zu bytes of 16-byte aligned workspace are needed", need);
+  welvet_status st = require_device();
+  if (st.code) return st;
+  const bool vec = dim % 4 == 0 && dout_stride % 4 == 0 && dtable_stride % 4 == 0 && tok::aligned(d_dout, 16) &&
+                   tok::aligned(d_dtable, 16);
+  const auto go = [&](auto launch) {
+    return launch(vocab, dim, d_tokens, n, scale, d_dout, dout_stride, d_dtable, dtable_stride, d_ws,
+                  (hipStream_t)stream);
+  };
+  WH_HIP(accumulate ? (vec ? go(launch_gradient<true, true>) : go(launch_gradient<false, true>))
+                    : (vec ? go(launch_gradient<true, false>) : go(launch_gradient<false, false>)));
+  return ok();
+}
+
+}  // extern "C"

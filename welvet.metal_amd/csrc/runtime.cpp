@@ -550,6 +550,11 @@ welvet_status backward_device(welvet_dense_session *s, const float *d_x, const f
 
 }  // namespace
 
+DevStore wh::rt::session_store(welvet_dense_session *s, std::unique_lock<std::mutex> *lock) {
+  *lock = std::unique_lock<std::mutex>(s->mu);
+  return s->W.dev();
+}
+
 extern "C" {
 
 const char *welvet_version(void) { return "0.71"; }

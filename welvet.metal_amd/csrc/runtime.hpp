@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/welvet_c.h"
 #include "codec.hpp"
 #include "kernels.hpp"
@@ -115,6 +117,10 @@ welvet_status store_sgd(Store *w, const float *d_dW, double lr, int *d_flag, hip
 welvet_status store_native(const Store &w, uint8_t *out, size_t cap, size_t *len, hipStream_t s);
 welvet_status store_export(const Store &w, float *d_out, hipStream_t s);
 bool dims_ok(int32_t rows, int32_t cols);
+
+// A mounted session's store as the kernels take it; *lock holds the session
+// until the caller has enqueued what reads it.
+DevStore session_store(welvet_dense_session *s, std::unique_lock<std::mutex> *lock);
 
 // Volume hooks for the model sessions (volume.cpp): bind a ready store (taken
 // over), read a bound cell's store, change the batch, and

@@ -55,6 +55,14 @@ class Blob(C.Structure):
     _fields_ = [("data", C.POINTER(C.c_uint8)), ("size", C.c_size_t)]
 _vp = C.c_void_p
 _i32 = C.c_int32
+_i64 = C.c_int64
+
+
+class AdaptersDesc(C.Structure):
+    """welvet_hip_adapters: a stack of low-rank adapters in device memory."""
+    _fields_ = [("dtype", C.c_int32), ("count", C.c_int32), ("rank", C.c_int32),
+                ("inn", C.c_int32), ("out", C.c_int32), ("d_down", C.c_void_p),
+                ("d_up", C.c_void_p), ("d_ranks", C.c_void_p), ("d_scales", C.c_void_p)]
 
 
 def _fp(a):
@@ -161,6 +169,26 @@ def lib() -> C.CDLL:
         L.welvet_hip_set_tuning.restype = _i32
         L.welvet_hip_probe_read.argtypes = [_vp, C.c_uint64, _vp, _vp]
         L.welvet_hip_probe_read.restype = Status
+        st = C.c_size_t
+        L.welvet_hip_embedding_forward.argtypes = [_i32] * 3 + [_vp, _i64, _vp, _i32, C.c_float,
+                                                                _vp, _i64, _vp]
+        L.welvet_hip_embedding_store_forward.argtypes = [_vp, _vp, _i32, C.c_float, _vp, _i64, _vp]
+        L.welvet_hip_embedding_backward_bytes.argtypes = [_i32] * 3 + [C.POINTER(st)]
+        L.welvet_hip_embedding_backward.argtypes = [_i32] * 2 + [_vp, _i32, C.c_float, _vp, _i64,
+                                                                 _i32, _vp, _i64, _vp, st, _vp]
+        _ad = C.POINTER(AdaptersDesc)
+        L.welvet_hip_adapters_bytes.argtypes = [_ad, _i32, C.POINTER(st)]
+        L.welvet_hip_adapters_forward.argtypes = [_ad, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i64,
+                                                  _vp, _vp, st, _vp]
+        L.welvet_hip_adapters_backward.argtypes = [_ad, _vp, _i64, _vp, _i32, _vp, _vp, _i64, _vp,
+                                                   _i64, _vp, _i64, _i32, _vp, _vp, _vp, st, _vp]
+        L.welvet_hip_distill_bytes.argtypes = [_i32] * 4 + [C.POINTER(st)]
+        L.welvet_hip_distill.argtypes = [_i32] * 3 + [_vp, _i64, _i32] + [_vp] * 4 + \
+            [C.c_float, _vp, _vp, _i64, _vp, st, _vp]
+        for nm in ("embedding_forward", "embedding_store_forward", "embedding_backward_bytes",
+                   "embedding_backward", "adapters_bytes", "adapters_forward", "adapters_backward",
+                   "distill_bytes", "distill"):
+            getattr(L, "welvet_hip_" + nm).restype = Status
         coord = [_vp] + [_i32] * 4
         L.welvet_hip_grid_new.argtypes = [_i32] * 5 + [C.POINTER(_vp)]
         L.welvet_hip_grid_new.restype = Status
@@ -626,3 +654,108 @@ class Grid:
         check(lib().welvet_hip_grid_native(self.h, *coord, out.ctypes.data_as(_u8), out.size,
                                            C.byref(n), C.byref(s)))
         return out, s.value
+
+
+# ---- token ends of a network and adapters beside its layers: device pointers
+# (ints) and a hipStream_t int; each returns once enqueued.  Strides count
+# elements between rows (None: the rows follow one another).
+
+def embedding_forward(dtype, vocab, dim, d_table, d_tokens, n, d_out, scale=1.0, table_stride=None,
+                      out_stride=None, stream=None, status=False):
+    """welvet_hip_embedding_forward: out[t] = scale * table[tokens[t]]."""
+    st = lib().welvet_hip_embedding_forward(
+        dtype, vocab, dim, d_table, dim if table_stride is None else table_stride, d_tokens, n,
+        scale, d_out, dim if out_stride is None else out_stride, stream)
+    if status:
+        return st
+    check(st)
+
+
+def embedding_store_forward(session, d_tokens, n, d_out, scale=1.0, out_stride=None, stream=None,
+                            status=False):
+    """welvet_hip_embedding_store_forward: rows of a Session's store."""
+    st = lib().welvet_hip_embedding_store_forward(
+        session.h, d_tokens, n, scale, d_out, session.inn if out_stride is None else out_stride,
+        stream)
+    if status:
+        return st
+    check(st)
+
+
+def embedding_backward_bytes(vocab, dim, n) -> int:
+    b = C.c_size_t()
+    check(lib().welvet_hip_embedding_backward_bytes(vocab, dim, n, C.byref(b)))
+    return b.value
+
+
+def embedding_backward(vocab, dim, d_tokens, n, d_dout, d_dtable, scale=1.0, accumulate=False,
+                       dout_stride=None, dtable_stride=None, ws=None, ws_bytes=0, stream=None,
+                       status=False):
+    """welvet_hip_embedding_backward: dtable (+)= scale * sums of dout by token."""
+    st = lib().welvet_hip_embedding_backward(
+        vocab, dim, d_tokens, n, scale, d_dout, dim if dout_stride is None else dout_stride,
+        1 if accumulate else 0, d_dtable, dim if dtable_stride is None else dtable_stride, ws,
+        ws_bytes, stream)
+    if status:
+        return st
+    check(st)
+
+
+class Adapters:
+    """welvet_hip_adapters_*: a stack of low-rank adapters beside a projection
+    inn -> out (factors down [count][rank][inn], up [count][rank][out])."""
+
+    def __init__(self, dtype, count, rank, inn, out, d_down, d_up, d_ranks=None, d_scales=None):
+        self.desc = AdaptersDesc(dtype, count, rank, inn, out, d_down, d_up, d_ranks, d_scales)
+        self._ref = C.byref(self.desc)
+
+    def workspace_bytes(self, n) -> int:
+        b = C.c_size_t()
+        check(lib().welvet_hip_adapters_bytes(self._ref, n, C.byref(b)))
+        return b.value
+
+    def forward(self, d_x, d_ids, n, d_base, d_y, d_h=None, x_stride=None, base_stride=None,
+                y_stride=None, ws=None, ws_bytes=0, stream=None, status=False):
+        """y = base + scale * (x . down^T) . up, each row with its own adapter."""
+        d = self.desc
+        st = lib().welvet_hip_adapters_forward(
+            self._ref, d_x, d.inn if x_stride is None else x_stride, d_ids, n, d_base,
+            d.out if base_stride is None else base_stride, d_y,
+            d.out if y_stride is None else y_stride, d_h, ws, ws_bytes, stream)
+        if status:
+            return st
+        check(st)
+
+    def backward(self, d_x, d_ids, n, d_h, d_dy, d_dx_base=None, d_dx=None, d_ddown=None,
+                 d_dup=None, accumulate=False, x_stride=None, dy_stride=None, dx_base_stride=None,
+                 dx_stride=None, ws=None, ws_bytes=0, stream=None, status=False):
+        """dx, ddown and dup (each where its pointer is given)."""
+        d = self.desc
+        st = lib().welvet_hip_adapters_backward(
+            self._ref, d_x, d.inn if x_stride is None else x_stride, d_ids, n, d_h, d_dy,
+            d.out if dy_stride is None else dy_stride, d_dx_base,
+            d.inn if dx_base_stride is None else dx_base_stride, d_dx,
+            d.inn if dx_stride is None else dx_stride, 1 if accumulate else 0, d_ddown, d_dup, ws,
+            ws_bytes, stream)
+        if status:
+            return st
+        check(st)
+
+
+def distill_bytes(dtype, n, vocab, k) -> int:
+    b = C.c_size_t()
+    check(lib().welvet_hip_distill_bytes(dtype, n, vocab, k, C.byref(b)))
+    return b.value
+
+
+def distill(dtype, n, vocab, d_logits, k, d_index, d_teacher, d_loss=None, d_dlogits=None,
+            temperature=1.0, d_weight=None, d_teacher_lse=None, logits_stride=None,
+            dlogits_stride=None, ws=None, ws_bytes=0, stream=None, status=False):
+    """welvet_hip_distill: the loss against a teacher's top logits and its gradient."""
+    st = lib().welvet_hip_distill(
+        dtype, n, vocab, d_logits, vocab if logits_stride is None else logits_stride, k, d_index,
+        d_teacher, d_teacher_lse, d_weight, temperature, d_loss, d_dlogits,
+        vocab if dlogits_stride is None else dlogits_stride, ws, ws_bytes, stream)
+    if status:
+        return st
+    check(st)
