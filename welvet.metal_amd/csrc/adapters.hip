@@ -28,13 +28,13 @@ using v4f = __attribute__((ext_vector_type(4))) float;
 __device__ inline v4f mfma(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 constexpr int kMaxRank = 256;
-constexpr int kFewRows = 128;  // tiles of one row up to here
+constexpr int kFewRows = 128;  // a block a row up to here
 
 // The rows of a launch: position p -> row and adapter (count: none).
 struct RowMap {
   const int32_t *key;    // adapter by position (sorted), or by row
   const int32_t *order;  // row by position; null: the row itself
-  int n, count, tile;    // tile: positions a block takes together (16 or 1)
+  int n, count;
   __device__ int row(int p) const { return order ? order[p] : p; }
   __device__ int adapter(int p) const {
     const uint32_t a = (uint32_t)key[p];
@@ -61,98 +61,296 @@ struct Hidden {
   }
 };
 
-// Four values at row + k of a row of `width`: zeros past its end.
-template <bool VEC>
-__device__ inline float4 load4(const float *row, int k, int width) {
-  if constexpr (VEC) return k < width ? *(const float4 *)(row + k) : make_float4(0, 0, 0, 0);
-  float f[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = k + i < width ? row[k + i] : 0.0f;
-  return make_float4(f[0], f[1], f[2], f[3]);
-}
-template <class T, bool VEC>
-__device__ inline float4 load4t(const typename T::raw *row, int k, int width) {
-  if constexpr (VEC && sizeof(typename T::raw) == 4) {
-    return k < width ? *(const float4 *)(row + k) : make_float4(0, 0, 0, 0);
-  } else if constexpr (VEC) {
-    const ushort4 u = k < width ? *(const ushort4 *)(row + k) : make_ushort4(0, 0, 0, 0);
-    return make_float4(T::get(u.x), T::get(u.y), T::get(u.z), T::get(u.w));
-  } else {
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = k + i < width ? T::get(row[k + i]) : 0.0f;
-    return make_float4(f[0], f[1], f[2], f[3]);
-  }
-}
-template <bool VEC>
-__device__ inline void store4(float *row, int k, int width, float4 v) {
-  if constexpr (VEC) {
-    if (k < width) *(float4 *)(row + k) = v;
-  } else {
-    const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k + i < width) row[k + i] = f[i];
-  }
-}
-__device__ inline float get4(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
 // --------------------------------------------------------- rows by a factor
 // hidden[split][row][j] = sum over the split's k of x[row][k] factor_a[j][k].
-// D[i = row][j = rank] of 16 x 16 x 4 MFMAs: lane l holds row (or rank) l % 16
-// and k = 4 (l / 16) + s for the s-th of four MFMAs, so both operands are one
-// 4-value load a lane.  A block's waves take 16 k in turn and add up in LDS.
+// D[i = row][j = rank] of 16 x 16 x 4 MFMAs: lane l holds row (or rank) l % 16,
+// and four lanes l / 16 share its k.  Rank rows past the adapter's repeat its
+// last one and are dropped at the end.
+//
+// Few rows: a block one row and a split of the width, where the MFMA's 16 rows
+// are the same one (what is read counts, not what is multiplied).  A wave's
+// step is 64 k, 16 (l / 16) + s for the s-th of sixteen MFMAs: whole 128-byte
+// lines of every rank row.  The block's waves take the steps in turn, the next
+// one's loads in flight, and add up in LDS.
 constexpr int kDownWaves = 8;
-template <class T, bool VEC, int RT>
-__global__ void __launch_bounds__(kDownWaves * 64) down_kernel(RowMap rows, Factor fac, const float *__restrict__ x,
-                                                               int64_t xstride, Hidden out, int split_len) {
-  __shared__ float red[kDownWaves][16][RT * 16 + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
-  const int p0 = blockIdx.x * rows.tile, live = min(rows.tile, rows.n - p0), j0 = blockIdx.z * RT * 16;
-  const int kbegin = blockIdx.y * split_len, kend = min(kbegin + split_len, fac.width);
-  const int mine = min(lo, live - 1);  // lanes past the tile's rows repeat its last
-  const int row = rows.row(p0 + mine), key = rows.adapter(p0 + mine);
-  const float *xrow = x + (int64_t)row * xstride;
-  float *hidden = out.p + (int64_t)blockIdx.y * out.n * out.rank;
-  for (int i0 = 0; i0 < live;) {
-    const int a = __builtin_amdgcn_readlane(key, i0);
-    // the run of positions [i0, i1) of adapter a
-    const uint64_t same = __ballot(lane < live && key == a);
-    const int i1 = i0 + __popcll(same >> i0);
-    const int ra = a < rows.count ? fac.rank_of(a) : 0;
-    v4f acc[RT] = {};
-    if (ra > j0) {
-      const typename T::raw *f = (const typename T::raw *)fac.p + ((int64_t)a * fac.rank + j0) * fac.width;
-      const int most = ra - j0;
-      for (int k = kbegin + wave * 16; k < kend; k += kDownWaves * 16) {
-        const float4 xv = load4<VEC>(xrow, k + 4 * q, kend);
-        float4 fv[RT];
+constexpr int kStep = 64;
+// 16 neighbouring factor values
+template <class T>
+struct Hex {
+  static constexpr int kWords = (int)sizeof(typename T::raw);
+  uint4 v[kWords];
+  __device__ inline void load(const typename T::raw *p) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int j = t * 16 + lo;
-          fv[t] = j < most ? load4t<T, VEC>(f + (int64_t)j * fac.width, k + 4 * q, kend) : make_float4(0, 0, 0, 0);
+    for (int i = 0; i < kWords; ++i) __builtin_memcpy(&v[i], p + i * T::kPer16, 16);
+  }
+  __device__ inline float get(int s) const {
+    const uint4 &w = v[s / T::kPer16];
+    const int e = s % T::kPer16;
+    const int at = e * (int)sizeof(typename T::raw) / 4;
+    const uint32_t word = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
+    if constexpr (sizeof(typename T::raw) == 4) return T::get(word);
+    else return T::get((uint16_t)(word >> (16 * (e & 1))));
+  }
+};
+template <class T, int RT>
+__global__ void __launch_bounds__(kDownWaves * 64) down_row_kernel(RowMap rows, Factor fac,
+                                                                   const float *__restrict__ x, int64_t xstride,
+                                                                   Hidden out, int split_len) {
+  using raw = typename T::raw;
+  __shared__ float red[kDownWaves][RT * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lo = lane & 15, q = lane >> 4;
+  const int row = blockIdx.x, j0 = blockIdx.z * RT * 16;
+  const int kbegin = blockIdx.y * split_len, kend = min(kbegin + split_len, fac.width);
+  const int first = kbegin + wave * kStep;
+  const int full = first + kStep <= kend ? (kend - first - kStep) / (kDownWaves * kStep) + 1 : 0;  // whole steps
+  const float *xrow = x + (int64_t)row * xstride;
+  const int a = rows.adapter(row), ra = a < rows.count ? fac.rank_of(a) : 0;
+  if (ra > j0) {
+    v4f acc[RT] = {};
+    const raw *frow[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      frow[t] = (const raw *)fac.p + ((int64_t)a * fac.rank + min(j0 + t * 16 + lo, ra - 1)) * fac.width;
+    float4 xv[2][4];
+    Hex<T> fv[2][RT];
+    const auto load = [&](int d, int step) {
+      const int k = first + min(step, full - 1) * (kDownWaves * kStep) + 16 * q;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) __builtin_memcpy(&xv[d][m], xrow + k + 4 * m, 16);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) fv[d][t].load(frow[t] + k);
+      issued();
+    };
+    const auto multiply = [&](int d) {
+#pragma unroll
+      for (int s = 0; s < 16; ++s)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = mfma(get4(xv[d][s / 4], s & 3), fv[d][t].get(s), acc[t]);
+    };
+    if (full > 0) {
+      // no condition between a load and its use: the compiler would move the
+      // load past it
+      load(0, 0);
+      for (int step = 1; step < full; step += 2) {
+        load(1, step);
+        multiply(0);
+        load(0, step + 1);
+        multiply(1);
+      }
+      if (full & 1) multiply(0);
+    }
+    const int k = first + full * (kDownWaves * kStep);  // the rest of the width, one wave's
+    if (k < kend) {
+#pragma unroll 1
+      for (int s = 0; s < kStep; s += 16) {
+        const float4 xs = load4(xrow, k + s + 4 * q, kend);
+        float4 fs[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) fs[t] = Quad<T>::load(frow[t], k + s + 4 * q, kend).floats();
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[t] = mfma(get4(xs, m), get4(fs[t], m), acc[t]);
+      }
+    }
+    if (q == 0)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) red[wave][t * 16 + lo] = acc[t][0];
+  }
+  __syncthreads();
+  const int j = threadIdx.x;
+  if (j < min(RT * 16, fac.rank - j0)) {
+    float sum = 0.0f;
+    if (j0 + j < ra)
+#pragma unroll
+      for (int w = 0; w < kDownWaves; ++w) sum += red[w][j];
+    out.p[((int64_t)blockIdx.y * out.n + row) * out.rank + j0 + j] = sum;
+  }
+}
+
+// An adapter's sums over a block's rows, D[i = rank][j = column]: into the
+// gradient where all its rows lie in the block, else into the block's partial
+// (slot 0: its rows began earlier, slot 1: they go on) for sum_kernel.
+struct Sum {
+  const float *hidden, *x;
+  int64_t xstride;
+  int width, chunk, across;  // chunk: rows of a block; across: blocks along the width
+  float *grad, *part;
+};
+template <bool ACC, int RT, bool NARROW>
+__device__ inline void store_sums(const v4f (&acc)[RT][4], const Factor &fac, int a, int ra, int j0, int q,
+                                  const Cols<NARROW> &cols, bool began, bool goes_on, const Sum &job) {
+  const int64_t size = (int64_t)fac.rank * job.width;
+  const float scale = fac.scale_of(a);
+  const bool whole = began && !goes_on;
+  float *to = whole ? job.grad + (int64_t)a * size : job.part + ((int64_t)blockIdx.y * 2 + (began ? 1 : 0)) * size;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = j0 + 16 * t + 4 * q + r;
+      if (j >= fac.rank || !cols.any()) continue;
+      float4 v = j < ra ? make_float4(acc[t][0][r], acc[t][1][r], acc[t][2][r], acc[t][3][r])
+                        : make_float4(0, 0, 0, 0);  // rank rows past the adapter's
+      float *at = to + (int64_t)j * job.width;
+      if (whole) {
+        v = j < ra ? mul4(v, scale) : v;
+        if constexpr (ACC) v = add4(cols.load(at), v);
+      }
+      cols.store(at, v);
+    }
+}
+
+// The same for many rows, a block a slice of the width: the slice's factor
+// values stay in registers while an adapter's rows pass, 16 at a time, the next
+// 16 rows' loads in flight.  Every wave holds 64 columns, its products are
+// added up across the block in LDS, and the slices' sums are left for
+// fold_kernel: hidden[slice][row][j].  A lane's 64-byte pieces of a row start at
+// its wave's column + 16 m + 4 (l / 16), m < 4.
+//
+// SUMS: the rows also give the second product that reads them, sum over the
+// adapter's rows of job.hidden[row][j] x[row][c] (outer_kernel below has its
+// terms), so that x is read from HBM once for both: a wave's 16 x 64 part is
+// turned in LDS to the columns-by-rows order of that product.
+constexpr int kSliceWaves = 8;
+constexpr int kSlice = kSliceWaves * 64;
+constexpr int kMaxChunk = 512;
+template <class T, int RT, bool SUMS, bool ACC, bool NARROW>
+__global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, Sum job, float *__restrict__ hidden) {
+  constexpr int kPitch = 68;  // floats of a turned row: reads by columns fall on different banks
+  using raw = typename T::raw;
+  __shared__ float red[kSliceWaves][16][RT * 16 + 1];
+  __shared__ float4 turn4[SUMS ? kSliceWaves * 16 * kPitch / 4 : 1];
+  __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lo = lane & 15, q = lane >> 4;
+  const int width = fac.width, c0 = blockIdx.x * kSlice + wave * 64, j0 = blockIdx.z * RT * 16;
+  const int p0 = blockIdx.y * job.chunk, p1 = min(p0 + job.chunk, rows.n);
+  const int ranks = min(RT * 16, fac.rank - j0);
+  float *turn = (float *)turn4 + (SUMS ? wave * 16 * kPitch : 0);
+  float *to_hidden = hidden + (int64_t)blockIdx.x * rows.n * fac.rank + j0;
+  for (int i = threadIdx.x; i < p1 - p0; i += kSlice) {
+    row_s[i] = rows.row(p0 + i);
+    key_s[i] = rows.adapter(p0 + i);
+  }
+  __syncthreads();
+  for (int i0 = p0; i0 < p1;) {
+    const int a = __builtin_amdgcn_readfirstlane(key_s[i0 - p0]);
+    int i1 = p1;  // the end of a's run here
+    for (int step = i0, hi = p1; step < hi;) {
+      const int mid = (step + hi) >> 1;
+      if (__builtin_amdgcn_readfirstlane(key_s[mid - p0]) == a) step = mid + 1;
+      else i1 = hi = mid;
+    }
+    const int ra = a < rows.count ? fac.rank_of(a) : 0;
+    v4f sums[RT][4] = {};
+    if (ra > j0) {
+      Quad<T> fv[RT][4];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const raw *row = (const raw *)fac.p + ((int64_t)a * fac.rank + min(j0 + 16 * t + lo, ra - 1)) * width;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const Cols<NARROW> cols(c0 + 16 * m + 4 * q, width);
+          fv[t][m] = cols.template load<T>(row);
+          fv[t][m].drop(cols.skip);
+        }
+      }
+      // values of a piece past the row's end, or another piece's, count as zeros
+      const auto own = [&](int m, const float4 &v) {
+        const Cols<NARROW> cols(c0 + 16 * m + 4 * q, width);
+        return make_float4(cols.skip < 1 ? v.x : 0.0f, cols.skip < 2 ? v.y : 0.0f, cols.skip < 3 ? v.z : 0.0f,
+                           cols.skip < 4 ? v.w : 0.0f);
+      };
+      const float *hcol[RT];
+      if constexpr (SUMS) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) hcol[t] = job.hidden + min(j0 + 16 * t + lo, ra - 1);
+      }
+      float4 xv[2][4];
+      float hv[2][RT][4];
+      const int tiles = (i1 - i0 + 15) / 16;
+      const auto load = [&](int d, int tile) {
+        const int p = i0 + 16 * min(tile, tiles - 1);
+        const float *row = job.x + (int64_t)row_s[min(p + lo, i1 - 1) - p0] * job.xstride;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) xv[d][m] = Cols<NARROW>(c0 + 16 * m + 4 * q, width).load(row);
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int64_t from = row_s[min(p + 4 * r + q, i1 - 1) - p0];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) hv[d][t][r] = hcol[t][from * fac.rank];
+          }
+        }
+        issued();
+      };
+      const auto multiply = [&](int d, int tile) {
+        const int p = i0 + 16 * tile;
+        v4f acc[RT] = {};
+        float4 x[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          x[m] = own(m, xv[d][m]);
+          if constexpr (SUMS) x[m] = keep4(p + lo < i1, x[m]);
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int m = 0; m < 4; ++m) {
+          if constexpr (SUMS) *(float4 *)(turn + lo * kPitch + 16 * m + 4 * q) = x[m];
 #pragma unroll
-          for (int t = 0; t < RT; ++t) acc[t] = mfma(get4(xv, s), get4(fv[t], s), acc[t]);
+          for (int t = 0; t < RT; ++t) {
+            const float4 f = fv[t][m].floats();
+#pragma unroll
+            for (int s = 0; s < 4; ++s) acc[t] = mfma(get4(x[m], s), get4(f, s), acc[t]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) red[wave][4 * q + r][16 * t + lo] = acc[t][r];
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float4 v = *(const float4 *)(turn + (4 * r + q) * kPitch + 4 * lo);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              const float h = p + 4 * r + q < i1 ? hv[d][t][r] : 0.0f;
+#pragma unroll
+              for (int m = 0; m < 4; ++m) sums[t][m] = mfma(h, get4(v, m), sums[t][m]);
+            }
+          }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < 16 * ranks; e += kSlice) {
+          const int i = e / ranks, j = e % ranks;
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kSliceWaves; ++w) sum += red[w][i][j];
+          if (p + i < i1) to_hidden[(int64_t)row_s[p + i - p0] * fac.rank + j] = j0 + j < ra ? sum : 0.0f;
+        }
+        __syncthreads();
+      };
+      load(0, 0);
+      int tile = 0;
+      for (; tile + 1 < tiles; tile += 2) {
+        load(1, tile + 1);
+        multiply(0, tile);
+        load(0, tile + 2);
+        multiply(1, tile + 1);
       }
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) red[wave][4 * q + r][t * 16 + lo] = acc[t][r];
+      if (tile < tiles) multiply(0, tile);
+    } else {
+      for (int e = threadIdx.x; e < (i1 - i0) * ranks; e += kSlice)
+        to_hidden[(int64_t)row_s[i0 - p0 + e / ranks] * fac.rank + e % ranks] = 0.0f;
     }
-    __syncthreads();
-    const int width = min(RT * 16, fac.rank - j0);
-    for (int e = threadIdx.x; e < (i1 - i0) * width; e += kDownWaves * 64) {
-      const int i = i0 + e / width, j = e % width;
-      float sum = 0.0f;
-      if (j0 + j < ra)
-#pragma unroll
-        for (int w = 0; w < kDownWaves; ++w) sum += red[w][i][j];
-      hidden[(int64_t)rows.row(p0 + i) * out.rank + j0 + j] = sum;
+    if constexpr (SUMS) {
+      if (a >= rows.count) break;  // rows without an adapter come last
+      const bool began = i0 > p0 || p0 == 0 || rows.adapter(p0 - 1) != a;
+      const bool goes_on = i1 == p1 && p1 < rows.n && rows.adapter(p1) == a;
+      const Cols<NARROW> cols(c0 + 4 * lo, width);
+      store_sums<ACC>(sums, fac, a, ra, j0, q, cols, began, goes_on, job);
     }
-    __syncthreads();
     i0 = i1;
   }
 }
@@ -161,181 +359,269 @@ __global__ void __launch_bounds__(kDownWaves * 64) down_kernel(RowMap rows, Fact
 // y[row] = base[row] + s_a sum_j hidden[row][j] factor_a[j].  D[i = row][j =
 // column]: lane l holds columns 4 (l % 16) + m of its wave's 64 for the m-th
 // of four accumulators, so a row's part is stored as 16-byte words; ranks 4
-// (l / 16) + s of each 16 for the s-th MFMA.  Block: four waves, 256 columns.
-template <class T, bool VEC, int RT>
-__global__ void __launch_bounds__(256) up_kernel(RowMap rows, Factor fac, Hidden h, const float *base,
-                                                 int64_t bstride, float *y, int64_t ystride,
-                                                 float *__restrict__ hsum, int tiles) {
+// (l / 16) + s of each 16 for the s-th MFMA.  Block: four waves, 256 columns,
+// `per` tiles of 32 rows one after the other; the tile's hidden values lie in
+// LDS, the adapter's factor in registers as long as it stays the same.
+constexpr int kUpRows = 32;
+template <class T, int RT, bool NARROW>
+__global__ void __launch_bounds__(256) up_kernel(RowMap rows, Factor fac, const float *__restrict__ hidden,
+                                                 const float *base, int64_t bstride, float *y, int64_t ystride,
+                                                 int per) {
+  constexpr int TT = kUpRows / 16, kPitch = RT * 16 + 4;
+  using raw = typename T::raw;
+  __shared__ float4 hs4[kUpRows * kPitch / 4];
+  float *hs = (float *)hs4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
-  const int c = blockIdx.x * 256 + wave * 64 + 4 * lo;
-  for (int tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
-    const int p0 = tile * rows.tile, live = min(rows.tile, rows.n - p0);
-    if (hsum && blockIdx.x == 0)
-      for (int e = threadIdx.x; e < live * fac.rank; e += 256) {
-        const int row = rows.row(p0 + e / fac.rank);
-        hsum[(int64_t)row * fac.rank + e % fac.rank] = h.at(row, e % fac.rank);
-      }
-    const int mine = min(lo, live - 1);
-    const int row = rows.row(p0 + mine), key = rows.adapter(p0 + mine);
-    int out_row[4], out_key[4];
-    float4 sum[4];
+  const Cols<NARROW> cols(blockIdx.x * 256 + wave * 64 + 4 * lo, fac.width);
+  int held = -1;
+  Quad<T> fv[RT][4];
+  const auto load_factor = [&](int a, int ra, int g) {  // rank rows past the adapter's: zeros
+    const raw *f = (const raw *)fac.p + (int64_t)a * fac.rank * fac.width;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {  // the rows this lane's accumulators belong to
-      out_row[r] = __shfl(row, 4 * q + r);
-      out_key[r] = __shfl(key, 4 * q + r);
-      sum[r] = make_float4(0, 0, 0, 0);
-      if (base && 4 * q + r < live && c < fac.width) sum[r] = load4<VEC>(base + (int64_t)out_row[r] * bstride, c, fac.width);
-    }
-    for (int i0 = 0; i0 < live;) {
-      const int a = __builtin_amdgcn_readlane(key, i0);
-      const uint64_t same = __ballot(lane < live && key == a);
-      i0 += __popcll(same >> i0);
-      if (a >= rows.count) continue;
-      const int ra = fac.rank_of(a);
-      const float scale = fac.scale_of(a);
-      const typename T::raw *f = (const typename T::raw *)fac.p + (int64_t)a * fac.rank * fac.width;
-      v4f acc[4] = {};
-      for (int g = 0; g < ra; g += 16 * RT) {
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        fv[t][s] = cols.template load<T>(f + (int64_t)min(g + 16 * t + 4 * q + s, ra - 1) * fac.width);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (g + 16 * t + 4 * q + s >= ra) fv[t][s] = Quad<T>{};
+  };
+  for (int p0 = blockIdx.y * per * kUpRows; p0 < min(((int)blockIdx.y + 1) * per * kUpRows, rows.n); p0 += kUpRows) {
+    const int live = min(kUpRows, rows.n - p0);
+    const int mine = min(lane & (kUpRows - 1), live - 1);
+    const int row = rows.row(p0 + mine), key = rows.adapter(p0 + mine);
+    int out_key[TT][4];
+    float4 sum[TT][4];
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // the rows this lane's accumulators belong to
+        const int at = 16 * i + 4 * q + r, from = __shfl(row, at);
+        out_key[i][r] = __shfl(key, at);
+        sum[i][r] = make_float4(0, 0, 0, 0);
+        if (base) sum[i][r] = cols.load(base + (int64_t)from * bstride);
+      }
+    for (int g = 0; g < fac.rank; g += 16 * RT) {
+      const int wide = min(16 * RT, fac.rank - g);
+      __syncthreads();
+      for (int e = threadIdx.x; e < kUpRows * RT * 4; e += 256) {
+        const int i = e / (RT * 4), j = e % (RT * 4) * 4;
+        const float *from = hidden + (int64_t)rows.row(p0 + min(i, live - 1)) * fac.rank + g;
+        *(float4 *)(hs + i * kPitch + j) = load4(from, j, wide);
+      }
+      __syncthreads();
+      for (int i0 = 0; i0 < live;) {
+        const int a = __builtin_amdgcn_readlane(key, i0);
+        const uint64_t same = __ballot(lane < live && key == a);
+        i0 += __popcll(same >> i0);
+        if (a >= rows.count) continue;
+        const int ra = fac.rank_of(a);
+        if (ra <= g) continue;
+        if (held != a || fac.rank > 16 * RT) load_factor(a, ra, g);
+        held = a;
+        const float scale = fac.scale_of(a);
+        v4f acc[TT][4] = {};
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const int j = g + 16 * t + 4 * q;
-          float hv[4];
-          float4 fv[4];
+          if (16 * t >= ra - g) break;
+          float4 hv[TT];
+#pragma unroll
+          for (int i = 0; i < TT; ++i) hv[i] = *(const float4 *)(hs + (16 * i + lo) * kPitch + 16 * t + 4 * q);
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            hv[s] = j + s < ra ? h.at(row, j + s) : 0.0f;
-            fv[s] = j + s < ra && c < fac.width ? load4t<T, VEC>(f + (int64_t)(j + s) * fac.width, c, fac.width)
-                                                : make_float4(0, 0, 0, 0);
+            const float4 f = fv[t][s].floats();
+#pragma unroll
+            for (int i = 0; i < TT; ++i)
+#pragma unroll
+              for (int m = 0; m < 4; ++m) acc[i][m] = mfma(get4(hv[i], s), get4(f, m), acc[i][m]);
           }
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) acc[m] = mfma(hv[s], get4(fv[s], m), acc[m]);
         }
-      }
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (out_key[r] == a)
-          sum[r] = make_float4(fmaf(scale, acc[0][r], sum[r].x), fmaf(scale, acc[1][r], sum[r].y),
-                               fmaf(scale, acc[2][r], sum[r].z), fmaf(scale, acc[3][r], sum[r].w));
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (out_key[i][r] == a)
+              sum[i][r] = fma4(scale, make_float4(acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]), sum[i][r]);
+      }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * q + r < live) store4<VEC>(y + (int64_t)out_row[r] * ystride, c, fac.width, sum[r]);
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 16 * i + 4 * q + r;
+        const int to = __shfl(row, at);
+        if (at < live && cols.any()) cols.store(y + (int64_t)to * ystride, sum[i][r]);
+      }
   }
+}
+
+// The same for few rows: a block one row's 1024 columns, four a thread, the
+// hidden values from LDS, rank by rank with eight factor loads ahead.
+template <class T, bool NARROW>
+__global__ void __launch_bounds__(256) up_row_kernel(RowMap rows, Factor fac, Hidden h, const float *base,
+                                                     int64_t bstride, float *y, int64_t ystride,
+                                                     float *__restrict__ hsum) {
+  __shared__ float hs[kMaxRank];
+  const int row = blockIdx.y, a = rows.adapter(row);
+  const Cols<NARROW> cols(blockIdx.x * 1024 + 4 * threadIdx.x, fac.width);
+  const int ra = a < rows.count ? fac.rank_of(a) : 0;
+  if ((int)threadIdx.x < fac.rank) {
+    const float v = h.at(row, threadIdx.x);
+    hs[threadIdx.x] = v;
+    if (hsum && blockIdx.x == 0) hsum[(int64_t)row * fac.rank + threadIdx.x] = v;
+  }
+  float4 sum = make_float4(0, 0, 0, 0);
+  if (base && cols.any()) sum = cols.load(base + (int64_t)row * bstride);
+  __syncthreads();
+  if (!cols.any()) return;
+  if (ra > 0) {
+    const typename T::raw *f = (const typename T::raw *)fac.p + (int64_t)a * fac.rank * fac.width;
+    float4 acc = make_float4(0, 0, 0, 0);
+    for (int j0 = 0; j0 < ra; j0 += 8) {
+      Quad<T> v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = cols.template load<T>(f + (int64_t)min(j0 + j, ra - 1) * fac.width);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= ra) break;
+        acc = fma4(hs[j0 + j], v[j].floats(), acc);
+      }
+    }
+    sum = fma4(fac.scale_of(a), acc, sum);
+  }
+  cols.store(y + (int64_t)row * ystride, sum);
 }
 
 // ------------------------------------------------ sums over an adapter's rows
 // grad_a[j][c] = s_a sum over a's rows of hidden[row][j] x[row][c].  D[i =
-// rank][j = column]: a wave 64 columns (as above), four rows an MFMA.  A block
-// takes kSumRows positions of the sorted rows; an adapter whose rows end
-// inside them is written from registers, one that reaches into a neighbour's
-// leaves a partial (slot 0: began earlier, slot 1: goes on) for sum_kernel.
-constexpr int kSumRows = 512;
-template <bool VEC, bool ACC, int RT>
-__global__ void __launch_bounds__(256) outer_kernel(RowMap rows, Factor fac, Hidden h, const float *__restrict__ x,
-                                                    int64_t xstride, float *__restrict__ grad,
-                                                    float *__restrict__ part) {
+// rank][j = column]: a wave 64 columns (as above), four rows an MFMA, DEPTH
+// MFMA steps of loads ahead.  A block takes `chunk` positions of the sorted
+// rows.
+// A launch does the sums of both factors where both are asked for.
+struct Sums {
+  Sum of[2];
+  int count;
+};
+template <bool ACC, int RT, bool NARROW>
+__global__ void __launch_bounds__(256) outer_kernel(RowMap rows, Factor fac, Sums sums) {
+  constexpr int DEPTH = RT >= 4 ? 4 : 8;
+  __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
+  const bool second = (int)blockIdx.x >= sums.of[0].across;
+  const Sum &job = sums.of[second ? 1 : 0];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
-  const int c = blockIdx.x * 256 + wave * 64 + 4 * lo, j0 = blockIdx.z * RT * 16;
-  const int p0 = blockIdx.y * kSumRows, p1 = min(p0 + kSumRows, rows.n);
-  const int64_t size = (int64_t)fac.rank * fac.width;
+  const int across = (int)blockIdx.x - (second ? sums.of[0].across : 0);
+  const int j0 = blockIdx.z * RT * 16;
+  const int width = job.width, chunk = job.chunk, p0 = (int)blockIdx.y * chunk;
+  if (p0 >= rows.n) return;
+  const Cols<NARROW> cols(across * 256 + wave * 64 + 4 * lo, width);
+  const int p1 = min(p0 + chunk, rows.n);
+  for (int i = threadIdx.x; i < p1 - p0; i += 256) {
+    row_s[i] = rows.row(p0 + i);
+    key_s[i] = rows.adapter(p0 + i);
+  }
+  __syncthreads();
   for (int i0 = p0; i0 < p1;) {
-    const int a = rows.adapter(i0);
+    const int a = __builtin_amdgcn_readfirstlane(key_s[i0 - p0]);
     if (a >= rows.count) break;  // rows without an adapter come last
     int i1 = p1;                 // the end of a's run here
     for (int step = i0, hi = p1; step < hi;) {
       const int mid = (step + hi) >> 1;
-      if (rows.adapter(mid) == a) step = mid + 1;
+      if (__builtin_amdgcn_readfirstlane(key_s[mid - p0]) == a) step = mid + 1;
       else i1 = hi = mid;
     }
     const bool began = i0 > p0 || p0 == 0 || rows.adapter(p0 - 1) != a;
     const bool goes_on = i1 == p1 && p1 < rows.n && rows.adapter(p1) == a;
     const int ra = fac.rank_of(a);
     v4f acc[RT][4] = {};
-    if (ra > j0)
-      for (int p = i0; p < i1; p += 4) {
-        const bool in = p + q < i1;
-        const int row = in ? rows.row(p + q) : 0;
-        float4 xv = make_float4(0, 0, 0, 0);
-        if (in && c < fac.width) xv = load4<VEC>(x + (int64_t)row * xstride, c, fac.width);
-        float hv[RT];
+    if (ra > j0) {
+      const int steps = (i1 - i0 + 3) / 4;
+      const float *hcol[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) hv[t] = in && j0 + 16 * t + lo < ra ? h.at(row, j0 + 16 * t + lo) : 0.0f;
+      for (int t = 0; t < RT; ++t) hcol[t] = job.hidden + min(j0 + 16 * t + lo, ra - 1);
+      float4 xv[DEPTH];
+      float hv[DEPTH][RT];
+      const auto load = [&](int d, int step) {  // steps past the last repeat its last row
+        const int64_t row = row_s[min(i0 + 4 * step + q, i1 - 1) - p0];
+        xv[d] = cols.load(job.x + row * job.xstride);
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < RT; ++t) hv[d][t] = hcol[t][row * fac.rank];
+        issued();
+      };
 #pragma unroll
-          for (int m = 0; m < 4; ++m) acc[t][m] = mfma(hv[t], get4(xv, m), acc[t][m]);
-      }
-    const float scale = fac.scale_of(a);
-    const bool whole = began && !goes_on;
-    float *to = whole ? grad + (int64_t)a * size : part + ((int64_t)blockIdx.y * 2 + (began ? 1 : 0)) * size;
+      for (int d = 0; d < DEPTH; ++d) load(d, d);
+      for (int step = 0; step < steps; step += DEPTH) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+        for (int d = 0; d < DEPTH; ++d) {
+          if (step + d < steps) {
+            const bool on = i0 + 4 * (step + d) + q < i1;
+            const float4 xs = keep4(on, xv[d]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = j0 + 16 * t + 4 * q + r;
-        if (j >= fac.rank || c >= fac.width) continue;
-        float4 v = j < ra ? make_float4(acc[t][0][r], acc[t][1][r], acc[t][2][r], acc[t][3][r])
-                          : make_float4(0, 0, 0, 0);  // 0 times a NaN of x is not 0
-        float *at = to + (int64_t)j * fac.width;
-        if (whole) {
-          v = j < ra ? make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale) : v;
-          if constexpr (ACC) {
-            const float4 o = load4<VEC>(at, c, fac.width);
-            v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+            for (int t = 0; t < RT; ++t) {
+              const float hs = on ? hv[d][t] : 0.0f;
+#pragma unroll
+              for (int m = 0; m < 4; ++m) acc[t][m] = mfma(hs, get4(xs, m), acc[t][m]);
+            }
           }
+          load(d, step + d + DEPTH);
         }
-        store4<VEC>(at, c, fac.width, v);
       }
+    }
+    store_sums<ACC>(acc, fac, a, ra, j0, q, cols, began, goes_on, job);
     i0 = i1;
   }
 }
 
-// The adapters outer_kernel did not write: their partials added up in order,
+// The adapters that no block wrote whole: their partials added up in order,
 // zeros for those no row names.
 template <bool ACC>
-__global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, const float *__restrict__ part,
-                                                  float *__restrict__ grad) {
-  const int a = blockIdx.y;
-  int bound[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    int lo = 0, hi = rows.n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (rows.key[mid] < a + e) lo = mid + 1;
-      else hi = mid;
-    }
-    bound[e] = lo;
-  }
-  const int64_t size = (int64_t)fac.rank * fac.width;
-  float *to = grad + (int64_t)a * size;
-  if (bound[0] == bound[1]) {
-    if constexpr (!ACC)
-      for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 256) to[e] = 0.0f;
-    return;
-  }
-  const int first = bound[0] / kSumRows, last = (bound[1] - 1) / kSumRows;
-  if (first == last) return;
-  const int ra = fac.rank_of(a);
+__global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, Sums sums) {
+  const Sum &job = sums.of[blockIdx.z];
+  const float *part = job.part;
+  const int a = blockIdx.y, chunk = job.chunk;
+  const int begin = first_at_least(rows.key, rows.n, a), end = first_at_least(rows.key, rows.n, a + 1);
+  const int size = fac.rank * job.width;
+  float *to = job.grad + (int64_t)a * size;
+  const int first = begin / chunk, last = (end - 1) / chunk;
+  const bool none = begin == end;
+  if (none ? ACC : first == last) return;
+  const int edge = fac.rank_of(a) * job.width;
   const float scale = fac.scale_of(a);
-  for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 256) {
-    // its first block's rows went on (slot 1), every later one's began earlier
-    float v = part[((int64_t)first * 2 + 1) * size + e];
-    for (int b = first + 1; b <= last; ++b) v += part[(int64_t)b * 2 * size + e];
-    v = e < (int64_t)ra * fac.width ? v * scale : 0.0f;
-    to[e] = ACC ? to[e] + v : v;
+  for (int e = (blockIdx.x * 256 + threadIdx.x) * 4; e < size; e += gridDim.x * 1024) {
+    float4 v = make_float4(0, 0, 0, 0);
+    if (!none) {
+      // its first block's rows went on (slot 1), every later one's began earlier
+      v = load4(part + ((int64_t)first * 2 + 1) * size, e, size);
+      int b = first + 1;
+      for (; b + 4 <= last + 1; b += 4) {
+        float4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = load4(part + (int64_t)(b + i) * 2 * size, e, size);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v = add4(v, w[i]);
+      }
+      for (; b <= last; ++b) v = add4(v, load4(part + (int64_t)b * 2 * size, e, size));
+      v = make_float4(e < edge ? v.x * scale : 0.0f, e + 1 < edge ? v.y * scale : 0.0f,
+                      e + 2 < edge ? v.z * scale : 0.0f, e + 3 < edge ? v.w * scale : 0.0f);
+      if constexpr (ACC) v = add4(load4(to, e, size), v);
+    }
+    store4(to, e, size, v);
   }
 }
 
 // ------------------------------------------------------------------ launches
-// Blocks along k where the row tiles alone leave CUs idle: at least 512
+// Few rows: blocks along k where the rows alone leave CUs idle, at least 512
 // values of the width each.
-int splits_of(int n, int width) {
-  const int tiles = n <= kFewRows ? n : (n + 15) / 16;
-  return std::max(1, std::min({16, 512 / std::max(1, tiles), width / 512}));
+int splits_of(int n, int width) { return std::max(1, std::min({16, 512 / std::max(1, n), width / 512})); }
+int slices_of(int width) { return (width + kSlice - 1) / kSlice; }
+// Rows of a block of slice_kernel or outer_kernel: as many as leave two blocks
+// to every CU, `across` of them along the width.
+int chunk_of(int n, int across) {
+  const int64_t rows = (int64_t)n * across / 512 / 16 * 16;
+  return (int)std::max<int64_t>(16, std::min<int64_t>(kMaxChunk, rows));
 }
+int rank_groups(int rank) { return rank <= 64 ? 1 : (rank + 63) / 64; }
 
 struct Call {
   int32_t dtype;
@@ -350,89 +636,164 @@ void by_rank(int rank, F &&f) {
   else f(std::integral_constant<int, 4>{});
 }
 template <class F>
-void by_vec(bool vec, F &&f) {
-  if (vec) f(std::true_type{});
+void by_flag(bool flag, F &&f) {
+  if (flag) f(std::true_type{});
   else f(std::false_type{});
 }
 
-bool vec_ok(const Factor &f, int32_t dtype, std::initializer_list<std::pair<const void *, int64_t>> f32) {
-  bool ok = f.width % 4 == 0 && aligned(f.p, 4 * float_size(dtype));
-  for (auto &pe : f32) ok = ok && aligned(pe.first, 16) && pe.second % 4 == 0;
-  return ok;
-}
-
-hipError_t launch_down(const Call &c, const Factor &fac, const float *x, int64_t xstride, const Hidden &out) {
-  const int split_len = (((fac.width + out.splits - 1) / out.splits) + 15) / 16 * 16;
-  const int tiles = (c.rows.n + c.rows.tile - 1) / c.rows.tile;
+hipError_t launch_down_rows(const Call &c, const Factor &fac, const float *x, int64_t xstride, const Hidden &out) {
+  const int split_len = (((fac.width + out.splits - 1) / out.splits) + kStep - 1) / kStep * kStep;
   by_rank(fac.rank, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-    const dim3 grid(tiles, out.splits, (fac.rank + 16 * RT - 1) / (16 * RT));
-    by_vec(vec_ok(fac, c.dtype, {{x, xstride}}), [&](auto vec) {
-      with_type(c.dtype, [&](auto t) {
-        down_kernel<decltype(t), decltype(vec)::value, RT>
-            <<<grid, kDownWaves * 64, 0, c.s>>>(c.rows, fac, x, xstride, out, split_len);
+    const dim3 grid(c.rows.n, out.splits, rank_groups(fac.rank));
+    with_type(c.dtype, [&](auto t) {
+      down_row_kernel<decltype(t), RT><<<grid, kDownWaves * 64, 0, c.s>>>(c.rows, fac, x, xstride, out, split_len);
+    });
+  });
+  return hipGetLastError();
+}
+
+// hidden's slices added up.
+__global__ void __launch_bounds__(256) fold_kernel(const float *__restrict__ from, int slices, int64_t size,
+                                                   float *__restrict__ to) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= size) return;
+  if (e + 4 <= size) {
+    float4 v = load4(from + e, 0, 4);
+    int s = 1;
+    for (; s + 4 <= slices; s += 4) {
+      float4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = load4(from + (int64_t)(s + i) * size + e, 0, 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v = add4(v, w[i]);
+    }
+    for (; s < slices; ++s) v = add4(v, load4(from + (int64_t)s * size + e, 0, 4));
+    store4(to + e, v);
+  } else {
+    for (int64_t i = e; i < size; ++i) {
+      float v = from[i];
+      for (int s = 1; s < slices; ++s) v += from[(int64_t)s * size + i];
+      to[i] = v;
+    }
+  }
+}
+
+// hidden [n][rank] of many rows, and with `sums` the sums of job.
+hipError_t launch_slices(const Call &c, const Factor &fac, const Sum &job, bool sums, bool accumulate, float *slices,
+                         float *hidden) {
+  const int count = slices_of(fac.width);
+  float *to = count > 1 ? slices : hidden;
+  by_rank(fac.rank, [&](auto rt) {
+    constexpr int RT = decltype(rt)::value;
+    const dim3 grid(count, (c.rows.n + job.chunk - 1) / job.chunk, rank_groups(fac.rank));
+    with_type(c.dtype, [&](auto t) {
+      by_flag(fac.width < 4, [&](auto narrow) {
+        constexpr bool N = decltype(narrow)::value;
+        if (!sums) slice_kernel<decltype(t), RT, false, false, N><<<grid, kSlice, 0, c.s>>>(c.rows, fac, job, to);
+        else if (accumulate) slice_kernel<decltype(t), RT, true, true, N><<<grid, kSlice, 0, c.s>>>(c.rows, fac, job, to);
+        else slice_kernel<decltype(t), RT, true, false, N><<<grid, kSlice, 0, c.s>>>(c.rows, fac, job, to);
       });
     });
   });
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || count == 1) return e;
+  const int64_t size = (int64_t)c.rows.n * fac.rank;
+  fold_kernel<<<(uint32_t)((size + 1023) / 1024), 256, 0, c.s>>>(slices, count, size, hidden);
   return hipGetLastError();
 }
 
 hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const float *base, int64_t bstride, float *y,
                      int64_t ystride, float *hsum) {
-  const int tiles = (c.rows.n + c.rows.tile - 1) / c.rows.tile;
+  if (c.rows.order == nullptr) {
+    const dim3 grid((fac.width + 1023) / 1024, c.rows.n);
+    with_type(c.dtype, [&](auto t) {
+      by_flag(fac.width < 4, [&](auto narrow) {
+        up_row_kernel<decltype(t), decltype(narrow)::value>
+            <<<grid, 256, 0, c.s>>>(c.rows, fac, h, base, bstride, y, ystride, hsum);
+      });
+    });
+    return hipGetLastError();
+  }
   by_rank(fac.rank, [&](auto rt) {
-    const dim3 grid((fac.width + 255) / 256, std::min(tiles, 65535));
-    by_vec(vec_ok(fac, c.dtype, {{base, base ? bstride : 0}, {y, ystride}}), [&](auto vec) {
-      with_type(c.dtype, [&](auto t) {
-        up_kernel<decltype(t), decltype(vec)::value, decltype(rt)::value>
-            <<<grid, 256, 0, c.s>>>(c.rows, fac, h, base, bstride, y, ystride, hsum, tiles);
+    const int tiles = (c.rows.n + kUpRows - 1) / kUpRows, across = (fac.width + 255) / 256;
+    const int per = std::max(1, std::min<int>(8, (int64_t)tiles * across / 1024));
+    const dim3 grid(across, (tiles + per - 1) / per);
+    with_type(c.dtype, [&](auto t) {
+      by_flag(fac.width < 4, [&](auto narrow) {
+        up_kernel<decltype(t), decltype(rt)::value, decltype(narrow)::value>
+            <<<grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, per);
       });
     });
   });
   return hipGetLastError();
 }
 
-hipError_t launch_outer(const Call &c, const Factor &fac, const Hidden &h, const float *x, int64_t xstride,
-                        bool accumulate, float *grad, float *part) {
-  if (c.rows.n > 0) by_rank(fac.rank, [&](auto rt) {
+// `outer`: how many of the sums, from the first on, slice_kernel has not done.
+hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int outer, bool accumulate) {
+  int across = 0, chunks = 0;
+  int64_t size = 0;
+  bool narrow = false;
+  for (int i = 0; i < sums.count; ++i) {
+    if (i < outer) {
+      across += sums.of[i].across;
+      narrow = narrow || sums.of[i].width < 4;
+      chunks = std::max(chunks, (c.rows.n + sums.of[i].chunk - 1) / sums.of[i].chunk);
+    }
+    size = std::max(size, (int64_t)fac.rank * sums.of[i].width);
+  }
+  if (c.rows.n > 0 && outer > 0) by_rank(fac.rank, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-    const dim3 grid((fac.width + 255) / 256, (c.rows.n + kSumRows - 1) / kSumRows, (fac.rank + 16 * RT - 1) / (16 * RT));
-    const bool ok = fac.width % 4 == 0 && aligned(x, 16) && xstride % 4 == 0 && aligned(grad, 16);
-    by_vec(ok, [&](auto vec) {
-      by_vec(accumulate, [&](auto acc) {
-        outer_kernel<decltype(vec)::value, decltype(acc)::value, RT>
-            <<<grid, 256, 0, c.s>>>(c.rows, fac, h, x, xstride, grad, part);
+    const dim3 grid(across, chunks, (fac.rank + 16 * RT - 1) / (16 * RT));
+    by_flag(accumulate, [&](auto acc) {
+      by_flag(narrow, [&](auto nar) {
+        outer_kernel<decltype(acc)::value, RT, decltype(nar)::value><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
       });
     });
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t size = (int64_t)fac.rank * fac.width;
-  const dim3 grid((uint32_t)std::min<int64_t>((size + 255) / 256, 1024), c.rows.count);
-  by_vec(accumulate, [&](auto acc) {
-    sum_kernel<decltype(acc)::value><<<grid, 256, 0, c.s>>>(c.rows, fac, part, grad);
+  const dim3 grid((uint32_t)std::min<int64_t>((size + 1023) / 1024, 1024), c.rows.count, sums.count);
+  by_flag(accumulate, [&](auto acc) {
+    sum_kernel<decltype(acc)::value><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
   });
   return hipGetLastError();
 }
 
+// The workspace's parts.
 struct Sizes {
-  size_t order = 0, hidden = 0, part = 0;
-  size_t total() const { return order + hidden + part; }
+  size_t order = 0, hidden = 0, one = 0, part[2] = {0, 0};  // hidden: by split or slice; one: added up
+  size_t total() const { return order + hidden + one + part[0] + part[1]; }
 };
 Sizes sizes_of(const welvet_hip_adapters &d, int n, bool backward) {
   Sizes z;
   if (n == 0) return z;
-  if (backward || n > kFewRows) z.order = order_bytes(n);
-  const int splits = splits_of(n, backward ? d.out : d.in);
-  z.hidden = pad256((size_t)splits * n * d.rank * sizeof(float));
-  if (backward)
-    z.part = pad256(((size_t)n + kSumRows - 1) / kSumRows * 2 * d.rank * (size_t)std::max(d.in, d.out) * sizeof(float));
+  const size_t one = (size_t)n * d.rank * sizeof(float);
+  const int width = backward ? d.out : d.in;
+  if (!backward && n <= kFewRows) {
+    z.hidden = pad256(splits_of(n, width) * one);
+    return z;
+  }
+  z.order = order_bytes(n);
+  z.one = pad256(one);
+  if (slices_of(width) > 1) z.hidden = pad256(slices_of(width) * one);
+  if (backward) {
+    // each factor's sums in blocks of rows; dup's in those of slice_kernel or
+    // outer_kernel, whichever is the more
+    const int groups = rank_groups(d.rank);
+    const auto bytes = [&](int w, int across) {
+      const size_t chunk = chunk_of(n, across * groups);
+      return pad256((n + chunk - 1) / chunk * 2 * d.rank * (size_t)w * sizeof(float));
+    };
+    z.part[0] = bytes(d.in, (d.in + 255) / 256);
+    z.part[1] = std::max(bytes(d.out, (d.out + 255) / 256), bytes(d.out, slices_of(d.out)));
+  }
   return z;
 }
 
 bool desc_ok(const welvet_hip_adapters *d, int32_t n) {
-  return d && n >= 0 && n <= (1 << 24) && d->count > 0 && d->count <= 65535 && d->rank > 0 && d->rank <= kMaxRank &&
-         d->in > 0 && d->out > 0 && d->in <= INT32_MAX - 512 && d->out <= INT32_MAX - 512;
+  return d && n >= 0 && n <= (1 << 23) && d->count > 0 && d->count <= 65535 && d->rank > 0 && d->rank <= kMaxRank &&
+         d->in > 0 && d->out > 0 && (int64_t)d->rank * std::max(d->in, d->out) <= INT32_MAX / 2;
 }
 
 }  // namespace
@@ -478,18 +839,25 @@ welvet_status welvet_hip_adapters_forward(const welvet_hip_adapters *desc, const
     return make_status(kInvalid, "adapters: %zu bytes of 16-byte aligned workspace are needed", z.total());
   st = require_device();
   if (st.code || n == 0) return st;
-  Call c{desc->dtype, {d_ids, nullptr, n, desc->count, 1}, (hipStream_t)stream};
-  if (n > kFewRows) {
-    tok::Order o;
-    WH_HIP(tok::launch_order(d_ids, n, desc->count, d_ws, &o, c.s));
-    c.rows = {o.skey, o.order, n, desc->count, 16};
-  }
+  Call c{desc->dtype, {d_ids, nullptr, n, desc->count}, (hipStream_t)stream};
   const Factor down{desc->d_down, desc->d_ranks, desc->d_scales, desc->rank, desc->in};
   const Factor up{desc->d_up, desc->d_ranks, desc->d_scales, desc->rank, desc->out};
-  Hidden h{(float *)((char *)d_ws + z.order), splits_of(n, desc->in), n, desc->rank};
-  if (h.splits == 1 && d_h) h.p = d_h;
-  WH_HIP(launch_down(c, down, d_x, x_stride, h));
-  WH_HIP(launch_up(c, up, h, d_base, base_stride, d_y, y_stride, h.p == d_h ? nullptr : d_h));
+  if (n <= kFewRows) {
+    Hidden h{(float *)d_ws, splits_of(n, desc->in), n, desc->rank};
+    if (h.splits == 1 && d_h) h.p = d_h;
+    WH_HIP(launch_down_rows(c, down, d_x, x_stride, h));
+    WH_HIP(launch_up(c, up, h, d_base, base_stride, d_y, y_stride, h.p == d_h ? nullptr : d_h));
+    return ok();
+  }
+  tok::Order o;
+  char *at = (char *)d_ws;
+  WH_HIP(tok::launch_order(d_ids, n, desc->count, at, &o, c.s));
+  c.rows = {o.skey, o.order, n, desc->count};
+  at += z.order;
+  float *one = d_h ? d_h : (float *)at, *slices = (float *)(at + z.one);
+  const Sum job{nullptr, d_x, x_stride, desc->in, chunk_of(n, slices_of(desc->in) * rank_groups(desc->rank)), 0, nullptr, nullptr};
+  WH_HIP(launch_slices(c, down, job, false, false, slices, one));
+  WH_HIP(launch_up(c, up, Hidden{one, 1, n, desc->rank}, d_base, base_stride, d_y, y_stride, nullptr));
   return ok();
 }
 
@@ -514,26 +882,33 @@ welvet_status welvet_hip_adapters_backward(const welvet_hip_adapters *desc, cons
     return make_status(kInvalid, "adapters backward: %zu bytes of 16-byte aligned workspace are needed", z.total());
   st = require_device();
   if (st.code) return st;
-  Call c{desc->dtype, {nullptr, nullptr, n, desc->count, 16}, (hipStream_t)stream};
-  float *part = nullptr;
-  Hidden g{nullptr, 1, n, desc->rank};
+  Call c{desc->dtype, {nullptr, nullptr, n, desc->count}, (hipStream_t)stream};
   const Factor down{desc->d_down, desc->d_ranks, desc->d_scales, desc->rank, desc->in};
   const Factor up{desc->d_up, desc->d_ranks, desc->d_scales, desc->rank, desc->out};
+  char *at = (char *)d_ws;
+  float *const g = (float *)(at + z.order), *const slices = (float *)(at + z.order + z.one);
+  float *const part = (float *)(at + z.order + z.one + z.hidden), *const part2 = (float *)((char *)part + z.part[0]);
+  const int groups = rank_groups(desc->rank);
+  const bool need_g = n > 0 && (d_dx || d_ddown), fused = need_g && d_dup;
+  const auto sum_of = [&](const float *hidden, const float *x, int64_t stride, int width, float *grad, float *part, bool slice) {
+    const int across = slice ? slices_of(width) : (width + 255) / 256;
+    return Sum{hidden, x, stride, width, chunk_of(n, across * groups), across, grad, part};
+  };
+  const Sum dup = sum_of(d_h, d_dy, dy_stride, desc->out, d_dup, part2, need_g);
   if (n > 0) {
     tok::Order o;
-    WH_HIP(tok::launch_order(d_ids, n, desc->count, d_ws, &o, c.s));
+    WH_HIP(tok::launch_order(d_ids, n, desc->count, at, &o, c.s));
     c.rows.key = o.skey;
     c.rows.order = o.order;
-    g.p = (float *)((char *)d_ws + z.order);
-    g.splits = splits_of(n, desc->out);
-    part = (float *)((char *)d_ws + z.order + z.hidden);
-    if (d_dx || d_ddown) WH_HIP(launch_down(c, up, d_dy, dy_stride, g));
-    if (d_dx) WH_HIP(launch_up(c, down, g, d_dx_base, dx_base_stride, d_dx, dx_stride, nullptr));
   }
-  if (d_ddown) WH_HIP(launch_outer(c, down, g, d_x, x_stride, accumulate != 0, d_ddown, part));
-  if (d_dup)
-    WH_HIP(launch_outer(c, up, Hidden{const_cast<float *>(d_h), 1, n, desc->rank}, d_dy, dy_stride, accumulate != 0,
-                        d_dup, part));
+  if (need_g) WH_HIP(launch_slices(c, up, dup, fused, accumulate != 0, slices, g));
+  if (n > 0 && d_dx)
+    WH_HIP(launch_up(c, down, Hidden{g, 1, n, desc->rank}, d_dx_base, dx_base_stride, d_dx, dx_stride, nullptr));
+  Sums sums{};
+  if (d_ddown) sums.of[sums.count++] = sum_of(g, d_x, x_stride, desc->in, d_ddown, part, false);
+  const int outer = sums.count + (d_dup && !fused ? 1 : 0);
+  if (d_dup) sums.of[sums.count++] = dup;
+  if (sums.count) WH_HIP(launch_sums(c, down, sums, outer, accumulate != 0));
   return ok();
 }
 

@@ -15,72 +15,24 @@ namespace {
 
 using namespace tok;
 
-// A thread's columns of a block's column tile: four neighbours as one 16-byte
-// word (VEC: dim, strides and pointers allow it), or four blockDim apart.
-template <bool VEC>
-struct Cols {
-  int c0;  // first column
-  int step, dim;
-  __device__ Cols(int tile, int dim_) : dim(dim_) {
-    const int width = 4 * blockDim.x;
-    c0 = VEC ? tile * width + 4 * threadIdx.x : tile * width + threadIdx.x;
-    step = VEC ? 1 : blockDim.x;
-  }
-  __device__ bool any() const { return c0 < dim; }
-  __device__ float4 load(const float *row) const {
-    if constexpr (VEC) return *(const float4 *)(row + c0);
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c0 + i * step < dim ? row[c0 + i * step] : 0.0f;
-    return make_float4(v[0], v[1], v[2], v[3]);
-  }
-  __device__ void store(float *row, float4 v) const {
-    if constexpr (VEC) {
-      *(float4 *)(row + c0) = v;
-    } else {
-      const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i * step < dim) row[c0 + i * step] = f[i];
-    }
-  }
-};
-
-__device__ inline float4 add4(float4 a, float4 b) {
-  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
-}
-__device__ inline float4 mul4(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
-
 // ---------------------------------------------------------------- forward
 // A block takes ROWS tokens and a column tile; a thread four columns of each
 // row, all rows' loads in flight before the first store.
-template <class T, bool VEC, int ROWS>
+template <class T, int ROWS, bool NARROW>
 __global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__restrict__ table, int64_t tstride,
                                                      uint32_t vocab, int dim, const int32_t *__restrict__ tokens,
                                                      int n, float scale, float *__restrict__ out, int64_t ostride,
                                                      int tiles) {
   const int group = blockIdx.x / tiles;
-  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (!cols.any()) return;
-  float4 v[ROWS];
+  Quad<T> v[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int t = group * ROWS + r;
     const uint32_t id = t < n ? (uint32_t)tokens[t] : vocab;
-    v[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (id >= vocab) continue;
-    const typename T::raw *row = table + (int64_t)id * tstride;
-    if constexpr (VEC && sizeof(typename T::raw) == 4) {
-      v[r] = *(const float4 *)(row + cols.c0);
-    } else if constexpr (VEC) {
-      const ushort4 u = *(const ushort4 *)(row + cols.c0);
-      v[r] = make_float4(T::get(u.x), T::get(u.y), T::get(u.z), T::get(u.w));
-    } else {
-      float f[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = cols.c0 + i * cols.step < dim ? T::get(row[cols.c0 + i * cols.step]) : 0.0f;
-      v[r] = make_float4(f[0], f[1], f[2], f[3]);
-    }
+    v[r] = Quad<T>{};
+    if (id < vocab) v[r] = cols.template load<T>(table + (int64_t)id * tstride);
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -88,7 +40,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__re
     if (t >= n) break;
     // padding stays +0 also under a negative scale
     const bool pad = (uint32_t)tokens[t] >= vocab;
-    cols.store(out + (int64_t)t * ostride, pad ? v[r] : mul4(v[r], scale));
+    cols.store(out + (int64_t)t * ostride, pad ? v[r].floats() : mul4(v[r].floats(), scale));
   }
 }
 
@@ -137,23 +89,18 @@ constexpr int kDirect = 256;
 constexpr int kRun = 32;
 constexpr int kZeroRows = 8;  // table rows of a zeroing block
 
-template <bool VEC, bool ACC>
-__device__ inline void put_row(const Cols<VEC> &cols, float *row, float4 sum, float scale) {
+template <bool ACC, bool NARROW>
+__device__ inline void put_row(const Cols<NARROW> &cols, float *row, const float4 &sum, float scale) {
   float4 v = mul4(sum, scale);
   if constexpr (ACC) v = add4(cols.load(row), v);
   cols.store(row, v);
 }
 
-template <bool VEC>
 __device__ inline void zero_row(float *row, int dim) {
-  if constexpr (VEC) {
-    for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) *(float4 *)(row + c) = make_float4(0, 0, 0, 0);
-  } else {
-    for (int c = threadIdx.x; c < dim; c += blockDim.x) row[c] = 0.0f;
-  }
+  for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) store4(row, c, dim, make_float4(0, 0, 0, 0));
 }
 
-template <bool VEC, bool ACC>
+template <bool ACC, bool NARROW>
 __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__ tokens, int n, uint32_t vocab,
                                                      int dim, const float *__restrict__ dout, int64_t dstride,
                                                      float scale, float *__restrict__ dtable, int64_t tstride,
@@ -174,7 +121,7 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     }
     __syncthreads();
     for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row<VEC>(dtable + (int64_t)(v0 + r) * tstride, dim);
+      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim);
     return;
   }
   if (threadIdx.x == 0) count_s = 0;
@@ -197,7 +144,7 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
   }
   __syncthreads();
   const int count = count_s;
-  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (count == 0 || !cols.any()) return;
   float4 sum = make_float4(0, 0, 0, 0);
   int r = 0;
@@ -209,21 +156,10 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
   }
   for (; r < count; ++r) sum = add4(sum, cols.load(dout + (int64_t)rows_s[r] * dstride));
-  put_row<VEC, ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
 }
 
-// The first place of the sorted keys whose key is >= v.
-__device__ inline int first_at_least(const int32_t *__restrict__ skey, int n, uint32_t v) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((uint32_t)skey[mid] < v) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
-template <bool VEC, bool ACC>
+template <bool ACC, bool NARROW>
 __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ skey,
                                                    const int32_t *__restrict__ order, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ dout, int64_t dstride, float scale,
@@ -232,13 +168,13 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
   if ((int)blockIdx.x >= adders) {
     __shared__ int named[kZeroRows];
     const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)adders) * kZeroRows;
-    if (threadIdx.x < kZeroRows) {
-      const int at = first_at_least(skey, n, v0 + threadIdx.x);
-      named[threadIdx.x] = at < n && (uint32_t)skey[at] == v0 + threadIdx.x;
+    for (uint32_t d = threadIdx.x >> 6; d < kZeroRows; d += blockDim.x >> 6) {  // a wave a row
+      const int at = first_at_least(skey, n, (int32_t)min(v0 + d, vocab));
+      if ((threadIdx.x & 63) == 0) named[d] = at < n && (uint32_t)skey[at] == v0 + d;
     }
     __syncthreads();
     for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row<VEC>(dtable + (int64_t)(v0 + r) * tstride, dim);
+      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim);
     return;
   }
   __shared__ int32_t key_s[kRun + 2];  // with the neighbours' nearest
@@ -250,7 +186,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
   }
   if (threadIdx.x < kRun) row_s[threadIdx.x] = p0 + (int)threadIdx.x < n ? order[p0 + threadIdx.x] : 0;
   __syncthreads();
-  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (!cols.any()) return;
   const int32_t before = key_s[0], after = key_s[kRun + 1];
   int32_t cur = key_s[1];
@@ -260,7 +196,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
     if ((uint32_t)cur >= vocab) return;  // padding, or past the last row
     if (!began) cols.store(part + (int64_t)(2 * chunk) * dim, sum);
     else if (goes_on) cols.store(part + (int64_t)(2 * chunk + 1) * dim, sum);
-    else put_row<VEC, ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale);
+    else put_row<ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale);
   };
 #pragma unroll 1
   for (int r0 = 0; r0 < kRun; r0 += 8) {
@@ -287,7 +223,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
 
 // Tokens whose rows fill more than one block's: the block where one begins
 // adds its later blocks' slot 0 to its own slot 1, in order.
-template <bool VEC, bool ACC>
+template <bool ACC, bool NARROW>
 __global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ skey, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ part, float scale,
                                                    float *__restrict__ dtable, int64_t tstride, int tiles) {
@@ -296,20 +232,20 @@ __global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ s
   const int32_t mine = skey[p1 - 1];
   if ((uint32_t)mine >= vocab || skey[p1] != mine) return;
   if (p0 > 0 && skey[p0 - 1] == mine) return;  // began earlier
-  const Cols<VEC> cols(blockIdx.x % tiles, dim);
+  const int last = (first_at_least(skey, n, mine + 1) - 1) / kRun;
+  const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (!cols.any()) return;
-  const int last = (first_at_least(skey, n, (uint32_t)mine + 1) - 1) / kRun;
   float4 sum = cols.load(part + (int64_t)(2 * chunk + 1) * dim);
-  int c = chunk + 1;
-  for (; c + 4 <= last + 1; c += 4) {
+  int b = chunk + 1;
+  for (; b + 4 <= last + 1; b += 4) {
     float4 v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = cols.load(part + (int64_t)(2 * (c + k)) * dim);
+    for (int k = 0; k < 4; ++k) v[k] = cols.load(part + (int64_t)(2 * (b + k)) * dim);
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
   }
-  for (; c <= last; ++c) sum = add4(sum, cols.load(part + (int64_t)(2 * c) * dim));
-  put_row<VEC, ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+  for (; b <= last; ++b) sum = add4(sum, cols.load(part + (int64_t)(2 * b) * dim));
+  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
 }
 
 int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
@@ -320,14 +256,14 @@ size_t gradient_bytes(int dim, int n) {
   return order_bytes(n) + pad256(chunks * 2 * (size_t)dim * sizeof(float));
 }
 
-template <bool VEC, bool ACC>
+template <bool ACC, bool NARROW>
 hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, float scale, const float *dout,
                            int64_t dstride, float *dtable, int64_t tstride, void *ws, hipStream_t s) {
   const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
   const int64_t zeros = ACC ? 0 : ((int64_t)vocab + kZeroRows - 1) / kZeroRows;
   if (n <= kDirect) {
     if (n == 0 && ACC) return hipSuccess;
-    direct_kernel<VEC, ACC><<<(uint32_t)((int64_t)n * tiles + zeros), threads, 0, s>>>(
+    direct_kernel<ACC, NARROW><<<(uint32_t)((int64_t)n * tiles + zeros), threads, 0, s>>>(
         tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles);
     return hipGetLastError();
   }
@@ -336,10 +272,10 @@ hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, flo
   if (e != hipSuccess) return e;
   float *part = (float *)((char *)ws + order_bytes(n));
   const int64_t chunks = ((int64_t)n + kRun - 1) / kRun, adders = chunks * tiles;
-  sums_kernel<VEC, ACC><<<(uint32_t)(adders + zeros), threads, 0, s>>>(
+  sums_kernel<ACC, NARROW><<<(uint32_t)(adders + zeros), threads, 0, s>>>(
       o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, part, tiles, (int)adders);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  join_kernel<VEC, ACC><<<(uint32_t)adders, threads, 0, s>>>(o.skey, n, (uint32_t)vocab, dim, part, scale, dtable,
+  join_kernel<ACC, NARROW><<<(uint32_t)adders, threads, 0, s>>>(o.skey, n, (uint32_t)vocab, dim, part, scale, dtable,
                                                             tstride, tiles);
   return hipGetLastError();
 }
@@ -370,8 +306,6 @@ welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t
     return make_status(kInvalid, "embedding: device pointers must be aligned to their elements");
   welvet_status st = require_device();
   if (st.code || n == 0) return st;
-  const bool vec = dim % 4 == 0 && table_stride % 4 == 0 && out_stride % 4 == 0 && tok::aligned(d_table, 4 * size) &&
-                   tok::aligned(d_out, 16);
   const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
   // four rows a block where there are blocks enough for every CU several times over
   const int rows = (int64_t)n * tiles >= 8192 ? 4 : 1;
@@ -383,8 +317,8 @@ welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t
                                                           (uint32_t)vocab, dim, d_tokens, n, scale, d_out, out_stride,
                                                           tiles);
     };
-    if (vec) rows == 4 ? go(lookup_kernel<T, true, 4>) : go(lookup_kernel<T, true, 1>);
-    else rows == 4 ? go(lookup_kernel<T, false, 4>) : go(lookup_kernel<T, false, 1>);
+    if (dim < 4) rows == 4 ? go(lookup_kernel<T, 4, true>) : go(lookup_kernel<T, 1, true>);
+    else rows == 4 ? go(lookup_kernel<T, 4, false>) : go(lookup_kernel<T, 1, false>);
   });
   WH_HIP(hipGetLastError());
   return ok();
@@ -426,14 +360,10 @@ welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t dim, const in
     return make_status(kInvalid, "embedding backward: %zu bytes of 16-byte aligned workspace are needed", need);
   welvet_status st = require_device();
   if (st.code) return st;
-  const bool vec = dim % 4 == 0 && dout_stride % 4 == 0 && dtable_stride % 4 == 0 && tok::aligned(d_dout, 16) &&
-                   tok::aligned(d_dtable, 16);
-  const auto go = [&](auto launch) {
-    return launch(vocab, dim, d_tokens, n, scale, d_dout, dout_stride, d_dtable, dtable_stride, d_ws,
-                  (hipStream_t)stream);
-  };
-  WH_HIP(accumulate ? (vec ? go(launch_gradient<true, true>) : go(launch_gradient<false, true>))
-                    : (vec ? go(launch_gradient<true, false>) : go(launch_gradient<false, false>)));
+  const auto launch = dim < 4 ? (accumulate ? launch_gradient<true, true> : launch_gradient<false, true>)
+                              : (accumulate ? launch_gradient<true, false> : launch_gradient<false, false>);
+  WH_HIP(launch(
+      vocab, dim, d_tokens, n, scale, d_dout, dout_stride, d_dtable, dtable_stride, d_ws, (hipStream_t)stream));
   return ok();
 }
 

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "runtime.hpp"
@@ -37,6 +38,95 @@ struct BF16 {
   __device__ static inline float get(raw v) { return u2f((uint32_t)v << 16); }
   __device__ static inline raw put(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 };
+
+// Four values wherever they lie: the hardware loads and stores words at any
+// alignment of their elements, so rows of any width and stride take this path.
+template <class T>
+struct Quad {
+  using raw = typename T::raw;
+  using bits = std::conditional_t<sizeof(raw) == 4, uint4, uint2>;
+  bits v;
+  __device__ inline float get(int i) const {
+    if constexpr (sizeof(raw) == 4) return T::get(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+    else return T::get((raw)((i < 2 ? v.x : v.y) >> (16 * (i & 1))));
+  }
+  __device__ inline float4 floats() const { return make_float4(get(0), get(1), get(2), get(3)); }
+  __device__ static inline Quad load(const raw *p) {
+    Quad q;
+    __builtin_memcpy(&q.v, p, sizeof(q.v));
+    return q;
+  }
+  // zeros in the place of the first `skip` values
+  __device__ inline void drop(int skip) {
+    if constexpr (sizeof(raw) == 4) {
+      v.x = skip < 1 ? v.x : 0;
+      v.y = skip < 2 ? v.y : 0;
+      v.z = skip < 3 ? v.z : 0;
+      v.w = skip < 4 ? v.w : 0;
+    } else {
+      v.x = skip < 1 ? v.x : skip < 2 ? v.x & 0xffff0000u : 0;
+      v.y = skip < 3 ? v.y : skip < 4 ? v.y & 0xffff0000u : 0;
+    }
+  }
+  // the values at row + k, zeros from `width` on
+  __device__ static inline Quad load(const raw *row, int k, int width) {
+    if (k + 4 <= width) return load(row + k);
+    raw r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = k + i < width ? row[k + i] : (raw)0;
+    return load(r);
+  }
+};
+__device__ inline void store4(float *p, const float4 &v) { __builtin_memcpy(p, &v, sizeof(v)); }
+__device__ inline void store4(float *row, int k, int width, const float4 &v) {
+  if (k + 4 <= width) return store4(row + k, v);
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k + i < width) row[k + i] = f[i];
+}
+__device__ inline float4 load4(const float *row, int k, int width) { return Quad<F32>::load((const uint32_t *)row, k, width).floats(); }
+// A thread's four columns of a row from c on.  Where those pass the row's end
+// it takes the row's last four, `skip` of them another thread's (all, past the
+// end), so every load is one word without a condition; only its own are
+// stored.  Rows of fewer than four columns (NARROW) go value by value.
+template <bool NARROW>
+struct Cols {
+  int c, skip, width;
+  __device__ Cols(int first, int width_) : width(width_) {
+    skip = NARROW ? 0 : max(0, first + 4 - width);
+    c = first - skip;
+  }
+  __device__ bool any() const { return NARROW ? c < width : skip < 4; }
+  template <class T>
+  __device__ Quad<T> load(const typename T::raw *row) const {
+    if constexpr (NARROW) return Quad<T>::load(row, c, width);
+    else return Quad<T>::load(row + c);
+  }
+  __device__ float4 load(const float *row) const { return load<F32>((const uint32_t *)row).floats(); }
+  __device__ void store(float *row, const float4 &v) const {
+    if constexpr (NARROW) return store4(row, c, width, v);
+    if (skip == 0) return store4(row + c, v);
+    if (skip < 2) row[c + 1] = v.y;
+    if (skip < 3) row[c + 2] = v.z;
+    if (skip < 4) row[c + 3] = v.w;
+  }
+};
+__device__ inline float4 add4(const float4 &a, const float4 &b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+__device__ inline float4 mul4(const float4 &a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
+__device__ inline float4 fma4(float s, const float4 &a, const float4 &b) {
+  return make_float4(fmaf(s, a.x, b.x), fmaf(s, a.y, b.y), fmaf(s, a.z, b.z), fmaf(s, a.w, b.w));
+}
+// A select that keeps no trace of the value left out.
+__device__ inline float4 keep4(bool on, const float4 &v) {
+  return make_float4(on ? v.x : 0.0f, on ? v.y : 0.0f, on ? v.z : 0.0f, on ? v.w : 0.0f);
+}
+__device__ inline float get4(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// Keeps loads in the order they are written in: a wait for the oldest of
+// several steps' loads must leave the later ones in flight.
+__device__ inline void issued() { __builtin_amdgcn_sched_barrier(0); }
 
 // Elements of one 16-byte word, and back.
 template <class T>
@@ -78,72 +168,79 @@ inline auto with_type(int32_t dtype, F &&f) {
 //
 // Ranks are counted, not sorted: a row's place among kChunk rows is the number
 // of rows before it, one compare and one add per pair.  A block takes 64 rows,
-// one a lane, and its 16 waves a sixteenth of the chunk each, whose keys are
-// wave-uniform (scalar) operands.  More rows than a chunk: each chunk by
-// itself, then every row's places in the other chunks by binary search there.
-constexpr int kChunk = 4096;
+// one a lane, and its 16 waves a sixteenth of the chunk each, read from LDS as
+// words of four that all lanes share.  More rows than a chunk: each chunk by
+// itself, then every row's places in the other chunks by binary search there,
+// four threads a row.
+constexpr int kChunk = 2048;
 
 static __global__ void __launch_bounds__(1024) rank_kernel(const int32_t *__restrict__ key, int n, uint32_t limit,
-                                                    int32_t *__restrict__ skey, int32_t *__restrict__ order) {
+                                                           int32_t *__restrict__ skey, int32_t *__restrict__ order) {
+  __shared__ uint4 keys[kChunk / 4];
   __shared__ int count[16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = blockIdx.x * 64 + lane;
-  const int begin = blockIdx.x * 64 / kChunk * kChunk, end = min(begin + kChunk, n);
-  const uint32_t mine = i < n ? min((uint32_t)key[i], limit) : limit;
-  const int per = (((end - begin) + 15) / 16 + 63) & ~63;  // this wave's rows, whole groups of 64
-  const int lo = min(begin + wave * per, end), hi = min(lo + per, end);
-  const int own = blockIdx.x * 64;
+  const int own = blockIdx.x * 64, i = own + lane, begin = own / kChunk * kChunk;
+  uint32_t *flat = (uint32_t *)keys;
+  for (int j = threadIdx.x; j < kChunk; j += 1024)
+    // past the end: after every row, whatever its key
+    flat[j] = begin + j < n ? min((uint32_t)key[begin + j], limit) : 0xffffffffu;
+  __syncthreads();
+  const uint32_t mine = i < n ? flat[i - begin] : limit;
+  const int at = own - begin;
   int less = 0;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    const int stop = min(j0 + 64, hi);
-    if (j0 == own) {
-      for (int j = j0; j < stop; ++j) {
-        const uint32_t u = min((uint32_t)key[j], limit);
-        less += (u < mine || (u == mine && j < i)) ? 1 : 0;
-      }
+  // 128 keys a wave, in words of four: the word's side of the block's rows is
+  // the same for all of it
+#pragma unroll 4
+  for (int w = wave * (kChunk / 64); w < (wave + 1) * (kChunk / 64); ++w) {
+    const uint4 u = keys[w];
+    const int j = w * 4;
+    if (j >= at && j < at + 64) {
+      less += (u.x < mine || (u.x == mine && j < at + lane)) ? 1 : 0;
+      less += (u.y < mine || (u.y == mine && j + 1 < at + lane)) ? 1 : 0;
+      less += (u.z < mine || (u.z == mine && j + 2 < at + lane)) ? 1 : 0;
+      less += (u.w < mine || (u.w == mine && j + 3 < at + lane)) ? 1 : 0;
     } else {
-      const uint32_t bound = mine + (j0 < own ? 1u : 0u);  // equal keys of earlier rows come first
-      int j = j0;
-      for (; j + 8 <= stop; j += 8) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) less += min((uint32_t)key[j + k], limit) < bound ? 1 : 0;
-      }
-      for (; j < stop; ++j) less += min((uint32_t)key[j], limit) < bound ? 1 : 0;
+      const uint32_t bound = mine + (j < at ? 1u : 0u);  // equal keys of earlier rows come first
+      less += u.x < bound ? 1 : 0;
+      less += u.y < bound ? 1 : 0;
+      less += u.z < bound ? 1 : 0;
+      less += u.w < bound ? 1 : 0;
     }
   }
   count[wave][lane] = less;
   __syncthreads();
   if (wave == 0 && i < n) {
-    int at = begin;
+    int to = begin;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) at += count[w][lane];
-    skey[at] = (int32_t)mine;
-    order[at] = i;
+    for (int w = 0; w < 16; ++w) to += count[w][lane];
+    skey[to] = (int32_t)mine;
+    order[to] = i;
   }
 }
 
 // Joins the sorted chunks: a row's place is its place in its own chunk plus
 // the rows before it in each other one (equal keys of earlier chunks first).
-constexpr int kMergeStage = 4;  // chunks in LDS at a time
+constexpr int kStage = 8 * kChunk;  // keys in LDS at a time
 static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__restrict__ ckey,
-                                                     const int32_t *__restrict__ corder, int n,
-                                                     int32_t *__restrict__ skey, int32_t *__restrict__ order) {
-  __shared__ int32_t keys[kMergeStage * kChunk];
-  const int p = blockIdx.x * 1024 + threadIdx.x;
+                                                            const int32_t *__restrict__ corder, int n,
+                                                            int32_t *__restrict__ skey, int32_t *__restrict__ order) {
+  __shared__ int4 keys4[kStage / 4];
+  int32_t *keys = (int32_t *)keys4;
+  const int p = blockIdx.x * 256 + (threadIdx.x >> 2), part = threadIdx.x & 3;
   const int own = p / kChunk;
   const int32_t mine = p < n ? ckey[p] : 0;
-  int at = p - own * kChunk;
-  for (int s0 = 0; s0 < n; s0 += kMergeStage * kChunk) {
-    const int len = min(kMergeStage * kChunk, n - s0);
+  int at = 0;
+  for (int s0 = 0; s0 < n; s0 += kStage) {
+    const int len = min(kStage, n - s0);
     __syncthreads();
-    for (int j = threadIdx.x; j < len; j += 1024) keys[j] = ckey[s0 + j];
+    for (int j = threadIdx.x; j < len / 4; j += 1024) keys4[j] = *(const int4 *)(ckey + s0 + 4 * j);
+    if ((int)threadIdx.x < (len & 3)) keys[len / 4 * 4 + threadIdx.x] = ckey[s0 + len / 4 * 4 + threadIdx.x];
     __syncthreads();
-    if (p >= n) continue;
-    for (int c0 = 0; c0 < len; c0 += kChunk) {
+    for (int c0 = part * kChunk; c0 < len; c0 += 4 * kChunk) {
       const int c = (s0 + c0) / kChunk;
       if (c == own) continue;
-      const int bound = mine + (c < own ? 1 : 0);  // keys are below 2^31: no overflow past limit
-      int lo = 0, hi = min(kChunk, len - c0);      // the first place whose key is >= bound
+      const int32_t bound = mine + (c < own ? 1 : 0);  // keys are below 2^31 - 1
+      int lo = 0, hi = min(kChunk, len - c0);          // the first place whose key is >= bound
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (keys[c0 + mid] < bound) lo = mid + 1;
@@ -152,10 +249,28 @@ static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__res
       at += lo;
     }
   }
-  if (p < n) {
+  at += __shfl_xor(at, 1);
+  at += __shfl_xor(at, 2);
+  if (p < n && part == 0) {
+    at += p - own * kChunk;
     skey[at] = mine;
     order[at] = corder[p];
   }
+}
+
+// The first place of the sorted keys whose key is >= v; a whole wave calls it
+// and looks at 64 places a time.
+__device__ inline int first_at_least(const int32_t *__restrict__ skey, int n, int32_t v) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) / 64, p = lo + lane * step;
+    const int below = __popcll(__ballot(p < hi && skey[p] < v));
+    if (below == 0) return lo;
+    hi = min(hi, lo + below * step);
+    lo = lo + (below - 1) * step + 1;
+  }
+  return lo;
 }
 
 inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -174,7 +289,7 @@ inline hipError_t launch_order(const int32_t *key, int n, int32_t limit, void *w
   rank_kernel<<<(n + 63) / 64, 1024, 0, s>>>(key, n, (uint32_t)limit, ck, co);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || one) return e;
-  merge_kernel<<<(n + 1023) / 1024, 1024, 0, s>>>(ck, co, n, out->skey, out->order);
+  merge_kernel<<<(n + 255) / 256, 1024, 0, s>>>(ck, co, n, out->skey, out->order);
   return hipGetLastError();
 }
 
