@@ -206,8 +206,10 @@ __device__ inline void store_sums(const v4f (&acc)[RT][4], const Factor &fac, in
 // values stay in registers while an adapter's rows pass, 16 at a time, the next
 // 16 rows' loads in flight.  Every wave holds 64 columns, its products are
 // added up across the block in LDS, and the slices' sums are left for
-// fold_kernel: hidden[slice][row][j].  A lane's 64-byte pieces of a row start at
-// its wave's column + 16 m + 4 (l / 16), m < 4.
+// fold_kernel: hidden[slice][row][j].  A lane's four 16-byte pieces of a row
+// start at its wave's column + 16 m + 4 (l / 16).  A wave whose columns pass
+// the row's end takes the row's last 64, the first `skip` of them (another
+// wave's) as zeros; rows of fewer than 64 columns (NARROW) go value by value.
 //
 // SUMS: the rows also give the second product that reads them, sum over the
 // adapter's rows of job.hidden[row][j] x[row][c] (outer_kernel below has its
@@ -217,15 +219,18 @@ constexpr int kSliceWaves = 8;
 constexpr int kSlice = kSliceWaves * 64;
 constexpr int kMaxChunk = 512;
 template <class T, int RT, bool SUMS, bool ACC, bool NARROW>
-__global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, Sum job, float *__restrict__ hidden) {
+__global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(RowMap rows, Factor fac, Sum job,
+                                                                              float *__restrict__ hidden) {
   constexpr int kPitch = 68;  // floats of a turned row: reads by columns fall on different banks
   using raw = typename T::raw;
   __shared__ float red[kSliceWaves][16][RT * 16 + 1];
   __shared__ float4 turn4[SUMS ? kSliceWaves * 16 * kPitch / 4 : 1];
+  __shared__ float hs[SUMS ? 2 : 1][16][RT * 16];
   __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = lane & 15, q = lane >> 4;
-  const int width = fac.width, c0 = blockIdx.x * kSlice + wave * 64, j0 = blockIdx.z * RT * 16;
+  const int width = fac.width, own = blockIdx.x * kSlice + wave * 64, j0 = blockIdx.z * RT * 16;
+  const int c0 = NARROW ? own : min(own, width - 64), skip = own - c0;
   const int p0 = blockIdx.y * job.chunk, p1 = min(p0 + job.chunk, rows.n);
   const int ranks = min(RT * 16, fac.rank - j0);
   float *turn = (float *)turn4 + (SUMS ? wave * 16 * kPitch : 0);
@@ -252,58 +257,72 @@ __global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, 
         const raw *row = (const raw *)fac.p + ((int64_t)a * fac.rank + min(j0 + 16 * t + lo, ra - 1)) * width;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const Cols<NARROW> cols(c0 + 16 * m + 4 * q, width);
-          fv[t][m] = cols.template load<T>(row);
-          fv[t][m].drop(cols.skip);
+          if constexpr (NARROW) fv[t][m] = Quad<T>::load(row, c0 + 16 * m + 4 * q, width);
+          else fv[t][m] = Quad<T>::load(row + c0 + 16 * m + 4 * q);
         }
       }
-      // values of a piece past the row's end, or another piece's, count as zeros
-      const auto own = [&](int m, const float4 &v) {
-        const Cols<NARROW> cols(c0 + 16 * m + 4 * q, width);
-        return make_float4(cols.skip < 1 ? v.x : 0.0f, cols.skip < 2 ? v.y : 0.0f, cols.skip < 3 ? v.z : 0.0f,
-                           cols.skip < 4 ? v.w : 0.0f);
-      };
-      const float *hcol[RT];
-      if constexpr (SUMS) {
+      if (skip > 0) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) hcol[t] = job.hidden + min(j0 + 16 * t + lo, ra - 1);
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) fv[t][m].drop(skip - (16 * m + 4 * q));
       }
-      float4 xv[2][4];
-      float hv[2][RT][4];
+      Quad<F32> xv[2][4];
+      constexpr int kHidden = (RT * 256 + kSlice - 1) / kSlice;  // a thread's hidden values of a tile
+      float hn[kHidden];
       const int tiles = (i1 - i0 + 15) / 16;
       const auto load = [&](int d, int tile) {
         const int p = i0 + 16 * min(tile, tiles - 1);
-        const float *row = job.x + (int64_t)row_s[min(p + lo, i1 - 1) - p0] * job.xstride;
+        const uint32_t *row = (const uint32_t *)job.x + (int64_t)row_s[min(p + lo, i1 - 1) - p0] * job.xstride;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) xv[d][m] = Cols<NARROW>(c0 + 16 * m + 4 * q, width).load(row);
-        if constexpr (SUMS) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int64_t from = row_s[min(p + 4 * r + q, i1 - 1) - p0];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) hv[d][t][r] = hcol[t][from * fac.rank];
-          }
+        for (int m = 0; m < 4; ++m) {
+          if constexpr (NARROW) xv[d][m] = Quad<F32>::load(row, c0 + 16 * m + 4 * q, width);
+          else xv[d][m] = Quad<F32>::load(row + c0 + 4 * q + 16 * m);
         }
         issued();
       };
+      const auto load_hidden = [&](int tile) {
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int n = 0; n < kHidden; ++n) {
+            const int e = threadIdx.x + n * kSlice, p = i0 + 16 * tile + e / (RT * 16), j = j0 + e % (RT * 16);
+            hn[n] = job.hidden[(int64_t)row_s[min(p, i1 - 1) - p0] * fac.rank + min(j, ra - 1)];
+          }
+          issued();
+        }
+      };
+      const auto store_hidden = [&](int tile) {
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int n = 0; n < kHidden; ++n) {
+            const int e = threadIdx.x + n * kSlice;
+            if (e < RT * 256)  // no rows past the run
+              (&hs[tile & 1][0][0])[e] = i0 + 16 * tile + e / (RT * 16) < i1 ? hn[n] : 0.0f;
+          }
+        }
+      };
       const auto multiply = [&](int d, int tile) {
         const int p = i0 + 16 * tile;
-        v4f acc[RT] = {};
-        float4 x[4];
+        if (skip > 0) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          x[m] = own(m, xv[d][m]);
-          if constexpr (SUMS) x[m] = keep4(p + lo < i1, x[m]);
+          for (int m = 0; m < 4; ++m) xv[d][m].drop(skip - (16 * m + 4 * q));
         }
+        if (SUMS && p + 16 > i1) {  // the run's last tile: no rows past it
+#pragma unroll
+          for (int m = 0; m < 4; ++m) xv[d][m].drop(p + lo < i1 ? 0 : 4);
+        }
+        v4f acc[RT] = {};
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) fv[t][m].pin();
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          if constexpr (SUMS) *(float4 *)(turn + lo * kPitch + 16 * m + 4 * q) = x[m];
+          if constexpr (SUMS) *(uint4 *)(turn + lo * kPitch + 16 * m + 4 * q) = xv[d][m].v;
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const float4 f = fv[t][m].floats();
+          for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) acc[t] = mfma(get4(x[m], s), get4(f, s), acc[t]);
-          }
+            for (int t = 0; t < RT; ++t) acc[t] = mfma(xv[d][m].get(s), fv[t][m].get(s), acc[t]);
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t)
@@ -315,27 +334,33 @@ __global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, 
             const float4 v = *(const float4 *)(turn + (4 * r + q) * kPitch + 4 * lo);
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-              const float h = p + 4 * r + q < i1 ? hv[d][t][r] : 0.0f;
+              const float h = hs[tile & 1][4 * r + q][16 * t + lo];
 #pragma unroll
               for (int m = 0; m < 4; ++m) sums[t][m] = mfma(h, get4(v, m), sums[t][m]);
             }
           }
         }
+        store_hidden(tile + 1);
         __syncthreads();
-        for (int e = threadIdx.x; e < 16 * ranks; e += kSlice) {
-          const int i = e / ranks, j = e % ranks;
+        for (int e = threadIdx.x; e < 16 * RT * 16; e += kSlice) {
+          const int i = e / (RT * 16), j = e % (RT * 16);
           float sum = 0.0f;
 #pragma unroll
           for (int w = 0; w < kSliceWaves; ++w) sum += red[w][i][j];
-          if (p + i < i1) to_hidden[(int64_t)row_s[p + i - p0] * fac.rank + j] = j0 + j < ra ? sum : 0.0f;
+          if (p + i < i1 && j < ranks) to_hidden[(int64_t)row_s[p + i - p0] * fac.rank + j] = j0 + j < ra ? sum : 0.0f;
         }
         __syncthreads();
       };
+      load_hidden(0);
       load(0, 0);
+      store_hidden(0);
+      __syncthreads();
       int tile = 0;
       for (; tile + 1 < tiles; tile += 2) {
+        load_hidden(tile + 1);
         load(1, tile + 1);
         multiply(0, tile);
+        load_hidden(tile + 2);
         load(0, tile + 2);
         multiply(1, tile + 1);
       }
@@ -348,7 +373,7 @@ __global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, 
       if (a >= rows.count) break;  // rows without an adapter come last
       const bool began = i0 > p0 || p0 == 0 || rows.adapter(p0 - 1) != a;
       const bool goes_on = i1 == p1 && p1 < rows.n && rows.adapter(p1) == a;
-      const Cols<NARROW> cols(c0 + 4 * lo, width);
+      const Cols<NARROW> cols(c0 + 4 * lo, NARROW ? 0 : max(0, skip - 4 * lo), width);
       store_sums<ACC>(sums, fac, a, ra, j0, q, cols, began, goes_on, job);
     }
     i0 = i1;
@@ -360,19 +385,23 @@ __global__ void __launch_bounds__(kSlice) slice_kernel(RowMap rows, Factor fac, 
 // column]: lane l holds columns 4 (l % 16) + m of its wave's 64 for the m-th
 // of four accumulators, so a row's part is stored as 16-byte words; ranks 4
 // (l / 16) + s of each 16 for the s-th MFMA.  Block: four waves, 256 columns,
-// `per` tiles of 32 rows one after the other; the tile's hidden values lie in
-// LDS, the adapter's factor in registers as long as it stays the same.
-constexpr int kUpRows = 32;
+// `per` tiles of 16 rows one after the other, the next tile's loads in flight,
+// the adapter's factor in registers as long as it stays the same.
+constexpr int kMaxPer = 16;
 template <class T, int RT, bool NARROW>
-__global__ void __launch_bounds__(256) up_kernel(RowMap rows, Factor fac, const float *__restrict__ hidden,
-                                                 const float *base, int64_t bstride, float *y, int64_t ystride,
-                                                 int per) {
-  constexpr int TT = kUpRows / 16, kPitch = RT * 16 + 4;
+__global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
+                                                                const float *__restrict__ hidden, const float *base,
+                                                                int64_t bstride, float *y, int64_t ystride, int per) {
   using raw = typename T::raw;
-  __shared__ float4 hs4[kUpRows * kPitch / 4];
-  float *hs = (float *)hs4;
+  __shared__ int row_s[kMaxPer * 16], key_s[kMaxPer * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
   const Cols<NARROW> cols(blockIdx.x * 256 + wave * 64 + 4 * lo, fac.width);
+  const int p0 = blockIdx.y * per * 16, p1 = min(p0 + per * 16, rows.n);
+  for (int i = threadIdx.x; i < p1 - p0; i += 256) {
+    row_s[i] = rows.row(p0 + i);
+    key_s[i] = rows.adapter(p0 + i);
+  }
+  __syncthreads();
   int held = -1;
   Quad<T> fv[RT][4];
   const auto load_factor = [&](int a, int ra, int g) {  // rank rows past the adapter's: zeros
@@ -388,73 +417,77 @@ __global__ void __launch_bounds__(256) up_kernel(RowMap rows, Factor fac, const 
       for (int s = 0; s < 4; ++s)
         if (g + 16 * t + 4 * q + s >= ra) fv[t][s] = Quad<T>{};
   };
-  for (int p0 = blockIdx.y * per * kUpRows; p0 < min(((int)blockIdx.y + 1) * per * kUpRows, rows.n); p0 += kUpRows) {
-    const int live = min(kUpRows, rows.n - p0);
-    const int mine = min(lane & (kUpRows - 1), live - 1);
-    const int row = rows.row(p0 + mine), key = rows.adapter(p0 + mine);
-    int out_key[TT][4];
-    float4 sum[TT][4];
+  const bool whole = fac.rank % 4 == 0;
+  const auto load_hidden = [&](float4 (&hv)[RT], int tile, int g) {
+    const float *from = hidden + (int64_t)row_s[min(16 * tile + lo, p1 - p0 - 1)] * fac.rank + g;
 #pragma unroll
-    for (int i = 0; i < TT; ++i)
+    for (int t = 0; t < RT; ++t) {
+      const int j = 16 * t + 4 * q;
+      if (whole) hv[t] = keep4(g + j < fac.rank, load4(from + (g + j < fac.rank ? j : 0), 0, 4));
+      else hv[t] = load4(from, j, fac.rank - g);
+    }
+  };
+  float4 hv[2][RT], bv[2][4];
+  const int tiles = (p1 - p0 + 15) / 16;
+  const auto load = [&](int d, int tile_) {
+    const int tile = min(tile_, tiles - 1);
+    load_hidden(hv[d], tile, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {  // the rows this lane's accumulators belong to
-        const int at = 16 * i + 4 * q + r, from = __shfl(row, at);
-        out_key[i][r] = __shfl(key, at);
-        sum[i][r] = make_float4(0, 0, 0, 0);
-        if (base) sum[i][r] = cols.load(base + (int64_t)from * bstride);
-      }
-    for (int g = 0; g < fac.rank; g += 16 * RT) {
-      const int wide = min(16 * RT, fac.rank - g);
-      __syncthreads();
-      for (int e = threadIdx.x; e < kUpRows * RT * 4; e += 256) {
-        const int i = e / (RT * 4), j = e % (RT * 4) * 4;
-        const float *from = hidden + (int64_t)rows.row(p0 + min(i, live - 1)) * fac.rank + g;
-        *(float4 *)(hs + i * kPitch + j) = load4(from, j, wide);
-      }
-      __syncthreads();
-      for (int i0 = 0; i0 < live;) {
-        const int a = __builtin_amdgcn_readlane(key, i0);
-        const uint64_t same = __ballot(lane < live && key == a);
-        i0 += __popcll(same >> i0);
-        if (a >= rows.count) continue;
+    for (int r = 0; r < 4; ++r) {  // the rows this lane's accumulators belong to
+      bv[d][r] = make_float4(0, 0, 0, 0);
+      if (base) bv[d][r] = cols.load(base + (int64_t)row_s[min(16 * tile + 4 * q + r, p1 - p0 - 1)] * bstride);
+    }
+    issued();
+  };
+  const auto work = [&](int d, int tile) {
+    const int at = 16 * tile, live = min(16, p1 - p0 - at);
+    const int key = key_s[at + min(lo, live - 1)];
+    for (int i0 = 0; i0 < live;) {
+      const int a = __builtin_amdgcn_readlane(key, i0);
+      const uint64_t same = __ballot(lane < live && key == a);
+      const int i1 = i0 + __popcll(same >> i0);
+      if (a < rows.count) {
         const int ra = fac.rank_of(a);
-        if (ra <= g) continue;
-        if (held != a || fac.rank > 16 * RT) load_factor(a, ra, g);
-        held = a;
-        const float scale = fac.scale_of(a);
-        v4f acc[TT][4] = {};
+        v4f acc[4] = {};
+        for (int g = 0; g < ra; g += 16 * RT) {
+          if (held != a || fac.rank > 16 * RT) load_factor(a, ra, g);
+          held = a;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          if (16 * t >= ra - g) break;
-          float4 hv[TT];
+          for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int i = 0; i < TT; ++i) hv[i] = *(const float4 *)(hs + (16 * i + lo) * kPitch + 16 * t + 4 * q);
+            for (int s = 0; s < 4; ++s) fv[t][s].pin();
+          if (g > 0) load_hidden(hv[d], tile, g);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const float4 f = fv[t][s].floats();
+          for (int t = 0; t < RT; ++t) {
+            if (16 * t >= ra - g) break;
 #pragma unroll
-            for (int i = 0; i < TT; ++i)
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
-              for (int m = 0; m < 4; ++m) acc[i][m] = mfma(get4(hv[i], s), get4(f, m), acc[i][m]);
+              for (int m = 0; m < 4; ++m) acc[m] = mfma(get4(hv[d][t], s), fv[t][s].get(m), acc[m]);
           }
         }
+        if (fac.rank > 16 * RT && i1 < live) load_hidden(hv[d], tile, 0);  // for the tile's next adapter
+        const float scale = fac.scale_of(a);
 #pragma unroll
-        for (int i = 0; i < TT; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (out_key[i][r] == a)
-              sum[i][r] = fma4(scale, make_float4(acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]), sum[i][r]);
+        for (int r = 0; r < 4; ++r)
+          if (4 * q + r >= i0 && 4 * q + r < i1)
+            bv[d][r] = fma4(scale, make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]), bv[d][r]);
       }
+      i0 = i1;
     }
 #pragma unroll
-    for (int i = 0; i < TT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 16 * i + 4 * q + r;
-        const int to = __shfl(row, at);
-        if (at < live && cols.any()) cols.store(y + (int64_t)to * ystride, sum[i][r]);
-      }
+    for (int r = 0; r < 4; ++r)
+      if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)row_s[at + 4 * q + r] * ystride, bv[d][r]);
+  };
+  load(0, 0);
+  int tile = 0;
+  for (; tile + 1 < tiles; tile += 2) {
+    load(1, tile + 1);
+    work(0, tile);
+    load(0, tile + 2);
+    work(1, tile + 1);
   }
+  if (tile < tiles) work(0, tile);
 }
 
 // The same for few rows: a block one row's 1024 columns, four a thread, the
@@ -505,7 +538,7 @@ struct Sums {
   int count;
 };
 template <bool ACC, int RT, bool NARROW>
-__global__ void __launch_bounds__(256) outer_kernel(RowMap rows, Factor fac, Sums sums) {
+__global__ void __launch_bounds__(256, 4) outer_kernel(RowMap rows, Factor fac, Sums sums) {
   constexpr int DEPTH = RT >= 4 ? 4 : 8;
   __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
   const bool second = (int)blockIdx.x >= sums.of[0].across;
@@ -618,7 +651,7 @@ int slices_of(int width) { return (width + kSlice - 1) / kSlice; }
 // Rows of a block of slice_kernel or outer_kernel: as many as leave two blocks
 // to every CU, `across` of them along the width.
 int chunk_of(int n, int across) {
-  const int64_t rows = (int64_t)n * across / 512 / 16 * 16;
+  const int64_t rows = ((int64_t)n * across + 512 * 16 - 1) / (512 * 16) * 16;
   return (int)std::max<int64_t>(16, std::min<int64_t>(kMaxChunk, rows));
 }
 int rank_groups(int rank) { return rank <= 64 ? 1 : (rank + 63) / 64; }
@@ -688,7 +721,7 @@ hipError_t launch_slices(const Call &c, const Factor &fac, const Sum &job, bool 
     constexpr int RT = decltype(rt)::value;
     const dim3 grid(count, (c.rows.n + job.chunk - 1) / job.chunk, rank_groups(fac.rank));
     with_type(c.dtype, [&](auto t) {
-      by_flag(fac.width < 4, [&](auto narrow) {
+      by_flag(fac.width < 64, [&](auto narrow) {
         constexpr bool N = decltype(narrow)::value;
         if (!sums) slice_kernel<decltype(t), RT, false, false, N><<<grid, kSlice, 0, c.s>>>(c.rows, fac, job, to);
         else if (accumulate) slice_kernel<decltype(t), RT, true, true, N><<<grid, kSlice, 0, c.s>>>(c.rows, fac, job, to);
@@ -716,8 +749,8 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
     return hipGetLastError();
   }
   by_rank(fac.rank, [&](auto rt) {
-    const int tiles = (c.rows.n + kUpRows - 1) / kUpRows, across = (fac.width + 255) / 256;
-    const int per = std::max(1, std::min<int>(8, (int64_t)tiles * across / 1024));
+    const int tiles = (c.rows.n + 15) / 16, across = (fac.width + 255) / 256;
+    const int per = std::max(1, std::min<int>(kMaxPer, (int64_t)tiles * across / 1024));
     const dim3 grid(across, (tiles + per - 1) / per);
     with_type(c.dtype, [&](auto t) {
       by_flag(fac.width < 4, [&](auto narrow) {

@@ -68,6 +68,11 @@ struct Quad {
       v.y = skip < 3 ? v.y : skip < 4 ? v.y & 0xffff0000u : 0;
     }
   }
+  // keeps a 16-bit quad packed through a loop: without it the compiler converts
+  // it once ahead of the loop and holds twice the registers
+  __device__ inline void pin() {
+    if constexpr (sizeof(raw) == 2) asm volatile("" : "+v"(v.x), "+v"(v.y));
+  }
   // the values at row + k, zeros from `width` on
   __device__ static inline Quad load(const raw *row, int k, int width) {
     if (k + 4 <= width) return load(row + k);
@@ -97,6 +102,7 @@ struct Cols {
     skip = NARROW ? 0 : max(0, first + 4 - width);
     c = first - skip;
   }
+  __device__ Cols(int c_, int skip_, int width_) : c(c_), skip(skip_), width(width_) {}
   __device__ bool any() const { return NARROW ? c < width : skip < 4; }
   template <class T>
   __device__ Quad<T> load(const typename T::raw *row) const {
