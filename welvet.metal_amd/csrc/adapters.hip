@@ -202,6 +202,56 @@ __device__ inline void store_sums(const v4f (&acc)[RT][4], const Factor &fac, in
     }
 }
 
+// f32 products at the bf16 MFMA's rate, for 16-bit factors: x is cut into
+// three bf16 parts without rounding (8 + 8 + 8 significand bits), a bf16 value
+// is one part and an f16 value (11 bits) two, so the part products are exact;
+// of f16's six the smallest, below 2^-24 of the product, is left out.  Where a
+// sum comes out as Inf or NaN (a part product can be one where the product is
+// not) the caller does it again by f32 products.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+__device__ inline v4f mfma16(const uint4 &a, const uint4 &b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <class T>
+constexpr int kParts = std::is_same_v<T, BF16> ? 1 : 2;
+// the upper halves of two words, the first's below
+__device__ inline uint32_t upper2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+// Eight values as bf16 parts, the next part's source left in v.
+__device__ inline uint4 take_part(uint4 (&v)[2]) {
+  const uint4 part = {upper2(v[0].x, v[0].y), upper2(v[0].z, v[0].w), upper2(v[1].x, v[1].y), upper2(v[1].z, v[1].w)};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[i].x = f2u(u2f(v[i].x) - u2f(v[i].x & 0xffff0000u));
+    v[i].y = f2u(u2f(v[i].y) - u2f(v[i].y & 0xffff0000u));
+    v[i].z = f2u(u2f(v[i].z) - u2f(v[i].z & 0xffff0000u));
+    v[i].w = f2u(u2f(v[i].w) - u2f(v[i].w & 0xffff0000u));
+  }
+  return part;
+}
+// Two quads of a 16-bit factor as parts.
+template <class T>
+__device__ inline void factor_parts(const Quad<T> &a, const Quad<T> &b, uint4 (&p)[2]) {
+  if constexpr (kParts<T> == 1) {
+    p[0] = {a.v.x, a.v.y, b.v.x, b.v.y};
+  } else {
+    uint4 v[2] = {{f2u(a.get(0)), f2u(a.get(1)), f2u(a.get(2)), f2u(a.get(3))},
+                  {f2u(b.get(0)), f2u(b.get(1)), f2u(b.get(2)), f2u(b.get(3))}};
+    p[0] = take_part(v);
+    p[1] = take_part(v);
+  }
+}
+__device__ inline void pin(uint4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+// Value i of eight from its parts (exact).
+template <class T>
+__device__ inline float from_parts(const uint4 (&p)[2], int i) {
+  const auto half = [&](const uint4 &w) {
+    const uint32_t word = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
+    return u2f(i & 1 ? word & 0xffff0000u : word << 16);
+  };
+  if constexpr (kParts<T> == 1) return half(p[0]);
+  else return half(p[0]) + half(p[1]);
+}
+
 // The same for many rows, a block a slice of the width: the slice's factor
 // values stay in registers while an adapter's rows pass, 16 at a time, the next
 // 16 rows' loads in flight.  Every wave holds 64 columns, its products are
@@ -222,6 +272,9 @@ template <class T, int RT, bool SUMS, bool ACC, bool NARROW>
 __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(RowMap rows, Factor fac, Sum job,
                                                                               float *__restrict__ hidden) {
   constexpr int kPitch = 68;  // floats of a turned row: reads by columns fall on different banks
+  // part products where the f32 MFMAs of both products would bind; f16's two
+  // parts do not fit the registers beside more than 16 ranks
+  constexpr bool SPLIT = SUMS && (std::is_same_v<T, BF16> || (std::is_same_v<T, F16> && RT == 1));
   using raw = typename T::raw;
   __shared__ float red[kSliceWaves][16][RT * 16 + 1];
   __shared__ float4 turn4[SUMS ? kSliceWaves * 16 * kPitch / 4 : 1];
@@ -251,7 +304,8 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
     const int ra = a < rows.count ? fac.rank_of(a) : 0;
     v4f sums[RT][4] = {};
     if (ra > j0) {
-      Quad<T> fv[RT][4];
+      Quad<T> fv[RT][4];     // f32 factors
+      uint4 fp[RT][2][2];    // 16-bit ones: the parts of pieces 2 i and 2 i + 1
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const raw *row = (const raw *)fac.p + ((int64_t)a * fac.rank + min(j0 + 16 * t + lo, ra - 1)) * width;
@@ -266,6 +320,12 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int m = 0; m < 4; ++m) fv[t][m].drop(skip - (16 * m + 4 * q));
+      }
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) factor_parts(fv[t][2 * i], fv[t][2 * i + 1], fp[t][i]);
       }
       Quad<F32> xv[2][4];
       constexpr int kHidden = (RT * 256 + kSlice - 1) / kSlice;  // a thread's hidden values of a tile
@@ -312,17 +372,55 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
           for (int m = 0; m < 4; ++m) xv[d][m].drop(p + lo < i1 ? 0 : 4);
         }
         v4f acc[RT] = {};
+        if constexpr (SUMS) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+          for (int m = 0; m < 4; ++m) *(uint4 *)(turn + lo * kPitch + 16 * m + 4 * q) = xv[d][m].v;
+        }
+        if constexpr (!SPLIT) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m) fv[t][m].pin();
+          for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          if constexpr (SUMS) *(uint4 *)(turn + lo * kPitch + 16 * m + 4 * q) = xv[d][m].v;
+            for (int m = 0; m < 4; ++m) fv[t][m].pin();
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
+          for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) acc[t] = mfma(xv[d][m].get(s), fv[t][m].get(s), acc[t]);
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+              for (int t = 0; t < RT; ++t) acc[t] = mfma(xv[d][m].get(s), fv[t][m].get(s), acc[t]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint4 v[2] = {xv[d][2 * i].v, xv[d][2 * i + 1].v};
+            const uint4 hi = take_part(v), mid = take_part(v), low = take_part(v);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              acc[t] = mfma16(low, fp[t][i][0], acc[t]);
+              if constexpr (kParts<T> == 2) acc[t] = mfma16(mid, fp[t][i][1], acc[t]);
+              acc[t] = mfma16(mid, fp[t][i][0], acc[t]);
+              if constexpr (kParts<T> == 2) acc[t] = mfma16(hi, fp[t][i][1], acc[t]);
+              acc[t] = mfma16(hi, fp[t][i][0], acc[t]);
+            }
+          }
+          bool odd = false;
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) odd = odd || !isfinite(acc[t][r]);
+          if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              acc[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                uint4 parts[2] = {fp[t][m / 2][0], fp[t][m / 2][1]};
+                pin(parts[0]);  // else converted ahead of the loop, in registers of their own
+                pin(parts[1]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                  acc[t] = mfma(xv[d][m].get(s), from_parts<T>(parts, 4 * (m & 1) + s), acc[t]);
+              }
+            }
+          }
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t)
@@ -387,11 +485,12 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 // (l / 16) + s of each 16 for the s-th MFMA.  Block: four waves, 256 columns,
 // `per` tiles of 16 rows one after the other, the next tile's loads in flight,
 // the adapter's factor in registers as long as it stays the same.
-constexpr int kMaxPer = 16;
+constexpr int kMaxPer = 4;
 template <class T, int RT, bool NARROW>
 __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
                                                                 const float *__restrict__ hidden, const float *base,
-                                                                int64_t bstride, float *y, int64_t ystride, int per) {
+                                                                int64_t bstride, float *y, int64_t ystride, int per,
+                                                                bool nt) {
   using raw = typename T::raw;
   __shared__ int row_s[kMaxPer * 16], key_s[kMaxPer * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
@@ -477,7 +576,7 @@ __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Fa
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)row_s[at + 4 * q + r] * ystride, bv[d][r]);
+      if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)row_s[at + 4 * q + r] * ystride, bv[d][r], nt);
   };
   load(0, 0);
   int tile = 0;
@@ -608,38 +707,51 @@ __global__ void __launch_bounds__(256, 4) outer_kernel(RowMap rows, Factor fac, 
 
 // The adapters that no block wrote whole: their partials added up in order,
 // zeros for those no row names.
-template <bool ACC>
+// WORDS: 16-byte words a thread, one where the values are few.
+template <bool ACC, int WORDS>
 __global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, Sums sums) {
   const Sum &job = sums.of[blockIdx.z];
   const float *part = job.part;
-  const int a = blockIdx.y, chunk = job.chunk;
-  const int begin = first_at_least(rows.key, rows.n, a), end = first_at_least(rows.key, rows.n, a + 1);
-  const int size = fac.rank * job.width;
+  const int a = blockIdx.y, chunk = job.chunk, size = fac.rank * job.width;
+  if ((int64_t)blockIdx.x * (WORDS * 1024) >= size) return;
+  const int2 at = rows_of(rows.key, rows.n, a);
   float *to = job.grad + (int64_t)a * size;
-  const int first = begin / chunk, last = (end - 1) / chunk;
-  const bool none = begin == end;
+  const int first = at.x / chunk, last = (at.y - 1) / chunk;
+  const bool none = at.x == at.y;
   if (none ? ACC : first == last) return;
-  const int edge = fac.rank_of(a) * job.width;
+  const int edge = fac.rank_of(a) * job.width, e0 = blockIdx.x * (WORDS * 1024) + threadIdx.x * 4;
   const float scale = fac.scale_of(a);
-  for (int e = (blockIdx.x * 256 + threadIdx.x) * 4; e < size; e += gridDim.x * 1024) {
-    float4 v = make_float4(0, 0, 0, 0);
-    if (!none) {
-      // its first block's rows went on (slot 1), every later one's began earlier
-      v = load4(part + ((int64_t)first * 2 + 1) * size, e, size);
-      int b = first + 1;
-      for (; b + 4 <= last + 1; b += 4) {
-        float4 w[4];
+  float4 v[WORDS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = load4(part + (int64_t)(b + i) * 2 * size, e, size);
+  for (int i = 0; i < WORDS; ++i) v[i] = make_float4(0, 0, 0, 0);
+  if (!none) {
+    constexpr int kAhead = 4 / WORDS;  // blocks whose loads are in flight together
+    // its first block's rows went on (slot 1), every later one's began earlier
+    const auto block = [&](int b) { return part + ((int64_t)b * 2 + (b == first ? 1 : 0)) * size; };
+    int b = first;
+    for (; b + kAhead - 1 <= last; b += kAhead) {
+      float4 w[kAhead][WORDS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v = add4(v, w[i]);
-      }
-      for (; b <= last; ++b) v = add4(v, load4(part + (int64_t)b * 2 * size, e, size));
-      v = make_float4(e < edge ? v.x * scale : 0.0f, e + 1 < edge ? v.y * scale : 0.0f,
-                      e + 2 < edge ? v.z * scale : 0.0f, e + 3 < edge ? v.w * scale : 0.0f);
-      if constexpr (ACC) v = add4(load4(to, e, size), v);
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[k][i] = load4(block(b + k), e0 + i * 1024, size);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) v[i] = add4(v[i], w[k][i]);
     }
-    store4(to, e, size, v);
+    for (; b <= last; ++b)
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) v[i] = add4(v[i], load4(block(b), e0 + i * 1024, size));
+  }
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    const int e = e0 + i * 1024;
+    if (e >= size) break;
+    float4 r = make_float4(e < edge ? v[i].x * scale : 0.0f, e + 1 < edge ? v[i].y * scale : 0.0f,
+                           e + 2 < edge ? v[i].z * scale : 0.0f, e + 3 < edge ? v[i].w * scale : 0.0f);
+    if constexpr (ACC) r = add4(load4(to, e, size), r);
+    store4(to, e, size, r);
   }
 }
 
@@ -750,12 +862,15 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
   }
   by_rank(fac.rank, [&](auto rt) {
     const int tiles = (c.rows.n + 15) / 16, across = (fac.width + 255) / 256;
+    // four tiles a block at most: blocks that pass the rows in launch order keep
+    // HBM at 5.3 TB/s, with eight tiles 4.6 (8192 x 4096 f32 read and written)
     const int per = std::max(1, std::min<int>(kMaxPer, (int64_t)tiles * across / 1024));
+    const bool nt = (int64_t)c.rows.n * fac.width * 4 > kKept;
     const dim3 grid(across, (tiles + per - 1) / per);
     with_type(c.dtype, [&](auto t) {
       by_flag(fac.width < 4, [&](auto narrow) {
         up_kernel<decltype(t), decltype(rt)::value, decltype(narrow)::value>
-            <<<grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, per);
+            <<<grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, per, nt);
       });
     });
   });
@@ -786,9 +901,13 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((uint32_t)std::min<int64_t>((size + 1023) / 1024, 1024), c.rows.count, sums.count);
+  const bool wide = size * c.rows.count * sums.count >= (int64_t)4096 * 1024;  // four blocks a CU at four words
+  const int per = wide ? 4096 : 1024;
+  const dim3 grid((uint32_t)((size + per - 1) / per), c.rows.count, sums.count);
   by_flag(accumulate, [&](auto acc) {
-    sum_kernel<decltype(acc)::value><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
+    by_flag(wide, [&](auto w) {
+      sum_kernel<decltype(acc)::value, decltype(w)::value ? 4 : 1><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
+    });
   });
   return hipGetLastError();
 }

@@ -22,25 +22,23 @@ template <class T, int ROWS, bool NARROW>
 __global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__restrict__ table, int64_t tstride,
                                                      uint32_t vocab, int dim, const int32_t *__restrict__ tokens,
                                                      int n, float scale, float *__restrict__ out, int64_t ostride,
-                                                     int tiles) {
+                                                     int tiles, bool nt) {
   const int group = blockIdx.x / tiles;
   const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (!cols.any()) return;
   Quad<T> v[ROWS];
+  uint32_t id[ROWS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int t = group * ROWS + r;
-    const uint32_t id = t < n ? (uint32_t)tokens[t] : vocab;
-    v[r] = Quad<T>{};
-    if (id < vocab) v[r] = cols.template load<T>(table + (int64_t)id * tstride);
-  }
+  for (int r = 0; r < ROWS; ++r) id[r] = (uint32_t)tokens[min(group * ROWS + r, n - 1)];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)  // padding reads row 0
+    v[r] = cols.template load<T>(table + (int64_t)(id[r] < vocab ? id[r] : 0) * tstride);
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int t = group * ROWS + r;
     if (t >= n) break;
-    // padding stays +0 also under a negative scale
-    const bool pad = (uint32_t)tokens[t] >= vocab;
-    cols.store(out + (int64_t)t * ostride, pad ? v[r].floats() : mul4(v[r].floats(), scale));
+    // padding is +0, also under a negative scale
+    cols.store(out + (int64_t)t * ostride, keep4(id[r] < vocab, mul4(v[r].floats(), scale)), nt);
   }
 }
 
@@ -315,7 +313,7 @@ welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t
     const auto go = [&](auto kernel) {
       kernel<<<blocks, threads, 0, (hipStream_t)stream>>>((const typename T::raw *)d_table, table_stride,
                                                           (uint32_t)vocab, dim, d_tokens, n, scale, d_out, out_stride,
-                                                          tiles);
+                                                          tiles, (int64_t)n * dim * 4 > tok::kKept);
     };
     if (dim < 4) rows == 4 ? go(lookup_kernel<T, 4, true>) : go(lookup_kernel<T, 1, true>);
     else rows == 4 ? go(lookup_kernel<T, 4, false>) : go(lookup_kernel<T, 1, false>);

@@ -83,6 +83,12 @@ struct Quad {
   }
 };
 __device__ inline void store4(float *p, const float4 &v) { __builtin_memcpy(p, &v, sizeof(v)); }
+// The same past the caches' keeping: results larger than they hold.
+typedef float nt4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ inline void store4_nt(float *p, const float4 &v) {
+  __builtin_nontemporal_store(nt4{v.x, v.y, v.z, v.w}, (nt4 *)p);
+}
+constexpr int64_t kKept = 64 << 20;  // results up to these bytes are stored to stay in the caches
 __device__ inline void store4(float *row, int k, int width, const float4 &v) {
   if (k + 4 <= width) return store4(row + k, v);
   const float f[4] = {v.x, v.y, v.z, v.w};
@@ -110,9 +116,9 @@ struct Cols {
     else return Quad<T>::load(row + c);
   }
   __device__ float4 load(const float *row) const { return load<F32>((const uint32_t *)row).floats(); }
-  __device__ void store(float *row, const float4 &v) const {
+  __device__ void store(float *row, const float4 &v, bool nt = false) const {
     if constexpr (NARROW) return store4(row, c, width, v);
-    if (skip == 0) return store4(row + c, v);
+    if (skip == 0) return nt ? store4_nt(row + c, v) : store4(row + c, v);
     if (skip < 2) row[c + 1] = v.y;
     if (skip < 3) row[c + 2] = v.z;
     if (skip < 4) row[c + 3] = v.w;
@@ -173,19 +179,20 @@ inline auto with_type(int32_t dtype, F &&f) {
 // rows' own, so sums over a key's rows are the same on every run.
 //
 // Ranks are counted, not sorted: a row's place among kChunk rows is the number
-// of rows before it, one compare and one add per pair.  A block takes 64 rows,
-// one a lane, and its 16 waves a sixteenth of the chunk each, read from LDS as
-// words of four that all lanes share.  More rows than a chunk: each chunk by
-// itself, then every row's places in the other chunks by binary search there,
-// four threads a row.
+// of rows before it, one compare and one add per pair.  A block takes 16 rows;
+// four lanes of each of its 16 waves share a row and look at 32 keys each, in
+// words of four from LDS.  More rows than a chunk: each chunk by itself, then
+// every row's places in the other chunks by binary search there, four threads
+// a row.  (2048 rows: 64 rows a block and a lane a row took 8 us on 32 CUs.)
 constexpr int kChunk = 2048;
+constexpr int kRankRows = 16;
 
 static __global__ void __launch_bounds__(1024) rank_kernel(const int32_t *__restrict__ key, int n, uint32_t limit,
                                                            int32_t *__restrict__ skey, int32_t *__restrict__ order) {
   __shared__ uint4 keys[kChunk / 4];
-  __shared__ int count[16][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int own = blockIdx.x * 64, i = own + lane, begin = own / kChunk * kChunk;
+  __shared__ int count[16][kRankRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
+  const int own = blockIdx.x * kRankRows, i = own + lo, begin = own / kChunk * kChunk;
   uint32_t *flat = (uint32_t *)keys;
   for (int j = threadIdx.x; j < kChunk; j += 1024)
     // past the end: after every row, whatever its key
@@ -194,31 +201,30 @@ static __global__ void __launch_bounds__(1024) rank_kernel(const int32_t *__rest
   const uint32_t mine = i < n ? flat[i - begin] : limit;
   const int at = own - begin;
   int less = 0;
-  // 128 keys a wave, in words of four: the word's side of the block's rows is
-  // the same for all of it
-#pragma unroll 4
-  for (int w = wave * (kChunk / 64); w < (wave + 1) * (kChunk / 64); ++w) {
-    const uint4 u = keys[w];
-    const int j = w * 4;
-    if (j >= at && j < at + 64) {
-      less += (u.x < mine || (u.x == mine && j < at + lane)) ? 1 : 0;
-      less += (u.y < mine || (u.y == mine && j + 1 < at + lane)) ? 1 : 0;
-      less += (u.z < mine || (u.z == mine && j + 2 < at + lane)) ? 1 : 0;
-      less += (u.w < mine || (u.w == mine && j + 3 < at + lane)) ? 1 : 0;
-    } else {
-      const uint32_t bound = mine + (j < at ? 1u : 0u);  // equal keys of earlier rows come first
-      less += u.x < bound ? 1 : 0;
-      less += u.y < bound ? 1 : 0;
-      less += u.z < bound ? 1 : 0;
-      less += u.w < bound ? 1 : 0;
+#pragma unroll
+  for (int w = 0; w < kChunk / 256; ++w) {
+    const int word = (w * 16 + wave) * 4 + q, j = word * 4;
+    const uint4 u = keys[word];
+    const uint32_t bound = mine + (j < at ? 1u : 0u);  // equal keys of earlier rows come first
+    less += u.x < bound ? 1 : 0;
+    less += u.y < bound ? 1 : 0;
+    less += u.z < bound ? 1 : 0;
+    less += u.w < bound ? 1 : 0;
+    if (j >= at && j < at + kRankRows) {  // the block's own rows, counted as later ones above
+      less += (u.x == mine && j < at + lo) ? 1 : 0;
+      less += (u.y == mine && j + 1 < at + lo) ? 1 : 0;
+      less += (u.z == mine && j + 2 < at + lo) ? 1 : 0;
+      less += (u.w == mine && j + 3 < at + lo) ? 1 : 0;
     }
   }
-  count[wave][lane] = less;
+  less += __shfl_xor(less, 16);
+  less += __shfl_xor(less, 32);
+  if (q == 0) count[wave][lo] = less;
   __syncthreads();
-  if (wave == 0 && i < n) {
+  if (threadIdx.x < kRankRows && i < n) {
     int to = begin;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) to += count[w][lane];
+    for (int w = 0; w < 16; ++w) to += count[w][lo];
     skey[to] = (int32_t)mine;
     order[to] = i;
   }
@@ -264,6 +270,26 @@ static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__res
   }
 }
 
+// The first places of the sorted keys whose keys are >= v and >= v + 1: the
+// rows of key v.  A whole wave calls it, each half looking at 32 places a time.
+__device__ inline int2 rows_of(const int32_t *__restrict__ skey, int n, int32_t v) {
+  const int lane = threadIdx.x & 31;
+  const int32_t mine = v + ((threadIdx.x & 32) ? 1 : 0);
+  int lo = 0, hi = n;
+  while (__any(lo < hi)) {
+    const int step = (hi - lo + 31) / 32, p = lo + lane * step;
+    const uint64_t both = __ballot(lo < hi && p < hi && skey[p] < mine);
+    const int below = __popc((threadIdx.x & 32) ? (uint32_t)(both >> 32) : (uint32_t)both);
+    if (below == 0) {
+      hi = lo;
+    } else if (lo < hi) {
+      hi = min(hi, lo + below * step);
+      lo = lo + (below - 1) * step + 1;
+    }
+  }
+  return {__builtin_amdgcn_readlane(lo, 0), __builtin_amdgcn_readlane(lo, 32)};
+}
+
 // The first place of the sorted keys whose key is >= v; a whole wave calls it
 // and looks at 64 places a time.
 __device__ inline int first_at_least(const int32_t *__restrict__ skey, int n, int32_t v) {
@@ -292,7 +318,7 @@ inline hipError_t launch_order(const int32_t *key, int n, int32_t limit, void *w
   out->order = (int32_t *)(p + step);
   const bool one = n <= kChunk;
   int32_t *ck = one ? out->skey : (int32_t *)(p + 2 * step), *co = one ? out->order : (int32_t *)(p + 3 * step);
-  rank_kernel<<<(n + 63) / 64, 1024, 0, s>>>(key, n, (uint32_t)limit, ck, co);
+  rank_kernel<<<(n + kRankRows - 1) / kRankRows, 1024, 0, s>>>(key, n, (uint32_t)limit, ck, co);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || one) return e;
   merge_kernel<<<(n + 255) / 256, 1024, 0, s>>>(ck, co, n, out->skey, out->order);
