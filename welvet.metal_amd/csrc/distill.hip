@@ -65,25 +65,36 @@ __device__ inline Stat join(Stat a, Stat b, float c) {
   const Shift h(fmaxf(a.m, b.m), c);
   return {h.m, a.s * rescale(a.m, c, h) + b.s * rescale(b.m, c, h)};
 }
-template <int N>
-__device__ inline void take(Stat &a, const float (&z)[N], float c) {
-  float m = z[0];
+// A thread's pair as it grows, with the offset of its maximum.
+struct Running {
+  float m = -INFINITY, s = 0.0f, mc = 0.0f;
+  template <int N>
+  __device__ inline void take(const float (&z)[N], float c) {
+    float top = z[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
-  if (m > a.m) {
-    const Shift h(m, c);
-    a.s *= rescale(a.m, c, h);
-    a.m = m;
+    for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+    if (top > m) {
+      const Shift h(top, c);
+      s *= rescale(m, c, h);
+      m = top;
+      mc = h.mc;
+    }
+    float e[N];
+    if (__builtin_expect(fabsf(mc) == INFINITY, 0)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f((z[i] - m) * c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(z[i], c, -mc));
+    }
+#pragma unroll
+    for (int n = N / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int i = 0; i < n; ++i) e[i] += e[i + n];
+    s += e[0];
   }
-  const Shift h(a.m, c);
-  if (__builtin_expect(h.huge, 0)) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) a.s += __builtin_amdgcn_exp2f((z[i] - h.m) * c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) a.s += __builtin_amdgcn_exp2f(fmaf(z[i], c, -h.mc));
-  }
-}
+  __device__ inline Stat stat() const { return {m, s}; }
+};
 
 // The block's pair, on every thread.
 template <int WAVES>
@@ -138,54 +149,80 @@ template <class T>
 __device__ inline float logit(const Args &a, int row, int v) {
   return T::get(((const typename T::raw *)a.logits + (int64_t)row * a.stride)[v]);
 }
-// Fills e, *mass = the sum of q; false where the row has no entry.  zs: the
-// entries' logits of this row, or null for reading them.
+// Three steps, so that a row's own loads can be in flight between them: the
+// entries' loads, the distribution q, the student's logits at the entries.
 template <class T, int WAVES>
-__device__ inline bool read_teacher(const Args &a, int row, const float *zs, Entries &e, float *mass) {
-  const double inv = 1.0 / (double)a.temperature;
-  if (threadIdx.x == 0) e.some = 0;
-  __syncthreads();
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
-    const int v = a.index[(int64_t)row * a.k + i];
-    const float l = a.teacher[(int64_t)row * a.k + i];
-    const bool live = v >= 0 && v < a.vocab && l != -INFINITY;
-    e.index[i] = live ? v : -1;
-    e.q[i] = l;
-    e.z[i] = !live ? 0.0f : zs ? zs[i] : logit<T>(a, row, v);
-    if (live) top = fmaxf(top, l), e.some = 1;
-  }
-  __syncthreads();
-  if (!e.some) return false;
-  double most;
-  if (a.teacher_lse == nullptr) {
+struct Teacher {
+  static constexpr int kPer = (kMaxEntries + WAVES * 64 - 1) / (WAVES * 64);
+  int index[kPer];
+  float l[kPer];
+  __device__ inline void load(const Args &a, int row) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    if ((threadIdx.x & 63) == 0) e.wave[threadIdx.x >> 6] = top;
+    for (int n = 0; n < kPer; ++n) {
+      const int i = threadIdx.x + n * WAVES * 64;
+      index[n] = -1;
+      l[n] = -INFINITY;
+      if (i < a.k) {
+        index[n] = a.index[(int64_t)row * a.k + i];
+        l[n] = a.teacher[(int64_t)row * a.k + i];
+      }
+    }
+  }
+  // Fills e.index and e.q; *mass = the sum of q; false where the row has no entry.
+  __device__ inline bool weigh(const Args &a, int row, Entries &e, float *mass) {
+    const double inv = 1.0 / (double)a.temperature;
+    if (threadIdx.x == 0) e.some = 0;
     __syncthreads();
-    top = e.wave[0];
+    float top = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, e.wave[w]);
+    for (int n = 0; n < kPer; ++n) {
+      if (index[n] < 0 || index[n] >= a.vocab || l[n] == -INFINITY) index[n] = -1;
+      else top = fmaxf(top, l[n]), e.some = 1;
+    }
     __syncthreads();
-    most = (double)top * inv;
-  } else {
-    most = (double)a.teacher_lse[row];
+    if (!e.some) return false;
+    double most;
+    if (a.teacher_lse == nullptr) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+      if ((threadIdx.x & 63) == 0) e.wave[threadIdx.x >> 6] = top;
+      __syncthreads();
+      top = e.wave[0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) top = fmaxf(top, e.wave[w]);
+      __syncthreads();
+      most = (double)top * inv;
+    } else {
+      most = (double)a.teacher_lse[row];
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) {
+      l[n] = (float)((double)l[n] * inv - most);
+      if (index[n] >= 0) sum += expf(l[n]);
+    }
+    sum = block_sum<WAVES>(sum, e.wave);
+    const float log_sum = a.teacher_lse == nullptr ? logf(sum) : 0.0f;
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) {
+      const int i = threadIdx.x + n * WAVES * 64;
+      if (i >= a.k) break;
+      e.index[i] = index[n];
+      e.q[i] = l[n] - log_sum;
+    }
+    *mass = a.teacher_lse == nullptr ? 1.0f : sum;
+    __syncthreads();
+    return true;
   }
-  float sum = 0.0f;
-  for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
-    e.q[i] = (float)((double)e.q[i] * inv - most);
-    if (e.index[i] >= 0) sum += expf(e.q[i]);
+  // e.z, from zs (this row's logits at the entries) or the row itself.
+  __device__ inline void gather(const Args &a, int row, const float *zs, Entries &e) {
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) {
+      const int i = threadIdx.x + n * WAVES * 64;
+      if (i < a.k && index[n] >= 0) e.z[i] = zs ? zs[i] : logit<T>(a, row, index[n]);
+    }
   }
-  sum = block_sum<WAVES>(sum, e.wave);
-  if (a.teacher_lse == nullptr) {
-    const float log_sum = logf(sum);
-    for (int i = threadIdx.x; i < a.k; i += WAVES * 64) e.q[i] -= log_sum;
-    sum = 1.0f;
-  }
-  *mass = sum;
-  __syncthreads();
-  return true;
-}
+};
 
 // loss of a row from the pair of its logits; every thread calls it.
 template <int WAVES>
@@ -233,13 +270,17 @@ __device__ inline void write_entries(const Args &a, int row, const Entries &e, i
   }
 }
 
-// Dense values of n logits at z: term * g.
-template <class T>
+// Dense values: term * g, for a row whose offset does not overflow, or does.
+template <bool HUGE>
+__device__ inline float dense(float z, float c, const Shift &h, float g) {
+  return __builtin_amdgcn_exp2f(HUGE ? (z - h.m) * c : fmaf(z, c, -h.mc)) * g;
+}
+template <class T, bool HUGE>
 __device__ inline uint4 grad_word(const uint4 &word, float c, const Shift &h, float g) {
   float f[T::kPer16];
   unpack16<T>(word, f);
 #pragma unroll
-  for (int i = 0; i < T::kPer16; ++i) f[i] = term(f[i], c, h) * g;
+  for (int i = 0; i < T::kPer16; ++i) f[i] = dense<HUGE>(f[i], c, h, g);
   return pack16<T>(f);
 }
 template <class T, int THREADS>
@@ -249,21 +290,165 @@ __device__ inline void zero_grad(typename T::raw *out, int n) {
   if ((int)threadIdx.x < span.head + span.tail) out[span.edge(threadIdx.x)] = 0;
 }
 
-// A block's part of a row.
+// Words that are not looked at again: past the caches, which then keep those
+// of the row's end that are.
+typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+__device__ inline void put_word(uint4 *p, const uint4 &v) {
+  __builtin_nontemporal_store(w4{v.x, v.y, v.z, v.w}, (w4 *)p);
+}
+__device__ inline uint4 get_word(const uint4 *p) {
+  const w4 v = __builtin_nontemporal_load((const w4 *)p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// A row a block.  Of each thread's 16-byte words of it HOLD stay in registers
+// and LDSW in LDS between the two passes, what is left is read again.  The
+// teacher's loads go out first, then the row's, and the teacher's arithmetic
+// runs while those are under way.  Two blocks a CU, so that one's exponentials
+// (about 200 us of the whole) run under the other's loads and stores: 4096 x
+// 131072 bf16, an eighth of the rows left out, takes 418 us with 8 waves and
+// 8 + 8 words held, 438 with 8 + 0, 573 with 16 waves and the whole row in
+// registers (one block a CU).
+template <class T, int WAVES, int HOLD, int LDSW, bool GRAD>
+__global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
+  constexpr int kThreads = WAVES * 64;
+  __shared__ Stat lds[WAVES];
+  __shared__ Entries e;
+  __shared__ uint4 more[LDSW > 0 ? LDSW * kThreads : 1];
+  const int row = blockIdx.x, n = a.vocab;
+  const float weight = a.weight ? a.weight[row] : 1.0f;
+  const Span<T> in((const typename T::raw *)a.logits + (int64_t)row * a.stride, n);
+  typename T::raw *out = GRAD ? (typename T::raw *)a.grad + (int64_t)row * a.gstride : nullptr;
+  float mass = 0.0f;
+  Teacher<T, WAVES> teacher;
+  uint4 held[HOLD];
+  bool live = weight != 0.0f;
+  if (live) {
+    teacher.load(a, row);
+    issued();
+#pragma unroll
+    for (int r = 0; r < HOLD; ++r)
+      if (r * kThreads < in.words) held[r] = get_word(in.word(min(r * kThreads + (int)threadIdx.x, in.words - 1)));
+    issued();
+    live = teacher.weigh(a, row, e, &mass);
+  }
+  if (!live) {
+    if (threadIdx.x == 0 && a.loss) a.loss[row] = 0.0f;
+    if constexpr (GRAD) zero_grad<T, kThreads>(out, n);
+    return;
+  }
+  teacher.gather(a, row, nullptr, e);
+  Running run;
+#pragma unroll
+  for (int r = 0; r < HOLD; ++r)
+    if (r * kThreads + (int)threadIdx.x < in.words) {
+      float f[T::kPer16];
+      unpack16<T>(held[r], f);
+      run.take(f, a.c);
+    }
+  {
+    int i = HOLD * kThreads + threadIdx.x;
+    if constexpr (LDSW > 0) {
+      for (int r0 = 0; r0 < LDSW && i < in.words; r0 += 4) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = get_word(in.word(min(i + k * kThreads, in.words - 1)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (i < in.words) {
+            more[(r0 + k) * kThreads + threadIdx.x] = w[k];
+            float f[T::kPer16];
+            unpack16<T>(w[k], f);
+            run.take(f, a.c);
+          }
+          i += kThreads;
+        }
+      }
+    }
+    for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
+      uint4 w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float f[T::kPer16];
+        unpack16<T>(w[k], f);
+        run.take(f, a.c);
+      }
+    }
+    for (; i < in.words; i += kThreads) {
+      float f[T::kPer16];
+      unpack16<T>(*in.word(i), f);
+      run.take(f, a.c);
+    }
+  }
+  if ((int)threadIdx.x < in.head + in.tail) {
+    const float f[1] = {T::get(in.p[in.edge(threadIdx.x)])};
+    run.take(f, a.c);
+  }
+  const Stat st = block_join<WAVES>(run.stat(), a.c, lds);
+  if (a.loss) write_loss<WAVES>(a, row, e, st, weight);
+  if constexpr (GRAD) {
+    const Shift h(st.m, a.c);
+    const float c = a.c, wt = weight * a.temperature;
+    const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
+    const auto write = [&](auto huge) {
+      constexpr bool H = decltype(huge)::value;
+      if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
+        uint4 *to = (uint4 *)(out + in.head);
+#pragma unroll
+        for (int r = 0; r < HOLD; ++r) {
+          const int i = r * kThreads + threadIdx.x;
+          if (i < in.words) put_word(to + i, grad_word<T, H>(held[r], c, h, g));
+        }
+        int i = HOLD * kThreads + threadIdx.x;
+        if constexpr (LDSW > 0) {
+          for (int r = 0; r < LDSW && i < in.words; ++r, i += kThreads)
+            put_word(to + i, grad_word<T, H>(more[r * kThreads + threadIdx.x], c, h, g));
+        }
+        for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
+          uint4 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) put_word(to + i + k * kThreads, grad_word<T, H>(w[k], c, h, g));
+        }
+        for (; i < in.words; i += kThreads) put_word(to + i, grad_word<T, H>(*in.word(i), c, h, g));
+        if ((int)threadIdx.x < in.head + in.tail) {
+          const int at = in.edge(threadIdx.x);
+          out[at] = T::put(dense<H>(T::get(in.p[at]), c, h, g));
+        }
+      } else {
+        for (int i = threadIdx.x; i < n; i += kThreads) out[i] = T::put(dense<H>(T::get(in.p[i]), c, h, g));
+      }
+    };
+    if (h.huge) write(std::true_type{});
+    else write(std::false_type{});
+    __syncthreads();
+    write_entries<T, WAVES>(a, row, e, 0, n, h, g, wt);
+  }
+}
+
+// Few rows: `parts` blocks a row.
 //   STATS  the part's pair into pairs[row][part], and by part 0 the entries'
 //          logits into zs[row][k]
-//   else   the part's gradient, and by part 0 the loss: the row's pair from
-//          `pairs`, or from the part itself where that is null (one part)
+//   else   the part's gradient, and by part 0 the loss
 template <class T, int WAVES, bool STATS>
-__global__ void __launch_bounds__(WAVES * 64) distill_kernel(Args a, int parts, int len, Stat *pairs, float *zs) {
+__global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int parts, int len, Stat *pairs, float *zs) {
   constexpr int kThreads = WAVES * 64;
   __shared__ Stat lds[WAVES];
   const int row = blockIdx.x / parts, part = blockIdx.x % parts, begin = part * len;
   const int n = min(len, a.vocab - begin);
   const float weight = a.weight ? a.weight[row] : 1.0f;
   const Span<T> in((const typename T::raw *)a.logits + (int64_t)row * a.stride + begin, n);
-  Stat st{-INFINITY, 0.0f};
-  const auto stats = [&] {
+  if constexpr (STATS) {
+    Running run;
+    if (weight == 0.0f) return;
+    if (part == 0)
+      for (int i = threadIdx.x; i < a.k; i += kThreads) {
+        const int v = a.index[(int64_t)row * a.k + i];
+        if (v >= 0 && v < a.vocab) zs[(int64_t)row * a.k + i] = logit<T>(a, row, v);
+      }
     int i = threadIdx.x;
     for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
       uint4 w[4];
@@ -273,67 +458,67 @@ __global__ void __launch_bounds__(WAVES * 64) distill_kernel(Args a, int parts, 
       for (int k = 0; k < 4; ++k) {
         float f[T::kPer16];
         unpack16<T>(w[k], f);
-        take(st, f, a.c);
+        run.take(f, a.c);
       }
     }
     for (; i < in.words; i += kThreads) {
       float f[T::kPer16];
       unpack16<T>(*in.word(i), f);
-      take(st, f, a.c);
+      run.take(f, a.c);
     }
     if ((int)threadIdx.x < in.head + in.tail) {
       const float f[1] = {T::get(in.p[in.edge(threadIdx.x)])};
-      take(st, f, a.c);
+      run.take(f, a.c);
     }
-    st = block_join<WAVES>(st, a.c, lds);
-  };
-  if constexpr (STATS) {
-    if (weight == 0.0f) return;
-    if (part == 0)
-      for (int i = threadIdx.x; i < a.k; i += kThreads) {
-        const int v = a.index[(int64_t)row * a.k + i];
-        if (v >= 0 && v < a.vocab) zs[(int64_t)row * a.k + i] = logit<T>(a, row, v);
-      }
-    stats();
+    const Stat st = block_join<WAVES>(run.stat(), a.c, lds);
     if (threadIdx.x == 0) pairs[(int64_t)row * parts + part] = st;
   } else {
     __shared__ Entries e;
     typename T::raw *out = a.grad ? (typename T::raw *)a.grad + (int64_t)row * a.gstride + begin : nullptr;
     float mass = 0.0f;
-    if (weight == 0.0f || !read_teacher<T, WAVES>(a, row, zs ? zs + (int64_t)row * a.k : nullptr, e, &mass)) {
+    Teacher<T, WAVES> teacher;
+    bool live = weight != 0.0f;
+    if (live) {
+      teacher.load(a, row);
+      live = teacher.weigh(a, row, e, &mass);
+    }
+    if (!live) {
       if (threadIdx.x == 0 && part == 0 && a.loss) a.loss[row] = 0.0f;
       if (out) zero_grad<T, kThreads>(out, n);
       return;
     }
-    if (pairs == nullptr) {
-      stats();
-    } else {
-      for (int i = threadIdx.x; i < parts; i += kThreads) st = join(st, pairs[(int64_t)row * parts + i], a.c);
-      st = block_join<WAVES>(st, a.c, lds);
-    }
+    teacher.gather(a, row, zs + (int64_t)row * a.k, e);
+    Stat st{-INFINITY, 0.0f};
+    for (int i = threadIdx.x; i < parts; i += kThreads) st = join(st, pairs[(int64_t)row * parts + i], a.c);
+    st = block_join<WAVES>(st, a.c, lds);
     if (part == 0 && a.loss) write_loss<WAVES>(a, row, e, st, weight);
     if (!out) return;
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
     const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
-    if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
-      uint4 *to = (uint4 *)(out + in.head);
-      int i = threadIdx.x;
-      for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
-        uint4 w[4];
+    const auto write = [&](auto huge) {
+      constexpr bool H = decltype(huge)::value;
+      if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
+        uint4 *to = (uint4 *)(out + in.head);
+        int i = threadIdx.x;
+        for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
+          uint4 w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
+          for (int k = 0; k < 4; ++k) w[k] = *in.word(i + k * kThreads);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) to[i + k * kThreads] = grad_word<T>(w[k], c, h, g);
+          for (int k = 0; k < 4; ++k) to[i + k * kThreads] = grad_word<T, H>(w[k], c, h, g);
+        }
+        for (; i < in.words; i += kThreads) to[i] = grad_word<T, H>(*in.word(i), c, h, g);
+        if ((int)threadIdx.x < in.head + in.tail) {
+          const int at = in.edge(threadIdx.x);
+          out[at] = T::put(dense<H>(T::get(in.p[at]), c, h, g));
+        }
+      } else {
+        for (int i = threadIdx.x; i < n; i += kThreads) out[i] = T::put(dense<H>(T::get(in.p[i]), c, h, g));
       }
-      for (; i < in.words; i += kThreads) to[i] = grad_word<T>(*in.word(i), c, h, g);
-      if ((int)threadIdx.x < in.head + in.tail) {
-        const int at = in.edge(threadIdx.x);
-        out[at] = T::put(term(T::get(in.p[at]), c, h) * g);
-      }
-    } else {
-      for (int i = threadIdx.x; i < n; i += kThreads) out[i] = T::put(term(T::get(in.p[i]), c, h) * g);
-    }
+    };
+    if (h.huge) write(std::true_type{});
+    else write(std::false_type{});
     __syncthreads();
     write_entries<T, WAVES>(a, row, e, begin, n, h, g, wt);
   }
@@ -355,16 +540,26 @@ template <class T>
 hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
   const int most = parts_of(n, a.vocab);
   if (most == 1) {
-    distill_kernel<T, 16, false><<<n, 1024, 0, s>>>(a, 1, a.vocab, nullptr, nullptr);
+    const int words = a.vocab / T::kPer16;
+    if (a.grad == nullptr) {
+      if (words <= 2048) distill_row_kernel<T, 4, 8, 0, false><<<n, 256, 0, s>>>(a);
+      else distill_row_kernel<T, 8, 16, 0, false><<<n, 512, 0, s>>>(a);
+    } else if (words <= 2048) {
+      distill_row_kernel<T, 4, 8, 0, true><<<n, 256, 0, s>>>(a);
+    } else if (words <= 4096) {
+      distill_row_kernel<T, 8, 8, 0, true><<<n, 512, 0, s>>>(a);
+    } else {
+      distill_row_kernel<T, 8, 8, 8, true><<<n, 512, 0, s>>>(a);
+    }
     return hipGetLastError();
   }
   const int len = part_len(a.vocab, most), parts = (a.vocab + len - 1) / len;
   Stat *pairs = (Stat *)ws;
   float *zs = (float *)((char *)ws + pairs_bytes(n, a.vocab));
-  distill_kernel<T, 4, true><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
+  distill_part_kernel<T, 4, true><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  distill_kernel<T, 4, false><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
+  distill_part_kernel<T, 4, false><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
   return hipGetLastError();
 }
 
