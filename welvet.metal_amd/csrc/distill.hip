@@ -142,8 +142,7 @@ struct Entries {
   int index[kMaxEntries];
   float q[kMaxEntries];  // log q
   float z[kMaxEntries];  // the student's logit, read before its gradient may take its place
-  float wave[16];
-  int some;
+  float top[16], sum[16];  // by wave
 };
 template <class T>
 __device__ inline float logit(const Args &a, int row, int v) {
@@ -168,40 +167,32 @@ struct Teacher {
       }
     }
   }
-  // Fills e.index and e.q; *mass = the sum of q; false where the row has no entry.
+  // Fills e.index and e.q (each thread its own entries: a barrier follows before
+  // another reads them); *mass = the sum of q; false where the row has no entry.
   __device__ inline bool weigh(const Args &a, int row, Entries &e, float *mass) {
     const double inv = 1.0 / (double)a.temperature;
-    if (threadIdx.x == 0) e.some = 0;
-    __syncthreads();
     float top = -INFINITY;
 #pragma unroll
     for (int n = 0; n < kPer; ++n) {
       if (index[n] < 0 || index[n] >= a.vocab || l[n] == -INFINITY) index[n] = -1;
-      else top = fmaxf(top, l[n]), e.some = 1;
+      else top = fmaxf(top, l[n] == l[n] ? l[n] : INFINITY);  // NaN: an entry, and q NaN throughout
     }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if ((threadIdx.x & 63) == 0) e.top[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (!e.some) return false;
-    double most;
-    if (a.teacher_lse == nullptr) {
+    top = e.top[0];
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-      if ((threadIdx.x & 63) == 0) e.wave[threadIdx.x >> 6] = top;
-      __syncthreads();
-      top = e.wave[0];
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) top = fmaxf(top, e.wave[w]);
-      __syncthreads();
-      most = (double)top * inv;
-    } else {
-      most = (double)a.teacher_lse[row];
-    }
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, e.top[w]);
+    if (top == -INFINITY) return false;
+    const double most = a.teacher_lse == nullptr ? (double)top * inv : (double)a.teacher_lse[row];
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < kPer; ++n) {
       l[n] = (float)((double)l[n] * inv - most);
       if (index[n] >= 0) sum += expf(l[n]);
     }
-    sum = block_sum<WAVES>(sum, e.wave);
+    sum = block_sum<WAVES>(sum, e.sum);
     const float log_sum = a.teacher_lse == nullptr ? logf(sum) : 0.0f;
 #pragma unroll
     for (int n = 0; n < kPer; ++n) {
@@ -211,7 +202,6 @@ struct Teacher {
       e.q[i] = l[n] - log_sum;
     }
     *mass = a.teacher_lse == nullptr ? 1.0f : sum;
-    __syncthreads();
     return true;
   }
   // e.z, from zs (this row's logits at the entries) or the row itself.
@@ -322,9 +312,9 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
   float mass = 0.0f;
   Teacher<T, WAVES> teacher;
   uint4 held[HOLD];
+  teacher.load(a, row);
   bool live = weight != 0.0f;
   if (live) {
-    teacher.load(a, row);
     issued();
 #pragma unroll
     for (int r = 0; r < HOLD; ++r)
@@ -387,7 +377,7 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
     run.take(f, a.c);
   }
   const Stat st = block_join<WAVES>(run.stat(), a.c, lds);
-  if (a.loss) write_loss<WAVES>(a, row, e, st, weight);
+  if constexpr (!GRAD) write_loss<WAVES>(a, row, e, st, weight);
   if constexpr (GRAD) {
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
@@ -426,6 +416,7 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
     else write(std::false_type{});
     __syncthreads();
     write_entries<T, WAVES>(a, row, e, 0, n, h, g, wt);
+    if (a.loss) write_loss<WAVES>(a, row, e, st, weight);
   }
 }
 
@@ -435,7 +426,7 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
 //   else   the part's gradient, and by part 0 the loss
 template <class T, int WAVES, bool STATS>
 __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int parts, int len, Stat *pairs, float *zs) {
-  constexpr int kThreads = WAVES * 64;
+  constexpr int kThreads = WAVES * 64, kHeld = 4;
   __shared__ Stat lds[WAVES];
   const int row = blockIdx.x / parts, part = blockIdx.x % parts, begin = part * len;
   const int n = min(len, a.vocab - begin);
@@ -477,9 +468,18 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
     typename T::raw *out = a.grad ? (typename T::raw *)a.grad + (int64_t)row * a.gstride + begin : nullptr;
     float mass = 0.0f;
     Teacher<T, WAVES> teacher;
+    Stat st{-INFINITY, 0.0f};
+    uint4 held[kHeld];
+    teacher.load(a, row);
     bool live = weight != 0.0f;
-    if (live) {
-      teacher.load(a, row);
+    if (live) {  // all the block's first loads, then the teacher's arithmetic
+      if ((int)threadIdx.x < parts) st = pairs[(int64_t)row * parts + threadIdx.x];
+      if (out) {
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r)
+          if (r * kThreads < in.words) held[r] = *in.word(min(r * kThreads + (int)threadIdx.x, in.words - 1));
+      }
+      issued();
       live = teacher.weigh(a, row, e, &mass);
     }
     if (!live) {
@@ -488,11 +488,12 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
       return;
     }
     teacher.gather(a, row, zs + (int64_t)row * a.k, e);
-    Stat st{-INFINITY, 0.0f};
-    for (int i = threadIdx.x; i < parts; i += kThreads) st = join(st, pairs[(int64_t)row * parts + i], a.c);
+    for (int i = threadIdx.x + kThreads; i < parts; i += kThreads) st = join(st, pairs[(int64_t)row * parts + i], a.c);
     st = block_join<WAVES>(st, a.c, lds);
-    if (part == 0 && a.loss) write_loss<WAVES>(a, row, e, st, weight);
-    if (!out) return;
+    if (!out) {
+      if (part == 0) write_loss<WAVES>(a, row, e, st, weight);
+      return;
+    }
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
     const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
@@ -500,7 +501,12 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
       constexpr bool H = decltype(huge)::value;
       if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
         uint4 *to = (uint4 *)(out + in.head);
-        int i = threadIdx.x;
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+          const int i = r * kThreads + threadIdx.x;
+          if (i < in.words) to[i] = grad_word<T, H>(held[r], c, h, g);
+        }
+        int i = kHeld * kThreads + threadIdx.x;
         for (; i + 3 * kThreads < in.words; i += 4 * kThreads) {
           uint4 w[4];
 #pragma unroll
@@ -521,14 +527,16 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
     else write(std::false_type{});
     __syncthreads();
     write_entries<T, WAVES>(a, row, e, begin, n, h, g, wt);
+    if (part == 0 && a.loss) write_loss<WAVES>(a, row, e, st, weight);
   }
 }
 
 // Parts of a row: one where there are rows for every CU, else as many as give
-// each CU two blocks of at least 4096 values.
+// each CU two blocks, down to 1024 values (4 rows of 32000 f32 logits, loss and
+// gradient: parts of 4096 and up 12.0 us, of 1024 and up 10.9).
 int parts_of(int n, int vocab) {
   if (n == 0 || n >= 256) return 1;
-  return std::max(1, std::min((512 + n - 1) / n, vocab / 4096));
+  return std::max(1, std::min((512 + n - 1) / n, vocab / 1024));
 }
 int part_len(int vocab, int parts) { return ((vocab + parts - 1) / parts + 63) / 64 * 64; }
 size_t pairs_bytes(int n, int vocab) { return pad256((size_t)n * parts_of(n, vocab) * sizeof(Stat)); }
@@ -543,7 +551,7 @@ hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
     const int words = a.vocab / T::kPer16;
     if (a.grad == nullptr) {
       if (words <= 2048) distill_row_kernel<T, 4, 8, 0, false><<<n, 256, 0, s>>>(a);
-      else distill_row_kernel<T, 8, 16, 0, false><<<n, 512, 0, s>>>(a);
+      else distill_row_kernel<T, 8, 8, 0, false><<<n, 512, 0, s>>>(a);
     } else if (words <= 2048) {
       distill_row_kernel<T, 4, 8, 0, true><<<n, 256, 0, s>>>(a);
     } else if (words <= 4096) {
