@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
   // parts do not fit the registers beside more than 16 ranks
   constexpr bool SPLIT = SUMS && (std::is_same_v<T, BF16> || (std::is_same_v<T, F16> && RT == 1));
   using raw = typename T::raw;
-  __shared__ float red[kSliceWaves][16][RT * 16 + 1];
+  __shared__ float red[2][kSliceWaves][16][RT * 16 + 1];  // by tile: one barrier each
   __shared__ float4 turn4[SUMS ? kSliceWaves * 16 * kPitch / 4 : 1];
   __shared__ float hs[SUMS ? 2 : 1][16][RT * 16];
   __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) red[wave][4 * q + r][16 * t + lo] = acc[t][r];
+          for (int r = 0; r < 4; ++r) red[tile & 1][wave][4 * q + r][16 * t + lo] = acc[t][r];
         if constexpr (SUMS) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -444,10 +444,9 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
           const int i = e / (RT * 16), j = e % (RT * 16);
           float sum = 0.0f;
 #pragma unroll
-          for (int w = 0; w < kSliceWaves; ++w) sum += red[w][i][j];
+          for (int w = 0; w < kSliceWaves; ++w) sum += red[tile & 1][w][i][j];
           if (p + i < i1 && j < ranks) to_hidden[(int64_t)row_s[p + i - p0] * fac.rank + j] = j0 + j < ra ? sum : 0.0f;
         }
-        __syncthreads();
       };
       load_hidden(0);
       load(0, 0);
@@ -483,110 +482,96 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 // column]: lane l holds columns 4 (l % 16) + m of its wave's 64 for the m-th
 // of four accumulators, so a row's part is stored as 16-byte words; ranks 4
 // (l / 16) + s of each 16 for the s-th MFMA.  Block: four waves, 256 columns,
-// `per` tiles of 16 rows one after the other, the next tile's loads in flight,
-// the adapter's factor in registers as long as it stays the same.
-constexpr int kMaxPer = 4;
+// 16 rows, all of its loads in flight together.  Short blocks that pass the
+// rows in launch order keep HBM busier than longer ones with the next rows'
+// loads ahead (8192 x 4096 f32 read and written: 64 rows a block 5.3 TB/s, 128
+// rows 4.6), and the factor read again by each comes from L2.
 template <class T, int RT, bool NARROW>
 __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
                                                                 const float *__restrict__ hidden, const float *base,
-                                                                int64_t bstride, float *y, int64_t ystride, int per,
-                                                                bool nt) {
+                                                                int64_t bstride, float *y, int64_t ystride, bool nt) {
   using raw = typename T::raw;
-  __shared__ int row_s[kMaxPer * 16], key_s[kMaxPer * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
-  const Cols<NARROW> cols(blockIdx.x * 256 + wave * 64 + 4 * lo, fac.width);
-  const int p0 = blockIdx.y * per * 16, p1 = min(p0 + per * 16, rows.n);
-  for (int i = threadIdx.x; i < p1 - p0; i += 256) {
-    row_s[i] = rows.row(p0 + i);
-    key_s[i] = rows.adapter(p0 + i);
-  }
-  __syncthreads();
-  int held = -1;
+  const int across = (fac.width + 255) / 256;
+  const Cols<NARROW> cols(blockIdx.x % across * 256 + wave * 64 + 4 * lo, fac.width);
+  const int p0 = blockIdx.x / across * 16, live = min(16, rows.n - p0);
+  const int mine = rows.row(p0 + min(lo, live - 1)), key = rows.adapter(p0 + min(lo, live - 1));
+  int to[4];  // the rows this lane's accumulators belong to
+#pragma unroll
+  for (int r = 0; r < 4; ++r) to[r] = __shfl(mine, 4 * q + r);
   Quad<T> fv[RT][4];
-  const auto load_factor = [&](int a, int ra, int g) {  // rank rows past the adapter's: zeros
+  const auto load_factor = [&](int a, int ra, int g) {
     const raw *f = (const raw *)fac.p + (int64_t)a * fac.rank * fac.width;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         fv[t][s] = cols.template load<T>(f + (int64_t)min(g + 16 * t + 4 * q + s, ra - 1) * fac.width);
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (g + 16 * t + 4 * q + s >= ra) fv[t][s] = Quad<T>{};
   };
+  float4 hv[RT], bv[4];
+  const float *from = hidden + (int64_t)mine * fac.rank;
   const bool whole = fac.rank % 4 == 0;
-  const auto load_hidden = [&](float4 (&hv)[RT], int tile, int g) {
-    const float *from = hidden + (int64_t)row_s[min(16 * tile + lo, p1 - p0 - 1)] * fac.rank + g;
+  const auto load_hidden = [&](int g) {  // zeros past the rank
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int j = 16 * t + 4 * q;
-      if (whole) hv[t] = keep4(g + j < fac.rank, load4(from + (g + j < fac.rank ? j : 0), 0, 4));
-      else hv[t] = load4(from, j, fac.rank - g);
+      const int j = g + 16 * t + 4 * q;
+      hv[t] = whole ? load4(from + (j < fac.rank ? j : 0), 0, 4) : load4(from, j, fac.rank);
     }
   };
-  float4 hv[2][RT], bv[2][4];
-  const int tiles = (p1 - p0 + 15) / 16;
-  const auto load = [&](int d, int tile_) {
-    const int tile = min(tile_, tiles - 1);
-    load_hidden(hv[d], tile, 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {  // the rows this lane's accumulators belong to
-      bv[d][r] = make_float4(0, 0, 0, 0);
-      if (base) bv[d][r] = cols.load(base + (int64_t)row_s[min(16 * tile + 4 * q + r, p1 - p0 - 1)] * bstride);
-    }
-    issued();
+  int a = __builtin_amdgcn_readfirstlane(key), ra = 0;
+  float scale = 0.0f;
+  const auto begin = [&] {
+    ra = a < rows.count ? fac.rank_of(a) : 0;
+    scale = a < rows.count ? fac.scale_of(a) : 0.0f;
+    if (ra > 0) load_factor(a, ra, 0);
   };
-  const auto work = [&](int d, int tile) {
-    const int at = 16 * tile, live = min(16, p1 - p0 - at);
-    const int key = key_s[at + min(lo, live - 1)];
-    for (int i0 = 0; i0 < live;) {
-      const int a = __builtin_amdgcn_readlane(key, i0);
-      const uint64_t same = __ballot(lane < live && key == a);
-      const int i1 = i0 + __popcll(same >> i0);
-      if (a < rows.count) {
-        const int ra = fac.rank_of(a);
-        v4f acc[4] = {};
-        for (int g = 0; g < ra; g += 16 * RT) {
-          if (held != a || fac.rank > 16 * RT) load_factor(a, ra, g);
-          held = a;
+  begin();
+  load_hidden(0);
 #pragma unroll
-          for (int t = 0; t < RT; ++t)
+  for (int r = 0; r < 4; ++r) {
+    bv[r] = make_float4(0, 0, 0, 0);
+    if (base) bv[r] = cols.load(base + (int64_t)to[r] * bstride);
+  }
+  issued();
+  for (int i0 = 0;;) {
+    const uint64_t same = __ballot(lane < live && key == a);
+    const int i1 = i0 + __popcll(same >> i0);
+    if (ra > 0) {
+      v4f acc[4] = {};
+      for (int g = 0; g < ra; g += 16 * RT) {
+        if (g > 0) {
+          load_factor(a, ra, g);
+          load_hidden(g);
+        }
 #pragma unroll
-            for (int s = 0; s < 4; ++s) fv[t][s].pin();
-          if (g > 0) load_hidden(hv[d], tile, g);
+        for (int t = 0; t < RT; ++t) {
+          if (16 * t >= ra - g) break;
+          const int j = g + 16 * t + 4 * q;
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            if (16 * t >= ra - g) break;
+          for (int s = 0; s < 4; ++s) {
+            // rank rows past the adapter's are not its: zeros on both sides
+            const float h = j + s < ra ? get4(hv[t], s) : 0.0f;
+            const float4 f = keep4(j + s < ra, fv[t][s].floats());
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-              for (int m = 0; m < 4; ++m) acc[m] = mfma(get4(hv[d][t], s), fv[t][s].get(m), acc[m]);
+            for (int m = 0; m < 4; ++m) acc[m] = mfma(h, get4(f, m), acc[m]);
           }
         }
-        if (fac.rank > 16 * RT && i1 < live) load_hidden(hv[d], tile, 0);  // for the tile's next adapter
-        const float scale = fac.scale_of(a);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (4 * q + r >= i0 && 4 * q + r < i1)
-            bv[d][r] = fma4(scale, make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]), bv[d][r]);
       }
-      i0 = i1;
-    }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)row_s[at + 4 * q + r] * ystride, bv[d][r], nt);
-  };
-  load(0, 0);
-  int tile = 0;
-  for (; tile + 1 < tiles; tile += 2) {
-    load(1, tile + 1);
-    work(0, tile);
-    load(0, tile + 2);
-    work(1, tile + 1);
+      for (int r = 0; r < 4; ++r)
+        if (4 * q + r >= i0 && 4 * q + r < i1)
+          bv[r] = fma4(scale, make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]), bv[r]);
+    }
+    if (i1 >= live) break;
+    const bool again = ra > 16 * RT;  // hv holds a later group
+    i0 = i1;
+    a = __builtin_amdgcn_readlane(key, i0);
+    begin();
+    if (again) load_hidden(0);
   }
-  if (tile < tiles) work(0, tile);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)to[r] * ystride, bv[r], nt);
 }
 
 // The same for few rows: a block one row's 1024 columns, four a thread, the
@@ -637,20 +622,26 @@ struct Sums {
   int count;
 };
 template <bool ACC, int RT, bool NARROW>
-__global__ void __launch_bounds__(256, 4) outer_kernel(RowMap rows, Factor fac, Sums sums) {
+__global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) outer_kernel(RowMap rows, Factor fac, Sums sums) {
   constexpr int DEPTH = RT >= 4 ? 4 : 8;
-  __shared__ int row_s[kMaxChunk], key_s[kMaxChunk];
+  __shared__ float4 half_s[RT][4][256];
+  // the rows' offsets: a 64-bit product for each load costs as much as its MFMAs
+  __shared__ int64_t x_s[kMaxChunk];
+  __shared__ int h_s[kMaxChunk], key_s[kMaxChunk];
   const bool second = (int)blockIdx.x >= sums.of[0].across;
   const Sum &job = sums.of[second ? 1 : 0];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), lo = lane & 15, q = lane >> 4;
   const int across = (int)blockIdx.x - (second ? sums.of[0].across : 0);
   const int j0 = blockIdx.z * RT * 16;
   const int width = job.width, chunk = job.chunk, p0 = (int)blockIdx.y * chunk;
   if (p0 >= rows.n) return;
   const Cols<NARROW> cols(across * 256 + wave * 64 + 4 * lo, width);
   const int p1 = min(p0 + chunk, rows.n);
-  for (int i = threadIdx.x; i < p1 - p0; i += 256) {
-    row_s[i] = rows.row(p0 + i);
+  for (int i = threadIdx.x; i < p1 - p0; i += 512) {
+    const int row = rows.row(p0 + i);
+    x_s[i] = row * job.xstride;
+    h_s[i] = row * fac.rank;
     key_s[i] = rows.adapter(p0 + i);
   }
   __syncthreads();
@@ -668,17 +659,18 @@ __global__ void __launch_bounds__(256, 4) outer_kernel(RowMap rows, Factor fac, 
     const int ra = fac.rank_of(a);
     v4f acc[RT][4] = {};
     if (ra > j0) {
-      const int steps = (i1 - i0 + 3) / 4;
+      const int steps = (i1 - i0 + 7) / 8;  // of this half, every second four rows
       const float *hcol[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) hcol[t] = job.hidden + min(j0 + 16 * t + lo, ra - 1);
       float4 xv[DEPTH];
       float hv[DEPTH][RT];
-      const auto load = [&](int d, int step) {  // steps past the last repeat its last row
-        const int64_t row = row_s[min(i0 + 4 * step + q, i1 - 1) - p0];
-        xv[d] = cols.load(job.x + row * job.xstride);
+      const auto load = [&](int d, int step) {  // rows past the last repeat it
+        const int at = min(i0 + 8 * step + 4 * half + q, i1 - 1) - p0;
+        xv[d] = cols.load(job.x + x_s[at]);
+        const int h = h_s[at];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) hv[d][t] = hcol[t][row * fac.rank];
+        for (int t = 0; t < RT; ++t) hv[d][t] = hcol[t][h];
         issued();
       };
 #pragma unroll
@@ -687,20 +679,40 @@ __global__ void __launch_bounds__(256, 4) outer_kernel(RowMap rows, Factor fac, 
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
           if (step + d < steps) {
-            const bool on = i0 + 4 * (step + d) + q < i1;
-            const float4 xs = keep4(on, xv[d]);
+            if (i0 + 8 * (step + d) + 8 > i1) {  // the run's end: no rows past it
+              const bool on = i0 + 8 * (step + d) + 4 * half + q < i1;
+              xv[d] = keep4(on, xv[d]);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-              const float hs = on ? hv[d][t] : 0.0f;
-#pragma unroll
-              for (int m = 0; m < 4; ++m) acc[t][m] = mfma(hs, get4(xs, m), acc[t][m]);
+              for (int t = 0; t < RT; ++t) hv[d][t] = on ? hv[d][t] : 0.0f;
             }
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+              for (int m = 0; m < 4; ++m) acc[t][m] = mfma(hv[d][t], get4(xv[d], m), acc[t][m]);
           }
           load(d, step + d + DEPTH);
         }
       }
     }
-    store_sums<ACC>(acc, fac, a, ra, j0, q, cols, began, goes_on, job);
+    // the second half's sums on top of the first's
+    if (half == 1)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          half_s[t][m][threadIdx.x - 256] = make_float4(acc[t][m][0], acc[t][m][1], acc[t][m][2], acc[t][m][3]);
+    __syncthreads();
+    if (half == 0) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float4 v = half_s[t][m][threadIdx.x];
+          acc[t][m] += v4f{v.x, v.y, v.z, v.w};
+        }
+      store_sums<ACC>(acc, fac, a, ra, j0, q, cols, began, goes_on, job);
+    }
+    __syncthreads();
     i0 = i1;
   }
 }
@@ -861,16 +873,12 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
     return hipGetLastError();
   }
   by_rank(fac.rank, [&](auto rt) {
-    const int tiles = (c.rows.n + 15) / 16, across = (fac.width + 255) / 256;
-    // four tiles a block at most: blocks that pass the rows in launch order keep
-    // HBM at 5.3 TB/s, with eight tiles 4.6 (8192 x 4096 f32 read and written)
-    const int per = std::max(1, std::min<int>(kMaxPer, (int64_t)tiles * across / 1024));
+    const int64_t grid = (int64_t)((fac.width + 255) / 256) * ((c.rows.n + 15) / 16);
     const bool nt = (int64_t)c.rows.n * fac.width * 4 > kKept;
-    const dim3 grid(across, (tiles + per - 1) / per);
     with_type(c.dtype, [&](auto t) {
       by_flag(fac.width < 4, [&](auto narrow) {
         up_kernel<decltype(t), decltype(rt)::value, decltype(narrow)::value>
-            <<<grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, per, nt);
+            <<<(uint32_t)grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, nt);
       });
     });
   });
@@ -895,7 +903,7 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
     const dim3 grid(across, chunks, (fac.rank + 16 * RT - 1) / (16 * RT));
     by_flag(accumulate, [&](auto acc) {
       by_flag(narrow, [&](auto nar) {
-        outer_kernel<decltype(acc)::value, RT, decltype(nar)::value><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
+        outer_kernel<decltype(acc)::value, RT, decltype(nar)::value><<<grid, 512, 0, c.s>>>(c.rows, fac, sums);
       });
     });
   });
@@ -944,7 +952,7 @@ Sizes sizes_of(const welvet_hip_adapters &d, int n, bool backward) {
 }
 
 bool desc_ok(const welvet_hip_adapters *d, int32_t n) {
-  return d && n >= 0 && n <= (1 << 23) && d->count > 0 && d->count <= 65535 && d->rank > 0 && d->rank <= kMaxRank &&
+  return d && n >= 0 && n <= (1 << 23) && (int64_t)n * d->rank <= INT32_MAX && d->count > 0 && d->count <= 65535 && d->rank > 0 && d->rank <= kMaxRank &&
          d->in > 0 && d->out > 0 && (int64_t)d->rank * std::max(d->in, d->out) <= INT32_MAX / 2;
 }
 

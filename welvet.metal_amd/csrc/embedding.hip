@@ -83,26 +83,30 @@ constexpr int kDirect = 256;
 // More: rows in the tokens' order, kRun of them a block and column tile.  A
 // token whose rows end inside the block's is written from registers; one that
 // reaches into a neighbour's leaves a partial row (slot 0: began earlier,
-// slot 1: goes on), and join_kernel adds those up, in order.
+// slot 1: goes on), and finish_kernel adds those up, in order.
 constexpr int kRun = 32;
-constexpr int kZeroRows = 8;  // table rows of a zeroing block
+constexpr int kZeroRows = 4;  // table rows of a zeroing block
 
 template <bool ACC, bool NARROW>
-__device__ inline void put_row(const Cols<NARROW> &cols, float *row, const float4 &sum, float scale) {
+__device__ inline void put_row(const Cols<NARROW> &cols, float *row, const float4 &sum, float scale, bool nt) {
   float4 v = mul4(sum, scale);
   if constexpr (ACC) v = add4(cols.load(row), v);
-  cols.store(row, v);
+  cols.store(row, v, nt);
 }
 
-__device__ inline void zero_row(float *row, int dim) {
-  for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) store4(row, c, dim, make_float4(0, 0, 0, 0));
+__device__ inline void zero_row(float *row, int dim, bool nt) {
+  const float4 zero = make_float4(0, 0, 0, 0);
+  for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) {
+    if (nt && c + 4 <= dim) store4_nt(row + c, zero);
+    else store4(row, c, dim, zero);
+  }
 }
 
 template <bool ACC, bool NARROW>
 __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__ tokens, int n, uint32_t vocab,
                                                      int dim, const float *__restrict__ dout, int64_t dstride,
                                                      float scale, float *__restrict__ dtable, int64_t tstride,
-                                                     int tiles) {
+                                                     int tiles, bool nt) {
   __shared__ int32_t tok_s[kDirect];
   __shared__ int rows_s[kDirect];
   __shared__ int count_s;
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     }
     __syncthreads();
     for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim);
+      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim, nt);
     return;
   }
   if (threadIdx.x == 0) count_s = 0;
@@ -154,7 +158,7 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
   }
   for (; r < count; ++r) sum = add4(sum, cols.load(dout + (int64_t)rows_s[r] * dstride));
-  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale, nt);
 }
 
 template <bool ACC, bool NARROW>
@@ -162,19 +166,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
                                                    const int32_t *__restrict__ order, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ dout, int64_t dstride, float scale,
                                                    float *__restrict__ dtable, int64_t tstride,
-                                                   float *__restrict__ part, int tiles, int adders) {
-  if ((int)blockIdx.x >= adders) {
-    __shared__ int named[kZeroRows];
-    const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)adders) * kZeroRows;
-    for (uint32_t d = threadIdx.x >> 6; d < kZeroRows; d += blockDim.x >> 6) {  // a wave a row
-      const int at = first_at_least(skey, n, (int32_t)min(v0 + d, vocab));
-      if ((threadIdx.x & 63) == 0) named[d] = at < n && (uint32_t)skey[at] == v0 + d;
-    }
-    __syncthreads();
-    for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim);
-    return;
-  }
+                                                   float *__restrict__ part, int tiles, bool nt) {
   __shared__ int32_t key_s[kRun + 2];  // with the neighbours' nearest
   __shared__ int32_t row_s[kRun];
   const int chunk = blockIdx.x / tiles, p0 = chunk * kRun;
@@ -194,7 +186,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
     if ((uint32_t)cur >= vocab) return;  // padding, or past the last row
     if (!began) cols.store(part + (int64_t)(2 * chunk) * dim, sum);
     else if (goes_on) cols.store(part + (int64_t)(2 * chunk + 1) * dim, sum);
-    else put_row<ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale);
+    else put_row<ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale, nt);
   };
 #pragma unroll 1
   for (int r0 = 0; r0 < kRun; r0 += 8) {
@@ -220,11 +212,26 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
 }
 
 // Tokens whose rows fill more than one block's: the block where one begins
-// adds its later blocks' slot 0 to its own slot 1, in order.
+// adds its later blocks' slot 0 to its own slot 1, in order.  The blocks after
+// those write the rows without a token, under whose stores the joins' waits
+// lie (32000 x 4096, 16384 tokens: 11 us less than a launch of its own).
 template <bool ACC, bool NARROW>
-__global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ skey, int n, uint32_t vocab, int dim,
+__global__ void __launch_bounds__(256) finish_kernel(const int32_t *__restrict__ skey, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ part, float scale,
-                                                   float *__restrict__ dtable, int64_t tstride, int tiles) {
+                                                   float *__restrict__ dtable, int64_t tstride, int tiles, int joins,
+                                                   bool nt) {
+  if ((int)blockIdx.x >= joins) {
+    __shared__ int named[kZeroRows];
+    const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)joins) * kZeroRows;
+    for (uint32_t d = threadIdx.x >> 5; d < kZeroRows; d += blockDim.x >> 5) {  // half a wave a row
+      const int at = first_by_half(skey, n, (int32_t)min(v0 + d, vocab));
+      if ((threadIdx.x & 31) == 0) named[d] = at < n && (uint32_t)skey[at] == v0 + d;
+    }
+    __syncthreads();
+    for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
+      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim, nt);
+    return;
+  }
   const int chunk = blockIdx.x / tiles, p0 = chunk * kRun, p1 = p0 + kRun;
   if (p1 >= n) return;
   const int32_t mine = skey[p1 - 1];
@@ -235,15 +242,15 @@ __global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ s
   if (!cols.any()) return;
   float4 sum = cols.load(part + (int64_t)(2 * chunk + 1) * dim);
   int b = chunk + 1;
-  for (; b + 4 <= last + 1; b += 4) {
-    float4 v[4];
+  for (; b + 8 <= last + 1; b += 8) {
+    float4 v[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = cols.load(part + (int64_t)(2 * (b + k)) * dim);
+    for (int k = 0; k < 8; ++k) v[k] = cols.load(part + (int64_t)(2 * (b + k)) * dim);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
+    for (int k = 0; k < 8; ++k) sum = add4(sum, v[k]);
   }
   for (; b <= last; ++b) sum = add4(sum, cols.load(part + (int64_t)(2 * b) * dim));
-  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale);
+  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale, nt);
 }
 
 int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
@@ -258,23 +265,24 @@ template <bool ACC, bool NARROW>
 hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, float scale, const float *dout,
                            int64_t dstride, float *dtable, int64_t tstride, void *ws, hipStream_t s) {
   const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
+  const bool nt = (int64_t)vocab * dim * 4 > kKept;
   const int64_t zeros = ACC ? 0 : ((int64_t)vocab + kZeroRows - 1) / kZeroRows;
   if (n <= kDirect) {
     if (n == 0 && ACC) return hipSuccess;
     direct_kernel<ACC, NARROW><<<(uint32_t)((int64_t)n * tiles + zeros), threads, 0, s>>>(
-        tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles);
+        tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles, nt);
     return hipGetLastError();
   }
   Order o;
   hipError_t e = launch_order(tokens, n, vocab, ws, &o, s);
   if (e != hipSuccess) return e;
   float *part = (float *)((char *)ws + order_bytes(n));
-  const int64_t chunks = ((int64_t)n + kRun - 1) / kRun, adders = chunks * tiles;
-  sums_kernel<ACC, NARROW><<<(uint32_t)(adders + zeros), threads, 0, s>>>(
-      o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, part, tiles, (int)adders);
+  const int64_t chunks = ((int64_t)n + kRun - 1) / kRun, blocks = chunks * tiles;
+  sums_kernel<ACC, NARROW><<<(uint32_t)blocks, threads, 0, s>>>(o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride,
+                                                               scale, dtable, tstride, part, tiles, nt);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  join_kernel<ACC, NARROW><<<(uint32_t)adders, threads, 0, s>>>(o.skey, n, (uint32_t)vocab, dim, part, scale, dtable,
-                                                            tstride, tiles);
+  finish_kernel<ACC, NARROW><<<(uint32_t)(blocks + zeros), threads, 0, s>>>(
+      o.skey, n, (uint32_t)vocab, dim, part, scale, dtable, tstride, tiles, (int)blocks, nt);
   return hipGetLastError();
 }
 

@@ -270,15 +270,14 @@ static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__res
   }
 }
 
-// The first places of the sorted keys whose keys are >= v and >= v + 1: the
-// rows of key v.  A whole wave calls it, each half looking at 32 places a time.
-__device__ inline int2 rows_of(const int32_t *__restrict__ skey, int n, int32_t v) {
+// The first place of the sorted keys whose key is >= v, for each half of a wave
+// its own v; the whole wave calls it, each half looking at 32 places a time.
+__device__ inline int first_by_half(const int32_t *__restrict__ skey, int n, int32_t v) {
   const int lane = threadIdx.x & 31;
-  const int32_t mine = v + ((threadIdx.x & 32) ? 1 : 0);
   int lo = 0, hi = n;
   while (__any(lo < hi)) {
     const int step = (hi - lo + 31) / 32, p = lo + lane * step;
-    const uint64_t both = __ballot(lo < hi && p < hi && skey[p] < mine);
+    const uint64_t both = __ballot(lo < hi && p < hi && skey[p] < v);
     const int below = __popc((threadIdx.x & 32) ? (uint32_t)(both >> 32) : (uint32_t)both);
     if (below == 0) {
       hi = lo;
@@ -287,6 +286,11 @@ __device__ inline int2 rows_of(const int32_t *__restrict__ skey, int n, int32_t 
       lo = lo + (below - 1) * step + 1;
     }
   }
+  return lo;
+}
+// The sorted rows of key v, from .x up to .y; a whole wave calls it.
+__device__ inline int2 rows_of(const int32_t *__restrict__ skey, int n, int32_t v) {
+  const int lo = first_by_half(skey, n, v + ((threadIdx.x & 32) ? 1 : 0));
   return {__builtin_amdgcn_readlane(lo, 0), __builtin_amdgcn_readlane(lo, 32)};
 }
 
