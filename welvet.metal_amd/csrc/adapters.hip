@@ -28,7 +28,6 @@ using v4f = __attribute__((ext_vector_type(4))) float;
 __device__ inline v4f mfma(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 constexpr int kMaxRank = 256;
-constexpr int kFewRows = 128;  // a block a row up to here
 
 // The rows of a launch: position p -> row and adapter (count: none).
 struct RowMap {
@@ -55,78 +54,83 @@ struct Hidden {
   int splits, n, rank;
   __device__ float at(int row, int j) const {
     const float *q = p + (int64_t)row * rank + j;
+    const int64_t step = (int64_t)n * rank;
     float v = q[0];
-    for (int s = 1; s < splits; ++s) v += q[(int64_t)s * n * rank];
+    for (int s = 1; s < splits; s += 8) {  // eight loads in flight
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = q[min(s + i, splits - 1) * step];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v = s + i < splits ? v + w[i] : v;
+    }
+    return v;
+  }
+  // Four neighbouring ones, zeros past the rank.
+  __device__ float4 at4(int row, int j) const {
+    if (rank % 4 != 0) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = j + i < rank ? at(row, j + i) : 0.0f;
+      return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    if (j >= rank) return make_float4(0, 0, 0, 0);
+    const float *q = p + (int64_t)row * rank + j;
+    const int64_t step = (int64_t)n * rank;
+    float4 v = load4(q, 0, 4);
+    for (int s = 1; s < splits; s += 4) {
+      float4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = load4(q + min(s + i, splits - 1) * step, 0, 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v = s + i < splits ? add4(v, w[i]) : v;
+    }
     return v;
   }
 };
 
 // --------------------------------------------------------- rows by a factor
 // hidden[split][row][j] = sum over the split's k of x[row][k] factor_a[j][k].
-// D[i = row][j = rank] of 16 x 16 x 4 MFMAs: lane l holds row (or rank) l % 16,
-// and four lanes l / 16 share its k.  Rank rows past the adapter's repeat its
-// last one and are dropped at the end.
 //
-// Few rows: a block one row and a split of the width, where the MFMA's 16 rows
-// are the same one (what is read counts, not what is multiplied).  A wave's
-// step is 64 k, 16 (l / 16) + s for the s-th of sixteen MFMAs: whole 128-byte
-// lines of every rank row.  The block's waves take the steps in turn, the next
-// one's loads in flight, and add up in LDS.
-constexpr int kDownWaves = 8;
-constexpr int kStep = 64;
-// 16 neighbouring factor values
-template <class T>
-struct Hex {
-  static constexpr int kWords = (int)sizeof(typename T::raw);
-  uint4 v[kWords];
-  __device__ inline void load(const typename T::raw *p) {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) __builtin_memcpy(&v[i], p + i * T::kPer16, 16);
-  }
-  __device__ inline float get(int s) const {
-    const uint4 &w = v[s / T::kPer16];
-    const int e = s % T::kPer16;
-    const int at = e * (int)sizeof(typename T::raw) / 4;
-    const uint32_t word = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
-    if constexpr (sizeof(typename T::raw) == 4) return T::get(word);
-    else return T::get((uint16_t)(word >> (16 * (e & 1))));
-  }
-};
-template <class T, int RT>
+// Few rows: a block one row, R ranks and a split of the width.  What is read
+// counts here, and every lane reads its own: four neighbouring k of x and of
+// each rank row, 256 k a wave's step, the block's waves in turn with the next
+// step's loads in flight.  (Lanes of an MFMA would share an x value sixteen
+// times and load it as often: f32 2048x8192 rank 8 n256 DOWNOLD -> DOWNNEW us.)
+// A rank's 64 lane sums are folded so that each exchange halves the values.
+// Rank rows past the adapter's repeat its last one and are dropped at the end.
+constexpr int kDownWaves = 4;
+constexpr int kStep = 256;
+template <class T, int R>
 __global__ void __launch_bounds__(kDownWaves * 64) down_row_kernel(RowMap rows, Factor fac,
                                                                    const float *__restrict__ x, int64_t xstride,
                                                                    Hidden out, int split_len) {
   using raw = typename T::raw;
-  __shared__ float red[kDownWaves][RT * 16];
+  __shared__ float red[kDownWaves][R];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lo = lane & 15, q = lane >> 4;
-  const int row = blockIdx.x, j0 = blockIdx.z * RT * 16;
+  const int row = blockIdx.x, j0 = blockIdx.z * R;
   const int kbegin = blockIdx.y * split_len, kend = min(kbegin + split_len, fac.width);
   const int first = kbegin + wave * kStep;
   const int full = first + kStep <= kend ? (kend - first - kStep) / (kDownWaves * kStep) + 1 : 0;  // whole steps
   const float *xrow = x + (int64_t)row * xstride;
-  const int a = rows.adapter(row), ra = a < rows.count ? fac.rank_of(a) : 0;
+  const int a = __builtin_amdgcn_readfirstlane(rows.adapter(row)), ra = a < rows.count ? fac.rank_of(a) : 0;
   if (ra > j0) {
-    v4f acc[RT] = {};
-    const raw *frow[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-      frow[t] = (const raw *)fac.p + ((int64_t)a * fac.rank + min(j0 + t * 16 + lo, ra - 1)) * fac.width;
-    float4 xv[2][4];
-    Hex<T> fv[2][RT];
+    float acc[R] = {};
+    const raw *f = (const raw *)fac.p + ((int64_t)a * fac.rank + j0) * fac.width;
+    const int last = min(R, ra - j0) - 1;
+    Quad<F32> xv[2];
+    Quad<T> fv[2][R];
     const auto load = [&](int d, int step) {
-      const int k = first + min(step, full - 1) * (kDownWaves * kStep) + 16 * q;
+      const int k = first + min(step, full - 1) * (kDownWaves * kStep) + 4 * lane;
+      xv[d] = Quad<F32>::load((const uint32_t *)xrow + k);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) __builtin_memcpy(&xv[d][m], xrow + k + 4 * m, 16);
-#pragma unroll
-      for (int t = 0; t < RT; ++t) fv[d][t].load(frow[t] + k);
+      for (int j = 0; j < R; ++j) fv[d][j] = Quad<T>::load(f + (int64_t)min(j, last) * fac.width + k);
       issued();
     };
     const auto multiply = [&](int d) {
 #pragma unroll
-      for (int s = 0; s < 16; ++s)
+      for (int j = 0; j < R; ++j)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = mfma(get4(xv[d][s / 4], s & 3), fv[d][t].get(s), acc[t]);
+        for (int m = 0; m < 4; ++m) acc[j] = fmaf(xv[d].get(m), fv[d][j].get(m), acc[j]);
     };
     if (full > 0) {
       // no condition between a load and its use: the compiler would move the
@@ -142,25 +146,33 @@ __global__ void __launch_bounds__(kDownWaves * 64) down_row_kernel(RowMap rows, 
     }
     const int k = first + full * (kDownWaves * kStep);  // the rest of the width, one wave's
     if (k < kend) {
-#pragma unroll 1
-      for (int s = 0; s < kStep; s += 16) {
-        const float4 xs = load4(xrow, k + s + 4 * q, kend);
-        float4 fs[RT];
+      const Quad<F32> xs = Quad<F32>::load((const uint32_t *)xrow, k + 4 * lane, kend);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) fs[t] = Quad<T>::load(frow[t], k + s + 4 * q, kend).floats();
+      for (int j = 0; j < R; ++j) {
+        const Quad<T> fs = Quad<T>::load(f + (int64_t)min(j, last) * fac.width, k + 4 * lane, kend);
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-          for (int t = 0; t < RT; ++t) acc[t] = mfma(get4(xs, m), get4(fs[t], m), acc[t]);
+        for (int m = 0; m < 4; ++m) acc[j] = fmaf(xs.get(m), fs.get(m), acc[j]);
       }
     }
-    if (q == 0)
+    int own = 0;  // the rank whose sum the lane ends with
 #pragma unroll
-      for (int t = 0; t < RT; ++t) red[wave][t * 16 + lo] = acc[t][0];
+    for (int half = R / 2, mask = 32, bit = 1; half > 0; half /= 2, mask /= 2, bit *= 2) {
+      const bool upper = lane & mask;
+      own += upper ? bit : 0;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float mine = upper ? acc[2 * i + 1] : acc[2 * i], other = upper ? acc[2 * i] : acc[2 * i + 1];
+        acc[i] = mine + __shfl_xor(other, mask);
+      }
+    }
+    float sum = acc[0];
+#pragma unroll
+    for (int mask = 32 / R; mask > 0; mask /= 2) sum += __shfl_xor(sum, mask);
+    if ((lane & (64 / R - 1)) == 0) red[wave][own] = sum;
   }
   __syncthreads();
   const int j = threadIdx.x;
-  if (j < min(RT * 16, fac.rank - j0)) {
+  if (j < min(R, fac.rank - j0)) {
     float sum = 0.0f;
     if (j0 + j < ra)
 #pragma unroll
@@ -574,41 +586,58 @@ __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Fa
     if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)to[r] * ystride, bv[r], nt);
 }
 
-// The same for few rows: a block one row's 1024 columns, four a thread, the
-// hidden values from LDS, rank by rank with eight factor loads ahead.
+// The same for few rows: a block one row's columns, four a thread, the hidden
+// values (added up from their splits) from LDS, rank by rank with eight to
+// sixteen factor loads ahead.
+template <class T, bool NARROW>
+__device__ inline void spread_row(const RowMap &rows, const Factor &fac, const Hidden &h, const float *base,
+                                  int64_t bstride, float *y, int64_t ystride, float *hsum, int row, int c0,
+                                  float (&hs)[kMaxRank]) {
+  const int a = rows.adapter(row);
+  const Cols<NARROW> cols(c0, fac.width);
+  const int ra = a < rows.count ? fac.rank_of(a) : 0;
+  const typename T::raw *f = (const typename T::raw *)fac.p + (int64_t)(ra > 0 ? a : 0) * fac.rank * fac.width;
+  float4 sum = make_float4(0, 0, 0, 0);
+  Quad<T> v[2][8];
+  const auto load = [&](Quad<T> (&to)[8], int j0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to[j] = cols.template load<T>(f + (int64_t)max(min(j0 + j, ra - 1), 0) * fac.width);
+    issued();
+  };
+  if (base && cols.any()) sum = cols.load(base + (int64_t)row * bstride);
+  if (ra > 0) load(v[0], 0);
+  if ((int)threadIdx.x < fac.rank) {
+    const float at = h.at(row, threadIdx.x);
+    hs[threadIdx.x] = at;
+    if (hsum) hsum[(int64_t)row * fac.rank + threadIdx.x] = at;
+  }
+  __syncthreads();
+  if (ra > 0) {
+    float4 acc = make_float4(0, 0, 0, 0);
+    const auto add = [&](const Quad<T> (&from)[8], int j0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= ra) break;
+        acc = fma4(hs[j0 + j], from[j].floats(), acc);
+      }
+    };
+    for (int j0 = 0; j0 < ra; j0 += 16) {
+      load(v[1], j0 + 8);
+      add(v[0], j0);
+      load(v[0], j0 + 16);
+      add(v[1], j0 + 8);
+    }
+    sum = fma4(fac.scale_of(a), acc, sum);
+  }
+  if (cols.any()) cols.store(y + (int64_t)row * ystride, sum);
+}
 template <class T, bool NARROW>
 __global__ void __launch_bounds__(256) up_row_kernel(RowMap rows, Factor fac, Hidden h, const float *base,
                                                      int64_t bstride, float *y, int64_t ystride,
                                                      float *__restrict__ hsum) {
   __shared__ float hs[kMaxRank];
-  const int row = blockIdx.y, a = rows.adapter(row);
-  const Cols<NARROW> cols(blockIdx.x * 1024 + 4 * threadIdx.x, fac.width);
-  const int ra = a < rows.count ? fac.rank_of(a) : 0;
-  if ((int)threadIdx.x < fac.rank) {
-    const float v = h.at(row, threadIdx.x);
-    hs[threadIdx.x] = v;
-    if (hsum && blockIdx.x == 0) hsum[(int64_t)row * fac.rank + threadIdx.x] = v;
-  }
-  float4 sum = make_float4(0, 0, 0, 0);
-  if (base && cols.any()) sum = cols.load(base + (int64_t)row * bstride);
-  __syncthreads();
-  if (!cols.any()) return;
-  if (ra > 0) {
-    const typename T::raw *f = (const typename T::raw *)fac.p + (int64_t)a * fac.rank * fac.width;
-    float4 acc = make_float4(0, 0, 0, 0);
-    for (int j0 = 0; j0 < ra; j0 += 8) {
-      Quad<T> v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = cols.template load<T>(f + (int64_t)min(j0 + j, ra - 1) * fac.width);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j0 + j >= ra) break;
-        acc = fma4(hs[j0 + j], v[j].floats(), acc);
-      }
-    }
-    sum = fma4(fac.scale_of(a), acc, sum);
-  }
-  cols.store(y + (int64_t)row * ystride, sum);
+  spread_row<T, NARROW>(rows, fac, h, base, bstride, y, ystride, blockIdx.x == 0 ? hsum : nullptr, blockIdx.y,
+                        blockIdx.x * 1024 + 4 * threadIdx.x, hs);
 }
 
 // ------------------------------------------------ sums over an adapter's rows
@@ -767,10 +796,139 @@ __global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, Sums 
   }
 }
 
+// ------------------------------------------------------ few rows, backward
+// Everything that follows from g of few rows, in one launch: blocks that sum
+// one adapter's rows into some columns of a gradient (its rows found by a scan
+// of all ids, in their order; the terms as in outer_kernel; zeros where no row
+// is the adapter's), then blocks that each spread one row's g over 2048 columns
+// of dx.  A wave sums 64 columns of 32 rows; `parts` of a block's eight share
+// columns and add up in LDS: two where adapters are many, more for long runs of
+// few adapters, whose blocks alone would not fill the CUs.
+constexpr int kFewRows = 2048;       // rows at most
+constexpr int kFewAcross = 1 << 20;  // blocks in the grid's x: 2^32 threads at most
+struct FewSum {
+  Hidden h;
+  const float *x;
+  int64_t xstride;
+  int width, across, first;  // across: blocks along the width; first: blocks before its own
+  float *grad;
+};
+struct FewSums {
+  FewSum of[2];
+  int count, parts;
+  int blocks, total, groups;  // total: with the rows' blocks; groups: of 16 RT ranks
+};
+template <class T, int RT, bool ACC, bool NARROW>
+__global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) few_kernel(RowMap rows, Factor fac, FewSums sums, Hidden g,
+                                                                 const float *base, int64_t bstride, float *dx,
+                                                                 int64_t dxstride) {
+  constexpr int kPitch = RT * 16;
+  // the hidden values of 256 rows, later the sums of half the waves
+  __shared__ float4 both_s[RT * 1024];
+  float *const hs = (float *)both_s;
+  __shared__ int list[kFewRows], found[8];
+  __shared__ float spread_s[kMaxRank];
+  int block = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+  if (block >= sums.total) return;
+  if (block >= sums.blocks) {
+    block -= sums.blocks;
+    const int across = (fac.width + 2047) / 2048;
+    spread_row<T, NARROW>(rows, fac, g, base, bstride, dx, dxstride, nullptr, block / across,
+                          block % across * 2048 + 4 * threadIdx.x, spread_s);
+    return;
+  }
+  const bool second = sums.count > 1 && block >= sums.of[1].first;
+  const FewSum &job = sums.of[second ? 1 : 0];
+  block -= job.first;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = 8 / sums.parts, part = wave / waves, lo = lane & 15, q = lane >> 4;
+  const int a = block / (job.across * sums.groups), j0 = block / job.across % sums.groups * RT * 16;
+  const Cols<NARROW> cols((block % job.across * waves + wave % waves) * 64 + 4 * lo, job.width);
+  const int ra = fac.rank_of(a);
+  int total = 0;
+  for (int r0 = 0; r0 < rows.n; r0 += 512) {
+    const int row = r0 + threadIdx.x;
+    const bool mine = row < rows.n && rows.adapter(row) == a;
+    const uint64_t same = __ballot(mine);
+    if (lane == 0) found[wave] = __popcll(same);
+    __syncthreads();
+    int at = total + __popcll(same & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      at += w < wave ? found[w] : 0;
+      total += found[w];
+    }
+    if (mine) list[at] = row;
+    __syncthreads();
+  }
+  if (ACC && total == 0) return;
+  v4f acc[RT][4] = {};
+  for (int i0 = 0; i0 < total && ra > j0; i0 += 32 * sums.parts) {
+    const int h0 = 32 * part;
+    const bool any = i0 + h0 < total;
+    float4 xv[8];
+    if (any) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+        xv[d] = cols.load(job.x + list[min(i0 + h0 + 4 * d + q, total - 1)] * job.xstride);
+      issued();
+    }
+    for (int e = threadIdx.x; e < min(32 * sums.parts, total - i0 + 3) * RT * 4; e += 512) {
+      const int i = e / (RT * 4), j = j0 + e % (RT * 4) * 4;
+      float4 h = make_float4(0, 0, 0, 0);
+      if (i0 + i < total && j < ra) h = job.h.at4(list[i0 + i], j);
+      if (j + 4 > ra) h = make_float4(j < ra ? h.x : 0.0f, j + 1 < ra ? h.y : 0.0f, j + 2 < ra ? h.z : 0.0f, 0.0f);
+      *(float4 *)(hs + i * kPitch + j - j0) = h;
+    }
+    __syncthreads();
+    if (any) {
+      if (i0 + h0 + 32 > total)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) xv[d] = keep4(i0 + h0 + 4 * d + q < total, xv[d]);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        if (i0 + h0 + 4 * d >= total) break;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            acc[t][m] = mfma(hs[(h0 + 4 * d + q) * kPitch + 16 * t + lo], get4(xv[d], m), acc[t][m]);
+      }
+    }
+    __syncthreads();
+  }
+  for (int upper = sums.parts / 2; upper > 0; upper /= 2) {  // the later parts' sums on top of the earlier ones'
+    if (total <= 32 * upper) continue;
+    const int at = threadIdx.x & (upper * waves * 64 - 1);
+    if (part >= upper && part < 2 * upper)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          both_s[(4 * t + m) * 256 + at] = make_float4(acc[t][m][0], acc[t][m][1], acc[t][m][2], acc[t][m][3]);
+    __syncthreads();
+    if (part < upper)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float4 v = both_s[(4 * t + m) * 256 + at];
+          acc[t][m] += v4f{v.x, v.y, v.z, v.w};
+        }
+    __syncthreads();
+  }
+  if (part == 0) {
+    const Sum to{nullptr, nullptr, 0, job.width, 0, 0, job.grad, nullptr};
+    store_sums<ACC>(acc, fac, a, ra, j0, q, cols, true, false, to);
+  }
+}
+
 // ------------------------------------------------------------------ launches
-// Few rows: blocks along k where the rows alone leave CUs idle, at least 512
-// values of the width each.
-int splits_of(int n, int width) { return std::max(1, std::min({16, 512 / std::max(1, n), width / 512})); }
+// Few rows: blocks along k where the rows alone leave CUs idle, at least a step
+// of each wave.
+int splits_of(int n, int width) {
+  return std::max(1, std::min({8, 1024 / std::max(1, n), width / (kDownWaves * kStep)}));
+}
 int slices_of(int width) { return (width + kSlice - 1) / kSlice; }
 // Rows of a block of slice_kernel or outer_kernel: as many as leave two blocks
 // to every CU, `across` of them along the width.
@@ -784,6 +942,7 @@ struct Call {
   int32_t dtype;
   RowMap rows;
   hipStream_t s;
+  bool accumulate = false;
 };
 
 template <class F>
@@ -800,12 +959,17 @@ void by_flag(bool flag, F &&f) {
 
 hipError_t launch_down_rows(const Call &c, const Factor &fac, const float *x, int64_t xstride, const Hidden &out) {
   const int split_len = (((fac.width + out.splits - 1) / out.splits) + kStep - 1) / kStep * kStep;
-  by_rank(fac.rank, [&](auto rt) {
-    constexpr int RT = decltype(rt)::value;
-    const dim3 grid(c.rows.n, out.splits, rank_groups(fac.rank));
-    with_type(c.dtype, [&](auto t) {
-      down_row_kernel<decltype(t), RT><<<grid, kDownWaves * 64, 0, c.s>>>(c.rows, fac, x, xstride, out, split_len);
-    });
+  with_type(c.dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto launch = [&](auto r) {
+      constexpr int R = decltype(r)::value;
+      const dim3 grid(c.rows.n, out.splits, (fac.rank + R - 1) / R);
+      down_row_kernel<T, R><<<grid, kDownWaves * 64, 0, c.s>>>(c.rows, fac, x, xstride, out, split_len);
+    };
+    constexpr int kMost = sizeof(typename T::raw) == 4 ? 8 : 16;  // two steps' words in registers
+    if (fac.rank <= 4) launch(std::integral_constant<int, 4>{});
+    else if (fac.rank <= 8) launch(std::integral_constant<int, 8>{});
+    else launch(std::integral_constant<int, kMost>{});
   });
   return hipGetLastError();
 }
@@ -885,6 +1049,44 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
   return hipGetLastError();
 }
 
+hipError_t launch_few(const Call &c, const Factor &fac, FewSums sums, const Hidden &g, const float *base,
+                      int64_t bstride, float *dx, int64_t dxstride) {
+  int64_t grid = 0;
+  bool narrow = dx && fac.width < 4;
+  hipError_t e = hipSuccess;
+  by_rank(fac.rank, [&](auto rt) {
+    constexpr int RT = decltype(rt)::value;
+    sums.groups = (fac.rank + 16 * RT - 1) / (16 * RT);
+    const int share = c.rows.n / c.rows.count;  // rows of an adapter
+    sums.parts = share >= 128 ? 8 : share >= 64 ? 4 : 2;
+    for (int i = 0; i < sums.count; ++i) {
+      FewSum &job = sums.of[i];
+      job.across = (job.width + 512 / sums.parts - 1) / (512 / sums.parts);
+      job.first = (int)grid;
+      grid += (int64_t)c.rows.count * sums.groups * job.across;
+      narrow = narrow || job.width < 4;
+    }
+    sums.blocks = (int)grid;
+    if (dx) grid += (int64_t)c.rows.n * ((fac.width + 2047) / 2048);
+    if (grid == 0) return;
+    if (grid > INT32_MAX - kFewAcross) {  // gradients of 2 TB
+      e = hipErrorInvalidValue;
+      return;
+    }
+    sums.total = (int)grid;
+    const dim3 blocks((uint32_t)std::min<int64_t>(grid, kFewAcross), (uint32_t)((grid + kFewAcross - 1) / kFewAcross));
+    with_type(c.dtype, [&](auto t) {
+      by_flag(c.accumulate, [&](auto acc) {
+        by_flag(narrow, [&](auto nar) {
+          few_kernel<decltype(t), RT, decltype(acc)::value, decltype(nar)::value>
+              <<<blocks, 512, 0, c.s>>>(c.rows, fac, sums, g, base, bstride, dx, dxstride);
+        });
+      });
+    });
+  });
+  return e != hipSuccess ? e : hipGetLastError();
+}
+
 // `outer`: how many of the sums, from the first on, slice_kernel has not done.
 hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int outer, bool accumulate) {
   int across = 0, chunks = 0;
@@ -920,6 +1122,22 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
   return hipGetLastError();
 }
 
+// Whether the rows go one by one.  They then read their factors each for
+// itself, from the L2s at some 6 TB/s, in two launches; sorted into tiles they
+// share them but take five or more, 12 us and a quarter more per rank at
+// least.  Forward, rows one by one against tiles (us): f32 1024x1024 rank 4
+// n400 8 / 15; bf16 4096x4096 rank 16 n256 12 / 17, n400 18.6 / 18.4; f16
+// 4096x11008 rank 64 n96 23 / 28, n256 42 / 34; bf16 8192x8192 rank 128 n64 24 /
+// 34, n192 63 / 44.  Backward, where the tiles' launches are six and their sums
+// pass through memory: bf16 4096x4096 rank 16 n512 28 / 48; f16 4096x11008 rank
+// 64 n64 26 / 72, n400 79 / 104; bf16 8192x8192 rank 128 n64 37 / 79, n256 117 /
+// 118, n400 185 / 132.
+bool few_rows(const welvet_hip_adapters &d, int n, bool backward) {
+  const int64_t bytes = (int64_t)n * d.rank * ((int64_t)d.in + d.out) * tok::float_size(d.dtype);
+  const int64_t limit = (75 << 20) + d.rank * (9 << 18);
+  return n <= kFewRows && (backward ? bytes / 3 : bytes) <= limit;
+}
+
 // The workspace's parts.
 struct Sizes {
   size_t order = 0, hidden = 0, one = 0, part[2] = {0, 0};  // hidden: by split or slice; one: added up
@@ -930,7 +1148,7 @@ Sizes sizes_of(const welvet_hip_adapters &d, int n, bool backward) {
   if (n == 0) return z;
   const size_t one = (size_t)n * d.rank * sizeof(float);
   const int width = backward ? d.out : d.in;
-  if (!backward && n <= kFewRows) {
+  if (few_rows(d, n, backward)) {
     z.hidden = pad256(splits_of(n, width) * one);
     return z;
   }
@@ -1002,7 +1220,7 @@ welvet_status welvet_hip_adapters_forward(const welvet_hip_adapters *desc, const
   Call c{desc->dtype, {d_ids, nullptr, n, desc->count}, (hipStream_t)stream};
   const Factor down{desc->d_down, desc->d_ranks, desc->d_scales, desc->rank, desc->in};
   const Factor up{desc->d_up, desc->d_ranks, desc->d_scales, desc->rank, desc->out};
-  if (n <= kFewRows) {
+  if (few_rows(*desc, n, false)) {
     Hidden h{(float *)d_ws, splits_of(n, desc->in), n, desc->rank};
     if (h.splits == 1 && d_h) h.p = d_h;
     WH_HIP(launch_down_rows(c, down, d_x, x_stride, h));
@@ -1042,9 +1260,18 @@ welvet_status welvet_hip_adapters_backward(const welvet_hip_adapters *desc, cons
     return make_status(kInvalid, "adapters backward: %zu bytes of 16-byte aligned workspace are needed", z.total());
   st = require_device();
   if (st.code) return st;
-  Call c{desc->dtype, {nullptr, nullptr, n, desc->count}, (hipStream_t)stream};
+  Call c{desc->dtype, {d_ids, nullptr, n, desc->count}, (hipStream_t)stream, accumulate != 0};
   const Factor down{desc->d_down, desc->d_ranks, desc->d_scales, desc->rank, desc->in};
   const Factor up{desc->d_up, desc->d_ranks, desc->d_scales, desc->rank, desc->out};
+  if (few_rows(*desc, n, true)) {
+    const Hidden g{(float *)d_ws, n > 0 ? splits_of(n, desc->out) : 1, n, desc->rank};
+    if (n > 0 && (d_dx || d_ddown)) WH_HIP(launch_down_rows(c, up, d_dy, dy_stride, g));
+    FewSums sums{};
+    if (d_ddown) sums.of[sums.count++] = {g, d_x, x_stride, desc->in, 0, 0, d_ddown};
+    if (d_dup) sums.of[sums.count++] = {{const_cast<float *>(d_h), 1, n, desc->rank}, d_dy, dy_stride, desc->out, 0, 0, d_dup};
+    WH_HIP(launch_few(c, down, sums, g, d_dx_base, dx_base_stride, d_dx, dx_stride));
+    return ok();
+  }
   char *at = (char *)d_ws;
   float *const g = (float *)(at + z.order), *const slices = (float *)(at + z.order + z.one);
   float *const part = (float *)(at + z.order + z.one + z.hidden), *const part2 = (float *)((char *)part + z.part[0]);
