@@ -498,10 +498,10 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 // rows in launch order keep HBM busier than longer ones with the next rows'
 // loads ahead (8192 x 4096 f32 read and written: 64 rows a block 5.3 TB/s, 128
 // rows 4.6), and the factor read again by each comes from L2.
-template <class T, int RT, bool NARROW>
+template <class T, int RT, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
                                                                 const float *__restrict__ hidden, const float *base,
-                                                                int64_t bstride, float *y, int64_t ystride, bool nt) {
+                                                                int64_t bstride, float *y, int64_t ystride) {
   using raw = typename T::raw;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, q = lane >> 4;
   const int across = (fac.width + 255) / 256;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Fa
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (4 * q + r < live && cols.any()) cols.store(y + (int64_t)to[r] * ystride, bv[r], nt);
+    if (4 * q + r < live && cols.any()) cols.template store<NT>(y + (int64_t)to[r] * ystride, bv[r]);
 }
 
 // The same for few rows: a block one row's columns, four a thread, the hidden
@@ -1040,10 +1040,13 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
     const int64_t grid = (int64_t)((fac.width + 255) / 256) * ((c.rows.n + 15) / 16);
     const bool nt = (int64_t)c.rows.n * fac.width * 4 > kKept;
     with_type(c.dtype, [&](auto t) {
-      by_flag(fac.width < 4, [&](auto narrow) {
-        up_kernel<decltype(t), decltype(rt)::value, decltype(narrow)::value>
-            <<<(uint32_t)grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride, nt);
-      });
+      const auto go = [&](auto narrow, auto past) {
+        up_kernel<decltype(t), decltype(rt)::value, decltype(narrow)::value, decltype(past)::value>
+            <<<(uint32_t)grid, 256, 0, c.s>>>(c.rows, fac, h.p, base, bstride, y, ystride);
+      };
+      if (fac.width < 4) go(std::true_type{}, std::false_type{});
+      else if (nt) go(std::false_type{}, std::true_type{});
+      else go(std::false_type{}, std::false_type{});
     });
   });
   return hipGetLastError();

@@ -18,11 +18,11 @@ using namespace tok;
 // ---------------------------------------------------------------- forward
 // A block takes ROWS tokens and a column tile; a thread four columns of each
 // row, all rows' loads in flight before the first store.
-template <class T, int ROWS, bool NARROW>
+template <class T, int ROWS, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__restrict__ table, int64_t tstride,
                                                      uint32_t vocab, int dim, const int32_t *__restrict__ tokens,
                                                      int n, float scale, float *__restrict__ out, int64_t ostride,
-                                                     int tiles, bool nt) {
+                                                     int tiles) {
   const int group = blockIdx.x / tiles;
   const Cols<NARROW> cols((blockIdx.x % tiles * blockDim.x + threadIdx.x) * 4, dim);
   if (!cols.any()) return;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const typename T::raw *__re
     const int t = group * ROWS + r;
     if (t >= n) break;
     // padding is +0, also under a negative scale
-    cols.store(out + (int64_t)t * ostride, keep4(id[r] < vocab, mul4(v[r].floats(), scale)), nt);
+    cols.template store<NT>(out + (int64_t)t * ostride, keep4(id[r] < vocab, mul4(v[r].floats(), scale)));
   }
 }
 
@@ -87,18 +87,48 @@ constexpr int kDirect = 256;
 constexpr int kRun = 32;
 constexpr int kZeroRows = 4;  // table rows of a zeroing block
 
-template <bool ACC, bool NARROW>
-__device__ inline void put_row(const Cols<NARROW> &cols, float *row, const float4 &sum, float scale, bool nt) {
+template <bool ACC, bool NT, bool NARROW>
+__device__ inline void put_row(const Cols<NARROW> &cols, float *row, const float4 &sum, float scale) {
   float4 v = mul4(sum, scale);
   if constexpr (ACC) v = add4(cols.load(row), v);
-  cols.store(row, v, nt);
+  cols.template store<NT>(row, v);
 }
 
-__device__ inline void zero_row(float *row, int dim, bool nt) {
+// A block's zeros into `len` floats, each store a part of one cache line (rows
+// of 4099 floats from their own start on: 224 us against 154 for a table of
+// 50000).
+template <bool NT>
+__device__ inline void zero_span(float *p, int len) {
   const float4 zero = make_float4(0, 0, 0, 0);
-  for (int c = 4 * threadIdx.x; c < dim; c += 4 * blockDim.x) {
-    if (nt && c + 4 <= dim) store4_nt(row + c, zero);
-    else store4(row, c, dim, zero);
+  const int head = (int)((uintptr_t)p >> 2 & 31);  // floats past a line's start
+  for (int c = 4 * (int)threadIdx.x - head; c < len; c += 4 * blockDim.x) {
+    if (c >= 0 && c + 4 <= len) {
+      if constexpr (NT) store4_nt(p + c, zero);
+      else store4(p + c, zero);
+    } else {
+      for (int i = max(0, -c); i < 4 && c + i < len; ++i) p[c + i] = 0.0f;
+    }
+  }
+}
+// Zeros everywhere, ahead of the rows that tokens name: where they are few, a
+// table written at the rate of a fill and those rows a second time take less
+// than looking each row up among the tokens (68880 x 3340: 2 tokens 135 us
+// against 171, 400 152 / 187, 8192 213 / 222; 50000 x 4099, 8192: 214 / 214).
+// One store a thread in blocks that follow the addresses reaches 6.9 TB/s; four
+// a thread 6.0, sixteen 5.3.
+__global__ void __launch_bounds__(256) fill_kernel(uint32_t vocab, int dim, float *__restrict__ table, int64_t stride,
+                                                   int64_t blocks) {
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const uint32_t at = (uint32_t)(b * 1024 % dim) + 4 * threadIdx.x;
+    uint32_t row = (uint32_t)(b * 1024 / dim) + at / (uint32_t)dim, c = at % (uint32_t)dim;
+    if (row < vocab && c + 4 <= (uint32_t)dim) {
+      store4(table + (int64_t)row * stride + c, make_float4(0, 0, 0, 0));
+    } else {
+      for (int i = 0; i < 4 && row < vocab; ++i) {
+        table[(int64_t)row * stride + c] = 0.0f;
+        if (++c == (uint32_t)dim) c = 0, ++row;
+      }
+    }
   }
 }
 
@@ -106,7 +136,7 @@ template <bool ACC, bool NARROW>
 __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__ tokens, int n, uint32_t vocab,
                                                      int dim, const float *__restrict__ dout, int64_t dstride,
                                                      float scale, float *__restrict__ dtable, int64_t tstride,
-                                                     int tiles, bool nt) {
+                                                     int tiles) {
   __shared__ int32_t tok_s[kDirect];
   __shared__ int rows_s[kDirect];
   __shared__ int count_s;
@@ -123,7 +153,7 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     }
     __syncthreads();
     for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim, nt);
+      if (!named[r]) zero_span<false>(dtable + (int64_t)(v0 + r) * tstride, dim);
     return;
   }
   if (threadIdx.x == 0) count_s = 0;
@@ -158,15 +188,15 @@ __global__ void __launch_bounds__(256) direct_kernel(const int32_t *__restrict__
     for (int k = 0; k < 4; ++k) sum = add4(sum, v[k]);
   }
   for (; r < count; ++r) sum = add4(sum, cols.load(dout + (int64_t)rows_s[r] * dstride));
-  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale, nt);
+  put_row<ACC, false>(cols, dtable + (int64_t)mine * tstride, sum, scale);
 }
 
-template <bool ACC, bool NARROW>
+template <bool ACC, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ skey,
                                                    const int32_t *__restrict__ order, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ dout, int64_t dstride, float scale,
                                                    float *__restrict__ dtable, int64_t tstride,
-                                                   float *__restrict__ part, int tiles, bool nt) {
+                                                   float *__restrict__ part, int tiles) {
   __shared__ int32_t key_s[kRun + 2];  // with the neighbours' nearest
   __shared__ int32_t row_s[kRun];
   const int chunk = blockIdx.x / tiles, p0 = chunk * kRun;
@@ -186,7 +216,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
     if ((uint32_t)cur >= vocab) return;  // padding, or past the last row
     if (!began) cols.store(part + (int64_t)(2 * chunk) * dim, sum);
     else if (goes_on) cols.store(part + (int64_t)(2 * chunk + 1) * dim, sum);
-    else put_row<ACC>(cols, dtable + (int64_t)cur * tstride, sum, scale, nt);
+    else put_row<ACC, NT>(cols, dtable + (int64_t)cur * tstride, sum, scale);
   };
 #pragma unroll 1
   for (int r0 = 0; r0 < kRun; r0 += 8) {
@@ -215,11 +245,10 @@ __global__ void __launch_bounds__(256) sums_kernel(const int32_t *__restrict__ s
 // adds its later blocks' slot 0 to its own slot 1, in order.  The blocks after
 // those write the rows without a token, under whose stores the joins' waits
 // lie (32000 x 4096, 16384 tokens: 11 us less than a launch of its own).
-template <bool ACC, bool NARROW>
+template <bool ACC, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256) finish_kernel(const int32_t *__restrict__ skey, int n, uint32_t vocab, int dim,
                                                    const float *__restrict__ part, float scale,
-                                                   float *__restrict__ dtable, int64_t tstride, int tiles, int joins,
-                                                   bool nt) {
+                                                   float *__restrict__ dtable, int64_t tstride, int tiles, int joins) {
   if ((int)blockIdx.x >= joins) {
     __shared__ int named[kZeroRows];
     const uint32_t v0 = ((uint32_t)blockIdx.x - (uint32_t)joins) * kZeroRows;
@@ -229,7 +258,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const int32_t *__restrict__
     }
     __syncthreads();
     for (int r = 0; r < kZeroRows && v0 + r < vocab; ++r)
-      if (!named[r]) zero_row(dtable + (int64_t)(v0 + r) * tstride, dim, nt);
+      if (!named[r]) zero_span<NT>(dtable + (int64_t)(v0 + r) * tstride, dim);
     return;
   }
   const int chunk = blockIdx.x / tiles, p0 = chunk * kRun, p1 = p0 + kRun;
@@ -250,7 +279,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const int32_t *__restrict__
     for (int k = 0; k < 8; ++k) sum = add4(sum, v[k]);
   }
   for (; b <= last; ++b) sum = add4(sum, cols.load(part + (int64_t)(2 * b) * dim));
-  put_row<ACC>(cols, dtable + (int64_t)mine * tstride, sum, scale, nt);
+  put_row<ACC, NT>(cols, dtable + (int64_t)mine * tstride, sum, scale);
 }
 
 int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
@@ -260,17 +289,26 @@ size_t gradient_bytes(int dim, int n) {
   const size_t chunks = ((size_t)n + kRun - 1) / kRun;
   return order_bytes(n) + pad256(chunks * 2 * (size_t)dim * sizeof(float));
 }
+constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads; more go round
+constexpr int kMostZeros = 1 << 26;       // rows that a launch looks up
 
 template <bool ACC, bool NARROW>
 hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, float scale, const float *dout,
                            int64_t dstride, float *dtable, int64_t tstride, void *ws, hipStream_t s) {
   const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
-  const bool nt = (int64_t)vocab * dim * 4 > kKept;
-  const int64_t zeros = ACC ? 0 : ((int64_t)vocab + kZeroRows - 1) / kZeroRows;
+  const bool nt = (int64_t)vocab * dim * 4 > kKept;  // the table past the caches
+  const bool fill = !ACC && (vocab > kMostZeros || (nt && n <= vocab / 8));
+  if (fill) {
+    const int64_t blocks = ((int64_t)vocab * dim + 1023) / 1024;
+    fill_kernel<<<(uint32_t)std::min(blocks, kMostBlocks), 256, 0, s>>>((uint32_t)vocab, dim, dtable, tstride, blocks);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const int64_t zeros = ACC || fill ? 0 : ((int64_t)vocab + kZeroRows - 1) / kZeroRows;
   if (n <= kDirect) {
-    if (n == 0 && ACC) return hipSuccess;
+    if ((int64_t)n * tiles + zeros == 0) return hipSuccess;
     direct_kernel<ACC, NARROW><<<(uint32_t)((int64_t)n * tiles + zeros), threads, 0, s>>>(
-        tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles, nt);
+        tokens, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, tiles);
     return hipGetLastError();
   }
   Order o;
@@ -278,17 +316,22 @@ hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, flo
   if (e != hipSuccess) return e;
   float *part = (float *)((char *)ws + order_bytes(n));
   const int64_t chunks = ((int64_t)n + kRun - 1) / kRun, blocks = chunks * tiles;
-  sums_kernel<ACC, NARROW><<<(uint32_t)blocks, threads, 0, s>>>(o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride,
-                                                               scale, dtable, tstride, part, tiles, nt);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
-  finish_kernel<ACC, NARROW><<<(uint32_t)(blocks + zeros), threads, 0, s>>>(
-      o.skey, n, (uint32_t)vocab, dim, part, scale, dtable, tstride, tiles, (int)blocks, nt);
-  return hipGetLastError();
+  const auto go = [&](auto past) {
+    constexpr bool NT = decltype(past)::value;
+    sums_kernel<ACC, NARROW, NT><<<(uint32_t)blocks, threads, 0, s>>>(
+        o.skey, o.order, n, (uint32_t)vocab, dim, dout, dstride, scale, dtable, tstride, part, tiles);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    finish_kernel<ACC, NARROW, NT><<<(uint32_t)(blocks + zeros), threads, 0, s>>>(
+        o.skey, n, (uint32_t)vocab, dim, part, scale, dtable, tstride, tiles, (int)blocks);
+    return hipGetLastError();
+  };
+  return nt && !NARROW ? go(std::true_type{}) : go(std::false_type{});
 }
 
-// A launch's blocks and the kernels' int counters: (n + vocab / 8) * tiles.
+// A launch's threads (2^32) and the kernels' int counters.
 bool sizes_ok(int32_t vocab, int32_t dim, int32_t n) {
-  return vocab > 0 && vocab < INT32_MAX && dim > 0 && n >= 0 &&
+  return vocab > 0 && vocab < INT32_MAX && dim > 0 && n >= 0 && n <= 1 << 27 &&
          ((int64_t)n + vocab) * ((dim + 1023) / 1024 + 1) < INT32_MAX;
 }
 
@@ -321,10 +364,12 @@ welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t
     const auto go = [&](auto kernel) {
       kernel<<<blocks, threads, 0, (hipStream_t)stream>>>((const typename T::raw *)d_table, table_stride,
                                                           (uint32_t)vocab, dim, d_tokens, n, scale, d_out, out_stride,
-                                                          tiles, (int64_t)n * dim * 4 > tok::kKept);
+                                                          tiles);
     };
-    if (dim < 4) rows == 4 ? go(lookup_kernel<T, 4, true>) : go(lookup_kernel<T, 1, true>);
-    else rows == 4 ? go(lookup_kernel<T, 4, false>) : go(lookup_kernel<T, 1, false>);
+    if (dim < 4) rows == 4 ? go(lookup_kernel<T, 4, true, false>) : go(lookup_kernel<T, 1, true, false>);
+    else if (rows == 1) go(lookup_kernel<T, 1, false, false>);
+    else if ((int64_t)n * dim * 4 > tok::kKept) go(lookup_kernel<T, 4, false, true>);
+    else go(lookup_kernel<T, 4, false, false>);
   });
   WH_HIP(hipGetLastError());
   return ok();
@@ -335,7 +380,7 @@ welvet_status welvet_hip_embedding_store_forward(welvet_dense_session *s, const 
   if (!s || n < 0 || (n > 0 && (!d_tokens || !d_out))) return make_status(kInvalid, "embedding: invalid argument");
   std::unique_lock<std::mutex> lock;
   const DevStore w = session_store(s, &lock);
-  if ((int64_t)n * ((w.cols + 1023) / 1024) > INT32_MAX) return make_status(kInvalid, "embedding: invalid argument");
+  if ((int64_t)n * ((w.cols + 1023) / 1024) >= 1 << 24) return make_status(kInvalid, "embedding: invalid argument");
   if (out_stride < w.cols) return make_status(kInvalid, "embedding: row stride below dim %d", w.cols);
   if (!tok::aligned(d_tokens, 4) || !tok::aligned(d_out, 4))
     return make_status(kInvalid, "embedding: device pointers must be aligned to their elements");

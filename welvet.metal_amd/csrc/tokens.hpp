@@ -83,12 +83,19 @@ struct Quad {
   }
 };
 __device__ inline void store4(float *p, const float4 &v) { __builtin_memcpy(p, &v, sizeof(v)); }
-// The same past the caches' keeping: results larger than they hold.
+// The same past the caches: results larger than the L2s hold.  Chosen by a
+// kernel's template argument: of two such stores on the two sides of a branch
+// the compiler makes one, a plain one.
 typedef float nt4 __attribute__((ext_vector_type(4), aligned(4)));
 __device__ inline void store4_nt(float *p, const float4 &v) {
   __builtin_nontemporal_store(nt4{v.x, v.y, v.z, v.w}, (nt4 *)p);
 }
-constexpr int64_t kKept = 64 << 20;  // results up to these bytes are stored to stay in the caches
+// Bytes of results up to which they may stay there: what the L2s hold.  Past
+// them a lookup of 16384 rows x 1024 takes 15.4 us against 20.4, of 16384 x
+// 4096 68 / 91, an adapter's 8192 x 4096 rows 89 / 102.  A kernel that does
+// nothing but read the result right after pays for it (64 MiB: 0.6 us, 128 MiB:
+// 12); a product's loads hide that.
+constexpr int64_t kKept = 32 << 20;
 __device__ inline void store4(float *row, int k, int width, const float4 &v) {
   if (k + 4 <= width) return store4(row + k, v);
   const float f[4] = {v.x, v.y, v.z, v.w};
@@ -116,9 +123,13 @@ struct Cols {
     else return Quad<T>::load(row + c);
   }
   __device__ float4 load(const float *row) const { return load<F32>((const uint32_t *)row).floats(); }
-  __device__ void store(float *row, const float4 &v, bool nt = false) const {
+  template <bool NT = false>
+  __device__ void store(float *row, const float4 &v) const {
     if constexpr (NARROW) return store4(row, c, width, v);
-    if (skip == 0) return nt ? store4_nt(row + c, v) : store4(row + c, v);
+    if (skip == 0) {
+      if constexpr (NT) return store4_nt(row + c, v);
+      else return store4(row + c, v);
+    }
     if (skip < 2) row[c + 1] = v.y;
     if (skip < 3) row[c + 2] = v.z;
     if (skip < 4) row[c + 3] = v.w;
