@@ -333,7 +333,7 @@ WELVET_API void welvet_hip_swiglu_release(welvet_hip_swiglu *s);
 
 /* Embedding: out[t] = scale * table[tokens[t]], t < n, rows of dim f32 values
  * from a [vocab][dim] table.  A token outside [0, vocab) is padding: a row of
- * zeros. */
+ * zeros.  n <= 2^27, (n + vocab) (dim / 1024 + 2) < 2^31. */
 WELVET_API welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t dim,
                                                       const void *d_table, int64_t table_stride,
                                                       const int32_t *d_tokens, int32_t n,
@@ -366,7 +366,7 @@ WELVET_API welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t di
  * device arrays; adapter a uses its first d_ranks[a] rank rows (NULL: all;
  * the rest is not read) and the factor d_scales[a] (NULL: 1).  Row t of n
  * takes adapter ids[t], none where that lies outside [0, count).
- * count <= 65535. */
+ * count <= 65535, n <= 2^23, n * rank < 2^31, rank * max(in, out) < 2^30. */
 typedef struct welvet_hip_adapters {
   int32_t dtype, count, rank, in, out;
   const void *d_down, *d_up;
@@ -399,9 +399,9 @@ WELVET_API welvet_status welvet_hip_adapters_backward(
     int64_t dx_base_stride, float *d_dx, int64_t dx_stride, int32_t accumulate, float *d_ddown,
     float *d_dup, void *d_ws, size_t ws_bytes, void *stream);
 
-/* Distillation from a teacher's top logits.  Row t < n holds logits z over
- * the vocabulary (Float32, Float16 or BFloat16; row stride `stride`), and the
- * teacher's k entries (k <= 1024) index[t][k], teacher[t][k] (f32 logits).
+/* Distillation from a teacher's top logits.  Row t < n <= 2^22 holds logits z
+ * over the vocabulary (Float32, Float16 or BFloat16; row stride `stride`), and
+ * the teacher's k entries (k <= 1024) index[t][k], teacher[t][k] (f32 logits).
  * With temperature T (0 < T, finite): q = softmax of the row's teacher / T,
  * or, where d_teacher_lse [n] is given, exp(teacher / T - teacher_lse[t])
  * (the log-sum of the teacher's whole row at T: q then sums to what its top

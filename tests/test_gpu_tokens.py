@@ -10,6 +10,8 @@ import pytest
 import pywelvet
 from devmem import Stream, _ok, hip
 from parity import assert_bit_equal
+import test_gpu_adapters as adapters
+import test_gpu_embedding as embedding
 from test_gpu_adapters import Case
 from tokmem import DT, U, Dev, within
 
@@ -90,7 +92,7 @@ def put(dev, a):
     _ok(hip().hipMemcpy(dev.ptr, a.ctypes.data, a.nbytes, 1), "hipMemcpy H2D")
 
 
-@pytest.mark.parametrize("n", [3, 40, 400])
+@pytest.mark.parametrize("n", [3, 40, 400, 2300])
 def test_replayed_from_a_graph(stream, n):
     """A captured step (lookups, adapters and distillation both ways, the
     table's gradient) replayed five times on new inputs, with eager calls
@@ -147,7 +149,7 @@ def test_replayed_from_a_graph(stream, n):
     store.close()
 
 
-@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("n", [20, 300, 2400])
 @pytest.mark.parametrize("rank", [1, 20])
 @pytest.mark.parametrize("dtype", DT)
 def test_adapters_with_values_not_finite(stream, dtype, rank, n):
@@ -198,3 +200,73 @@ def test_adapters_with_values_not_finite(stream, dtype, rank, n):
             assert np.array_equal(np.isnan(du[a][:, marked]), np.isnan(wu[:, marked]))
             hits = np.isinf(wu) & marked
             assert np.array_equal(du[a][hits], wu[hits])
+
+
+# tables of more than 32 MiB: filled first where tokens name few rows, else
+# their unnamed rows looked up; results stored past the caches
+@pytest.mark.parametrize("vocab,dim,n,extra", [
+    (9000, 1027, 200, 3), (20000, 515, 300, 0), (20000, 515, 2400, 5), (20000, 515, 6000, 0), (4200, 2052, 700, 4)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradients_of_large_tables(stream, vocab, dim, n, extra, accumulate):
+    embedding.test_gradient(stream.h, vocab, dim, n, extra, accumulate)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim,extra", [(515, 0), (516, 3), (2048, 4)])
+def test_lookups_of_large_results(stream, dtype, dim, extra):
+    embedding.test_lookup(stream.h, dtype, 300, dim, 9_000_000 // dim + 7, extra, 2.0)
+
+
+# more than 2048 rows are always sorted by their adapters; the last two shapes'
+# rows pass 32 MiB
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("shape", [
+    (1001, 777, 5, 4, 2100, "mixed", 0), (130, 70, 33, 7, 2300, "mixed", 2), (260, 196, 20, 9, 2200, "mixed", 4),
+    (96, 1028, 100, 3, 2500, "mixed", 0), (3, 2, 4, 2, 2100, "mixed", 1), (513, 257, 16, 2, 4200, "sorted", 1),
+    (64, 68, 4, 200, 4100, "mixed", 0), (600, 4100, 16, 1, 2100, "sorted", 0), (4100, 600, 33, 5, 2200, "mixed", 3)],
+    ids=lambda s: "-".join(map(str, s)))
+def test_many_rows_of_adapters(stream, dtype, shape):
+    adapters.test_forward_and_backward(stream.h, dtype, shape)
+
+
+def test_many_rows_of_adapters_elsewhere(stream):
+    """Without bases, added to gradients, without adapters, with another
+    tenant's NaN and in place, on sorted rows."""
+    adapters.test_without_bases_scales_or_h(stream.h, 2200)
+    adapters.test_accumulates(stream.h, 2300)
+    adapters.test_rows_without_an_adapter(stream.h, 2400)
+    adapters.test_tenants_do_not_meet(stream.h, 2500)
+    c = Case("float16", 100, 84, 8, 3, 2100).on_device()
+    y, h = c.forward(stream.h)
+    dx, _, _ = c.backward(stream.h, h)
+    yb, xb = Dev(c.base), Dev(c.dxb)
+    c.a.forward(c.d["x"].ptr, c.d["ids"].ptr, c.n, yb.ptr, yb.ptr, stream=stream.h, **c.ws)
+    assert_bit_equal(yb.get(), y, "y")
+    c.a.backward(None, c.d["ids"].ptr, c.n, None, c.d["dy"].ptr, d_dx_base=xb.ptr, d_dx=xb.ptr, stream=stream.h, **c.ws)
+    assert_bit_equal(xb.get(), dx, "dx")
+
+
+@pytest.mark.parametrize("n,count", [(64, 1), (130, 1), (256, 1), (200, 2), (1300, 3)])
+@pytest.mark.parametrize("rank", [3, 24, 40])
+def test_long_runs_row_by_row(stream, n, count, rank):
+    """Few adapters with many rows each, below the sorting's threshold."""
+    adapters.test_forward_and_backward(stream.h, "bfloat16", (132, 200, rank, count, n, "mixed", 0))
+
+
+@pytest.mark.parametrize("given", ["dx", "ddown", "dup"])
+@pytest.mark.parametrize("n", [6, 300, 2200])
+def test_one_gradient_alone(stream, n, given):
+    """Each of the backward's outputs by itself; of rows that go one by one
+    with the bits that it has beside the others."""
+    c = Case("bfloat16", 140, 264, 12, 5, n).on_device()
+    _, h = c.forward(stream.h)
+    outs = dict(zip(("dx", "ddown", "dup"), c.backward(stream.h, h)))
+    dh, out = Dev(h), Dev(np.full(outs[given].shape, np.nan, np.float32))
+    c.a.backward(c.d["x"].ptr if given == "ddown" else None, c.d["ids"].ptr, n, dh.ptr if given == "dup" else None,
+                 c.d["dy"].ptr, d_dx_base=c.d["dxb"].ptr if given == "dx" else None, stream=stream.h,
+                 **{"d_" + given: out.ptr}, **c.ws)
+    got = out.get()
+    if n <= 2048:
+        assert_bit_equal(got, outs[given], given)
+    outs[given] = got
+    adapters.check_backward(c, outs["dx"], outs["ddown"], outs["dup"], h)

@@ -5,16 +5,22 @@
 //   backward  g = dy . up_a^T              dx = dx_base + s_a g . down_a
 //             ddown_a = s_a sum_t g_t x_t  dup_a = s_a sum_t h_t dy_t
 // Both factors keep the rank first, so the two directions are the same three
-// products: rows by a factor over its width (down_kernel), rank values spread
-// over a width (up_kernel), and sums over an adapter's rows (outer_kernel).
-// Products and sums are f32 (the f32 MFMA, fma chains in its accumulators):
-// activations are f32 and a 16-bit factor is exact in f32.
+// products: rows by a factor over its width (down_row_kernel, slice_kernel),
+// rank values spread over a width (spread_row, up_kernel), and sums over an
+// adapter's rows (few_kernel, outer_kernel, and slice_kernel for dup, whose dy
+// it reads anyway).  Products and sums are f32: activations are f32 and a
+// 16-bit factor is exact in f32.
 //
-// Rows are taken in the order of their adapters (tokens.hpp), 16 of them a
-// tile, so a tile reads each of its adapters once; a tile of several adapters
-// computes all 16 rows with each and keeps the adapter's own, so no value of
-// another tenant's factor reaches a row, NaN or not.  Few rows (a decode
-// step) are tiles of one row in their own order, without the sorting launch.
+// Few rows go one by one in two launches, in their own order: latency and the
+// factors' reads through the L2s bound them (f32 1001x777 rank 5 n3: 11.9 us;
+// bf16 4096x11008 rank 16 n64: 11.6, 28 MB at 2.1 TB/s; backward, f32 2048x8192
+// rank 8 n256: 16.3).  Many rows are sorted by their adapters (tokens.hpp), so
+// that an adapter's rows pass a factor held in registers, and cost about the
+// activations' bytes (bf16 4096x4096 rank 16 n8192 forward: 89 us, 403 MB at
+// 4.5 TB/s; backward bf16 4096x11008 rank 32 n8192: 277 us, 787 MB at 2.8 TB/s,
+// of which the matrix pipe would take 105 with f32 MFMAs alone).  Rows of
+// different adapters never share a sum, so no value of another tenant's factor
+// reaches a row, NaN or not.
 #include <hip/hip_runtime.h>
 
 #include "tokens.hpp"
@@ -31,8 +37,8 @@ constexpr int kMaxRank = 256;
 
 // The rows of a launch: position p -> row and adapter (count: none).
 struct RowMap {
-  const int32_t *key;    // adapter by position (sorted), or by row
-  const int32_t *order;  // row by position; null: the row itself
+  const int32_t *key;    // adapter by position
+  const int32_t *order;  // row by position; null: the row itself, unsorted
   int n, count;
   __device__ int row(int p) const { return order ? order[p] : p; }
   __device__ int adapter(int p) const {
@@ -48,7 +54,7 @@ struct Factor {
   __device__ int rank_of(int a) const { return ranks ? min(max(ranks[a], 0), rank) : rank; }
   __device__ float scale_of(int a) const { return scales ? scales[a] : 1.0f; }
 };
-// The products of down_kernel: [splits][n][rank], to be added up.
+// Rows' products with a factor: [splits][n][rank], to be added up.
 struct Hidden {
   float *p;
   int splits, n, rank;
@@ -95,7 +101,7 @@ struct Hidden {
 // counts here, and every lane reads its own: four neighbouring k of x and of
 // each rank row, 256 k a wave's step, the block's waves in turn with the next
 // step's loads in flight.  (Lanes of an MFMA would share an x value sixteen
-// times and load it as often: f32 2048x8192 rank 8 n256 DOWNOLD -> DOWNNEW us.)
+// times and load it as often: f32 2048x8192 rank 8 n256 17 us, so 6.8.)
 // A rank's 64 lane sums are folded so that each exchange halves the values.
 // Rank rows past the adapter's repeat its last one and are dropped at the end.
 constexpr int kDownWaves = 4;
@@ -264,7 +270,7 @@ __device__ inline float from_parts(const uint4 (&p)[2], int i) {
   else return half(p[0]) + half(p[1]);
 }
 
-// The same for many rows, a block a slice of the width: the slice's factor
+// Many rows, a block a slice of the width: the slice's factor
 // values stay in registers while an adapter's rows pass, 16 at a time, the next
 // 16 rows' loads in flight.  Every wave holds 64 columns, its products are
 // added up across the block in LDS, and the slices' sums are left for
@@ -276,7 +282,9 @@ __device__ inline float from_parts(const uint4 (&p)[2], int i) {
 // SUMS: the rows also give the second product that reads them, sum over the
 // adapter's rows of job.hidden[row][j] x[row][c] (outer_kernel below has its
 // terms), so that x is read from HBM once for both: a wave's 16 x 64 part is
-// turned in LDS to the columns-by-rows order of that product.
+// turned in LDS to the columns-by-rows order of that product (bf16 4096x11008
+// rank 32 n8192, dy's 361 MB: 140 us, 2.6 TB/s; its MFMAs 45 and the turning's
+// LDS traffic 22 do not lie wholly under the loads).
 constexpr int kSliceWaves = 8;
 constexpr int kSlice = kSliceWaves * 64;
 constexpr int kMaxChunk = 512;
@@ -284,9 +292,10 @@ template <class T, int RT, bool SUMS, bool ACC, bool NARROW>
 __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(RowMap rows, Factor fac, Sum job,
                                                                               float *__restrict__ hidden) {
   constexpr int kPitch = 68;  // floats of a turned row: reads by columns fall on different banks
-  // part products where the f32 MFMAs of both products would bind; f16's two
-  // parts do not fit the registers beside more than 16 ranks
-  constexpr bool SPLIT = SUMS && (std::is_same_v<T, BF16> || (std::is_same_v<T, F16> && RT == 1));
+  // part products where f32 MFMAs would bind; f16's two parts do not fit the
+  // registers beside the sums of more than 16 ranks.  The same with and without
+  // SUMS: what dx comes out as does not depend on dup being asked for.
+  constexpr bool SPLIT = std::is_same_v<T, BF16> || (std::is_same_v<T, F16> && RT == 1);
   using raw = typename T::raw;
   __shared__ float red[2][kSliceWaves][16][RT * 16 + 1];  // by tile: one barrier each
   __shared__ float4 turn4[SUMS ? kSliceWaves * 16 * kPitch / 4 : 1];
@@ -497,7 +506,9 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 // 16 rows, all of its loads in flight together.  Short blocks that pass the
 // rows in launch order keep HBM busier than longer ones with the next rows'
 // loads ahead (8192 x 4096 f32 read and written: 64 rows a block 5.3 TB/s, 128
-// rows 4.6), and the factor read again by each comes from L2.
+// rows 4.6), and the factor read again by each comes from L2.  bf16 4096 wide,
+// rank 32, 8192 rows with a base: 58 us, 403 MB with the hidden values' at 4.6
+// TB/s before the stores went past the caches, a copy's rate.
 template <class T, int RT, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
                                                                 const float *__restrict__ hidden, const float *base,
@@ -644,8 +655,10 @@ __global__ void __launch_bounds__(256) up_row_kernel(RowMap rows, Factor fac, Hi
 // grad_a[j][c] = s_a sum over a's rows of hidden[row][j] x[row][c].  D[i =
 // rank][j = column]: a wave 64 columns (as above), four rows an MFMA, DEPTH
 // MFMA steps of loads ahead.  A block takes `chunk` positions of the sorted
-// rows.
-// A launch does the sums of both factors where both are asked for.
+// rows, half a block's waves every second four of them: long runs keep twice
+// the loads in flight.  A launch does the sums of both factors where both are
+// asked for.  x of 8192 x 4096, rank 32: 47 us, 2.9 TB/s; its MFMAs would take
+// 14, the rest waits for loads at three waves a SIMD.
 struct Sums {
   Sum of[2];
   int count;
@@ -803,7 +816,8 @@ __global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, Sums 
 // is the adapter's), then blocks that each spread one row's g over 2048 columns
 // of dx.  A wave sums 64 columns of 32 rows; `parts` of a block's eight share
 // columns and add up in LDS: two where adapters are many, more for long runs of
-// few adapters, whose blocks alone would not fill the CUs.
+// few adapters, whose blocks alone would not fill the CUs (f32 2048x8192 rank 8,
+// one adapter's 256 rows: two parts 16.7 us, eight 10.0).
 constexpr int kFewRows = 2048;       // rows at most
 constexpr int kFewAcross = 1 << 20;  // blocks in the grid's x: 2^32 threads at most
 struct FewSum {
@@ -1173,8 +1187,9 @@ Sizes sizes_of(const welvet_hip_adapters &d, int n, bool backward) {
 }
 
 bool desc_ok(const welvet_hip_adapters *d, int32_t n) {
-  return d && n >= 0 && n <= (1 << 23) && (int64_t)n * d->rank <= INT32_MAX && d->count > 0 && d->count <= 65535 && d->rank > 0 && d->rank <= kMaxRank &&
-         d->in > 0 && d->out > 0 && (int64_t)d->rank * std::max(d->in, d->out) <= INT32_MAX / 2;
+  return d && n >= 0 && n <= (1 << 23) && (int64_t)n * d->rank <= INT32_MAX && d->count > 0 && d->count <= 65535 &&
+         d->rank > 0 && d->rank <= kMaxRank && d->in > 0 && d->out > 0 &&
+         (int64_t)d->rank * std::max(d->in, d->out) <= INT32_MAX / 2;
 }
 
 }  // namespace

@@ -572,7 +572,7 @@ hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
 }
 
 bool sizes_ok(int32_t dtype, int32_t n, int32_t vocab, int32_t k) {
-  return n >= 0 && n <= (1 << 28) && vocab > 0 && vocab <= INT32_MAX - 64 && k > 0 && k <= kMaxEntries;
+  return n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= INT32_MAX - 64 && k > 0 && k <= kMaxEntries;
 }
 
 }  // namespace
