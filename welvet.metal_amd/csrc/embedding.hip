@@ -114,8 +114,10 @@ __device__ inline void zero_span(float *p, int len) {
 }
 // Zeros everywhere, ahead of the rows that tokens name: where they are few, a
 // table written at the rate of a fill and those rows a second time take less
-// than looking each row up among the tokens (68880 x 3340: 2 tokens 135 us
-// against 171, 400 152 / 187, 8192 213 / 222; 50000 x 4099, 8192: 214 / 214).
+// than looking each row up among the tokens.  32000 x 4096, fill against lookups
+// (us), tokens as many as a 16th of the rows 103 / 113, an 8th 120 / 121, a
+// quarter 148 / 132; 68880 x 3340: 177 / 209, 205 / 223, 257 / 247; 2 tokens 135 /
+// 171 (skewed tokens; uniform ones a few us further towards the lookups).
 // One store a thread in blocks that follow the addresses reaches 6.9 TB/s; four
 // a thread 6.0, sixteen 5.3.
 __global__ void __launch_bounds__(256) fill_kernel(uint32_t vocab, int dim, float *__restrict__ table, int64_t stride,
