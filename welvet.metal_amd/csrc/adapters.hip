@@ -950,10 +950,10 @@ int chunk_of(int n, int across) {
   const int64_t rows = ((int64_t)n * across + 512 * 16 - 1) / (512 * 16) * 16;
   return (int)std::max<int64_t>(16, std::min<int64_t>(kMaxChunk, rows));
 }
-// The forward's slices, without sums: about one block to every CU, for the slice
-// of the factor is read by each block (whole calls
-// with one and with two: bf16 4096x11008 rank 32, 2048 rows 56.6 us / 59.4, 8192
-// rows 211 / 212; 4096x4096 rank 16, 4100 rows 47.4 / 50.9).
+// The forward's slices, without sums: about one block to every CU, for each block
+// reads its slice of the factor (whole calls with one and with two: bf16
+// 4096x11008 rank 32, 2048 rows 56.6 us / 59.4, 8192 rows 211 / 212; 4096x4096
+// rank 16, 4100 rows 47.4 / 50.9).
 int forward_chunk_of(int n, int across) {
   const int64_t rows = ((int64_t)n * across + 256 * 8) / (256 * 16) * 16;
   return (int)std::max<int64_t>(16, std::min<int64_t>(kMaxChunk, rows));
@@ -1149,7 +1149,7 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
 
 // Whether the rows go one by one.  They then read their factors each for
 // itself, from the L2s at some 6 TB/s, in two launches; sorted into tiles they
-// share them but take five or more, 12 us and a quarter more per rank at
+// share them but take four or more, 12 us and a quarter more per rank at
 // least.  Forward, rows one by one against tiles (us): f32 1024x1024 rank 4
 // n400 8 / 15; bf16 4096x4096 rank 16 n256 12 / 17, n400 18.6 / 18.4; f16
 // 4096x11008 rank 64 n96 23 / 28, n256 42 / 34; bf16 8192x8192 rank 128 n64 24 /
