@@ -283,7 +283,7 @@ __device__ inline float from_parts(const uint4 (&p)[2], int i) {
 // adapter's rows of job.hidden[row][j] x[row][c] (outer_kernel below has its
 // terms), so that x is read from HBM once for both: a wave's 16 x 64 part is
 // turned in LDS to the columns-by-rows order of that product (bf16 4096x11008
-// rank 32 n8192, dy's 361 MB: 140 us, 2.6 TB/s; its MFMAs 45 and the turning's
+// rank 32 n8192, dy's 361 MB: 144 us, 2.5 TB/s; its MFMAs 45 and the turning's
 // LDS traffic 22 do not lie wholly under the loads).
 constexpr int kSliceWaves = 8;
 constexpr int kSlice = kSliceWaves * 64;
@@ -507,8 +507,7 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 // rows in launch order keep HBM busier than longer ones with the next rows'
 // loads ahead (8192 x 4096 f32 read and written: 64 rows a block 5.3 TB/s, 128
 // rows 4.6), and the factor read again by each comes from L2.  bf16 4096 wide,
-// rank 32, 8192 rows with a base: 58 us, 403 MB with the hidden values' at 4.6
-// TB/s before the stores went past the caches, a copy's rate.
+// rank 32, 8192 rows with a base: 61 us, 268 MB at 4.4 TB/s, about a copy's rate.
 template <class T, int RT, bool NARROW, bool NT>
 __global__ void __launch_bounds__(256, RT > 2 ? 3 : 4) up_kernel(RowMap rows, Factor fac,
                                                                 const float *__restrict__ hidden, const float *base,
@@ -657,7 +656,7 @@ __global__ void __launch_bounds__(256) up_row_kernel(RowMap rows, Factor fac, Hi
 // MFMA steps of loads ahead.  A block takes `chunk` positions of the sorted
 // rows, half a block's waves every second four of them: long runs keep twice
 // the loads in flight.  A launch does the sums of both factors where both are
-// asked for.  x of 8192 x 4096, rank 32: 47 us, 2.9 TB/s; its MFMAs would take
+// asked for.  x of 8192 x 4096, rank 32: 46 us, 2.9 TB/s; its MFMAs would take
 // 14, the rest waits for loads at three waves a SIMD.
 struct Sums {
   Sum of[2];
@@ -1148,7 +1147,7 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
 }
 
 // Whether the rows go one by one.  They then read their factors each for
-// itself, from the L2s at some 6 TB/s, in two launches; sorted into tiles they
+// itself, from the L2s at some 9 TB/s, in two launches; sorted into tiles they
 // share them but take four or more, 12 us and a quarter more per rank at
 // least.  Forward, rows one by one against tiles (us): f32 1024x1024 rank 4
 // n400 8 / 15; bf16 4096x4096 rank 16 n256 12 / 17, n400 18.6 / 18.4; f16
