@@ -192,6 +192,28 @@ def test_masked_logits(stream, dtype, n):
     assert np.isposinf(loss[3]) and np.isfinite(to_f64(grad[3], dtype)).all()
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n", [6, 256])
+@pytest.mark.parametrize("T", [2.0, 0.002])
+def test_logits_of_any_magnitude(stream, dtype, n, T):
+    """Rows masked throughout with the type's lowest value or a large one, and
+    rows whose logits lie around a large value of either sign, also the one (2^24
+    T / log2 e) where the kernels change the form of their exponents, so that a
+    row has threads on both sides.  The differences to the maximum are rounded
+    once more there: 3 |t| 2^-24, below the bound's 1200 where p is not zero."""
+    rng = np.random.default_rng(9)
+    z, index, teacher = inputs(rng, dtype, n, 8200, 12, absent=0)
+    teacher = teacher * np.float32(min(T, 1.0))  # teacher / T as spread as elsewhere
+    lowest = {"float32": np.finfo(np.float32).min, "float16": np.float16(-65504), "bfloat16": np.uint16(0xFF7F)}[dtype]
+    top = 65504 if dtype == "float16" else 3e38
+    edge = 2.0 ** 24 * T / 1.4426950408889634
+    z[0] = lowest
+    for row, at in ((1, -1e30), (2, 3e9), (3, edge), (4, -edge)):
+        at = np.clip(at, -top, top)
+        z[row] = to_bits(np.clip(at + T * rng.uniform(-8, 8, 8200), -top, top), dtype)
+    check(stream, dtype, z, index, teacher, T=T)
+
+
 @pytest.mark.parametrize("n", [3, 256])
 def test_rows_left_out(stream, n):
     """Weight 0 or no entry: zeros, whatever the logits; NaN logits stay in their own row."""

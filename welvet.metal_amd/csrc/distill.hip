@@ -13,10 +13,10 @@
 // running pair, joined across the block), the gradient a second: bound by
 // HBM, which reads each logit once where a row's block still holds it and
 // writes the gradient once.  Exponentials are taken as 2^(z c - m c) with
-// c = log2(e) / T in one fma: its rounding of m c is common to the row and
-// leaves p as it is; the loss takes the same c and m c in f64.  Where m c
-// overflows (a row masked with the type's lowest value throughout) they are
-// 2^((z - m) c).
+// c = log2(e) / T in one fma, whose rounding of m c the sums and g make up
+// for.  From |m c| = 2^24 on (a row masked with a large value throughout) that
+// rounding is more than a half, in the end more than the exponential's range:
+// they are then 2^((z - m) c).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -42,30 +42,31 @@ struct Args {
   int64_t gstride;
 };
 
-// Running maximum of z and sum of 2^(z c - mc), mc = m c as rounded.
+// Maximum of z and sum of 2^((z - m) c).
 struct Stat {
   float m, s;
 };
-// The exponent's offset; huge: m c overflows (m itself may be +inf).
+// The exponent's offset mc = m c as rounded; huge: of no use (m itself may be +inf).
+__device__ inline bool too_large(float mc) { return !(fabsf(mc) < 0x1p24f); }
 struct Shift {
   float m, mc;
   bool huge;
-  __device__ Shift(float m_, float c) : m(m_), mc(m_ == -INFINITY ? 0.0f : m_ * c) { huge = fabsf(mc) == INFINITY; }
+  __device__ Shift(float m_, float c) : m(m_), mc(m_ == -INFINITY ? 0.0f : m_ * c) { huge = too_large(mc); }
+  // what m c is past the offset taken for it
+  __device__ float rest(float c) const { return huge || m == -INFINITY ? 0.0f : fmaf(m, c, -mc); }
 };
 __device__ inline float term(float z, float c, const Shift &h) {
   return __builtin_amdgcn_exp2f(h.huge ? (z - h.m) * c : fmaf(z, c, -h.mc));
 }
-// The factor from a sum at maximum m to one at h's: between the offsets as
-// rounded, so 1 where they are equal.  An empty sum's (0) must not be NaN.
-__device__ inline float rescale(float m, float c, const Shift &h) {
-  if (m == -INFINITY) return 1.0f;
-  return __builtin_amdgcn_exp2f(h.huge ? (m - h.m) * c : m * c - h.mc);
+// The factor from a sum at maximum `from` to one at `to`; an empty sum's (0) must not be NaN.
+__device__ inline float rescale(float from, float to, float c) {
+  return from == to ? 1.0f : __builtin_amdgcn_exp2f((from - to) * c);
 }
 __device__ inline Stat join(Stat a, Stat b, float c) {
-  const Shift h(fmaxf(a.m, b.m), c);
-  return {h.m, a.s * rescale(a.m, c, h) + b.s * rescale(b.m, c, h)};
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.s * rescale(a.m, m, c) + b.s * rescale(b.m, m, c)};
 }
-// A thread's pair as it grows, with the offset of its maximum.
+// A thread's pair as it grows, its sum at the offset of its maximum.
 struct Running {
   float m = -INFINITY, s = 0.0f, mc = 0.0f;
   template <int N>
@@ -75,12 +76,14 @@ struct Running {
     for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
     if (top > m) {
       const Shift h(top, c);
-      s *= rescale(m, c, h);
+      float e = mc - h.mc;
+      if (__builtin_expect(h.huge || too_large(mc), 0)) e = (m - top) * c + h.rest(c) - Shift(m, c).rest(c);
+      s *= m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(e);
       m = top;
       mc = h.mc;
     }
     float e[N];
-    if (__builtin_expect(fabsf(mc) == INFINITY, 0)) {
+    if (__builtin_expect(too_large(mc), 0)) {
 #pragma unroll
       for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f((z[i] - m) * c);
     } else {
@@ -93,7 +96,7 @@ struct Running {
       for (int i = 0; i < n; ++i) e[i] += e[i + n];
     s += e[0];
   }
-  __device__ inline Stat stat() const { return {m, s}; }
+  __device__ inline Stat stat(float c) const { return {m, s * __builtin_amdgcn_exp2f(-Shift(m, c).rest(c))}; }
 };
 
 // The block's pair, on every thread.
@@ -217,8 +220,7 @@ struct Teacher {
 // loss of a row from the pair of its logits; every thread calls it.
 template <int WAVES>
 __device__ inline void write_loss(const Args &a, int row, const Entries &e, Stat st, float weight) {
-  const Shift h(st.m, a.c);
-  const double c = (double)a.c, mc = h.huge ? (double)h.m * c : (double)h.mc, log2s = log2((double)st.s);
+  const double c = (double)a.c, mc = (double)st.m * c, log2s = log2((double)st.s);
   double loss = 0.0;
   for (int i = threadIdx.x; i < a.k; i += WAVES * 64) {
     if (e.index[i] < 0) continue;
@@ -260,7 +262,7 @@ __device__ inline void write_entries(const Args &a, int row, const Entries &e, i
   }
 }
 
-// Dense values: term * g, for a row whose offset does not overflow, or does.
+// Dense values: term * g, for a row whose offset is not too large, or is.
 template <bool HUGE>
 __device__ inline float dense(float z, float c, const Shift &h, float g) {
   return __builtin_amdgcn_exp2f(HUGE ? (z - h.m) * c : fmaf(z, c, -h.mc)) * g;
@@ -376,12 +378,13 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
     const float f[1] = {T::get(in.p[in.edge(threadIdx.x)])};
     run.take(f, a.c);
   }
-  const Stat st = block_join<WAVES>(run.stat(), a.c, lds);
+  const Stat st = block_join<WAVES>(run.stat(a.c), a.c, lds);
   if constexpr (!GRAD) write_loss<WAVES>(a, row, e, st, weight);
   if constexpr (GRAD) {
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
-    const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
+    // no finite logit: p = 0
+    const float g = st.s == 0.0f ? 0.0f : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
     const auto write = [&](auto huge) {
       constexpr bool H = decltype(huge)::value;
       if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
@@ -461,7 +464,7 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
       const float f[1] = {T::get(in.p[in.edge(threadIdx.x)])};
       run.take(f, a.c);
     }
-    const Stat st = block_join<WAVES>(run.stat(), a.c, lds);
+    const Stat st = block_join<WAVES>(run.stat(a.c), a.c, lds);
     if (threadIdx.x == 0) pairs[(int64_t)row * parts + part] = st;
   } else {
     __shared__ Entries e;
@@ -496,7 +499,8 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
     }
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
-    const float g = st.s == 0.0f ? 0.0f : wt * mass / st.s;  // no finite logit: p = 0
+    // no finite logit: p = 0
+    const float g = st.s == 0.0f ? 0.0f : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
     const auto write = [&](auto huge) {
       constexpr bool H = decltype(huge)::value;
       if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
