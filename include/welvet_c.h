@@ -402,10 +402,10 @@ WELVET_API welvet_status welvet_hip_adapters_backward(
 /* Distillation from a teacher's top logits.  Row t < n <= 2^22 holds logits z
  * over the vocabulary (Float32, Float16 or BFloat16; row stride `stride`), and
  * the teacher's k entries (k <= 1024) index[t][k], teacher[t][k] (f32 logits).
- * With temperature T (0 < T, finite): q = softmax of the row's teacher / T,
- * or, where d_teacher_lse [n] is given, exp(teacher / T - teacher_lse[t])
- * (the log-sum of the teacher's whole row at T: q then sums to what its top
- * entries hold); p = softmax(z / T) over the vocabulary;
+ * With temperature T (0 < T, finite as log2(e) / T has to be): q = softmax of
+ * the row's teacher / T, or, where d_teacher_lse [n] is given, exp(teacher / T
+ * - teacher_lse[t]) (the log-sum of the teacher's whole row at T: q then sums
+ * to what its top entries hold); p = softmax(z / T) over the vocabulary;
  *   loss[t] = w T^2 sum_i q_i (log q_i - log p_index(i))
  *   dlogits[t][v] = w T (p_v sum_i q_i - sum of q_i over index(i) = v)
  * with w = weight[t] (d_weight NULL = 1): dlogits is the gradient of the

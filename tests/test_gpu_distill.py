@@ -287,3 +287,11 @@ def test_refusals(stream):
     assert call(logits=z.ptr + 1) == 1
     need = pywelvet.distill_bytes(1, 2, 32000, 3)
     assert need > 0 and call(vocab=32000, ws_bytes=need - 1) == 1 and call(vocab=32000, ws=None) == 1
+
+
+def test_smallest_temperature(stream):
+    """Where log2(e) / T is just a float: the larger logit has all of p."""
+    z, index = np.array([[0.5, 0.25, 0.5, -1.0]], np.float32), np.array([[1]], np.int32)
+    _, grad = run(stream, "float32", z, index, np.zeros((1, 1), np.float32), 4.3e-39, np.array([2.0 ** 126]))
+    T = float(np.float32(4.3e-39))
+    within(grad, 2.0 ** 126 * T * np.array([[0.5, -1.0, 0.5, 0.0]]), 64 * U, "gradient")

@@ -51,3 +51,11 @@ def test_embedding_workspace(n):
         assert got == 0
     else:
         assert got >= n * 4 * (4 if n > 4096 else 2) + -(-n // 32) * 2 * 100 * 4
+
+
+def test_temperatures_without_an_exponent_are_refused():
+    """log2(e) / T has to be a float: below some 4.24e-39 it is not, though 1 / T is."""
+    call = lambda T: pywelvet.distill(1, 1, 8, 16, 1, 16, 16, d_loss=16, temperature=T, status=True)  # noqa: E731
+    for T in (3e-39, 4.2e-39):
+        st = call(T)
+        assert st.code == 1 and b"temperature" in st.message

@@ -601,8 +601,9 @@ welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab, const 
   if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
   if (!sizes_ok(dtype, n, vocab, k) || (n > 0 && (!d_logits || !d_index || !d_teacher)) || (!d_loss && !d_dlogits))
     return make_status(kInvalid, "distill: invalid argument");
-  if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
-    return make_status(kInvalid, "distill: temperature must be positive and finite");
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(c))
+    return make_status(kInvalid, "distill: temperature must be positive and finite, as log2(e) / temperature");
   if (stride < vocab || (d_dlogits && dstride < vocab))
     return make_status(kInvalid, "distill: row stride below vocab %d", vocab);
   const int size = tok::float_size(dtype);
@@ -615,8 +616,8 @@ welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab, const 
     return make_status(kInvalid, "distill: %zu bytes of 16-byte aligned workspace are needed", need);
   welvet_status st = require_device();
   if (st.code || n == 0) return st;
-  const Args a{d_logits, stride,   vocab, k,      d_index,   d_teacher, d_teacher_lse, d_weight, temperature,
-               (float)(1.4426950408889634 / (double)temperature), d_loss, d_dlogits, dstride};
+  const Args a{d_logits, stride, vocab, k, d_index, d_teacher, d_teacher_lse, d_weight, temperature, c,
+               d_loss,   d_dlogits, dstride};
   WH_HIP(tok::with_type(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, d_ws, (hipStream_t)stream); }));
   return ok();
 }
