@@ -413,7 +413,9 @@ WELVET_API welvet_status welvet_hip_adapters_backward(
  * index lies outside [0, vocab) or whose logit is -inf is absent; a row
  * without entries, or of weight 0, has loss 0 and gradient 0 whatever its
  * logits.  A logit of -inf has p = 0 (and an infinite loss where an entry
- * names it); a row without a finite logit has p = 0.  d_loss [n] or
+ * names it); a row without a finite logit has p = 0.  A teacher logit that is
+ * NaN or +inf makes its row's q, loss and gradient what the formulas give: NaN,
+ * or infinite where the teacher's sum is given.  d_loss [n] or
  * d_dlogits may be NULL, not both; d_dlogits may be d_logits (the same
  * stride): the gradient then takes the logits' place. */
 WELVET_API welvet_status welvet_hip_distill_bytes(int32_t dtype, int32_t n, int32_t vocab,

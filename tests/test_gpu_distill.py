@@ -295,3 +295,34 @@ def test_smallest_temperature(stream):
     _, grad = run(stream, "float32", z, index, np.zeros((1, 1), np.float32), 4.3e-39, np.array([2.0 ** 126]))
     T = float(np.float32(4.3e-39))
     within(grad, 2.0 ** 126 * T * np.array([[0.5, -1.0, 0.5, 0.0]]), 64 * U, "gradient")
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("odd", [np.nan, np.inf])
+@pytest.mark.parametrize("n", [4, 256])
+def test_teacher_s_values_not_finite(stream, n, odd, given):
+    """A NaN or infinite teacher logit makes its row's q, so its loss and its
+    whole gradient, NaN (with the teacher's own sum given, an infinite logit's
+    q is infinite: the named column is NaN, the others infinite); so does a row
+    without a finite student logit beside it (0 times NaN).  Other rows keep
+    theirs, bit for bit."""
+    rng = np.random.default_rng(12)
+    z, index, teacher = inputs(rng, "float32", n, 4100, 8, absent=0)
+    lse = np.full(n, 14.0) if given else None
+    clean = run(stream, "float32", z, index, teacher, 1.3, None, lse)
+    teacher[1, 3] = teacher[2, 0] = odd
+    z[2] = -np.inf
+    loss, grad = run(stream, "float32", z, index, teacher, 1.3, None, lse)
+    rest = np.arange(n) % n != 1
+    rest[2] = False
+    assert_bit_equal(loss[rest], clean[0][rest], "loss")
+    assert_bit_equal(grad[rest], clean[1][rest], "gradient")
+    if given and odd == np.inf:
+        named = np.zeros(4100, bool)
+        named[index[1, 3]] = True
+        assert np.isnan(grad[1][named]).all()
+        # p below the float's range is 0, and 0 times infinity NaN
+        assert (np.isposinf(grad[1][~named]) | np.isnan(grad[1][~named])).all()
+    else:
+        assert np.isnan(loss[1]) and np.isnan(grad[1]).all()
+    assert not np.isfinite(loss[2]) and np.isnan(grad[2]).all()

@@ -204,7 +204,8 @@ struct Teacher {
       e.index[i] = index[n];
       e.q[i] = l[n] - log_sum;
     }
-    *mass = a.teacher_lse == nullptr ? 1.0f : sum;
+    // the entries' own sum leaves 1, or NaN where one of them is NaN or +inf
+    *mass = a.teacher_lse == nullptr ? sum / sum : sum;
     return true;
   }
   // e.z, from zs (this row's logits at the entries) or the row itself.
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
     // no finite logit: p = 0
-    const float g = st.s == 0.0f ? 0.0f : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
+    const float g = st.s == 0.0f ? 0.0f * mass : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
     const auto write = [&](auto huge) {
       constexpr bool H = decltype(huge)::value;
       if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
     const Shift h(st.m, a.c);
     const float c = a.c, wt = weight * a.temperature;
     // no finite logit: p = 0
-    const float g = st.s == 0.0f ? 0.0f : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
+    const float g = st.s == 0.0f ? 0.0f * mass : wt * mass / (st.s * __builtin_amdgcn_exp2f(h.rest(c)));
     const auto write = [&](auto huge) {
       constexpr bool H = decltype(huge)::value;
       if ((((uintptr_t)out ^ (uintptr_t)in.p) & 15) == 0) {
