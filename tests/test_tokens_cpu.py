@@ -59,3 +59,14 @@ def test_temperatures_without_an_exponent_are_refused():
     for T in (3e-39, 4.2e-39):
         st = call(T)
         assert st.code == 1 and b"temperature" in st.message
+
+
+def test_gradient_in_place_needs_the_logits_stride():
+    """Rows of another stride would be written over rows not yet read."""
+    call = lambda n, dstride: pywelvet.distill(  # noqa: E731
+        1, n, 8, 16, 1, 16, 16, d_dlogits=16, logits_stride=8, dlogits_stride=dstride, ws=16, ws_bytes=1 << 20,
+        status=True)
+    st = call(2, 9)
+    assert st.code == 1 and b"stride" in st.message
+    if not pywelvet.available():  # accepted: then there is no device
+        assert call(1, 9).code == 2 and call(2, 8).code == 2

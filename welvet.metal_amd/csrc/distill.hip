@@ -607,6 +607,8 @@ welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab, const 
     return make_status(kInvalid, "distill: temperature must be positive and finite, as log2(e) / temperature");
   if (stride < vocab || (d_dlogits && dstride < vocab))
     return make_status(kInvalid, "distill: row stride below vocab %d", vocab);
+  if (n > 1 && d_dlogits == d_logits && dstride != stride)
+    return make_status(kInvalid, "distill: a gradient in the logits' place needs their row stride");
   const int size = tok::float_size(dtype);
   if (!tok::aligned(d_logits, size) || !tok::aligned(d_dlogits, size) || !tok::aligned(d_index, 4) ||
       !tok::aligned(d_teacher, 4) || !tok::aligned(d_teacher_lse, 4) || !tok::aligned(d_weight, 4) ||
