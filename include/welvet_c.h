@@ -400,8 +400,9 @@ WELVET_API welvet_status welvet_hip_adapters_backward(
     float *d_dup, void *d_ws, size_t ws_bytes, void *stream);
 
 /* Distillation from a teacher's top logits.  Row t < n <= 2^22 holds logits z
- * over the vocabulary (Float32, Float16 or BFloat16; row stride `stride`), and
- * the teacher's k entries (k <= 1024) index[t][k], teacher[t][k] (f32 logits).
+ * over the vocabulary (Float32, Float16 or BFloat16; vocab <= 2^31 - 4096; row
+ * stride `stride`), and the teacher's k entries (k <= 1024) index[t][k],
+ * teacher[t][k] (f32 logits).
  * With temperature T (0 < T, finite as log2(e) / T has to be): q = softmax of
  * the row's teacher / T, or, where d_teacher_lse [n] is given, exp(teacher / T
  * - teacher_lse[t]) (the log-sum of the teacher's whole row at T: q then sums

@@ -70,3 +70,16 @@ def test_gradient_in_place_needs_the_logits_stride():
     assert st.code == 1 and b"stride" in st.message
     if not pywelvet.available():  # accepted: then there is no device
         assert call(1, 9).code == 2 and call(2, 8).code == 2
+
+
+@pytest.mark.parametrize("vocab", [2**31 - 1, 2**31 - 65, 2**31 - 70, 2**31 - 512, 2**31 - 4095])
+def test_vocabularies_past_an_int_are_refused(vocab):
+    """A block's steps along a row (up to 512 values past its end) are counted in int."""
+    b = C.c_size_t()
+    for n in (1, 300):
+        assert pywelvet.lib().welvet_hip_distill_bytes(3, n, vocab, 1, C.byref(b)).code == 1
+        assert pywelvet.distill(3, n, vocab, 16, 1, 16, 16, d_loss=16, ws=16, ws_bytes=1 << 30, status=True).code == 1
+
+
+def test_distill_workspace_of_the_largest_vocabulary():
+    assert pywelvet.distill_bytes(3, 1, 2**31 - 4096, 1) >= 512 * 8 + 4

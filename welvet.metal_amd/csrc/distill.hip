@@ -543,7 +543,7 @@ int parts_of(int n, int vocab) {
   if (n == 0 || n >= 256) return 1;
   return std::max(1, std::min((512 + n - 1) / n, vocab / 1024));
 }
-int part_len(int vocab, int parts) { return ((vocab + parts - 1) / parts + 63) / 64 * 64; }
+int part_len(int64_t vocab, int parts) { return (int)(((vocab + parts - 1) / parts + 63) / 64 * 64); }
 size_t pairs_bytes(int n, int vocab) { return pad256((size_t)n * parts_of(n, vocab) * sizeof(Stat)); }
 size_t workspace_bytes(int n, int vocab, int k) {
   return parts_of(n, vocab) == 1 ? 0 : pairs_bytes(n, vocab) + pad256((size_t)n * k * sizeof(float));
@@ -566,7 +566,7 @@ hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
     }
     return hipGetLastError();
   }
-  const int len = part_len(a.vocab, most), parts = (a.vocab + len - 1) / len;
+  const int len = part_len(a.vocab, most), parts = (int)(((int64_t)a.vocab + len - 1) / len);
   Stat *pairs = (Stat *)ws;
   float *zs = (float *)((char *)ws + pairs_bytes(n, a.vocab));
   distill_part_kernel<T, 4, true><<<n * parts, 256, 0, s>>>(a, parts, len, pairs, zs);
@@ -576,8 +576,9 @@ hipError_t launch_distill(const Args &a, int n, void *ws, hipStream_t s) {
   return hipGetLastError();
 }
 
-bool sizes_ok(int32_t dtype, int32_t n, int32_t vocab, int32_t k) {
-  return n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= INT32_MAX - 64 && k > 0 && k <= kMaxEntries;
+// vocab: a thread's steps along a row pass its end in int.
+bool sizes_ok(int32_t n, int32_t vocab, int32_t k) {
+  return n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= INT32_MAX - 4095 && k > 0 && k <= kMaxEntries;
 }
 
 }  // namespace
@@ -590,7 +591,7 @@ extern "C" {
 
 welvet_status welvet_hip_distill_bytes(int32_t dtype, int32_t n, int32_t vocab, int32_t k, size_t *bytes) {
   if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
-  if (!sizes_ok(dtype, n, vocab, k) || !bytes) return make_status(kInvalid, "distill: invalid argument");
+  if (!sizes_ok(n, vocab, k) || !bytes) return make_status(kInvalid, "distill: invalid argument");
   *bytes = workspace_bytes(n, vocab, k);
   return ok();
 }
@@ -600,7 +601,7 @@ welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vocab, const 
                                  const float *d_teacher_lse, const float *d_weight, float temperature, float *d_loss,
                                  void *d_dlogits, int64_t dstride, void *d_ws, size_t ws_bytes, void *stream) {
   if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
-  if (!sizes_ok(dtype, n, vocab, k) || (n > 0 && (!d_logits || !d_index || !d_teacher)) || (!d_loss && !d_dlogits))
+  if (!sizes_ok(n, vocab, k) || (n > 0 && (!d_logits || !d_index || !d_teacher)) || (!d_loss && !d_dlogits))
     return make_status(kInvalid, "distill: invalid argument");
   const float c = (float)(1.4426950408889634 / (double)temperature);
   if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(c))
