@@ -333,14 +333,17 @@ WELVET_API void welvet_hip_swiglu_release(welvet_hip_swiglu *s);
 
 /* Embedding: out[t] = scale * table[tokens[t]], t < n, rows of dim f32 values
  * from a [vocab][dim] table.  A token outside [0, vocab) is padding: a row of
- * zeros.  n <= 2^27, (n + vocab) (dim / 1024 + 2) < 2^31. */
+ * zeros.  dim <= 2^31 - 4096, n <= 2^27, (n + vocab) (dim / 1024 + 2) < 2^31,
+ * and n d < 2^36 with n rounded up to 4 and d = dim rounded up to 256 (above
+ * 1024: to 1024): what one launch takes. */
 WELVET_API welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t dim,
                                                       const void *d_table, int64_t table_stride,
                                                       const int32_t *d_tokens, int32_t n,
                                                       float scale, float *d_out,
                                                       int64_t out_stride, void *stream);
 /* The same from a mounted layer's store [out][in], any dtype, decoded as the
- * layer decodes it: an output layer's weights shared with the embedding. */
+ * layer decodes it: an output layer's weights shared with the embedding.
+ * n (dim / 1024, rounded up) < 2^24. */
 WELVET_API welvet_status welvet_hip_embedding_store_forward(welvet_dense_session *s,
                                                             const int32_t *d_tokens, int32_t n,
                                                             float scale, float *d_out,
@@ -350,7 +353,7 @@ WELVET_API welvet_status welvet_hip_embedding_store_forward(welvet_dense_session
  * that tokens name, the others left as they are (scale = -rate: an SGD step
  * on a Float32 table in place).  Padding's rows of dout are not read.  A
  * token's rows are added in f32 in their own order: the same bits on every
- * run. */
+ * run.  Sizes as above, and n <= 2^26 - 16; up to 256 tokens also n d < 2^33. */
 WELVET_API welvet_status welvet_hip_embedding_backward_bytes(int32_t vocab, int32_t dim,
                                                              int32_t n, size_t *bytes);
 WELVET_API welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t dim,

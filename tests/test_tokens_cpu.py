@@ -83,3 +83,36 @@ def test_vocabularies_past_an_int_are_refused(vocab):
 
 def test_distill_workspace_of_the_largest_vocabulary():
     assert pywelvet.distill_bytes(3, 1, 2**31 - 4096, 1) >= 512 * 8 + 4
+
+
+def embedding_codes(vocab, dim, n):
+    """Codes of the lookup, the gradient's workspace and the gradient."""
+    b = C.c_size_t()
+    return (pywelvet.embedding_forward(1, vocab, dim, 16, 16, n, 16, status=True).code,
+            pywelvet.lib().welvet_hip_embedding_backward_bytes(vocab, dim, n, C.byref(b)).code,
+            pywelvet.embedding_backward(vocab, dim, 16, n, 16, 16, ws=16, ws_bytes=1 << 62, status=True).code)
+
+
+@pytest.mark.parametrize("vocab,dim,n,lookup,gradient", [
+    (100, 256, 2**26 - 16, True, True),
+    (100, 256, 2**26 - 15, True, False),    # the order's 64 threads a row reach 2^32
+    (100, 256, 2**26, True, False),
+    (100, 256, 2**27, True, False),
+    (100, 257, 2**27, False, False),        # 2^25 blocks of 128 threads
+    (100, 512, 2**27 - 4, True, False),
+    (100, 512, 2**27 - 3, False, False),
+    (100, 1024, 2**26 - 64, True, True),
+    (100, 1025, 2**26 - 64, False, False),  # two tiles of columns
+    (2**25, 1024, 300, True, True),
+    (1, 2**31 - 4096, 1, True, True),
+    (1, 2**31 - 4096, 3, True, True),
+    (1, 2**31 - 4096, 16, True, False),     # up to 256 tokens: one a block
+    (1, 2**31 - 4095, 1, False, False),     # a thread's steps along a row pass an int
+    (1, 2**31 - 1, 1, False, False),
+    (1000, 2**31 - 1000, 2**27, False, False)])
+def test_launches_past_32_bits_are_refused(vocab, dim, n, lookup, gradient):
+    """What a launch cannot take is code 1 before anything is enqueued."""
+    codes = embedding_codes(vocab, dim, n) if not pywelvet.available() else None
+    if codes is None:
+        pytest.skip("accepted sizes would be launched")
+    assert codes == (2 if lookup else 1, 0 if gradient else 1, 2 if gradient else 1)

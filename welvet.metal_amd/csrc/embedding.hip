@@ -286,20 +286,35 @@ __global__ void __launch_bounds__(256) finish_kernel(const int32_t *__restrict__
   put_row<ACC, NT>(cols, dtable + (int64_t)mine * tstride, sum, scale);
 }
 
-int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
-
 size_t gradient_bytes(int dim, int n) {
   if (n <= kDirect) return 0;
   const size_t chunks = ((size_t)n + kRun - 1) / kRun;
   return order_bytes(n) + pad256(chunks * 2 * (size_t)dim * sizeof(float));
 }
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads; more go round
-constexpr int kMostZeros = 1 << 26;       // rows that a launch looks up
+constexpr int kMostZeros = 1 << 25;       // rows that a launch looks up
+
+// The kernels' int counters, which pass a row's end by a block's step, and a
+// lookup's threads (four rows each).
+int threads_for(int dim) { return std::min(256, ((dim + 3) / 4 + 63) / 64 * 64); }
+int64_t tiles_for(int dim) { return ((int64_t)dim + 4 * threads_for(dim) - 1) / (4 * threads_for(dim)); }
+bool sizes_ok(int32_t vocab, int32_t dim, int32_t n) {
+  return vocab > 0 && vocab < INT32_MAX && dim > 0 && dim <= INT32_MAX - 4095 && n >= 0 && n <= 1 << 27 &&
+         ((int64_t)n + vocab) * (tiles_for(dim) + 1) < INT32_MAX &&
+         ((int64_t)n + 3) / 4 * tiles_for(dim) * threads_for(dim) <= UINT32_MAX;
+}
+// The gradient's: the order's launch, and up to kDirect tokens a block for each
+// token and tile.  Those of the zero rows beside them have 2^31 threads at most
+// (kMostZeros), the sums' an eighth of a lookup's.
+bool gradient_ok(int32_t vocab, int32_t dim, int32_t n) {
+  return sizes_ok(vocab, dim, n) && order_launchable(n) &&
+         (n > kDirect || n * tiles_for(dim) * threads_for(dim) < (int64_t)1 << 31);
+}
 
 template <bool ACC, bool NARROW>
 hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, float scale, const float *dout,
                            int64_t dstride, float *dtable, int64_t tstride, void *ws, hipStream_t s) {
-  const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
+  const int threads = threads_for(dim), tiles = (int)tiles_for(dim);
   const bool nt = (int64_t)vocab * dim * 4 > kKept;  // the table past the caches
   const bool fill = !ACC && (vocab > kMostZeros || (nt && n <= vocab / 8));
   if (fill) {
@@ -333,12 +348,6 @@ hipError_t launch_gradient(int vocab, int dim, const int32_t *tokens, int n, flo
   return nt && !NARROW ? go(std::true_type{}) : go(std::false_type{});
 }
 
-// A launch's threads (2^32) and the kernels' int counters.
-bool sizes_ok(int32_t vocab, int32_t dim, int32_t n) {
-  return vocab > 0 && vocab < INT32_MAX && dim > 0 && n >= 0 && n <= 1 << 27 &&
-         ((int64_t)n + vocab) * ((dim + 1023) / 1024 + 1) < INT32_MAX;
-}
-
 }  // namespace
 }  // namespace wh
 
@@ -359,7 +368,7 @@ welvet_status welvet_hip_embedding_forward(int32_t dtype, int32_t vocab, int32_t
     return make_status(kInvalid, "embedding: device pointers must be aligned to their elements");
   welvet_status st = require_device();
   if (st.code || n == 0) return st;
-  const int threads = threads_for(dim), tiles = (dim + 4 * threads - 1) / (4 * threads);
+  const int threads = threads_for(dim), tiles = (int)tiles_for(dim);
   // four rows a block where there are blocks enough for every CU several times over
   const int rows = (int64_t)n * tiles >= 8192 ? 4 : 1;
   const uint32_t blocks = (uint32_t)(((int64_t)n + rows - 1) / rows * tiles);
@@ -395,7 +404,7 @@ welvet_status welvet_hip_embedding_store_forward(welvet_dense_session *s, const 
 }
 
 welvet_status welvet_hip_embedding_backward_bytes(int32_t vocab, int32_t dim, int32_t n, size_t *bytes) {
-  if (!sizes_ok(vocab, dim, n) || !bytes) return make_status(kInvalid, "embedding backward: invalid argument");
+  if (!gradient_ok(vocab, dim, n) || !bytes) return make_status(kInvalid, "embedding backward: invalid argument");
   *bytes = gradient_bytes(dim, n);
   return ok();
 }
@@ -404,7 +413,7 @@ welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t dim, const in
                                             float scale, const float *d_dout, int64_t dout_stride, int32_t accumulate,
                                             float *d_dtable, int64_t dtable_stride, void *d_ws, size_t ws_bytes,
                                             void *stream) {
-  if (!sizes_ok(vocab, dim, n) || !d_dtable || (n > 0 && (!d_tokens || !d_dout)))
+  if (!gradient_ok(vocab, dim, n) || !d_dtable || (n > 0 && (!d_tokens || !d_dout)))
     return make_status(kInvalid, "embedding backward: invalid argument");
   if (dout_stride < dim || dtable_stride < dim)
     return make_status(kInvalid, "embedding backward: row stride below dim %d", dim);

@@ -320,6 +320,8 @@ __device__ inline int first_at_least(const int32_t *__restrict__ skey, int n, in
   return lo;
 }
 
+// A launch takes fewer than 2^32 threads, the order's first 1024 for kRankRows rows.
+inline bool order_launchable(int64_t n) { return (n + kRankRows - 1) / kRankRows * 1024 <= UINT32_MAX; }
 inline size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
 // Workspace of the order: skey, order and, past one chunk, the chunks'.
 inline size_t order_bytes(int64_t n) { return pad256((size_t)n * 4) * (n > kChunk ? 4 : 2); }
