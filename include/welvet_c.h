@@ -369,7 +369,8 @@ WELVET_API welvet_status welvet_hip_embedding_backward(int32_t vocab, int32_t di
  * device arrays; adapter a uses its first d_ranks[a] rank rows (NULL: all;
  * the rest is not read) and the factor d_scales[a] (NULL: 1).  Row t of n
  * takes adapter ids[t], none where that lies outside [0, count).
- * count <= 65535, n <= 2^23, n * rank < 2^31, rank * max(in, out) < 2^30. */
+ * count <= 65535, n <= 2^23, n * rank < 2^31, rank * max(in, out) < 2^30, and
+ * n * out (n * in for dx) < 2^36 with n rounded up to 16, widths to 256. */
 typedef struct welvet_hip_adapters {
   int32_t dtype, count, rank, in, out;
   const void *d_down, *d_up;

@@ -116,3 +116,24 @@ def test_launches_past_32_bits_are_refused(vocab, dim, n, lookup, gradient):
     if codes is None:
         pytest.skip("accepted sizes would be launched")
     assert codes == (2 if lookup else 1, 0 if gradient else 1, 2 if gradient else 1)
+
+
+def test_adapters_launches_past_32_bits_are_refused():
+    """The rows' launch: 256 threads for 16 rows and 256 columns; of rows one by
+    one the gradients' blocks, counted in int."""
+    b = C.c_size_t()
+
+    def codes(count, rank, inn, out, n):
+        a = pywelvet.Adapters(1, count, rank, inn, out, 16, 16)
+        on = dict(ws=16, ws_bytes=1 << 62, status=True)
+        return (pywelvet.lib().welvet_hip_adapters_bytes(a._ref, n, C.byref(b)).code,
+                a.forward(16, 16, n, None, 16, **on).code,
+                a.backward(16, 16, n, None, 16, d_dx=16, **on).code,
+                a.backward(16, 16, n, 16, 16, d_ddown=16, d_dup=16, **on).code)
+    if pywelvet.available():
+        pytest.skip("accepted sizes would be launched")
+    assert codes(1, 1, 64, 8192 - 256, 2**23) == (0, 2, 2, 2)
+    assert codes(1, 1, 64, 8192, 2**23) == (0, 1, 2, 2)  # 2^24 blocks
+    assert codes(1, 1, 8191, 64, 2**23) == (0, 2, 1, 2)
+    assert codes(60000, 1, 2**24, 2**24, 1) == (0, 2, 2, 1)
+    assert codes(4, 1, 2**24, 2**24, 1) == (0, 2, 2, 2)

@@ -1045,6 +1045,9 @@ hipError_t launch_slices(const Call &c, const Factor &fac, const Sum &job, bool 
   return hipGetLastError();
 }
 
+// up_kernel's blocks; a launch takes fewer than 2^32 threads.
+int64_t up_blocks(int n, int width) { return (int64_t)((width + 255) / 256) * ((n + 15) / 16); }
+bool rows_launchable(int n, int width) { return up_blocks(n, width) * 256 <= UINT32_MAX; }
 hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const float *base, int64_t bstride, float *y,
                      int64_t ystride, float *hsum) {
   if (c.rows.order == nullptr) {
@@ -1058,7 +1061,7 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
     return hipGetLastError();
   }
   by_rank(fac.rank, [&](auto rt) {
-    const int64_t grid = (int64_t)((fac.width + 255) / 256) * ((c.rows.n + 15) / 16);
+    const int64_t grid = up_blocks(c.rows.n, fac.width);
     const bool nt = (int64_t)c.rows.n * fac.width * 4 > kKept;
     with_type(c.dtype, [&](auto t) {
       const auto go = [&](auto narrow, auto past) {
@@ -1073,32 +1076,35 @@ hipError_t launch_up(const Call &c, const Factor &fac, const Hidden &h, const fl
   return hipGetLastError();
 }
 
-hipError_t launch_few(const Call &c, const Factor &fac, FewSums sums, const Hidden &g, const float *base,
-                      int64_t bstride, float *dx, int64_t dxstride) {
+// Fills in the sums' blocks; false where all of them are too many for int
+// counters (gradients of 2 TB).
+bool plan_few(const RowMap &rows, const Factor &fac, bool dx, FewSums *sums) {
   int64_t grid = 0;
+  by_rank(fac.rank, [&](auto rt) { sums->groups = (fac.rank + 16 * decltype(rt)::value - 1) / (16 * decltype(rt)::value); });
+  const int share = rows.n / rows.count;  // rows of an adapter
+  sums->parts = share >= 128 ? 8 : share >= 64 ? 4 : 2;
+  for (int i = 0; i < sums->count; ++i) {
+    FewSum &job = sums->of[i];
+    job.across = (job.width + 512 / sums->parts - 1) / (512 / sums->parts);
+    job.first = (int)grid;
+    grid += (int64_t)rows.count * sums->groups * job.across;
+    if (grid > INT32_MAX - kFewAcross) return false;
+  }
+  sums->blocks = (int)grid;
+  if (dx) grid += (int64_t)rows.n * ((fac.width + 2047) / 2048);
+  sums->total = (int)grid;
+  return grid <= INT32_MAX - kFewAcross;
+}
+
+hipError_t launch_few(const Call &c, const Factor &fac, const FewSums &sums, const Hidden &g, const float *base,
+                      int64_t bstride, float *dx, int64_t dxstride) {
+  const int grid = sums.total;
+  if (grid == 0) return hipSuccess;
   bool narrow = dx && fac.width < 4;
-  hipError_t e = hipSuccess;
+  for (int i = 0; i < sums.count; ++i) narrow = narrow || sums.of[i].width < 4;
+  const dim3 blocks((uint32_t)std::min(grid, kFewAcross), (uint32_t)((grid + kFewAcross - 1) / kFewAcross));
   by_rank(fac.rank, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-    sums.groups = (fac.rank + 16 * RT - 1) / (16 * RT);
-    const int share = c.rows.n / c.rows.count;  // rows of an adapter
-    sums.parts = share >= 128 ? 8 : share >= 64 ? 4 : 2;
-    for (int i = 0; i < sums.count; ++i) {
-      FewSum &job = sums.of[i];
-      job.across = (job.width + 512 / sums.parts - 1) / (512 / sums.parts);
-      job.first = (int)grid;
-      grid += (int64_t)c.rows.count * sums.groups * job.across;
-      narrow = narrow || job.width < 4;
-    }
-    sums.blocks = (int)grid;
-    if (dx) grid += (int64_t)c.rows.n * ((fac.width + 2047) / 2048);
-    if (grid == 0) return;
-    if (grid > INT32_MAX - kFewAcross) {  // gradients of 2 TB
-      e = hipErrorInvalidValue;
-      return;
-    }
-    sums.total = (int)grid;
-    const dim3 blocks((uint32_t)std::min<int64_t>(grid, kFewAcross), (uint32_t)((grid + kFewAcross - 1) / kFewAcross));
     with_type(c.dtype, [&](auto t) {
       by_flag(c.accumulate, [&](auto acc) {
         by_flag(narrow, [&](auto nar) {
@@ -1108,7 +1114,7 @@ hipError_t launch_few(const Call &c, const Factor &fac, FewSums sums, const Hidd
       });
     });
   });
-  return e != hipSuccess ? e : hipGetLastError();
+  return hipGetLastError();
 }
 
 // `outer`: how many of the sums, from the first on, slice_kernel has not done.
@@ -1237,6 +1243,7 @@ welvet_status welvet_hip_adapters_forward(const welvet_hip_adapters *desc, const
     return make_status(kInvalid, "adapters: row stride below its row");
   for (const void *p : {(const void *)d_x, (const void *)d_ids, (const void *)d_base, (const void *)d_y, (const void *)d_h})
     if (!tok::aligned(p, 4)) return make_status(kInvalid, "adapters: device pointers must be aligned to their elements");
+  if (!rows_launchable(n, desc->out)) return make_status(kInvalid, "adapters: more than a launch takes");
   const Sizes z = sizes_of(*desc, n, false);
   if (z.total() > 0 && (!d_ws || ws_bytes < z.total() || !tok::aligned(d_ws, 16)))
     return make_status(kInvalid, "adapters: %zu bytes of 16-byte aligned workspace are needed", z.total());
@@ -1284,18 +1291,21 @@ welvet_status welvet_hip_adapters_backward(const welvet_hip_adapters *desc, cons
   const Sizes z = sizes_of(*desc, n, true);
   if (z.total() > 0 && (!d_ws || ws_bytes < z.total() || !tok::aligned(d_ws, 16)))
     return make_status(kInvalid, "adapters backward: %zu bytes of 16-byte aligned workspace are needed", z.total());
-  st = require_device();
-  if (st.code) return st;
   Call c{desc->dtype, {d_ids, nullptr, n, desc->count}, (hipStream_t)stream, accumulate != 0};
   const Factor down{desc->d_down, desc->d_ranks, desc->d_scales, desc->rank, desc->in};
   const Factor up{desc->d_up, desc->d_ranks, desc->d_scales, desc->rank, desc->out};
-  if (few_rows(*desc, n, true)) {
-    const Hidden g{(float *)d_ws, n > 0 ? splits_of(n, desc->out) : 1, n, desc->rank};
-    if (n > 0 && (d_dx || d_ddown)) WH_HIP(launch_down_rows(c, up, d_dy, dy_stride, g));
-    FewSums sums{};
-    if (d_ddown) sums.of[sums.count++] = {g, d_x, x_stride, desc->in, 0, 0, d_ddown};
-    if (d_dup) sums.of[sums.count++] = {{const_cast<float *>(d_h), 1, n, desc->rank}, d_dy, dy_stride, desc->out, 0, 0, d_dup};
-    WH_HIP(launch_few(c, down, sums, g, d_dx_base, dx_base_stride, d_dx, dx_stride));
+  const bool few = few_rows(*desc, n, true);
+  const Hidden few_g{(float *)d_ws, few && n > 0 ? splits_of(n, desc->out) : 1, n, desc->rank};
+  FewSums few_sums{};
+  if (d_ddown) few_sums.of[few_sums.count++] = {few_g, d_x, x_stride, desc->in, 0, 0, d_ddown};
+  if (d_dup) few_sums.of[few_sums.count++] = {{const_cast<float *>(d_h), 1, n, desc->rank}, d_dy, dy_stride, desc->out, 0, 0, d_dup};
+  if (few ? !plan_few(c.rows, down, d_dx != nullptr, &few_sums) : d_dx && !rows_launchable(n, desc->in))
+    return make_status(kInvalid, "adapters backward: more than a launch takes");
+  st = require_device();
+  if (st.code) return st;
+  if (few) {
+    if (n > 0 && (d_dx || d_ddown)) WH_HIP(launch_down_rows(c, up, d_dy, dy_stride, few_g));
+    WH_HIP(launch_few(c, down, few_sums, few_g, d_dx_base, dx_base_stride, d_dx, dx_stride));
     return ok();
   }
   char *at = (char *)d_ws;
