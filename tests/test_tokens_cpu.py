@@ -137,3 +137,10 @@ def test_adapters_launches_past_32_bits_are_refused():
     assert codes(1, 1, 8191, 64, 2**23) == (0, 2, 1, 2)
     assert codes(60000, 1, 2**24, 2**24, 1) == (0, 2, 2, 1)
     assert codes(4, 1, 2**24, 2**24, 1) == (0, 2, 2, 2)
+
+
+def test_adapters_workspace_of_another_dtype_is_unsupported():
+    b = C.c_size_t()
+    for dtype in (0, 4, 33):
+        a = pywelvet.Adapters(dtype, 1, 4, 8, 8, 16, 16)
+        assert pywelvet.lib().welvet_hip_adapters_bytes(a._ref, 4, C.byref(b)).code == 2

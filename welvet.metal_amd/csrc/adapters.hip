@@ -1228,6 +1228,8 @@ welvet_status check_call(const char *what, const welvet_hip_adapters *d, int32_t
 extern "C" {
 
 welvet_status welvet_hip_adapters_bytes(const welvet_hip_adapters *desc, int32_t n, size_t *bytes) {
+  if (desc && !tok::float_type(desc->dtype))
+    return make_status(kUnsupported, "adapters: unsupported dtype %d", desc->dtype);
   if (!desc_ok(desc, n) || !bytes) return make_status(kInvalid, "adapters: invalid argument");
   *bytes = std::max(sizes_of(*desc, n, false).total(), sizes_of(*desc, n, true).total());
   return ok();
