@@ -144,3 +144,22 @@ def test_adapters_workspace_of_another_dtype_is_unsupported():
     for dtype in (0, 4, 33):
         a = pywelvet.Adapters(dtype, 1, 4, 8, 8, 16, 16)
         assert pywelvet.lib().welvet_hip_adapters_bytes(a._ref, 4, C.byref(b)).code == 2
+
+
+def accepted(st):
+    """The checks passed: the call ran, or there is no device to run it on."""
+    return st.code != 1
+
+
+@pytest.mark.parametrize("dtype,vocab,k", [(1, 32000, 20), (3, 131072, 64), (2, 50257, 1024), (1, 2047, 5), (3, 5000, 1)])
+def test_distill_workspace_serves_smaller_batches(dtype, vocab, k):
+    """A workspace sized for n rows is enough for every smaller batch, on both
+    sides of the 256 rows from which a row has one block and needs none."""
+    sizes = [pywelvet.distill_bytes(dtype, n, vocab, k) for n in range(0, 600)]
+    assert sizes == sorted(sizes)
+    assert pywelvet.distill_bytes(dtype, 1 << 22, vocab, k) == sizes[-1]
+    if pywelvet.available():
+        return
+    for n in range(1, 300):
+        assert accepted(pywelvet.distill(dtype, n, vocab, 16, k, 16, 16, d_loss=16, ws=16, ws_bytes=sizes[-1],
+                                         status=True))

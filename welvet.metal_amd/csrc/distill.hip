@@ -536,17 +536,25 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
   }
 }
 
+constexpr int kRowBlocks = 256;  // rows from which each has one block
 // Parts of a row: one where there are rows for every CU, else as many as give
 // each CU two blocks, down to 1024 values (4 rows of 32000 f32 logits, loss and
 // gradient: parts of 4096 and up 12.0 us, of 1024 and up 10.9).
 int parts_of(int n, int vocab) {
-  if (n == 0 || n >= 256) return 1;
+  if (n == 0 || n >= kRowBlocks) return 1;
   return std::max(1, std::min((512 + n - 1) / n, vocab / 1024));
 }
 int part_len(int64_t vocab, int parts) { return (int)(((vocab + parts - 1) / parts + 63) / 64 * 64); }
 size_t pairs_bytes(int n, int vocab) { return pad256((size_t)n * parts_of(n, vocab) * sizeof(Stat)); }
 size_t workspace_bytes(int n, int vocab, int k) {
   return parts_of(n, vocab) == 1 ? 0 : pairs_bytes(n, vocab) + pad256((size_t)n * k * sizeof(float));
+}
+
+// Enough for any batch up to n: fewer rows can need more, as more parts.
+size_t most_workspace_bytes(int n, int vocab, int k) {
+  size_t most = 0;
+  for (int rows = 1; rows <= std::min(n, kRowBlocks - 1); ++rows) most = std::max(most, workspace_bytes(rows, vocab, k));
+  return most;
 }
 
 template <class T>
@@ -592,7 +600,7 @@ extern "C" {
 welvet_status welvet_hip_distill_bytes(int32_t dtype, int32_t n, int32_t vocab, int32_t k, size_t *bytes) {
   if (!tok::float_type(dtype)) return make_status(kUnsupported, "distill: unsupported dtype %d", dtype);
   if (!sizes_ok(n, vocab, k) || !bytes) return make_status(kInvalid, "distill: invalid argument");
-  *bytes = workspace_bytes(n, vocab, k);
+  *bytes = most_workspace_bytes(n, vocab, k);
   return ok();
 }
 
