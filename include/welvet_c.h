@@ -323,12 +323,13 @@ WELVET_API void welvet_hip_swiglu_release(welvet_hip_swiglu *s);
  * them.  All pointers named d_ are device memory; every call is enqueued on
  * `stream` (a hipStream_t; NULL = the HIP null stream), returns once enqueued,
  * allocates nothing and may be captured into a HIP graph.  Calls that take a
- * workspace (d_ws, at least the bytes the _bytes call names, 16-byte aligned;
- * NULL where that is 0) own it until the stream has passed them: calls that
- * may overlap need one each.  Strides count elements between rows.  Types are
- * dtype ids: 1 Float32, 2 Float16, 3 BFloat16 (code 2 for others).  Sizes,
- * null or misaligned pointers, strides below a row and short workspaces
- * answer code 1 before anything is enqueued.  Outputs must not overlap
+ * workspace (d_ws, 16-byte aligned; NULL where it is of 0 bytes) own it until
+ * the stream has passed them: calls that may overlap need one each.  The bytes
+ * that a _bytes call names for n rows are enough for every call of n rows or
+ * fewer.  Strides count elements between rows.  Types are dtype ids:
+ * 1 Float32, 2 Float16, 3 BFloat16 (code 2 for others).  Sizes, null or
+ * misaligned pointers, strides below a row and short workspaces answer code 1
+ * before anything is enqueued.  Outputs must not overlap
  * inputs except where a call says so. */
 
 /* Embedding: out[t] = scale * table[tokens[t]], t < n, rows of dim f32 values

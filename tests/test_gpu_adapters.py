@@ -326,3 +326,34 @@ def test_refusals(stream):
     assert bwd(d_dx=dx.ptr, ws_bytes=16) == 1
     with pytest.raises(pywelvet.WelvetError):
         stack(rank=0).workspace_bytes(4)
+
+
+def needed(call):
+    """The bytes that a refused call names, 0 where it takes none."""
+    st = call(ws=None, ws_bytes=0)
+    return int(st.message.split(b" bytes")[0].split()[-1]) if st.code else 0
+
+
+@pytest.mark.parametrize("dtype,inn,out,rank,count,n", [
+    ("float32", 1001, 777, 5, 4, 3), ("bfloat16", 4096, 1024, 16, 8, 64), ("float16", 2048, 512, 64, 4, 300),
+    ("bfloat16", 130, 3000, 33, 7, 2100), ("float32", 320, 64, 32, 5, 5000), ("float16", 513, 257, 16, 2, 2049)])
+def test_workspaces_of_the_needed_size(stream, dtype, inn, out, rank, count, n):
+    """The named workspace serves smaller batches too, so may be larger than
+    this one needs; nothing is written past what it needs."""
+    c = Case(dtype, inn, out, rank, count, n).on_device()
+    y, h = c.forward(stream)
+    dx, dd, du = c.backward(stream, h)
+    o = [Dev(np.full(a.shape, np.nan, np.float32)) for a in (y, h, dx, dd, du)]
+    dh = Dev(h)
+    calls = (lambda **ws: c.a.forward(c.d["x"].ptr, c.d["ids"].ptr, n, c.d["base"].ptr, o[0].ptr, o[1].ptr,
+                                      stream=stream, status=True, **ws),
+             lambda **ws: c.a.backward(c.d["x"].ptr, c.d["ids"].ptr, n, dh.ptr, c.d["dy"].ptr, c.d["dxb"].ptr, o[2].ptr,
+                                       o[3].ptr, o[4].ptr, stream=stream, status=True, **ws))
+    for call in calls:
+        need = needed(call)
+        assert need <= c.a.workspace_bytes(n)
+        ws = Dev(np.full(need, 0xFF, np.uint8))
+        assert call(ws=ws.ptr, ws_bytes=need).code == 0
+        ws.get()
+    for got, want, what in zip(o, (y, h, dx, dd, du), ("y", "h", "dx", "ddown", "dup")):
+        assert_bit_equal(got.get(), want, what)

@@ -163,3 +163,24 @@ def test_distill_workspace_serves_smaller_batches(dtype, vocab, k):
     for n in range(1, 300):
         assert accepted(pywelvet.distill(dtype, n, vocab, 16, k, 16, 16, d_loss=16, ws=16, ws_bytes=sizes[-1],
                                          status=True))
+
+
+@pytest.mark.parametrize("dtype,count,rank,inn,out", [
+    (3, 8, 16, 4096, 4096), (2, 4, 64, 4096, 4096), (3, 8, 32, 4096, 11008), (1, 1, 8, 2048, 8192),
+    (1, 3, 5, 1001, 777), (3, 2, 256, 8192, 64), (1, 5, 1, 1, 1), (2, 4, 130, 515, 20000)])
+def test_adapters_workspace_serves_smaller_batches(dtype, count, rank, inn, out):
+    """A workspace sized for n rows is enough for every smaller batch in both
+    directions, where rows go one by one and where they are sorted into blocks
+    whose length grows with n."""
+    a = pywelvet.Adapters(dtype, count, rank, inn, out, 16, 16)
+    ns = sorted({*range(0, 2100, 7), *(2 ** i + d for i in range(20) for d in (-1, 0, 1, 9)),
+                 *range(2040, 2060), *(16 * i + d for i in range(1, 130) for d in (0, 1))})
+    sizes = [a.workspace_bytes(n) for n in ns]
+    assert sizes == sorted(sizes)
+    if pywelvet.available():
+        return
+    for most in (130, 2049, 8192):
+        on = dict(ws=16, ws_bytes=a.workspace_bytes(most), status=True)
+        for n in (n for n in ns if 0 < n <= most):
+            assert accepted(a.forward(16, 16, n, None, 16, **on)), (n, most)
+            assert accepted(a.backward(16, 16, n, 16, 16, d_dx=16, d_ddown=16, d_dup=16, **on)), (n, most)

@@ -1199,6 +1199,32 @@ Sizes sizes_of(const welvet_hip_adapters &d, int n, bool backward) {
   return z;
 }
 
+// Enough for any batch up to n: few rows have their splits, and blocks of fewer
+// rows can be more.
+size_t most_bytes(const welvet_hip_adapters &d, int n, bool backward) {
+  const size_t row = d.rank * sizeof(float);
+  const int width = backward ? d.out : d.in;
+  // splits_of(r, width) r for r <= n: the width's splits, up to 1024 blocks, at least one
+  const int64_t few = std::min(n, kFewRows);
+  size_t most = pad256(std::max<int64_t>(few, std::min<int64_t>(few * splits_of(1, width), 1024)) * row);
+  if (few_rows(d, n, backward)) return most;
+  Sizes z = sizes_of(d, n, backward);
+  if (backward) {
+    const int groups = rank_groups(d.rank);
+    const auto bytes = [&](int w, int across) {
+      size_t chunks = 0;
+      for (int c = 16; c <= kMaxChunk; c += 16) {  // the most rows in blocks of c
+        const int64_t rows = c == kMaxChunk ? n : std::min<int64_t>(n, (int64_t)c * 512 / (across * groups));
+        chunks = std::max<size_t>(chunks, (rows + c - 1) / c);
+      }
+      return pad256(chunks * 2 * row * w);
+    };
+    z.part[0] = bytes(d.in, (d.in + 255) / 256);
+    z.part[1] = std::max(bytes(d.out, (d.out + 255) / 256), bytes(d.out, slices_of(d.out)));
+  }
+  return std::max(most, z.total());
+}
+
 bool desc_ok(const welvet_hip_adapters *d, int32_t n) {
   return d && n >= 0 && n <= (1 << 23) && (int64_t)n * d->rank <= INT32_MAX && d->count > 0 && d->count <= 65535 &&
          d->rank > 0 && d->rank <= kMaxRank && d->in > 0 && d->out > 0 &&
@@ -1231,7 +1257,7 @@ welvet_status welvet_hip_adapters_bytes(const welvet_hip_adapters *desc, int32_t
   if (desc && !tok::float_type(desc->dtype))
     return make_status(kUnsupported, "adapters: unsupported dtype %d", desc->dtype);
   if (!desc_ok(desc, n) || !bytes) return make_status(kInvalid, "adapters: invalid argument");
-  *bytes = std::max(sizes_of(*desc, n, false).total(), sizes_of(*desc, n, true).total());
+  *bytes = n > 0 ? std::max(most_bytes(*desc, n, false), most_bytes(*desc, n, true)) : 0;
   return ok();
 }
 
