@@ -326,3 +326,24 @@ def test_teacher_s_values_not_finite(stream, n, odd, given):
     else:
         assert np.isnan(loss[1]) and np.isnan(grad[1]).all()
     assert not np.isfinite(loss[2]) and np.isnan(grad[2]).all()
+
+
+@pytest.mark.parametrize("n,vocab,k", [(1, 32000, 20), (37, 9000, 1000), (170, 50257, 64), (255, 4099, 3)])
+def test_workspaces_of_the_needed_size(stream, n, vocab, k):
+    """The named workspace serves smaller batches too, so may be larger than
+    this one needs; nothing is written past what it needs."""
+    rng = np.random.default_rng(n)
+    z, index, teacher = inputs(rng, "bfloat16", n, vocab, k)
+    loss, grad = run(stream, "bfloat16", z, index, teacher)
+    d_z, d_i, d_t, out, d_g = (Dev(a) for a in (z, index, teacher, np.zeros(n, np.float32), np.zeros_like(z)))
+
+    def call(**ws):
+        return pywelvet.distill(3, n, vocab, d_z.ptr, k, d_i.ptr, d_t.ptr, out.ptr, d_g.ptr, stream=stream,
+                                status=True, **ws)
+    need = int(call(ws=None, ws_bytes=0).message.split(b" bytes")[0].split()[-1])
+    assert 0 < need <= pywelvet.distill_bytes(3, n, vocab, k)
+    ws = Dev(np.full(need, 0xFF, np.uint8))
+    assert call(ws=ws.ptr, ws_bytes=need).code == 0
+    ws.get()
+    assert_bit_equal(out.get(), loss, "loss")
+    assert_bit_equal(d_g.get(), grad, "gradient")
