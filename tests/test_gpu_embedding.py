@@ -228,3 +228,36 @@ def test_refusals(stream):
     with pywelvet.Session(np.zeros((4, 8), np.float32), 1) as s:
         assert pywelvet.embedding_store_forward(s, t.ptr, 4, a.ptr, out_stride=7, stream=stream, status=True).code == 1
         assert pywelvet.embedding_store_forward(s, None, 4, a.ptr, stream=stream, status=True).code == 1
+
+
+def sums_in_order(vocab, tok, dout):
+    """The gradient as f32 adds in the documented order: rows by (token, row),
+    in runs of 32 whose sums a token's later runs are added to."""
+    order = np.argsort(np.where((tok >= 0) & (tok < vocab), tok, vocab), kind="stable")
+    out, key = np.zeros((vocab, dout.shape[1]), np.float32), tok[order]
+    total = None
+    for i, t in enumerate(order):
+        if i == 0 or key[i] != key[i - 1] or i % 32 == 0:
+            part = np.zeros(dout.shape[1], np.float32)
+        part = part + dout[t]
+        last = i + 1 == len(order) or key[i + 1] != key[i]
+        if last or i % 32 == 31:
+            total = part if total is None else total + part
+            if last:
+                if 0 <= key[i] < vocab:
+                    out[key[i]] = total
+                total = None
+    return out
+
+
+# one chunk of 2048 sorted rows, joined chunks to 65536 rows, joined spans above
+# (twice from 2^19 on)
+@pytest.mark.parametrize("skewed", [False, True])
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 4095, 16385, 65536, 65537, 100003, 540001])
+def test_gradient_sums_in_row_order(stream, n, skewed):
+    rng = np.random.default_rng([n, skewed])
+    vocab = 3001
+    tok = (np.exp(rng.random(n) * np.log(vocab + 40)) if skewed else rng.integers(-20, vocab + 20, n)).astype(np.int32)
+    dout = rng.normal(0, 1, (n, 2)).astype(np.float32)
+    got = gradient(stream, vocab, 2, tok, dout, 2.0)
+    assert_bit_equal(got, sums_in_order(vocab, tok, dout) * np.float32(2.0), "gradient")

@@ -194,7 +194,7 @@ inline auto with_type(int32_t dtype, F &&f) {
 // four lanes of each of its 16 waves share a row and look at 32 keys each, in
 // words of four from LDS.  More rows than a chunk: each chunk by itself, then
 // every row's places in the other chunks by binary search there, four threads
-// a row.  (2048 rows: 64 rows a block and a lane a row took 8 us on 32 CUs.)
+// a row, up to kSpan rows.  (2048 rows: 64 rows a block and a lane a row took 8 us on 32 CUs.)
 constexpr int kChunk = 2048;
 constexpr int kRankRows = 16;
 
@@ -241,20 +241,21 @@ static __global__ void __launch_bounds__(1024) rank_kernel(const int32_t *__rest
   }
 }
 
-// Joins the sorted chunks: a row's place is its place in its own chunk plus
-// the rows before it in each other one (equal keys of earlier chunks first).
+// Joins the sorted chunks of each `span` rows (whole stages, or all rows): a
+// row's place is its place in its own chunk plus the rows before it in each
+// other one (equal keys of earlier chunks first).
 constexpr int kStage = 8 * kChunk;  // keys in LDS at a time
 static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__restrict__ ckey,
-                                                            const int32_t *__restrict__ corder, int n,
+                                                            const int32_t *__restrict__ corder, int n, int span,
                                                             int32_t *__restrict__ skey, int32_t *__restrict__ order) {
   __shared__ int4 keys4[kStage / 4];
   int32_t *keys = (int32_t *)keys4;
   const int p = blockIdx.x * 256 + (threadIdx.x >> 2), part = threadIdx.x & 3;
-  const int own = p / kChunk;
+  const int own = p / kChunk, begin = (int)blockIdx.x * 256 / span * span, end = min(n, begin + span);
   const int32_t mine = p < n ? ckey[p] : 0;
   int at = 0;
-  for (int s0 = 0; s0 < n; s0 += kStage) {
-    const int len = min(kStage, n - s0);
+  for (int s0 = begin; s0 < end; s0 += kStage) {
+    const int len = min(kStage, end - s0);
     __syncthreads();
     for (int j = threadIdx.x; j < len / 4; j += 1024) keys4[j] = *(const int4 *)(ckey + s0 + 4 * j);
     if ((int)threadIdx.x < (len & 3)) keys[len / 4 * 4 + threadIdx.x] = ckey[s0 + len / 4 * 4 + threadIdx.x];
@@ -275,9 +276,40 @@ static __global__ void __launch_bounds__(1024) merge_kernel(const int32_t *__res
   at += __shfl_xor(at, 1);
   at += __shfl_xor(at, 2);
   if (p < n && part == 0) {
-    at += p - own * kChunk;
+    at += begin + p - own * kChunk;
     skey[at] = mine;
     order[at] = corder[p];
+  }
+}
+
+// Joins each eight neighbouring runs of `run` sorted rows, eight threads a row:
+// every one searches a run of the row's eight in memory.
+static __global__ void __launch_bounds__(256) join_kernel(const int32_t *__restrict__ rkey,
+                                                          const int32_t *__restrict__ rorder, int n, int run,
+                                                          int32_t *__restrict__ skey, int32_t *__restrict__ order) {
+  const int p = (int)blockIdx.x * 32 + (threadIdx.x >> 3), part = threadIdx.x & 7;
+  const int own = p / run, first = own / 8 * 8;
+  const int32_t mine = p < n ? rkey[p] : 0;
+  const int64_t begin = (int64_t)(first + part) * run;
+  const int other = first + part;
+  int at = 0;
+  if (p < n && begin < n && other != own) {
+    const int32_t *keys = rkey + begin;
+    const int32_t bound = mine + (other < own ? 1 : 0);
+    int hi = (int)min((int64_t)run, n - begin);
+    while (at < hi) {
+      const int mid = (at + hi) >> 1;
+      if (keys[mid] < bound) at = mid + 1;
+      else hi = mid;
+    }
+  }
+  at += __shfl_xor(at, 1);
+  at += __shfl_xor(at, 2);
+  at += __shfl_xor(at, 4);
+  if (p < n && part == 0) {
+    at += first * run + p - own * run;
+    skey[at] = mine;
+    order[at] = rorder[p];
   }
 }
 
@@ -328,18 +360,36 @@ inline size_t order_bytes(int64_t n) { return pad256((size_t)n * 4) * (n > kChun
 struct Order {
   int32_t *skey, *order;
 };
+// Rows up to which one launch joins all chunks; its reads grow with the square
+// of the rows.  More are joined in spans of as many, eight neighbours at a time
+// (a gradient's whole call, us, by spans and in one launch: 100000 rows 76 / 74,
+// 131072 91 / 92, 262144 165 / 226, 2^20 708 / 2247; with spans of 32768 50000
+// rows take 52.5 for 49.9).
+constexpr int kSpan = 4 * kStage;
 inline hipError_t launch_order(const int32_t *key, int n, int32_t limit, void *ws, Order *out, hipStream_t s) {
   const size_t step = pad256((size_t)n * 4);
-  char *p = (char *)ws;
-  out->skey = (int32_t *)p;
-  out->order = (int32_t *)(p + step);
-  const bool one = n <= kChunk;
-  int32_t *ck = one ? out->skey : (int32_t *)(p + 2 * step), *co = one ? out->order : (int32_t *)(p + 3 * step);
-  rank_kernel<<<(n + kRankRows - 1) / kRankRows, 1024, 0, s>>>(key, n, (uint32_t)limit, ck, co);
+  int32_t *at[4];
+  for (int i = 0; i < 4; ++i) at[i] = (int32_t *)((char *)ws + i * step);
+  *out = {at[0], at[1]};
+  int passes = n > kChunk ? 1 : 0;  // each from one pair of arrays to the other, the last to the first
+  for (int64_t run = kSpan; run < n; run *= 8) ++passes;
+  int32_t *from_key = at[passes % 2 * 2], *from = at[passes % 2 * 2 + 1];
+  rank_kernel<<<(n + kRankRows - 1) / kRankRows, 1024, 0, s>>>(key, n, (uint32_t)limit, from_key, from);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || one) return e;
-  merge_kernel<<<(n + 255) / 256, 1024, 0, s>>>(ck, co, n, out->skey, out->order);
-  return hipGetLastError();
+  for (int64_t run = 0; e == hipSuccess && passes > 0; --passes) {
+    int32_t *to_key = at[(passes - 1) % 2 * 2], *to = at[(passes - 1) % 2 * 2 + 1];
+    if (run == 0) {
+      merge_kernel<<<(n + 255) / 256, 1024, 0, s>>>(from_key, from, n, kSpan, to_key, to);
+      run = kSpan;
+    } else {
+      join_kernel<<<(n + 31) / 32, 256, 0, s>>>(from_key, from, n, (int)run, to_key, to);
+      run *= 8;
+    }
+    e = hipGetLastError();
+    from_key = to_key;
+    from = to;
+  }
+  return e;
 }
 
 }  // namespace tok
