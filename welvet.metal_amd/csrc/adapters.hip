@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kDownWaves * 64) down_row_kernel(RowMap rows, 
 struct Sum {
   const float *hidden, *x;
   int64_t xstride;
-  int width, chunk, across;  // chunk: rows of a block; across: blocks along the width
+  int width, chunk;  // chunk: rows of a block
   float *grad, *part;
 };
 template <bool ACC, int RT, bool NARROW>
@@ -655,29 +655,22 @@ __global__ void __launch_bounds__(256) up_row_kernel(RowMap rows, Factor fac, Hi
 // rank][j = column]: a wave 64 columns (as above), four rows an MFMA, DEPTH
 // MFMA steps of loads ahead.  A block takes `chunk` positions of the sorted
 // rows, half a block's waves every second four of them: long runs keep twice
-// the loads in flight.  A launch does the sums of both factors where both are
-// asked for.  x of 8192 x 4096, rank 32: 46 us, 2.9 TB/s; its MFMAs would take
-// 14, the rest waits for loads at three waves a SIMD.
-struct Sums {
-  Sum of[2];
-  int count;
-};
+// the loads in flight.  It serves ddown, and dup where that is asked for alone:
+// beside others dup's sums are slice_kernel's.  x of 8192 x 4096, rank 32: 46
+// us, 2.9 TB/s; its MFMAs would take 14, the rest waits for loads at three
+// waves a SIMD.
 template <bool ACC, int RT, bool NARROW>
-__global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) outer_kernel(RowMap rows, Factor fac, Sums sums) {
+__global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) outer_kernel(RowMap rows, Factor fac, Sum job) {
   constexpr int DEPTH = RT >= 4 ? 4 : 8;
   __shared__ float4 half_s[RT][4][256];
   // the rows' offsets: a 64-bit product for each load costs as much as its MFMAs
   __shared__ int64_t x_s[kMaxChunk];
   __shared__ int h_s[kMaxChunk], key_s[kMaxChunk];
-  const bool second = (int)blockIdx.x >= sums.of[0].across;
-  const Sum &job = sums.of[second ? 1 : 0];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), lo = lane & 15, q = lane >> 4;
-  const int across = (int)blockIdx.x - (second ? sums.of[0].across : 0);
   const int j0 = blockIdx.z * RT * 16;
   const int width = job.width, chunk = job.chunk, p0 = (int)blockIdx.y * chunk;
-  if (p0 >= rows.n) return;
-  const Cols<NARROW> cols(across * 256 + wave * 64 + 4 * lo, width);
+  const Cols<NARROW> cols((int)blockIdx.x * 256 + wave * 64 + 4 * lo, width);
   const int p1 = min(p0 + chunk, rows.n);
   for (int i = threadIdx.x; i < p1 - p0; i += 512) {
     const int row = rows.row(p0 + i);
@@ -760,6 +753,10 @@ __global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) outer_kernel(RowMap rows,
 
 // The adapters that no block wrote whole: their partials added up in order,
 // zeros for those no row names.
+struct Sums {
+  Sum of[2];
+  int count;
+};
 // WORDS: 16-byte words a thread, one where the values are few.
 template <bool ACC, int WORDS>
 __global__ void __launch_bounds__(256) sum_kernel(RowMap rows, Factor fac, Sums sums) {
@@ -931,7 +928,7 @@ __global__ void __launch_bounds__(512, RT > 2 ? 2 : 4) few_kernel(RowMap rows, F
     __syncthreads();
   }
   if (part == 0) {
-    const Sum to{nullptr, nullptr, 0, job.width, 0, 0, job.grad, nullptr};
+    const Sum to{nullptr, nullptr, 0, job.width, 0, job.grad, nullptr};
     store_sums<ACC>(acc, fac, a, ra, j0, q, cols, true, false, to);
   }
 }
@@ -1117,25 +1114,17 @@ hipError_t launch_few(const Call &c, const Factor &fac, const FewSums &sums, con
   return hipGetLastError();
 }
 
-// `outer`: how many of the sums, from the first on, slice_kernel has not done.
-hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int outer, bool accumulate) {
-  int across = 0, chunks = 0;
+// `outer`: the one of the sums that slice_kernel has not done, if any.
+hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, const Sum *outer) {
   int64_t size = 0;
-  bool narrow = false;
-  for (int i = 0; i < sums.count; ++i) {
-    if (i < outer) {
-      across += sums.of[i].across;
-      narrow = narrow || sums.of[i].width < 4;
-      chunks = std::max(chunks, (c.rows.n + sums.of[i].chunk - 1) / sums.of[i].chunk);
-    }
-    size = std::max(size, (int64_t)fac.rank * sums.of[i].width);
-  }
-  if (c.rows.n > 0 && outer > 0) by_rank(fac.rank, [&](auto rt) {
+  for (int i = 0; i < sums.count; ++i) size = std::max(size, (int64_t)fac.rank * sums.of[i].width);
+  if (outer) by_rank(fac.rank, [&](auto rt) {
     constexpr int RT = decltype(rt)::value;
-    const dim3 grid(across, chunks, (fac.rank + 16 * RT - 1) / (16 * RT));
-    by_flag(accumulate, [&](auto acc) {
-      by_flag(narrow, [&](auto nar) {
-        outer_kernel<decltype(acc)::value, RT, decltype(nar)::value><<<grid, 512, 0, c.s>>>(c.rows, fac, sums);
+    const dim3 grid((outer->width + 255) / 256, (c.rows.n + outer->chunk - 1) / outer->chunk,
+                    (fac.rank + 16 * RT - 1) / (16 * RT));
+    by_flag(c.accumulate, [&](auto acc) {
+      by_flag(outer->width < 4, [&](auto nar) {
+        outer_kernel<decltype(acc)::value, RT, decltype(nar)::value><<<grid, 512, 0, c.s>>>(c.rows, fac, *outer);
       });
     });
   });
@@ -1144,7 +1133,7 @@ hipError_t launch_sums(const Call &c, const Factor &fac, const Sums &sums, int o
   const bool wide = size * c.rows.count * sums.count >= (int64_t)4096 * 1024;  // four blocks a CU at four words
   const int per = wide ? 4096 : 1024;
   const dim3 grid((uint32_t)((size + per - 1) / per), c.rows.count, sums.count);
-  by_flag(accumulate, [&](auto acc) {
+  by_flag(c.accumulate, [&](auto acc) {
     by_flag(wide, [&](auto w) {
       sum_kernel<decltype(acc)::value, decltype(w)::value ? 4 : 1><<<grid, 256, 0, c.s>>>(c.rows, fac, sums);
     });
@@ -1294,7 +1283,7 @@ welvet_status welvet_hip_adapters_forward(const welvet_hip_adapters *desc, const
   at += z.order;
   float *one = d_h ? d_h : (float *)at, *slices = (float *)(at + z.one);
   const int chunk = forward_chunk_of(n, slices_of(desc->in) * rank_groups(desc->rank));
-  const Sum job{nullptr, d_x, x_stride, desc->in, chunk, 0, nullptr, nullptr};
+  const Sum job{nullptr, d_x, x_stride, desc->in, chunk, nullptr, nullptr};
   WH_HIP(launch_slices(c, down, job, false, false, slices, one));
   WH_HIP(launch_up(c, up, Hidden{one, 1, n, desc->rank}, d_base, base_stride, d_y, y_stride, nullptr));
   return ok();
@@ -1340,26 +1329,25 @@ welvet_status welvet_hip_adapters_backward(const welvet_hip_adapters *desc, cons
   float *const g = (float *)(at + z.order), *const slices = (float *)(at + z.order + z.one);
   float *const part = (float *)(at + z.order + z.one + z.hidden), *const part2 = (float *)((char *)part + z.part[0]);
   const int groups = rank_groups(desc->rank);
-  const bool need_g = n > 0 && (d_dx || d_ddown), fused = need_g && d_dup;
+  const bool need_g = d_dx || d_ddown, fused = need_g && d_dup;
   const auto sum_of = [&](const float *hidden, const float *x, int64_t stride, int width, float *grad, float *part, bool slice) {
     const int across = slice ? slices_of(width) : (width + 255) / 256;
-    return Sum{hidden, x, stride, width, chunk_of(n, across * groups), across, grad, part};
+    return Sum{hidden, x, stride, width, chunk_of(n, across * groups), grad, part};
   };
   const Sum dup = sum_of(d_h, d_dy, dy_stride, desc->out, d_dup, part2, need_g);
-  if (n > 0) {
-    tok::Order o;
-    WH_HIP(tok::launch_order(d_ids, n, desc->count, at, &o, c.s));
-    c.rows.key = o.skey;
-    c.rows.order = o.order;
-  }
-  if (need_g) WH_HIP(launch_slices(c, up, dup, fused, accumulate != 0, slices, g));
-  if (n > 0 && d_dx)
+  tok::Order o;
+  WH_HIP(tok::launch_order(d_ids, n, desc->count, at, &o, c.s));
+  c.rows.key = o.skey;
+  c.rows.order = o.order;
+  if (need_g) WH_HIP(launch_slices(c, up, dup, fused, c.accumulate, slices, g));
+  if (d_dx)
     WH_HIP(launch_up(c, down, Hidden{g, 1, n, desc->rank}, d_dx_base, dx_base_stride, d_dx, dx_stride, nullptr));
   Sums sums{};
   if (d_ddown) sums.of[sums.count++] = sum_of(g, d_x, x_stride, desc->in, d_ddown, part, false);
-  const int outer = sums.count + (d_dup && !fused ? 1 : 0);
   if (d_dup) sums.of[sums.count++] = dup;
-  if (sums.count) WH_HIP(launch_sums(c, down, sums, outer, accumulate != 0));
+  // ddown, or dup alone; the slices have done dup beside dx, with no ddown
+  const Sum *outer = d_ddown || !fused ? &sums.of[0] : nullptr;
+  if (sums.count) WH_HIP(launch_sums(c, down, sums, outer));
   return ok();
 }
 
