@@ -261,3 +261,32 @@ def test_gradient_sums_in_row_order(stream, n, skewed):
     dout = rng.normal(0, 1, (n, 2)).astype(np.float32)
     got = gradient(stream, vocab, 2, tok, dout, 2.0)
     assert_bit_equal(got, sums_in_order(vocab, tok, dout) * np.float32(2.0), "gradient")
+
+
+# one column less and more than a block's 1024, several blocks, one column
+@pytest.mark.parametrize("dim", [1, 1023, 1025, 2051])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "fp8e4m3", "int8", "int4", "nf4", "fp4", "uint8", "binary",
+                                   "ternary", "int64", "complex64"])
+def test_store_lookup_of_wide_rows(stream, dtype, dim):
+    rng = np.random.default_rng(dim)
+    W = rng.normal(0, 1, (33, dim)).astype(np.float32)
+    tok = rng.integers(-2, 36, 300).astype(np.int32)
+    tok[:2] = 32, 0
+    with pywelvet.Session(W, 1, dtype=pywelvet.DTYPE[dtype]) as s:
+        values = s.export_f32()
+        d_k, out = Dev(tok), Dev(np.full((300, dim + 1), 9.0, np.float32))
+        pywelvet.embedding_store_forward(s, d_k.ptr, 300, out.ptr, scale=-0.5, out_stride=dim + 1, stream=stream)
+        got = out.get()
+    there = (tok >= 0) & (tok < 33)
+    want = np.where(there[:, None], values[np.where(there, tok, 0)] * np.float32(-0.5), np.float32(0))
+    assert_bit_equal(got[:, :dim], want.astype(np.float32), dtype)
+    assert (got[:, dim] == 9.0).all()
+
+
+def test_store_lookup_of_a_zero_scale(stream):
+    """A store whose scale is 0 decodes as 1, as in the layer's own products."""
+    raw = np.random.default_rng(1).integers(-128, 128, (5, 30)).astype(np.int8)
+    with pywelvet.Session((5, 30), 1, dtype=pywelvet.DTYPE["int8"], native=(raw.view(np.uint8).reshape(-1), 0.0)) as s:
+        d_k, out = Dev(np.arange(5, dtype=np.int32)), Dev(np.full((5, 30), 9.0, np.float32))
+        pywelvet.embedding_store_forward(s, d_k.ptr, 5, out.ptr, stream=stream)
+        assert_bit_equal(out.get(), raw.astype(np.float32), "rows")

@@ -184,3 +184,12 @@ def test_adapters_workspace_serves_smaller_batches(dtype, count, rank, inn, out)
         for n in (n for n in ns if 0 < n <= most):
             assert accepted(a.forward(16, 16, n, None, 16, **on)), (n, most)
             assert accepted(a.backward(16, 16, n, 16, 16, d_dx=16, d_ddown=16, d_dup=16, **on)), (n, most)
+
+
+@pytest.mark.parametrize("n", [257, 2047, 2048, 2049, 4096, 4097, 65536, 65537, 600001])
+def test_embedding_workspace_by_chunks(n):
+    """The order's two arrays, four past one chunk of 2048 tokens, and two
+    partial rows for every 32 tokens; not less for more tokens."""
+    got = pywelvet.embedding_backward_bytes(5000, 100, n)
+    assert got >= n * 4 * (4 if n > 2048 else 2) + -(-n // 32) * 2 * 100 * 4
+    assert got <= pywelvet.embedding_backward_bytes(5000, 100, n + 1)
