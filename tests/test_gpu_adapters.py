@@ -357,3 +357,29 @@ def test_workspaces_of_the_needed_size(stream, dtype, inn, out, rank, count, n):
         ws.get()
     for got, want, what in zip(o, (y, h, dx, dd, du), ("y", "h", "dx", "ddown", "dup")):
         assert_bit_equal(got.get(), want, what)
+
+
+@pytest.mark.parametrize("n", [40, 2200])
+@pytest.mark.parametrize("rank", [12, 20, 64])
+@pytest.mark.parametrize("dtype", DT)
+def test_small_activations(stream, dtype, rank, n):
+    """Activations and gradients near the type's least normal values (some
+    below, whose last bits count) through large factors: as near, norm-wise, as
+    ordinary ones."""
+    c = Case(dtype, 200, 640, rank, 2, n, ranks=[rank, rank - 3], scales=False, junk=False)
+    factor = 2.0 ** (12 if dtype == "float16" else 100)
+    for name in ("down", "up"):
+        setattr(c, name, to_bits(to_f64(getattr(c, name), dtype) * factor, dtype))
+    c.x, c.dy = c.x * np.float32(1e-37), c.dy * np.float32(1e-37)
+    c.on_device()
+    _, h = c.forward(stream, base=False)
+    down = c.down
+    c.down = to_bits(to_f64(down, dtype) / factor, dtype)  # dx of the size of g
+    c.on_device()
+    dx, _, _ = c.backward(stream, h, dxb=False)
+    far = 2.0 ** 100
+    for a, rows, back, up, s in c.groups():
+        want = far * (c.x[rows].astype(np.float64) @ to_f64(down[a, :len(back)], dtype).T)
+        norm_close(far * h[rows, :len(back)].astype(np.float64), want, 1e-6, "h")
+        want = far * (c.dy[rows].astype(np.float64) @ up.T) @ back
+        norm_close(far * dx[rows].astype(np.float64), want, 3e-6, "dx")

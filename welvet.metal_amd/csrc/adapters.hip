@@ -223,9 +223,16 @@ __device__ inline void store_sums(const v4f (&acc)[RT][4], const Factor &fac, in
 // f32 products at the bf16 MFMA's rate, for 16-bit factors: x is cut into
 // three bf16 parts without rounding (8 + 8 + 8 significand bits), a bf16 value
 // is one part and an f16 value (11 bits) two, so the part products are exact;
-// of f16's six the smallest, below 2^-24 of the product, is left out.  Where a
-// sum comes out as Inf or NaN (a part product can be one where the product is
-// not) the caller does it again by f32 products.
+// of f16's six the smallest, below 2^-24 of the product, is left out.  The caller
+// does again by f32 products
+//   sums that come out as Inf or NaN: a part product can be one where the
+//   product is not;
+//   sums of values below 2^-110 with bits below 2^-133, where bf16 ends.  In 64
+//   columns those come to less than 2^-127 of the largest factor value: half an
+//   ulp of a sum of kSmallSum while that is below kLargeFactor.  So values are
+//   looked at where a sum is smaller, or the factor has a larger one.
+constexpr uint32_t kSmallSum = 47u << 23;           // 2^-80, as bits
+constexpr uint32_t kLargeFactor = (127 + 23) << 7;  // 2^23, as bf16's
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ inline v4f mfma16(const uint4 &a, const uint4 &b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -246,6 +253,16 @@ __device__ inline uint4 take_part(uint4 (&v)[2]) {
   }
   return part;
 }
+__device__ inline void pin(uint4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+// Whether two parts leave one of the eight values more than a third holds.
+__device__ inline bool past_parts(const uint4 &a, const uint4 &b) {
+  uint4 v[2] = {a, b};
+  pin(v[0]);  // cut anew, rather than kept from the products
+  pin(v[1]);
+  take_part(v);
+  take_part(v);
+  return ((v[0].x | v[0].y | v[0].z | v[0].w | v[1].x | v[1].y | v[1].z | v[1].w) & 0xffff) != 0;
+}
 // Two quads of a 16-bit factor as parts.
 template <class T>
 __device__ inline void factor_parts(const Quad<T> &a, const Quad<T> &b, uint4 (&p)[2]) {
@@ -258,7 +275,6 @@ __device__ inline void factor_parts(const Quad<T> &a, const Quad<T> &b, uint4 (&
     p[1] = take_part(v);
   }
 }
-__device__ inline void pin(uint4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 // Value i of eight from its parts (exact).
 template <class T>
 __device__ inline float from_parts(const uint4 (&p)[2], int i) {
@@ -348,6 +364,17 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 #pragma unroll
           for (int i = 0; i < 2; ++i) factor_parts(fv[t][2 * i], fv[t][2 * i + 1], fp[t][i]);
       }
+      bool large = false;  // a factor value not below kLargeFactor
+      if constexpr (std::is_same_v<T, BF16>) {  // f16's are below
+        uint32_t most = 0;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            most = max(max(most, max(fv[t][m].v.x & 0x7fff, fv[t][m].v.x >> 16 & 0x7fff)),
+                       max(fv[t][m].v.y & 0x7fff, fv[t][m].v.y >> 16 & 0x7fff));
+        large = __any(most >= kLargeFactor);
+      }
       Quad<F32> xv[2][4];
       constexpr int kHidden = (RT * 256 + kSlice - 1) / kSlice;  // a thread's hidden values of a tile
       float hn[kHidden];
@@ -422,12 +449,22 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
               acc[t] = mfma16(hi, fp[t][i][0], acc[t]);
             }
           }
-          bool odd = false;
+          // outside [kSmallSum, infinity): below it the difference wraps
+          uint32_t far = 0;
 #pragma unroll
           for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) odd = odd || !isfinite(acc[t][r]);
-          if (__builtin_expect(__any(odd), 0)) {
+            for (int r = 0; r < 4; ++r) far = max(far, (f2u(acc[t][r]) << 1) - (kSmallSum << 1));
+          bool odd = large || __any(far >= (0x7f800000u - kSmallSum) << 1);
+          if (__builtin_expect(odd, 0)) {
+            bool again = past_parts(xv[d][0].v, xv[d][1].v) || past_parts(xv[d][2].v, xv[d][3].v);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) again = again || !isfinite(acc[t][r]);
+            odd = __any(again);
+          }
+          if (__builtin_expect(odd, 0)) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
               acc[t] = v4f{0, 0, 0, 0};
