@@ -17,7 +17,7 @@
 // rank 8 n256: 16.3).  Many rows are sorted by their adapters (tokens.hpp), so
 // that an adapter's rows pass a factor held in registers, and cost about the
 // activations' bytes (bf16 4096x4096 rank 16 n8192 forward: 89 us, 403 MB at
-// 4.5 TB/s; backward bf16 4096x11008 rank 32 n8192: 277 us, 787 MB at 2.8 TB/s,
+// 4.5 TB/s; backward bf16 4096x11008 rank 32 n8192: 281 us, 787 MB at 2.8 TB/s,
 // of which the matrix pipe would take 105 with f32 MFMAs alone).  Rows of
 // different adapters never share a sum, so no value of another tenant's factor
 // reaches a row, NaN or not.
@@ -299,7 +299,7 @@ __device__ inline float from_parts(const uint4 (&p)[2], int i) {
 // adapter's rows of job.hidden[row][j] x[row][c] (outer_kernel below has its
 // terms), so that x is read from HBM once for both: a wave's 16 x 64 part is
 // turned in LDS to the columns-by-rows order of that product (bf16 4096x11008
-// rank 32 n8192, dy's 361 MB: 144 us, 2.5 TB/s; its MFMAs 45 and the turning's
+// rank 32 n8192, dy's 361 MB: 145 us, 2.5 TB/s; its MFMAs 45 and the turning's
 // LDS traffic 22 do not lie wholly under the loads).
 constexpr int kSliceWaves = 8;
 constexpr int kSlice = kSliceWaves * 64;

@@ -299,9 +299,9 @@ __device__ inline uint4 get_word(const uint4 *p) {
 // teacher's loads go out first, then the row's, and the teacher's arithmetic
 // runs while those are under way.  Two blocks a CU, so that one's exponentials
 // (about 200 us of the whole) run under the other's loads and stores: 4096 x
-// 131072 bf16, an eighth of the rows left out, takes 418 us with 8 waves and
-// 8 + 8 words held, 438 with 8 + 0, 573 with 16 waves and the whole row in
-// registers (one block a CU).
+// 131072 bf16, 15 % of the rows left out, takes 423 us with 8 waves and 8 + 8
+// words held; 8 + 0 took 20 more, 16 waves with the whole row in registers (one
+// block a CU) 155.
 template <class T, int WAVES, int HOLD, int LDSW, bool GRAD>
 __global__ void __launch_bounds__(WAVES * 64, 4) distill_row_kernel(Args a) {
   constexpr int kThreads = WAVES * 64;
@@ -539,7 +539,8 @@ __global__ void __launch_bounds__(WAVES * 64) distill_part_kernel(Args a, int pa
 constexpr int kRowBlocks = 256;  // rows from which each has one block
 // Parts of a row: one where there are rows for every CU, else as many as give
 // each CU two blocks, down to 1024 values (4 rows of 32000 f32 logits, loss and
-// gradient: parts of 4096 and up 12.0 us, of 1024 and up 10.9).
+// gradient, calls one after the other: parts of 4096 and up 10.6 us, of 1024 and
+// up 9.7; 64 rows of 32000 bf16 14.8 and 14.0).
 int parts_of(int n, int vocab) {
   if (n == 0 || n >= kRowBlocks) return 1;
   return std::max(1, std::min((512 + n - 1) / n, vocab / 1024));
