@@ -361,13 +361,14 @@ def test_workspaces_of_the_needed_size(stream, dtype, inn, out, rank, count, n):
 
 @pytest.mark.parametrize("n", [40, 2200])
 @pytest.mark.parametrize("rank", [12, 20, 64])
-@pytest.mark.parametrize("dtype", DT)
-def test_small_activations(stream, dtype, rank, n):
+@pytest.mark.parametrize("dtype,power", [("float32", 100), ("float16", 12), ("bfloat16", 12), ("bfloat16", 22),
+                                         ("bfloat16", 100)])
+def test_small_activations(stream, dtype, power, rank, n):
     """Activations and gradients near the type's least normal values (some
     below, whose last bits count) through large factors: as near, norm-wise, as
     ordinary ones."""
     c = Case(dtype, 200, 640, rank, 2, n, ranks=[rank, rank - 3], scales=False, junk=False)
-    factor = 2.0 ** (12 if dtype == "float16" else 100)
+    factor = 2.0 ** power
     for name in ("down", "up"):
         setattr(c, name, to_bits(to_f64(getattr(c, name), dtype) * factor, dtype))
     c.x, c.dy = c.x * np.float32(1e-37), c.dy * np.float32(1e-37)
@@ -383,3 +384,18 @@ def test_small_activations(stream, dtype, rank, n):
         norm_close(far * h[rows, :len(back)].astype(np.float64), want, 1e-6, "h")
         want = far * (c.dy[rows].astype(np.float64) @ up.T) @ back
         norm_close(far * dx[rows].astype(np.float64), want, 3e-6, "dx")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_dx_of_sorted_rows_does_not_depend_on_dup(stream, dtype):
+    """dx alone has the bits that it has beside dup, also where the gradients
+    hold values whose products are looked at again."""
+    c = Case(dtype, 140, 264, 12, 5, 2201)
+    c.dy[np.random.default_rng(3).random(c.dy.shape) < 0.01] *= np.float32(1e-37)
+    c.on_device()
+    _, h = c.forward(stream)
+    dx, _, _ = c.backward(stream, h)
+    out = Dev(np.full(dx.shape, np.nan, np.float32))
+    c.a.backward(None, c.d["ids"].ptr, c.n, None, c.d["dy"].ptr, d_dx_base=c.d["dxb"].ptr, d_dx=out.ptr, stream=stream,
+                 **c.ws)
+    assert_bit_equal(out.get(), dx, "dx")

@@ -234,6 +234,7 @@ __device__ inline void store_sums(const v4f (&acc)[RT][4], const Factor &fac, in
 constexpr uint32_t kSmallSum = 47u << 23;           // 2^-80, as bits
 constexpr uint32_t kLargeFactor = (127 + 23) << 7;  // 2^23, as bf16's
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ inline v4f mfma16(const uint4 &a, const uint4 &b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -364,16 +365,19 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 #pragma unroll
           for (int i = 0; i < 2; ++i) factor_parts(fv[t][2 * i], fv[t][2 * i + 1], fp[t][i]);
       }
-      bool large = false;  // a factor value not below kLargeFactor
+      // what a sum's bits, past kSmallSum's, have to be below: all are looked at
+      // beside a factor value not below kLargeFactor
+      uint32_t fine = (0x7f800000u - kSmallSum) << 1;
       if constexpr (std::is_same_v<T, BF16>) {  // f16's are below
-        uint32_t most = 0;
+        u16x2 most = 0;
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int m = 0; m < 4; ++m)
-            most = max(max(most, max(fv[t][m].v.x & 0x7fff, fv[t][m].v.x >> 16 & 0x7fff)),
-                       max(fv[t][m].v.y & 0x7fff, fv[t][m].v.y >> 16 & 0x7fff));
-        large = __any(most >= kLargeFactor);
+            most = __builtin_elementwise_max(
+                most, __builtin_elementwise_max(__builtin_bit_cast(u16x2, fv[t][m].v.x & 0x7fff7fff),
+                                                __builtin_bit_cast(u16x2, fv[t][m].v.y & 0x7fff7fff)));
+        if (__any(max(most.x, most.y) >= kLargeFactor)) fine = 0;
       }
       Quad<F32> xv[2][4];
       constexpr int kHidden = (RT * 256 + kSlice - 1) / kSlice;  // a thread's hidden values of a tile
@@ -415,14 +419,15 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
 #pragma unroll
           for (int m = 0; m < 4; ++m) xv[d][m].drop(skip - (16 * m + 4 * q));
         }
-        if (SUMS && p + 16 > i1) {  // the run's last tile: no rows past it
-#pragma unroll
-          for (int m = 0; m < 4; ++m) xv[d][m].drop(p + lo < i1 ? 0 : 4);
-        }
         v4f acc[RT] = {};
         if constexpr (SUMS) {
 #pragma unroll
           for (int m = 0; m < 4; ++m) *(uint4 *)(turn + lo * kPitch + 16 * m + 4 * q) = xv[d][m].v;
+          // the run's last tile: no rows past it (the first product has them, as without SUMS)
+          if (p + 16 > i1 && p + lo >= i1) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) *(uint4 *)(turn + lo * kPitch + 16 * m + 4 * q) = make_uint4(0, 0, 0, 0);
+          }
         }
         if constexpr (!SPLIT) {
 #pragma unroll
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(kSlice, SUMS && RT > 2 ? 2 : 4) slice_kernel(R
           for (int t = 0; t < RT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) far = max(far, (f2u(acc[t][r]) << 1) - (kSmallSum << 1));
-          bool odd = large || __any(far >= (0x7f800000u - kSmallSum) << 1);
+          bool odd = __any(far >= fine);
           if (__builtin_expect(odd, 0)) {
             bool again = past_parts(xv[d][0].v, xv[d][1].v) || past_parts(xv[d][2].v, xv[d][3].v);
 #pragma unroll
