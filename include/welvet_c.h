@@ -434,6 +434,159 @@ WELVET_API welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vo
                                             int64_t dstride, void *d_ws, size_t ws_bytes,
                                             void *stream);
 
+/* ---- activations in 8 bits (extensions) ------------------------------------
+ * Rows of n tokens whose values are codes c in [-127, 127] and one scale a
+ * row, value = scale * c: what an integer product takes, and what a training
+ * step keeps of its activations, a quarter of f32's bytes, until its backward
+ * pass.  The calls follow the rules above (device pointers, streams, types,
+ * checks, workspaces); d_codes is 16-byte aligned, [n][stride]
+ * with the stride a multiple of 16 and at least the width rounded up to 16.
+ *   scale = max |x| / 127, rounded to f32;  c = x / scale to nearest, ties to
+ *   even, of the exact quotient (at most 127: a scale below 2^-126 is itself
+ *   rounded to few bits, and below 2^-150 it is 0)
+ * A row of zeros has scale 0.  A row that holds a NaN or an infinity has scale
+ * NaN and codes 0: whatever reads it is NaN.  Codes between the width and its
+ * multiple of 16 are written as 0 and may hold anything where they are read.
+ * n <= 2^24, widths <= 2^24. */
+typedef struct welvet_hip_rows8 {
+  int8_t *d_codes;
+  int64_t stride;
+  float *d_scales;
+} welvet_hip_rows8;
+/* x [n][width] (Float32, Float16 or BFloat16) into rows, and rows back into x,
+ * rounded to nearest even. */
+WELVET_API welvet_status welvet_hip_rows8_store(int32_t dtype, int32_t n, int32_t width,
+                                                const void *d_x, int64_t x_stride,
+                                                const welvet_hip_rows8 *rows, void *stream);
+WELVET_API welvet_status welvet_hip_rows8_load(int32_t dtype, int32_t n, int32_t width,
+                                               const welvet_hip_rows8 *rows, void *d_x,
+                                               int64_t x_stride, void *stream);
+/* SwiGLU's product of its two projections, h = silu(gate) * up, formed in f32
+ * from gate and up as given: into d_h (in `dtype`), into h8 in 8 bits (the
+ * next integer product's rows; from h in f32), or both; gate8 and up8 keep
+ * gate and up for the backward.  Any of gate8, up8, h8 and d_h may be NULL,
+ * not all. */
+WELVET_API welvet_status welvet_hip_rows8_swiglu(
+    int32_t dtype, int32_t n, int32_t width, const void *d_gate, int64_t gate_stride,
+    const void *d_up, int64_t up_stride, const welvet_hip_rows8 *gate8,
+    const welvet_hip_rows8 *up8, const welvet_hip_rows8 *h8, void *d_h, int64_t h_stride,
+    void *stream);
+/* Its backward at the values that gate8 and up8 hold: dgate = dh * up *
+ * silu'(gate), dup = dh * silu(gate).  d_dgate or d_dup may be d_dh (the same
+ * stride). */
+WELVET_API welvet_status welvet_hip_rows8_swiglu_backward(
+    int32_t dtype, int32_t n, int32_t width, const welvet_hip_rows8 *gate8,
+    const welvet_hip_rows8 *up8, const void *d_dh, int64_t dh_stride, void *d_dgate,
+    int64_t dgate_stride, void *d_dup, int64_t dup_stride, void *stream);
+
+/* A layer in -> out whose product runs in 8-bit integers: weights as rows of
+ * codes, a scale for each output channel, stored as rows8_store does; bias (held
+ * in f32) and act as in welvet_dense_mount.  in <= 131072 (a sum of products fits
+ * 32 bits), out <= 2^24, in out < 2^31.  Mounted from host values W [out*in], from device
+ * values (16-byte aligned; read on the null stream), from codes [out][in]
+ * in [-127, 127] and scales [out] on the host, or from a mounted Dense session
+ * of any dtype (its decoded weights, bias and activation; the session stays as
+ * it is).  A mounted layer does not change: calls on it may overlap. */
+typedef struct welvet_hip_int8 welvet_hip_int8;
+WELVET_API welvet_status welvet_hip_int8_mount(int32_t in, int32_t out, int32_t act, const float *W,
+                                               const double *bias, size_t bias_len,
+                                               welvet_hip_int8 **layer);
+WELVET_API welvet_status welvet_hip_int8_mount_device(int32_t in, int32_t out, int32_t act,
+                                                      const float *d_W, const double *bias,
+                                                      size_t bias_len, welvet_hip_int8 **layer);
+WELVET_API welvet_status welvet_hip_int8_mount_codes(int32_t in, int32_t out, int32_t act,
+                                                     const int8_t *codes, const float *scales,
+                                                     const double *bias, size_t bias_len,
+                                                     welvet_hip_int8 **layer);
+WELVET_API welvet_status welvet_hip_int8_mount_dense(welvet_dense_session *s,
+                                                     welvet_hip_int8 **layer);
+/* The layer's codes [out][in] and scales [out] (host; either may be NULL). */
+WELVET_API welvet_status welvet_hip_int8_weights(welvet_hip_int8 *layer, int8_t *codes,
+                                                 float *scales);
+/* The caller's work on the layer has to be done. */
+WELVET_API void welvet_hip_int8_release(welvet_hip_int8 *layer);
+/* The workspace that forward or product need for n rows or fewer. */
+WELVET_API welvet_status welvet_hip_int8_bytes(const welvet_hip_int8 *layer, int32_t n,
+                                               size_t *bytes);
+/* x [n][in] to 8 bits a row as rows8_store does, then
+ *   pre[t][o] = scale_t wscale_o sum_k c_tk w_ok + bias_o,  post = act(pre)
+ * with the sum exact and the rest in f32, whatever n: a row's results have the
+ * same bits in every batch.  Both are written in `dtype`, either may be NULL,
+ * not both.  rows (nullable) receives x's rows, the backward's checkpoint. */
+WELVET_API welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *layer, int32_t dtype,
+                                                 int32_t n, const void *d_x, int64_t x_stride,
+                                                 const welvet_hip_rows8 *rows, void *d_pre,
+                                                 int64_t pre_stride, void *d_post,
+                                                 int64_t post_stride, void *d_ws, size_t ws_bytes,
+                                                 void *stream);
+/* The same from rows already in 8 bits (one store for several layers). */
+WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, int32_t dtype,
+                                                 int32_t n, const welvet_hip_rows8 *rows,
+                                                 void *d_pre, int64_t pre_stride, void *d_post,
+                                                 int64_t post_stride, void *d_ws, size_t ws_bytes,
+                                                 void *stream);
+
+/* The backward of a layer in -> out from what it kept in 8 bits, at those
+ * values: pre8 its pre-activations (NULL with act = -1), x8 its input.
+ *   dpre = dy * act'(pre)              [n][out], in `dtype`
+ *   dw (+)= sum over rows of dpre x    [out][in], f32, contiguous
+ *   dx = dpre . W                      [n][in], in `dtype`, W the int8 layer's
+ * Any of d_dpre, d_dw (with x8) and d_dx (with `layer`, of the same sizes) may
+ * be NULL, not all; accumulate = 1 adds to dw.  d_dpre may be d_dy (the same
+ * stride).  A Dense layer of any dtype can keep its activations so: it takes
+ * dpre and dw here, and dx from its own weights.
+ * dpre enters the products before it is rounded to `dtype`, times its row's
+ * scale (dw) or its channel's (dx), as bf16 parts: three for Float32 (24
+ * bits), two for 16-bit types (16 bits or more), one for dx in BFloat16
+ * (rounded as its dy was); sums are f32, in a fixed order.  Such products below
+ * 2^-102 are held to an absolute 2^-126, and from 3.38e38 on count as
+ * infinite.  in and out <= 2^20, n <= 2^20. */
+WELVET_API welvet_status welvet_hip_rows8_backward_bytes(int32_t dtype, int32_t n, int32_t in,
+                                                         int32_t out, size_t *bytes);
+WELVET_API welvet_status welvet_hip_rows8_backward(
+    int32_t act, int32_t dtype, int32_t n, int32_t in, int32_t out, const void *d_dy,
+    int64_t dy_stride, const welvet_hip_rows8 *pre8, const welvet_hip_rows8 *x8,
+    const welvet_hip_int8 *layer, void *d_dpre, int64_t dpre_stride, void *d_dx,
+    int64_t dx_stride, int32_t accumulate, float *d_dw, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Rules that logits pass before an answer is taken from them.  Row t < n <=
+ * 2^20 holds logits z over the vocabulary (Float32, Float16 or BFloat16;
+ * vocab <= 2^30), and a history of tokens, d_history [n][history_stride] with
+ * d_history_len[t] of at most `history` (<= 2^20 - 1) entries (NULL: all), the
+ * first d_prompt_len[t] of them the prompt (NULL: none).  For each token v:
+ *   1 named anywhere in the history:  z = z > 0 ? z / r : z r
+ *   2 named c > 0 times after the prompt:  z = z - c f - p
+ *   3 z = z + each bias of the row's list that names v, in the list's order
+ *   4 z = -inf where the row's mask has v's bit clear, whatever z is
+ * with r = d_repetition[t], f = d_frequency[t], p = d_presence[t] (NULL: 1, 0,
+ * 0).  Entries outside [0, vocab) are padding, lengths outside [0, history]
+ * count as the nearer end.  The list: d_bias_index and d_bias, [n][biases],
+ * biases <= 1024.  The masks: d_masks [masks][mask_stride], bit v % 32 of word
+ * v / 32 (mask_stride of at least that many words); row t takes mask
+ * d_mask_id[t], none where that lies outside [0, masks) (d_mask_id NULL: mask
+ * t).  Rules 1 to 3 are formed in f64 and rounded once, to nearest even, to the
+ * logits' type; other logits keep their bits. */
+typedef struct welvet_hip_logit_rules {
+  int32_t history;
+  const int32_t *d_history;
+  int64_t history_stride;
+  const int32_t *d_history_len, *d_prompt_len;
+  const float *d_repetition, *d_frequency, *d_presence;
+  int32_t biases;
+  const int32_t *d_bias_index;
+  const float *d_bias;
+  int32_t masks;
+  const uint32_t *d_masks;
+  int64_t mask_stride;
+  const int32_t *d_mask_id;
+} welvet_hip_logit_rules;
+/* d_out may be d_logits (the same stride): then only the logits that a rule
+ * changes are read and written. */
+WELVET_API welvet_status welvet_hip_logits_rules(int32_t dtype, int32_t n, int32_t vocab,
+                                                 const void *d_logits, int64_t stride,
+                                                 const welvet_hip_logit_rules *rules, void *d_out,
+                                                 int64_t out_stride, void *stream);
+
 /* Kernel route of the forward: 0 auto, 1 GEMV, 2 MFMA GEMM, 3 element-wise. */
 WELVET_API void welvet_hip_set_forward_path(int32_t path);
 /* Route switch `key` := value, returns the previous value (-1 = unknown key,

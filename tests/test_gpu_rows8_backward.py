@@ -1,0 +1,183 @@
+"""welvet_hip_rows8_backward: a layer's backward from 8-bit activations against f64.
+
+Bounds.  The activations' values are rounded once (U |pre|, U of x), act' is
+within 64 U, dpre one rounding more and then its type's.  A product's terms
+carry that, one rounding of the scale's product and what the bf16 parts leave:
+2^-24, 2^-16 or 2^-8 of a term for three, two or one (each part is within 2^-8
+of what is left).  A sum of K terms in f32 is within (P K + 8) U of the sum of
+their magnitudes."""
+import numpy as np
+import pytest
+
+import pywelvet
+from devmem import Stream
+from parity import assert_bit_equal
+from rows8ref import ACTS, PRIME_ERR, Rows, act, act_prime, codes_of, values
+from test_gpu_rows8 import HALF_ULP, LEAST, matrix
+from tokmem import DT, U, Dev, to_bits, to_f64, within
+
+pytestmark = pytest.mark.gpu
+PARTS = {"float32": (3, 3), "float16": (2, 2), "bfloat16": (2, 1)}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    pywelvet.init()
+
+
+@pytest.fixture
+def stream():
+    s = Stream()
+    yield s.h
+    s.sync()
+    s.close()
+
+
+class Case:
+    def __init__(self, dtype, n, inn, out, name, seed=0, layer=True, extra=0, shift=0):
+        rng = np.random.default_rng([n, inn, out, seed])
+        self.dtype, self.n, self.inn, self.out, self.name, self.extra = dtype, n, inn, out, name, extra
+        self.xc, self.xs = codes_of(rng.normal(0, 1, (n, inn)).astype(np.float32) if n else np.zeros((0, inn)))
+        self.pc, self.ps = codes_of((rng.normal(0, 2, (n, out)) * np.exp(rng.normal(0, 1, (n, 1)))).astype(np.float32)
+                                    if n else np.zeros((0, out)))
+        self.x8, self.pre8 = Rows(n, inn, 1, self.xc, self.xs), Rows(n, out, 0, self.pc, self.ps)
+        self.d, self.dy_ptr, self.dy = matrix(rng.normal(0, 1, (n, out)) * 1e-2, dtype, extra, shift)
+        self.layer = pywelvet.Int8Layer(rng.normal(0, 1, (out, inn)) * np.exp(rng.normal(0, 1, (out, 1)))) if layer else None
+        self.item = to_bits(np.zeros(1), dtype).dtype
+        self.ws = Dev(np.full(max(16, pywelvet.rows8_backward_bytes(DT[dtype], n, inn, out)), 0xFF, np.uint8))
+
+    def run(self, stream, dpre=True, dx=True, dw=True, base=None, ws=None, in_place=False):
+        e = self.extra
+        a, b = Dev(np.full((self.n, self.out + e), 5, self.item)), Dev(np.full((self.n, self.inn + e), 5, self.item))
+        c = Dev(np.full((self.out, self.inn), 3.0, np.float32) if base is None else base)
+        ws = self.ws if ws is None else ws
+        pywelvet.rows8_backward(
+            pywelvet.ACT[self.name], DT[self.dtype], self.n, self.inn, self.out, self.dy_ptr,
+            pre=None if self.name == "linear" else self.pre8.desc, x=self.x8.desc if dw else None,
+            layer=self.layer if dx else None, d_dpre=(self.dy_ptr if in_place else a.ptr) if dpre else None,
+            d_dx=b.ptr if dx else None, d_dw=c.ptr if dw else None, accumulate=base is not None,
+            dy_stride=self.out + e, dpre_stride=self.out + e, dx_stride=self.inn + e, ws=ws.ptr, ws_bytes=ws.nbytes,
+            stream=stream)
+        ws.get()
+        a, b = a.get(), b.get()
+        assert (a[:, self.out:] == 5).all() and (b[:, self.inn:] == 5).all()
+        return (a[:, :self.out] if dpre else None, b[:, :self.inn] if dx else None, c.get() if dw else None)
+
+    def want(self):
+        pre = values(self.pc, self.ps)
+        prime = act_prime(pre, self.name)
+        dpre = self.dy * prime
+        smooth = self.name in ("silu", "gelu", "tanh", "sigmoid")
+        err = np.abs(self.dy) * (PRIME_ERR + U * np.abs(pre) if smooth else 0) + 3 * U * np.abs(dpre)
+        x = values(self.xc, self.xs)
+        return dpre, err, x
+
+    def check(self, stream, base=None, **kw):
+        dpre, dx, dw = self.run(stream, base=base, **kw)
+        want, err, x = self.want()
+        half, pw, px = HALF_ULP[self.dtype], *PARTS[self.dtype]
+        if dpre is not None and not kw.get("in_place"):
+            within(to_f64(dpre, self.dtype), want, err + half * (np.abs(want) + err) + LEAST[self.dtype], "dpre")
+        if dw is not None:
+            total, ab, more = want.T @ x, np.abs(want).T @ np.abs(x), err.T @ np.abs(x)
+            b = 0 if base is None else base
+            within(dw, total + b, more + ab * (2.0 ** (-8 * pw) + (pw * self.n + 12) * U)
+                   + U * np.abs(total + b) * 2 + 1e-36, "dw")
+        if dx is not None:
+            wc, ws = self.layer.weights()
+            W = values(wc, ws)
+            total, ab, more = want @ W, np.abs(want) @ np.abs(W), err @ np.abs(W)
+            bound = more + ab * (2.0 ** (-8 * px) + (px * self.out + 12) * U)
+            within(to_f64(dx, self.dtype), total, bound * 1.01 + half * np.abs(total) + LEAST[self.dtype] * 2, "dx")
+        return dpre, dx, dw
+
+
+SHAPES = [(1, 1, 1), (1, 40, 70), (3, 17, 5), (31, 64, 64), (32, 65, 63), (33, 100, 129), (100, 1001, 777),
+          (65, 300, 260), (256, 512, 1100), (700, 130, 33), (2100, 200, 128)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,inn,out", SHAPES)
+def test_backward(stream, dtype, n, inn, out):
+    case = Case(dtype, n, inn, out, ACTS[(n + inn) % len(ACTS)], extra=out % 3, shift=inn % 4)
+    dpre, dx, dw = case.check(stream)
+    again = case.run(stream)
+    for a, b, what in zip(again, (dpre, dx, dw), ("dpre", "dx", "dw")):
+        assert_bit_equal(a, b, what + " of a second run")
+    for k, what in enumerate(("dpre", "dx", "dw")):  # each alone has the same bits
+        only = case.run(stream, dpre=k == 0, dx=k == 1, dw=k == 2)
+        assert_bit_equal(only[k], (dpre, dx, dw)[k], what + " alone")
+    base = np.random.default_rng(1).normal(0, 1, (out, inn)).astype(np.float32)
+    case.check(stream, base=base)
+    case.run(stream, dx=False, dw=False, in_place=True)
+    placed = case.d.get()[inn % 4:].reshape(n, out + case.extra)[:, :out]
+    assert_bit_equal(placed, dpre, "dpre in dy's place")
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("name", ACTS)
+def test_every_activation(stream, dtype, name):
+    Case(dtype, 70, 90, 110, name, 1).check(stream)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_large_tiles(stream, dtype):
+    """Sizes past 256 x 256 tiles on every side, none of them a multiple."""
+    Case(dtype, 2900, 2900, 2900, "silu", 2, extra=1).check(stream)
+
+
+def test_gradients_against_differences(stream):
+    """The layer's own loss sum(dy act(x W^T)) at the values held, differentiated numerically."""
+    case = Case("float32", 6, 20, 9, "gelu", 3)
+    wc, ws = case.layer.weights()
+    W, x = values(wc, ws), values(case.xc, case.xs)
+    pre = x @ W.T * 0.1
+    case.pc, case.ps = codes_of(pre.astype(np.float32))
+    case.pre8 = Rows(6, 9, 0, case.pc, case.ps)
+    dpre, dx, dw = case.run(stream)
+    p, step = values(case.pc, case.ps), 1e-5
+    d = case.dy * (act(p + step, "gelu") - act(p - step, "gelu")) / (2 * step)
+    # differences are off by step^2 / 6 of a third derivative of at most 3 and f64's rounding over the step
+    size = np.abs(case.dy)
+    within(dpre, d, 1e-5 * size, "dpre")
+    within(dx, d @ W, 1e-5 * size @ np.abs(W) + 1e-6 * np.abs(d) @ np.abs(W), "dx")
+    within(dw, d.T @ x, 1e-5 * size.T @ np.abs(x) + 1e-6 * np.abs(d).T @ np.abs(x), "dw")
+
+
+def test_no_rows(stream):
+    case = Case("float32", 0, 30, 20, "silu", 4)
+    ones = np.ones((20, 30), np.float32)
+    assert (case.run(stream, dpre=False, dx=False, dw=True)[2] == 0).all()
+    assert_bit_equal(case.run(stream, dpre=False, dx=False, dw=True, base=ones)[2], ones, "added to")
+
+
+def test_values_that_are_not_finite(stream):
+    """A NaN row of the input makes dw NaN; an infinite gradient reaches its own
+    row of dx and its own channel of dw, and nothing else; other rows and channels stay."""
+    for dtype in DT:
+        case = Case(dtype, 40, 50, 60, "linear", 5)
+        dy = case.dy.copy()
+        dy[7, 9] = np.inf
+        case.d, case.dy_ptr, case.dy = matrix(dy, dtype)
+        dpre, dx, dw = case.run(stream)
+        dx, dw = to_f64(dx, dtype), dw.astype(np.float64)
+        assert not np.isfinite(dx[7]).any() and np.isfinite(np.delete(dx, 7, 0)).all()
+        assert not np.isfinite(dw[9]).any() and np.isfinite(np.delete(dw, 9, 0)).all()
+        # inf times a code: infinite where the code is not 0, as the formula has it
+        some = case.xc[7] != 0
+        assert np.isinf(dw[9][some]).all() and np.isnan(dw[9][~some]).all()
+        case = Case(dtype, 40, 50, 60, "linear", 5)
+        case.xs[3] = np.nan
+        case.x8 = Rows(40, 50, 1, case.xc, case.xs)
+        dpre, dx, dw = case.run(stream)
+        assert np.isnan(dw).all() and np.isfinite(to_f64(dx, dtype)).all()
+
+
+def test_a_smaller_batch_in_the_same_workspace(stream):
+    big = Case("bfloat16", 300, 130, 140, "silu", 6)
+    for n in (299, 64, 33, 1):
+        case = Case("bfloat16", n, 130, 140, "silu", 7)
+        want = case.check(stream)
+        got = case.run(stream, ws=big.ws)
+        for a, b in zip(got, want):
+            assert_bit_equal(a, b, f"{n} rows")

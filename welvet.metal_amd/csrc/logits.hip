@@ -1,0 +1,227 @@
+// logits.hip — rules that logits pass before an answer is taken from them.  For
+// token v of a row, named c times after the prompt:
+//   z = z > 0 ? z / r : z r  where the history names v at all
+//   z = z - c f - p          where c > 0
+//   z = z + the sum of v's biases, in the list's order
+//   z = -inf                 where the row's mask shuts v
+// A block takes a stretch of a row's vocabulary.  It counts the history's
+// tokens of that stretch in LDS (whole numbers: the order does not matter), a
+// word a token: how often it was said, whether the prompt names it, how many
+// biases do.  Then it passes over the stretch once: bound by HBM, as nothing of
+// what a mask shuts is read.  Tokens with a bias go last, a thread each.  In
+// place, only what changes is touched.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "rows8.hpp"
+
+namespace wh {
+namespace {
+
+using namespace r8;
+
+constexpr int kThreads = 512;
+constexpr int kStretch = 16384;       // tokens a block: 64 KB of counts, two blocks a CU
+constexpr int kMaxHistory = (1 << 20) - 1, kMaxBiases = 1024;
+constexpr uint32_t kCount = kMaxHistory, kBias = 1u << 20, kBiases = 0x7ffu << 20, kPrompt = 1u << 31;
+
+struct Args {
+  welvet_hip_logit_rules r;
+  const void *in;
+  void *out;
+  int64_t in_stride, out_stride;
+  int vocab, parts, len;  // parts stretches of len tokens a row
+};
+
+struct Row {
+  double repetition, frequency, presence;
+  __device__ inline double apply(double z, uint32_t word) const {
+    const uint32_t c = word & kCount;
+    if (c || (word & kPrompt)) z = z > 0.0 ? z / repetition : z * repetition;
+    if (c) z = z - (double)c * frequency - presence;
+    return z;
+  }
+};
+// Rounded once: through an f32 whose last bit tells that something was cut off.
+template <class T>
+__device__ inline typename T::raw rounded(double z) {
+  float f = (float)z;
+  if constexpr (sizeof(typename T::raw) == 2) {
+    uint32_t u = f2u(f);
+    if ((double)f != z && z == z) {
+      if (fabs((double)f) > fabs(z)) --u;
+      f = u2f(u | 1u);
+    }
+  }
+  return T::put(f);
+}
+template <class T>
+constexpr typename T::raw kShut = sizeof(typename T::raw) == 4 ? (typename T::raw)0xff800000u
+                                  : std::is_same_v<T, F16>     ? (typename T::raw)0xfc00u
+                                                               : (typename T::raw)0xff80u;
+
+template <class T, bool INPLACE>
+__global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
+  using raw = typename T::raw;
+  __shared__ uint4 words[kStretch / 4];
+  __shared__ int index[kMaxBiases];
+  __shared__ float bias[kMaxBiases];
+  uint32_t *count = (uint32_t *)words;
+  const int row = blockIdx.x / a.parts, begin = (int)(blockIdx.x % a.parts) * a.len;
+  const int len = min(a.len, a.vocab - begin), tid = threadIdx.x;
+  const raw *in = (const raw *)a.in + (int64_t)row * a.in_stride + begin;
+  raw *out = (raw *)a.out + (int64_t)row * a.out_stride + begin;
+  const uint32_t *mask = nullptr;
+  if (a.r.masks > 0) {
+    const int id = a.r.d_mask_id ? a.r.d_mask_id[row] : row;
+    if (id >= 0 && id < a.r.masks) mask = a.r.d_masks + id * a.r.mask_stride + begin / 32;
+  }
+  const auto open8 = [&](int c) -> uint32_t { return mask ? mask[c >> 5] >> (c & 31) & 0xffu : 0xffu; };
+  const int history = a.r.history > 0 && a.r.d_history_len ? min(max(a.r.d_history_len[row], 0), a.r.history) : a.r.history;
+  const int prompt = a.r.d_prompt_len ? min(max(a.r.d_prompt_len[row], 0), history) : 0;
+  const int32_t *said = a.r.d_history + (int64_t)row * a.r.history_stride;
+  const bool sparse = history > 0 || a.r.biases > 0;
+  if (sparse) {
+    for (int i = tid; i < (len + 3) / 4; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i = tid; i < history; i += kThreads) {
+      const int64_t v = (int64_t)said[i] - begin;
+      if (v < 0 || v >= len) continue;
+      if (i < prompt) atomicOr(&count[v], kPrompt);
+      else atomicAdd(&count[v], 1u);
+    }
+    for (int i = tid; i < a.r.biases; i += kThreads) {
+      const int64_t v = (int64_t)a.r.d_bias_index[(int64_t)row * a.r.biases + i] - begin;
+      const bool here = v >= 0 && v < len;
+      index[i] = here ? (int)v : -1;
+      bias[i] = a.r.d_bias[(int64_t)row * a.r.biases + i];
+      if (here) atomicAdd(&count[v], kBias);
+    }
+    __syncthreads();
+  }
+  const Row rules{a.r.d_repetition ? (double)a.r.d_repetition[row] : 1.0,
+                  a.r.d_frequency ? (double)a.r.d_frequency[row] : 0.0,
+                  a.r.d_presence ? (double)a.r.d_presence[row] : 0.0};
+  if (!INPLACE || mask) {
+    for (int c = tid * 8; c < len; c += kThreads * 8) {
+      const uint32_t open = open8(c);
+      Oct<T> o;
+      if constexpr (INPLACE) {
+        if (open == 0xffu) continue;
+        if (open == 0) {
+#pragma unroll
+          for (int w = 0; w < Oct<T>::kWords; ++w)
+            o.w[w] = sizeof(raw) == 4 ? (uint32_t)kShut<T> : (uint32_t)kShut<T> * 0x10001u;
+          o.store(out, c, len);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(open >> i & 1) && c + i < len) out[c + i] = kShut<T>;
+        }
+      } else {
+        raw r[8];
+        if (open) o.load(in, c, len);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = open >> i & 1 ? o.raw_at(i) : kShut<T>;
+        if (sparse && open) {
+          const uint4 w0 = words[c / 4], w1 = words[c / 4 + 1 < kStretch / 4 ? c / 4 + 1 : c / 4];
+          const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          if (w0.x | w0.y | w0.z | w0.w | w1.x | w1.y | w1.z | w1.w) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < len && (open >> i & 1) && (w[i] & (kCount | kPrompt)) && !(w[i] & kBiases))
+                r[i] = rounded<T>(rules.apply((double)o.get(i), w[i]));
+          }
+        }
+        __builtin_memcpy(o.w, r, sizeof(o.w));
+        o.store(out, c, len);
+      }
+    }
+  }
+  if (!sparse) return;
+  __syncthreads();  // what a token with a bias holds by now is written again
+  for (int i = tid; i < a.r.biases; i += kThreads) {
+    const int v = index[i];
+    if (v < 0 || !(open8(v & ~7) >> (v & 7) & 1)) continue;
+    const uint32_t w = count[v];
+    bool first = true;
+    if ((w & kBiases) != kBias)
+      for (int j = 0; j < i; ++j) first = first && index[j] != v;
+    if (!first) continue;
+    double z = rules.apply((double)T::get(in[v]), w);
+    if ((w & kBiases) == kBias) z += (double)bias[i];
+    else
+      for (int j = i; j < a.r.biases; ++j)
+        if (index[j] == v) z += (double)bias[j];
+    out[v] = rounded<T>(z);
+  }
+  if constexpr (INPLACE) {
+    for (int i = tid; i < history; i += kThreads) {
+      const int64_t v = (int64_t)said[i] - begin;
+      if (v < 0 || v >= len || !(open8((int)v & ~7) >> (v & 7) & 1)) continue;
+      if (count[v] & kBiases) continue;  // the words with a bias do not change here
+      const uint32_t w = atomicExch(&count[v], 0u);
+      if (w) out[v] = rounded<T>(rules.apply((double)T::get(in[v]), w));
+    }
+  }
+}
+
+// Stretches of a row: as many as give each CU two blocks, of 2048 tokens and
+// more, and no longer than the counts' place.
+void stretches(int n, int vocab, int *parts, int *len) {
+  const int64_t most = (vocab + kStretch - 1) / kStretch;
+  const int64_t p = std::max<int64_t>(most, std::min<int64_t>((512 + n - 1) / n, vocab / 2048));
+  *len = (int)(((vocab + p - 1) / p + 31) / 32 * 32);
+  *parts = (vocab + *len - 1) / *len;
+}
+
+}  // namespace
+}  // namespace wh
+
+using namespace wh;
+using namespace wh::rt;
+
+extern "C" {
+
+welvet_status welvet_hip_logits_rules(int32_t dtype, int32_t n, int32_t vocab, const void *d_logits, int64_t stride,
+                                      const welvet_hip_logit_rules *rules, void *d_out, int64_t out_stride,
+                                      void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "logits: unsupported dtype %d", dtype);
+  if (n < 0 || n > (1 << 20) || vocab <= 0 || vocab > (1 << 30) || !rules || (n > 0 && (!d_logits || !d_out)))
+    return make_status(kInvalid, "logits: invalid argument");
+  const welvet_hip_logit_rules &r = *rules;
+  if (r.history < 0 || r.history > kMaxHistory || r.biases < 0 || r.biases > kMaxBiases || r.masks < 0 ||
+      (r.history > 0 && (!r.d_history || r.history_stride < r.history)) ||
+      (r.biases > 0 && (!r.d_bias_index || !r.d_bias)) ||
+      (r.masks > 0 && (!r.d_masks || r.mask_stride < ((int64_t)vocab + 31) / 32)))
+    return make_status(kInvalid, "logits: invalid rules");
+  if (stride < vocab || out_stride < vocab) return make_status(kInvalid, "logits: row stride below vocab %d", vocab);
+  if (n > 1 && d_out == d_logits && out_stride != stride)
+    return make_status(kInvalid, "logits: a result in the logits' place needs their row stride");
+  const int size = tok::float_size(dtype);
+  if (!tok::aligned(d_logits, size) || !tok::aligned(d_out, size))
+    return make_status(kInvalid, "logits: device pointers must be aligned to their elements");
+  for (const void *p : {(const void *)r.d_history, (const void *)r.d_history_len, (const void *)r.d_prompt_len,
+                        (const void *)r.d_repetition, (const void *)r.d_frequency, (const void *)r.d_presence,
+                        (const void *)r.d_bias_index, (const void *)r.d_bias, (const void *)r.d_masks,
+                        (const void *)r.d_mask_id})
+    if (!tok::aligned(p, 4)) return make_status(kInvalid, "logits: device pointers must be aligned to their elements");
+  Args a{r, d_logits, d_out, stride, out_stride, vocab, 1, vocab};
+  if (n > 0) stretches(n, vocab, &a.parts, &a.len);
+  // a launch of fewer than 2^32 threads
+  if ((int64_t)n * a.parts >= (int64_t)1 << 23)
+    return make_status(kInvalid, "logits: %d rows of %d are more than a launch takes", n, vocab);
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  WH_HIP(tok::with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const unsigned blocks = (unsigned)(n * a.parts);
+    if (d_out == d_logits) rules_kernel<T, true><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
+    else rules_kernel<T, false><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
+    return hipGetLastError();
+  }));
+  return ok();
+}
+
+}  // extern "C"

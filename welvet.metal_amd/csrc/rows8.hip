@@ -1,0 +1,331 @@
+// rows8.hip — rows of activations in 8 bits: stored, read back, and SwiGLU's
+// product between them in both directions.  For a row x:
+//   s = max |x| / 127,  c_i = x_i / s to nearest even,  value s c_i
+//   h = silu(gate) up;  dgate = dh up silu'(gate),  dup = dh silu(gate)
+// Bound by HBM: a row a block, read once into registers, its largest magnitude
+// joined across the block, then its codes written.
+#include <hip/hip_runtime.h>
+
+#include "rows8.hpp"
+
+namespace wh {
+namespace r8 {
+namespace {
+
+// The block's maximum of each value, on every thread.  `lds` alternates
+// between a block's rows, so one barrier a row is enough.
+template <int WAVES, int N>
+__device__ inline void block_max(uint32_t (&top)[N], uint32_t *lds) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], off));
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds[i * WAVES + (threadIdx.x >> 6)] = top[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) top[i] = max(top[i], lds[i * WAVES + w]);
+  }
+}
+
+struct StoreArgs {
+  const void *x;
+  int64_t x_stride;
+  int8_t *codes;
+  int64_t codes_stride;
+  float *scales;
+  int n, width;
+};
+
+// GROUPS of eight values a thread stay in registers; a longer row is read again.
+template <class T, int WAVES, int GROUPS>
+__global__ void __launch_bounds__(WAVES * 64) store_kernel(StoreArgs a) {
+  constexpr int kThreads = WAVES * 64, kStep = kThreads * 8;
+  __shared__ uint32_t lds[2][WAVES];
+  const int end = (a.width + kPad - 1) / kPad * kPad, first = threadIdx.x * 8;
+  int turn = 0;
+  for (int row = blockIdx.x; row < a.n; row += gridDim.x, turn ^= 1) {
+    const typename T::raw *x = (const typename T::raw *)a.x + (int64_t)row * a.x_stride;
+    int8_t *codes = a.codes + (int64_t)row * a.codes_stride;
+    Oct<T> held[GROUPS];
+    uint32_t top[1] = {0};
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      if (g * kStep < a.width) held[g].load(x, min(first + g * kStep, a.width), a.width);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      if (g * kStep < a.width)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(held[g].get(i)));
+    for (int c = first + GROUPS * kStep; c < a.width; c += kStep) {
+      Oct<T> o;
+      o.load(x, c, a.width);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(o.get(i)));
+    }
+    block_max<WAVES>(top, lds[turn]);
+    const Scale q(top[0]);
+    if (threadIdx.x == 0) a.scales[row] = q.stored;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      if (first + g * kStep < end)
+        *(uint2 *)(codes + first + g * kStep) = codes8(q, [&](int i) { return held[g].get(i); });
+    for (int c = first + GROUPS * kStep; c < end; c += kStep) {
+      Oct<T> o;
+      o.load(x, c, a.width);
+      *(uint2 *)(codes + c) = codes8(q, [&](int i) { return o.get(i); });
+    }
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) load_kernel(StoreArgs a, int per_row) {
+  typename T::raw *x = (typename T::raw *)a.x;
+  const int64_t all = (int64_t)a.n * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per_row;
+    const int c = (int)(i - row * per_row) * 8;
+    const uint2 w = *(const uint2 *)(a.codes + row * a.codes_stride + c);
+    const float s = a.scales[row];
+    Oct<T> o;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.set(k, value_of(k < 4 ? w.x : w.y, k & 3) * s);
+    o.store(x + row * a.x_stride, c, a.width);
+  }
+}
+
+struct SwigluArgs {
+  const void *gate, *up;
+  int64_t gate_stride, up_stride;
+  welvet_hip_rows8 gate8, up8, h8;  // d_codes null: not asked for
+  void *h;
+  int64_t h_stride;
+  int n, width;
+};
+__device__ inline float product(float gate, float up) { return gate * Sigmoid(gate).z * up; }
+
+template <class T, int WAVES, int GROUPS>
+__global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
+  constexpr int kThreads = WAVES * 64, kStep = kThreads * 8;
+  using raw = typename T::raw;
+  __shared__ uint32_t lds[2][3 * WAVES];
+  const int end = (a.width + kPad - 1) / kPad * kPad, first = threadIdx.x * 8;
+  int turn = 0;
+  for (int row = blockIdx.x; row < a.n; row += gridDim.x, turn ^= 1) {
+    const raw *gate = (const raw *)a.gate + (int64_t)row * a.gate_stride;
+    const raw *up = (const raw *)a.up + (int64_t)row * a.up_stride;
+    raw *h = a.h ? (raw *)a.h + (int64_t)row * a.h_stride : nullptr;
+    Oct<T> g[GROUPS], u[GROUPS];
+    uint32_t top[3] = {0, 0, 0};
+    const auto look = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
+      Oct<T> ho;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float gv = go.get(i), uv = uo.get(i), hv = product(gv, uv);
+        top[0] = max(top[0], magnitude(gv));
+        top[1] = max(top[1], magnitude(uv));
+        top[2] = max(top[2], magnitude(hv));
+        ho.set(i, hv);
+      }
+      if (h) ho.store(h, c, a.width);
+    };
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k)
+      if (k * kStep < a.width) {
+        g[k].load(gate, min(first + k * kStep, a.width), a.width);
+        u[k].load(up, min(first + k * kStep, a.width), a.width);
+      }
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k)
+      if (k * kStep < a.width) look(g[k], u[k], first + k * kStep);
+    for (int c = first + GROUPS * kStep; c < a.width; c += kStep) {
+      Oct<T> go, uo;
+      go.load(gate, c, a.width);
+      uo.load(up, c, a.width);
+      look(go, uo, c);
+    }
+    block_max<WAVES>(top, lds[turn]);
+    const Scale qg(top[0]), qu(top[1]), qh(top[2]);
+    if (threadIdx.x == 0) {
+      if (a.gate8.d_codes) a.gate8.d_scales[row] = qg.stored;
+      if (a.up8.d_codes) a.up8.d_scales[row] = qu.stored;
+      if (a.h8.d_codes) a.h8.d_scales[row] = qh.stored;
+    }
+    const auto write = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
+      if (a.gate8.d_codes)
+        *(uint2 *)(a.gate8.d_codes + row * a.gate8.stride + c) = codes8(qg, [&](int i) { return go.get(i); });
+      if (a.up8.d_codes)
+        *(uint2 *)(a.up8.d_codes + row * a.up8.stride + c) = codes8(qu, [&](int i) { return uo.get(i); });
+      if (a.h8.d_codes)
+        *(uint2 *)(a.h8.d_codes + row * a.h8.stride + c) =
+            codes8(qh, [&](int i) { return product(go.get(i), uo.get(i)); });
+    };
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k)
+      if (first + k * kStep < end) write(g[k], u[k], first + k * kStep);
+    for (int c = first + GROUPS * kStep; c < end; c += kStep) {
+      Oct<T> go, uo;
+      go.load(gate, c, a.width);
+      uo.load(up, c, a.width);
+      write(go, uo, c);
+    }
+  }
+}
+
+struct SwigluBackArgs {
+  welvet_hip_rows8 gate8, up8;
+  const void *dh;
+  int64_t dh_stride;
+  void *dgate, *dup;
+  int64_t dgate_stride, dup_stride;
+  int n, width;
+};
+template <class T>
+__global__ void __launch_bounds__(256) swiglu_backward_kernel(SwigluBackArgs a, int per_row) {
+  using raw = typename T::raw;
+  const int64_t all = (int64_t)a.n * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per_row;
+    const int c = (int)(i - row * per_row) * 8;
+    const uint2 gw = *(const uint2 *)(a.gate8.d_codes + row * a.gate8.stride + c);
+    const uint2 uw = *(const uint2 *)(a.up8.d_codes + row * a.up8.stride + c);
+    const float gs = a.gate8.d_scales[row], us = a.up8.d_scales[row];
+    Oct<T> d, dg, du;
+    d.load((const raw *)a.dh + row * a.dh_stride, c, a.width);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float g = value_of(k < 4 ? gw.x : gw.y, k & 3) * gs, u = value_of(k < 4 ? uw.x : uw.y, k & 3) * us;
+      const Sigmoid z(g);
+      dg.set(k, d.get(k) * u * fmaf(g * z.z, z.co, z.z));
+      du.set(k, d.get(k) * (g * z.z));
+    }
+    dg.store((raw *)a.dgate + row * a.dgate_stride, c, a.width);
+    du.store((raw *)a.dup + row * a.dup_stride, c, a.width);
+  }
+}
+
+// Blocks of a kernel that walks `all` items 256 at a time.
+unsigned walk_blocks(int64_t all) { return (unsigned)std::min<int64_t>((all + 255) / 256, 65536); }
+unsigned row_blocks(int n) { return (unsigned)std::min(n, 65536); }
+
+}  // namespace
+
+hipError_t launch_store(int32_t dtype, int32_t n, int32_t width, const void *x, int64_t x_stride, int8_t *codes,
+                        int64_t codes_stride, float *scales, hipStream_t s) {
+  const StoreArgs a{x, x_stride, codes, codes_stride, scales, n, width};
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (width <= 1024) store_kernel<T, 1, 2><<<row_blocks(n), 64, 0, s>>>(a);
+    else if (width <= 8192) store_kernel<T, 4, 4><<<row_blocks(n), 256, 0, s>>>(a);
+    else store_kernel<T, 16, 4><<<row_blocks(n), 1024, 0, s>>>(a);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace r8
+}  // namespace wh
+
+using namespace wh;
+using namespace wh::rt;
+
+namespace {
+// What the rows' calls share: the type, the size, a float matrix of rows.
+bool matrix_ok(const void *p, int64_t stride, int32_t n, int32_t width) { return n == 0 || (p && stride >= width); }
+}  // namespace
+
+extern "C" {
+
+welvet_status welvet_hip_rows8_store(int32_t dtype, int32_t n, int32_t width, const void *d_x, int64_t x_stride,
+                                     const welvet_hip_rows8 *rows, void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "rows8: unsupported dtype %d", dtype);
+  if (!r8::size_ok(n, width) || !matrix_ok(d_x, x_stride, n, width)) return make_status(kInvalid, "rows8: invalid argument");
+  if (const char *why = r8::rows_fault(rows, n, width)) return make_status(kInvalid, "rows8: %s", why);
+  if (!tok::aligned(d_x, tok::float_size(dtype)))
+    return make_status(kInvalid, "rows8: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  WH_HIP(r8::launch_store(dtype, n, width, d_x, x_stride, rows->d_codes, rows->stride, rows->d_scales,
+                          (hipStream_t)stream));
+  return ok();
+}
+
+welvet_status welvet_hip_rows8_load(int32_t dtype, int32_t n, int32_t width, const welvet_hip_rows8 *rows, void *d_x,
+                                    int64_t x_stride, void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "rows8: unsupported dtype %d", dtype);
+  if (!r8::size_ok(n, width) || !matrix_ok(d_x, x_stride, n, width)) return make_status(kInvalid, "rows8: invalid argument");
+  if (const char *why = r8::rows_fault(rows, n, width)) return make_status(kInvalid, "rows8: %s", why);
+  if (!tok::aligned(d_x, tok::float_size(dtype)))
+    return make_status(kInvalid, "rows8: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  const int per_row = (width + 7) / 8;
+  const r8::StoreArgs a{d_x, x_stride, rows->d_codes, rows->stride, rows->d_scales, n, width};
+  WH_HIP(tok::with_type(dtype, [&](auto t) {
+    r8::load_kernel<decltype(t)><<<r8::walk_blocks((int64_t)n * per_row), 256, 0, (hipStream_t)stream>>>(a, per_row);
+    return hipGetLastError();
+  }));
+  return ok();
+}
+
+welvet_status welvet_hip_rows8_swiglu(int32_t dtype, int32_t n, int32_t width, const void *d_gate, int64_t gate_stride,
+                                      const void *d_up, int64_t up_stride, const welvet_hip_rows8 *gate8,
+                                      const welvet_hip_rows8 *up8, const welvet_hip_rows8 *h8, void *d_h,
+                                      int64_t h_stride, void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "rows8 swiglu: unsupported dtype %d", dtype);
+  if (!r8::size_ok(n, width) || !matrix_ok(d_gate, gate_stride, n, width) || !matrix_ok(d_up, up_stride, n, width) ||
+      (!gate8 && !up8 && !h8 && !d_h) || (d_h && h_stride < width))
+    return make_status(kInvalid, "rows8 swiglu: invalid argument");
+  for (const welvet_hip_rows8 *r : {gate8, up8, h8})
+    if (const char *why = r ? r8::rows_fault(r, n, width) : nullptr)
+      return make_status(kInvalid, "rows8 swiglu: %s", why);
+  const int size = tok::float_size(dtype);
+  if (!tok::aligned(d_gate, size) || !tok::aligned(d_up, size) || !tok::aligned(d_h, size))
+    return make_status(kInvalid, "rows8 swiglu: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  const welvet_hip_rows8 none{};
+  const r8::SwigluArgs a{d_gate, d_up, gate_stride, up_stride, gate8 ? *gate8 : none, up8 ? *up8 : none,
+                         h8 ? *h8 : none, d_h, h_stride, n, width};
+  WH_HIP(tok::with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    hipStream_t s = (hipStream_t)stream;
+    if (width <= 1024) r8::swiglu_kernel<T, 1, 2><<<r8::row_blocks(n), 64, 0, s>>>(a);
+    else if (width <= 8192) r8::swiglu_kernel<T, 8, 2><<<r8::row_blocks(n), 512, 0, s>>>(a);
+    else r8::swiglu_kernel<T, 16, 2><<<r8::row_blocks(n), 1024, 0, s>>>(a);
+    return hipGetLastError();
+  }));
+  return ok();
+}
+
+welvet_status welvet_hip_rows8_swiglu_backward(int32_t dtype, int32_t n, int32_t width, const welvet_hip_rows8 *gate8,
+                                               const welvet_hip_rows8 *up8, const void *d_dh, int64_t dh_stride,
+                                               void *d_dgate, int64_t dgate_stride, void *d_dup, int64_t dup_stride,
+                                               void *stream) {
+  if (!tok::float_type(dtype)) return make_status(kUnsupported, "rows8 swiglu: unsupported dtype %d", dtype);
+  if (!r8::size_ok(n, width) || !matrix_ok(d_dh, dh_stride, n, width) || !matrix_ok(d_dgate, dgate_stride, n, width) ||
+      !matrix_ok(d_dup, dup_stride, n, width) || (n > 0 && d_dgate == d_dup))
+    return make_status(kInvalid, "rows8 swiglu: invalid argument");
+  for (const welvet_hip_rows8 *r : {gate8, up8})
+    if (const char *why = r8::rows_fault(r, n, width)) return make_status(kInvalid, "rows8 swiglu: %s", why);
+  if (n > 1 && ((d_dgate == d_dh && dgate_stride != dh_stride) || (d_dup == d_dh && dup_stride != dh_stride)))
+    return make_status(kInvalid, "rows8 swiglu: a gradient in the place of dh needs its row stride");
+  const int size = tok::float_size(dtype);
+  if (!tok::aligned(d_dh, size) || !tok::aligned(d_dgate, size) || !tok::aligned(d_dup, size))
+    return make_status(kInvalid, "rows8 swiglu: device pointers must be aligned to their elements");
+  welvet_status st = require_device();
+  if (st.code || n == 0) return st;
+  const int per_row = (width + 7) / 8;
+  const r8::SwigluBackArgs a{*gate8, *up8, d_dh, dh_stride, d_dgate, d_dup, dgate_stride, dup_stride, n, width};
+  WH_HIP(tok::with_type(dtype, [&](auto t) {
+    r8::swiglu_backward_kernel<decltype(t)>
+        <<<r8::walk_blocks((int64_t)n * per_row), 256, 0, (hipStream_t)stream>>>(a, per_row);
+    return hipGetLastError();
+  }));
+  return ok();
+}
+
+}  // extern "C"

@@ -1,0 +1,167 @@
+// rows8.hpp — rows in 8 bits, shared by rows8.hip (storing them, SwiGLU),
+// int8.hip (products of them) and rows8_backward.hip: a row's values as codes
+// c in [-127, 127] and one scale s, value = s c.  Internal to the library.
+//   s = max |x| / 127, rounded to f32;  c = x / s, to nearest, ties to even
+// The code is that of the exact quotient: a product with 1 / s decides unless
+// it lies within 2^-13 of a half, where the remainder x - k s does, exactly.
+// A row of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and
+// codes 0, so whatever reads it is NaN.
+#pragma once
+
+#include "tokens.hpp"
+
+namespace wh {
+namespace r8 {
+
+using namespace tok;
+
+constexpr int kPad = 16;  // a row's codes: whole 16-byte words
+inline int64_t padded(int64_t width) { return (width + kPad - 1) / kPad * kPad; }
+
+struct Scale {
+  float stored;   // the row's scale
+  float s, inv;   // of the lifted values
+  float lift;     // 2^64 for rows whose scale is near the smallest float
+  bool finite;
+  // top: the largest magnitude's bits, above infinity's where a value is NaN
+  __device__ explicit Scale(uint32_t top) {
+    finite = top < 0x7f800000u;
+    stored = finite ? u2f(top) / 127.0f : u2f(0x7fc00000u);
+    lift = finite && stored < 0x1p-100f ? 0x1p64f : 1.0f;
+    s = stored * lift;
+    inv = finite && stored > 0.0f ? 1.0f / s : 0.0f;
+  }
+  __device__ inline int code(float x) const {
+    const float a = fabsf(x) * lift, q = a * inv;
+    float t = rintf(q);
+    if (fabsf(q - t) > 0.4999f) {
+      // within 127 2^-22 of a half: k + 1/2 against the quotient by the remainder,
+      // a multiple of a's or s's last place near s / 2, so the fma does not round
+      const float k = floorf(q), d = fmaf(-k, s, a), half = 0.5f * s;
+      t = d > half || (d == half && ((int)k & 1)) ? k + 1.0f : k;
+    }
+    t = fminf(t, 127.0f);  // a scale that was rounded down among the smallest floats
+    return (int)copysignf(t, x);
+  }
+};
+__device__ inline uint32_t magnitude(float x) { return f2u(x) & 0x7fffffffu; }
+
+// Eight neighbouring values wherever they lie, as floats; zeros from `width` on.
+template <class T>
+struct Oct {
+  using raw = typename T::raw;
+  static constexpr int kWords = sizeof(raw) * 2;
+  uint32_t w[kWords];
+  __device__ inline void load(const raw *row, int64_t c, int64_t width) {
+    if (c + 8 <= width) {
+      __builtin_memcpy(w, row + c, sizeof(w));
+      return;
+    }
+    raw r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = c + i < width ? row[c + i] : (raw)0;
+    __builtin_memcpy(w, r, sizeof(w));
+  }
+  __device__ inline raw raw_at(int i) const {
+    if constexpr (sizeof(raw) == 4) return w[i];
+    else return (raw)(w[i >> 1] >> (16 * (i & 1)));
+  }
+  __device__ inline float get(int i) const { return T::get(raw_at(i)); }
+  __device__ inline void set(int i, float v) {
+    if constexpr (sizeof(raw) == 4) w[i] = T::put(v);
+    else if (i & 1) w[i >> 1] = (w[i >> 1] & 0xffffu) | ((uint32_t)T::put(v) << 16);
+    else w[i >> 1] = (w[i >> 1] & 0xffff0000u) | T::put(v);
+  }
+  __device__ inline void store(raw *row, int64_t c, int64_t width) const {
+    if (c + 8 <= width) {
+      __builtin_memcpy(row + c, w, sizeof(w));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < width) row[c + i] = raw_at(i);
+  }
+};
+
+// Codes of eight values as two words (0 throughout in a row that is not finite).
+template <class F>
+__device__ inline uint2 codes8(const Scale &q, F &&value) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(uint8_t)q.code(value(i)) << (8 * (i & 3));
+  return q.finite ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
+}
+__device__ inline float value_of(uint32_t word, int i) { return (float)(int8_t)(word >> (8 * i)); }
+
+// z = 1 / (1 + e^-x) and 1 - z, each within 4 ulp: from e^-|x|, the argument's
+// product with log2 e carried past f32.
+struct Sigmoid {
+  float z, co;
+  __device__ explicit Sigmoid(float x) {
+    const float a = fabsf(x), t = -1.44269502f * a;
+    const float rest = fmaf(-1.44269502f, a, -t) - 1.92596299e-8f * a;
+    float e = __builtin_amdgcn_exp2f(t);
+    if (t > -126.0f) e = fmaf(e * rest, 0.693147181f, e);  // else e is 0 or about to be, and rest may be NaN
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    z = x < 0.0f ? e * r : r;
+    co = x < 0.0f ? r : e * r;
+    if (x != x) z = co = x;
+  }
+};
+// The activations and their derivatives in f32, by the formulas of act_value
+// and act_prime.
+__device__ inline float gelu_arg(float x) { return 1.59576912f * fmaf(0.044715f * x * x, x, x); }  // 2 u of 0.5 x (1 + tanh u)
+__device__ inline float act_f32(float x, int act) {
+  switch (act) {
+  case kReLU: return x > 0.0f ? x : 0.0f;
+  case kReLU2: return x < 0.0f ? 0.0f : x * x;
+  case kLeakyReLU: return x < 0.0f ? (float)((double)x * 0.01) : x;
+  case kSilu: return x * Sigmoid(x).z;
+  case kSigmoid: return Sigmoid(x).z;
+  case kTanh: return tanhf(x);
+  case kGELU: return x * Sigmoid(gelu_arg(x)).z;
+  }
+  return x;
+}
+__device__ inline float act_prime_f32(float x, int act) {
+  switch (act) {
+  case kSilu: {
+    const Sigmoid s(x);
+    return fmaf(x * s.z, s.co, s.z);
+  }
+  case kSigmoid: {
+    const Sigmoid s(x);
+    return s.z * s.co;
+  }
+  case kTanh: {
+    const Sigmoid s(2.0f * x);
+    return 4.0f * s.z * s.co;
+  }
+  case kGELU: {
+    if (fabsf(x) > 20.0f) return x > 0.0f ? 1.0f : 0.0f;  // where x x x may be infinite
+    const Sigmoid s(gelu_arg(x));
+    return fmaf(x * s.z * s.co, 1.59576912f * fmaf(0.134145f * x, x, 1.0f), s.z);
+  }
+  }
+  return act_prime_piecewise(x, act);
+}
+
+// What the rows' operators take: widths whose columns an int holds with a
+// block's steps past them, rows that a grid walks.
+constexpr int32_t kMaxWidth = 1 << 24, kMaxRows = 1 << 24;
+inline bool size_ok(int32_t n, int32_t width) { return n >= 0 && n <= kMaxRows && width > 0 && width <= kMaxWidth; }
+// A description of n rows: why it cannot be taken, or nullptr.
+inline const char *rows_fault(const welvet_hip_rows8 *r, int32_t n, int32_t width) {
+  if (!r) return "null rows";
+  if (n > 0 && (!r->d_codes || !r->d_scales)) return "null codes or scales";
+  if (!aligned(r->d_codes, 16) || r->stride % kPad != 0) return "codes and their stride must be multiples of 16 bytes";
+  if (!aligned(r->d_scales, 4)) return "device pointers must be aligned to their elements";
+  if (r->stride < padded(width)) return "stride of the codes below the width rounded up to 16";
+  return nullptr;
+}
+// rows8.hip: the store by itself, for the layers' weights and the forward.
+hipError_t launch_store(int32_t dtype, int32_t n, int32_t width, const void *x, int64_t x_stride, int8_t *codes,
+                        int64_t codes_stride, float *scales, hipStream_t s);
+
+}  // namespace r8
+}  // namespace wh

@@ -764,6 +764,28 @@ welvet_status welvet_hip_dense_export_f32(welvet_dense_session *s, float *W_out)
   return ok();
 }
 
+// The store's decoded weights, bias and activation as an int8 layer (int8.hip).
+welvet_status welvet_hip_int8_mount_dense(welvet_dense_session *s, welvet_hip_int8 **layer) {
+  if (!layer) return make_status(kInvalid, "int8: null layer");
+  *layer = nullptr;
+  if (!s) return make_status(kInvalid, "null session");
+  WH_HIP(hipSetDevice(g_dev.id));
+  std::lock_guard<std::mutex> lock(s->mu);
+  DevBuf w(s->stream);
+  WH_HIP(w.alloc((size_t)s->W.n() * sizeof(float)));
+  WH_HIP(launch_decode(s->W.dtype, s->W.body, s->W.n(), s->W.dev().scale, s->W.minv, w.as<float>(), s->stream));
+  std::vector<double> bias;
+  try {
+    bias.resize(s->W.bias_len);
+  } catch (...) {
+    return make_status(kInternal, "int8: out of memory");
+  }
+  if (!bias.empty())
+    WH_HIP(hipMemcpyAsync(bias.data(), s->W.bias, bias.size() * sizeof(double), hipMemcpyDeviceToHost, s->stream));
+  WH_HIP(hipStreamSynchronize(s->stream));
+  return welvet_hip_int8_mount_device(s->W.cols, s->W.rows, s->act, w.as<float>(), bias.data(), bias.size(), layer);
+}
+
 welvet_status welvet_hip_dense_backward(welvet_dense_session *s, const float *x, const float *pre,
                                         const float *gy, float *dX, float *dW) {
   if (!s || !x || !pre || !gy || !dX || !dW) return make_status(kInvalid, "null resident backward");

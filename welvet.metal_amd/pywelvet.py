@@ -65,6 +65,21 @@ class AdaptersDesc(C.Structure):
                 ("d_up", C.c_void_p), ("d_ranks", C.c_void_p), ("d_scales", C.c_void_p)]
 
 
+class Rows8(C.Structure):
+    """welvet_hip_rows8: rows in 8 bits in device memory."""
+    _fields_ = [("d_codes", C.c_void_p), ("stride", C.c_int64), ("d_scales", C.c_void_p)]
+
+
+class LogitRulesDesc(C.Structure):
+    """welvet_hip_logit_rules: what logits pass before an answer is taken."""
+    _fields_ = [("history", C.c_int32), ("d_history", C.c_void_p), ("history_stride", C.c_int64),
+                ("d_history_len", C.c_void_p), ("d_prompt_len", C.c_void_p),
+                ("d_repetition", C.c_void_p), ("d_frequency", C.c_void_p),
+                ("d_presence", C.c_void_p), ("biases", C.c_int32), ("d_bias_index", C.c_void_p),
+                ("d_bias", C.c_void_p), ("masks", C.c_int32), ("d_masks", C.c_void_p),
+                ("mask_stride", C.c_int64), ("d_mask_id", C.c_void_p)]
+
+
 def _fp(a):
     return None if a is None else a.ctypes.data_as(_f)
 
@@ -188,6 +203,34 @@ def lib() -> C.CDLL:
         for nm in ("embedding_forward", "embedding_store_forward", "embedding_backward_bytes",
                    "embedding_backward", "adapters_bytes", "adapters_forward", "adapters_backward",
                    "distill_bytes", "distill"):
+            getattr(L, "welvet_hip_" + nm).restype = Status
+        r8 = C.POINTER(Rows8)
+        mat = [_vp, _i64]  # a matrix in device memory and its row stride
+        L.welvet_hip_rows8_store.argtypes = [_i32] * 3 + mat + [r8, _vp]
+        L.welvet_hip_rows8_load.argtypes = [_i32] * 3 + [r8] + mat + [_vp]
+        L.welvet_hip_rows8_swiglu.argtypes = [_i32] * 3 + mat * 2 + [r8] * 3 + mat + [_vp]
+        L.welvet_hip_rows8_swiglu_backward.argtypes = [_i32] * 3 + [r8] * 2 + mat * 3 + [_vp]
+        L.welvet_hip_rows8_backward_bytes.argtypes = [_i32] * 4 + [C.POINTER(st)]
+        L.welvet_hip_rows8_backward.argtypes = [_i32] * 5 + mat + [r8, r8, _vp] + mat * 2 + \
+            [_i32, _vp, _vp, st, _vp]
+        layer = [_i32] * 3
+        L.welvet_hip_int8_mount.argtypes = layer + [_f, _d, st, C.POINTER(_vp)]
+        L.welvet_hip_int8_mount_device.argtypes = layer + [_vp, _d, st, C.POINTER(_vp)]
+        L.welvet_hip_int8_mount_codes.argtypes = layer + [C.POINTER(C.c_int8), _f, _d, st,
+                                                          C.POINTER(_vp)]
+        L.welvet_hip_int8_mount_dense.argtypes = [_vp, C.POINTER(_vp)]
+        L.welvet_hip_int8_weights.argtypes = [_vp, C.POINTER(C.c_int8), _f]
+        L.welvet_hip_int8_release.argtypes = [_vp]
+        L.welvet_hip_int8_release.restype = None
+        L.welvet_hip_int8_bytes.argtypes = [_vp, _i32, C.POINTER(st)]
+        L.welvet_hip_int8_forward.argtypes = [_vp, _i32, _i32] + mat + [r8] + mat * 2 + [_vp, st, _vp]
+        L.welvet_hip_int8_product.argtypes = [_vp, _i32, _i32, r8] + mat * 2 + [_vp, st, _vp]
+        L.welvet_hip_logits_rules.argtypes = [_i32] * 3 + mat + [C.POINTER(LogitRulesDesc)] + mat + \
+            [_vp]
+        for nm in ("rows8_store", "rows8_load", "rows8_swiglu", "rows8_swiglu_backward",
+                   "rows8_backward_bytes", "rows8_backward", "int8_mount", "int8_mount_device",
+                   "int8_mount_codes", "int8_mount_dense", "int8_weights", "int8_bytes",
+                   "int8_forward", "int8_product", "logits_rules"):
             getattr(L, "welvet_hip_" + nm).restype = Status
         coord = [_vp] + [_i32] * 4
         L.welvet_hip_grid_new.argtypes = [_i32] * 5 + [C.POINTER(_vp)]
@@ -759,3 +802,199 @@ def distill(dtype, n, vocab, d_logits, k, d_index, d_teacher, d_loss=None, d_dlo
     if status:
         return st
     check(st)
+
+
+# ---- activations in 8 bits: device pointers (ints) as above, rows as rows8().
+
+def rows8(d_codes, stride, d_scales) -> Rows8:
+    """Rows in 8 bits: codes [n][stride] and scales [n] in device memory."""
+    return Rows8(d_codes, stride, d_scales)
+
+
+def rows8_stride(width) -> int:
+    """The least stride of rows of `width` codes."""
+    return (width + 15) // 16 * 16
+
+
+def _r8(rows):
+    return None if rows is None else C.byref(rows)
+
+
+def rows8_store(dtype, n, width, d_x, rows, x_stride=None, stream=None, status=False):
+    """welvet_hip_rows8_store: x [n][width] into rows."""
+    st = lib().welvet_hip_rows8_store(dtype, n, width, d_x, width if x_stride is None else x_stride,
+                                      _r8(rows), stream)
+    if status:
+        return st
+    check(st)
+
+
+def rows8_load(dtype, n, width, rows, d_x, x_stride=None, stream=None, status=False):
+    """welvet_hip_rows8_load: the values that rows hold into x [n][width]."""
+    st = lib().welvet_hip_rows8_load(dtype, n, width, _r8(rows), d_x,
+                                     width if x_stride is None else x_stride, stream)
+    if status:
+        return st
+    check(st)
+
+
+def rows8_swiglu(dtype, n, width, d_gate, d_up, gate=None, up=None, h=None, d_h=None,
+                 gate_stride=None, up_stride=None, h_stride=None, stream=None, status=False):
+    """welvet_hip_rows8_swiglu: h = silu(gate) * up, and the rows that are asked for."""
+    st = lib().welvet_hip_rows8_swiglu(
+        dtype, n, width, d_gate, width if gate_stride is None else gate_stride, d_up,
+        width if up_stride is None else up_stride, _r8(gate), _r8(up), _r8(h), d_h,
+        width if h_stride is None else h_stride, stream)
+    if status:
+        return st
+    check(st)
+
+
+def rows8_swiglu_backward(dtype, n, width, gate, up, d_dh, d_dgate, d_dup, dh_stride=None,
+                          dgate_stride=None, dup_stride=None, stream=None, status=False):
+    """welvet_hip_rows8_swiglu_backward: dgate and dup at the values gate and up hold."""
+    st = lib().welvet_hip_rows8_swiglu_backward(
+        dtype, n, width, _r8(gate), _r8(up), d_dh, width if dh_stride is None else dh_stride,
+        d_dgate, width if dgate_stride is None else dgate_stride, d_dup,
+        width if dup_stride is None else dup_stride, stream)
+    if status:
+        return st
+    check(st)
+
+
+def rows8_backward_bytes(dtype, n, inn, out) -> int:
+    b = C.c_size_t()
+    check(lib().welvet_hip_rows8_backward_bytes(dtype, n, inn, out, C.byref(b)))
+    return b.value
+
+
+def rows8_backward(act, dtype, n, inn, out, d_dy, pre=None, x=None, layer=None, d_dpre=None,
+                   d_dx=None, d_dw=None, accumulate=False, dy_stride=None, dpre_stride=None,
+                   dx_stride=None, ws=None, ws_bytes=0, stream=None, status=False):
+    """welvet_hip_rows8_backward: dpre, dx (through an Int8Layer) and dw from rows."""
+    st = lib().welvet_hip_rows8_backward(
+        act, dtype, n, inn, out, d_dy, out if dy_stride is None else dy_stride, _r8(pre), _r8(x),
+        None if layer is None else layer.h, d_dpre, out if dpre_stride is None else dpre_stride,
+        d_dx, inn if dx_stride is None else dx_stride, 1 if accumulate else 0, d_dw, ws, ws_bytes,
+        stream)
+    if status:
+        return st
+    check(st)
+
+
+class Int8Layer:
+    """welvet_hip_int8_*: a layer whose product runs in 8-bit integers."""
+
+    def __init__(self, W, act=-1, bias=None):
+        W = _f32(W)
+        self.out, self.inn = W.shape
+        self._mount("welvet_hip_int8_mount", (self.inn, self.out, act, _fp(W)), bias)
+
+    @classmethod
+    def from_device(cls, d_W, inn, out, act=-1, bias=None):
+        """From f32 weights [out][inn] in device memory."""
+        self = cls.__new__(cls)
+        self.inn, self.out = inn, out
+        self._mount("welvet_hip_int8_mount_device", (inn, out, act, d_W), bias)
+        return self
+
+    @classmethod
+    def from_codes(cls, codes, scales, act=-1, bias=None):
+        """From codes [out][inn] (int8) and scales [out]."""
+        self = cls.__new__(cls)
+        codes, scales = np.ascontiguousarray(codes, np.int8), _f32(scales)
+        self.out, self.inn = codes.shape
+        assert scales.shape == (self.out,)
+        self._mount("welvet_hip_int8_mount_codes",
+                    (self.inn, self.out, act, codes.ctypes.data_as(C.POINTER(C.c_int8)),
+                     _fp(scales)), bias)
+        return self
+
+    @classmethod
+    def from_session(cls, session):
+        """From a mounted Session: its decoded weights, bias and activation."""
+        self = cls.__new__(cls)
+        self.inn, self.out = session.inn, session.out
+        self.h = _vp()
+        check(lib().welvet_hip_int8_mount_dense(session.h, C.byref(self.h)))
+        return self
+
+    def _mount(self, name, head, bias):
+        self.h = _vp()
+        b = None if bias is None else np.ascontiguousarray(bias, np.float64)
+        check(getattr(lib(), name)(*head, _dp(b), 0 if b is None else b.size, C.byref(self.h)))
+
+    def close(self):
+        if self.h:
+            lib().welvet_hip_int8_release(self.h)
+            self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def weights(self):
+        """Codes [out][inn] and scales [out]."""
+        codes, scales = np.zeros((self.out, self.inn), np.int8), np.zeros(self.out, np.float32)
+        check(lib().welvet_hip_int8_weights(self.h, codes.ctypes.data_as(C.POINTER(C.c_int8)),
+                                            _fp(scales)))
+        return codes, scales
+
+    def workspace_bytes(self, n) -> int:
+        b = C.c_size_t()
+        check(lib().welvet_hip_int8_bytes(self.h, n, C.byref(b)))
+        return b.value
+
+    def forward(self, dtype, n, d_x, rows=None, d_pre=None, d_post=None, x_stride=None,
+                pre_stride=None, post_stride=None, ws=None, ws_bytes=0, stream=None, status=False):
+        """x to 8 bits a row (into rows, where given), then pre and post."""
+        st = lib().welvet_hip_int8_forward(
+            self.h, dtype, n, d_x, self.inn if x_stride is None else x_stride, _r8(rows), d_pre,
+            self.out if pre_stride is None else pre_stride, d_post,
+            self.out if post_stride is None else post_stride, ws, ws_bytes, stream)
+        if status:
+            return st
+        check(st)
+
+    def product(self, dtype, n, rows, d_pre=None, d_post=None, pre_stride=None, post_stride=None,
+                ws=None, ws_bytes=0, stream=None, status=False):
+        """pre and post from rows already in 8 bits."""
+        st = lib().welvet_hip_int8_product(
+            self.h, dtype, n, _r8(rows), d_pre, self.out if pre_stride is None else pre_stride,
+            d_post, self.out if post_stride is None else post_stride, ws, ws_bytes, stream)
+        if status:
+            return st
+        check(st)
+
+
+class LogitRules:
+    """welvet_hip_logits_rules: penalties, biases and masks for rows of logits."""
+
+    def __init__(self, history=0, d_history=None, history_stride=None, d_history_len=None,
+                 d_prompt_len=None, d_repetition=None, d_frequency=None, d_presence=None, biases=0,
+                 d_bias_index=None, d_bias=None, masks=0, d_masks=None, mask_stride=None,
+                 d_mask_id=None):
+        self.desc = LogitRulesDesc(
+            history, d_history, history if history_stride is None else history_stride,
+            d_history_len, d_prompt_len, d_repetition, d_frequency, d_presence, biases,
+            d_bias_index, d_bias, masks, d_masks, 0, d_mask_id)
+        self.mask_stride = mask_stride  # None: the vocabulary's words
+
+    def apply(self, dtype, n, vocab, d_logits, d_out, stride=None, out_stride=None, stream=None,
+              status=False):
+        d = self.desc
+        d.mask_stride = (vocab + 31) // 32 if self.mask_stride is None else self.mask_stride
+        st = lib().welvet_hip_logits_rules(
+            dtype, n, vocab, d_logits, vocab if stride is None else stride, C.byref(d), d_out,
+            vocab if out_stride is None else out_stride, stream)
+        if status:
+            return st
+        check(st)
