@@ -21,7 +21,6 @@ using namespace r8;
 using namespace tiles;
 
 constexpr int kMaxIn = 131072, kMaxOut = 1 << 24;
-constexpr int kPitch = 128;  // bytes: whole stages of every kernel here
 
 struct Out {
   void *pre, *post;
@@ -38,11 +37,11 @@ __device__ inline float pre_of(int sum, float scale, float bias) { return fmaf((
 template <class T, int TILES>
 __global__ void __launch_bounds__(512) int8_few_kernel(const int8_t *__restrict__ codes, int64_t pitch,
                                                        const int8_t *__restrict__ x, int64_t x_stride, int last,
-                                                       Out o) {
+                                                       int steps, Out o) {
   constexpr int kWaves = 8, kAhead = TILES == 1 ? 8 : 4;
   __shared__ i32x4 part[kWaves][TILES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const int first = blockIdx.x * 16, steps = (int)(pitch / 64);
+  const int first = blockIdx.x * 16;
   const int8_t *w = codes + (int64_t)min(first + r, o.out - 1) * pitch + q * 16;
   const int8_t *xs[TILES];
 #pragma unroll
@@ -86,7 +85,7 @@ __global__ void __launch_bounds__(512) int8_few_kernel(const int8_t *__restrict_
     if (c >= o.out) break;
     const float pre = pre_of(sum[i], scale * o.w_scales[c], o.bias[c]);
     if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(pre);
-    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_f32(pre, o.act));
+    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_of<T>(pre, o.act));
   }
 }
 
@@ -94,26 +93,51 @@ __global__ void __launch_bounds__(512) int8_few_kernel(const int8_t *__restrict_
 template <class T, class Tile>
 __global__ void __launch_bounds__(Tile::kWaves * 64) int8_tile_kernel(Operands g, Out o, int tiles_m, int tiles_n) {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  float *x_scales = (float *)(lds + Tile::kResults);
   const Place at = place(tiles_m, tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
   Tile::run(g, m0, n0, acc, lds);
-  Tile::results(m0, n0, acc, [&](int row, int c, int sum) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) x_scales[i] = o.x_scales[min(m0 + i, o.n - 1)];
+  // a lane's channels are the same in all its rows
+  const int first = Tile::first_col(n0);
+  float scale[8], bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    scale[i] = o.w_scales[min(first + i, o.out - 1)];
+    bias[i] = o.bias[min(first + i, o.out - 1)];
+  }
+  __syncthreads();
+  Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
     if (row >= o.n || c >= o.out) return;
-    const float pre = pre_of(sum, o.x_scales[row] * o.w_scales[c], o.bias[c]);
-    if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(pre);
-    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_f32(pre, o.act));
+    const float s = x_scales[row - m0];
+    float v[8];
+    Oct<T> out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = pre_of(sum[i], s * scale[i], bias[i]);
+    if (o.pre) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out.set(i, v[i]);
+      out.store((typename T::raw *)o.pre + row * o.pre_stride, c, o.out);
+    }
+    if (o.post) {
+      act8<T>(v, o.act);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out.set(i, v[i]);
+      out.store((typename T::raw *)o.post + row * o.post_stride, c, o.out);
+    }
   });
 }
 
-using Large = Tile<Int8Op, 1, 2, 4, 4, 2, 4>;   // 256 x 256, eight waves
-using Medium = Tile<Int8Op, 1, 2, 2, 2, 2, 4>;  // 128 x 128, four
+using Large = Tile<Int8Op, 1, 2, 4, 4, 2>;   // 256 x 256, eight waves
+using Medium = Tile<Int8Op, 1, 2, 2, 2, 2>;  // 128 x 128, four
 
 template <class T, class Tile>
 hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_stride, const Out &o, hipStream_t s) {
   const int tm = (o.n + Tile::kRows - 1) / Tile::kRows, tn = (o.out + Tile::kCols - 1) / Tile::kCols;
   const Operands g{(const char *)x, x_stride, 0, o.n, (int)padded(l.in) - 16, (const char *)l.codes, l.pitch, l.out,
-                   (int)((l.in + 63) / 64)};
+                   (l.in + kStageBytes - 1) / kStageBytes};
   int8_tile_kernel<T, Tile><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, o, tm, tn);
   return hipGetLastError();
 }
@@ -122,11 +146,11 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
                           hipStream_t s) {
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int last = (int)padded(l.in) - 16;
+    const int last = (int)padded(l.in) - 16, steps = (l.in + 63) / 64;
     const unsigned blocks = (unsigned)((l.out + 15) / 16);
-    if (o.n <= 16) int8_few_kernel<T, 1><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, o);
-    else if (o.n <= 32) int8_few_kernel<T, 2><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, o);
-    else if (o.n <= 64) int8_few_kernel<T, 4><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, o);
+    if (o.n <= 16) int8_few_kernel<T, 1><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
+    else if (o.n <= 32) int8_few_kernel<T, 2><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
+    else if (o.n <= 64) int8_few_kernel<T, 4><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
     else if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 128)
       return launch_tiles<T, Large>(l, x, x_stride, o, s);
     else return launch_tiles<T, Medium>(l, x, x_stride, o, s);
@@ -134,7 +158,9 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
   });
 }
 
-size_t forward_bytes(int32_t in, int64_t n) { return pad256((size_t)n * padded(in)) + pad256((size_t)n * 4); }
+// The forward's own rows.
+int64_t row_bytes(int32_t in) { return spread(in); }
+size_t forward_bytes(int32_t in, int64_t n) { return pad256((size_t)n * row_bytes(in)) + pad256((size_t)n * 4); }
 
 void free_layer(welvet_hip_int8 *l) {
   if (!l) return;
@@ -149,7 +175,7 @@ bool shape_ok(int32_t in, int32_t out) { return in <= kMaxIn && out <= kMaxOut &
 // A layer with zeroed codes and its bias; the caller fills codes and scales.
 welvet_status new_layer(int32_t in, int32_t out, int32_t act, const double *bias, size_t bias_len,
                         welvet_hip_int8 **layer) {
-  auto *l = new (std::nothrow) welvet_hip_int8{in, out, act, (in + kPitch - 1) / kPitch * kPitch, nullptr, nullptr,
+  auto *l = new (std::nothrow) welvet_hip_int8{in, out, act, spread(in), nullptr, nullptr,
                                                nullptr};
   if (!l) return rt::make_status(kInternal, "int8: out of memory");
   std::vector<float> b;
@@ -293,7 +319,7 @@ welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *l, int32_t dtype, i
     return make_status(kInvalid, "int8: %zu bytes of 16-byte aligned workspace are needed", need);
   st = require_device();
   if (st.code || n == 0) return st;
-  welvet_hip_rows8 r{(int8_t *)d_ws, r8::padded(l->in), (float *)((char *)d_ws + tok::pad256(n * r8::padded(l->in)))};
+  welvet_hip_rows8 r{(int8_t *)d_ws, row_bytes(l->in), (float *)((char *)d_ws + tok::pad256(n * row_bytes(l->in)))};
   if (rows) r = *rows;
   const Out o{d_pre, d_post, pre_stride, post_stride, r.d_scales, l->scales, l->bias, n, l->out, l->act};
   WH_HIP(r8::launch_store(dtype, n, l->in, d_x, x_stride, r.d_codes, r.stride, r.d_scales, (hipStream_t)stream));

@@ -3,7 +3,7 @@
 
 #include <stdint.h>
 
-// Codes [out][pitch], zeros from `in` on, in whole 128 bytes; scales and bias
+// Codes [out][pitch], zeros from `in` on to whole 64 bytes and more; scales and bias
 // [out] (the bias zeros where none was given).
 struct welvet_hip_int8 {
   int32_t in, out, act;

@@ -58,15 +58,13 @@ __global__ void __launch_bounds__(WAVES * 64) store_kernel(StoreArgs a) {
       if (g * kStep < a.width) held[g].load(x, min(first + g * kStep, a.width), a.width);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
-      if (g * kStep < a.width)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(held[g].get(i)));
+      if (g * kStep < a.width) raise(top[0], held[g]);
     for (int c = first + GROUPS * kStep; c < a.width; c += kStep) {
       Oct<T> o;
       o.load(x, c, a.width);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(o.get(i)));
+      raise(top[0], o);
     }
+    top[0] = widened<T>(top[0]);
     block_max<WAVES>(top, lds[turn]);
     const Scale q(top[0]);
     if (threadIdx.x == 0) a.scales[row] = q.stored;
@@ -108,7 +106,8 @@ struct SwigluArgs {
 };
 __device__ inline float product(float gate, float up) { return gate * Sigmoid(gate).z * up; }
 
-template <class T, int WAVES, int GROUPS>
+// H8: h's own rows are asked for; its products are formed again for their codes.
+template <class T, int WAVES, int GROUPS, bool H8>
 __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
   constexpr int kThreads = WAVES * 64, kStep = kThreads * 8;
   using raw = typename T::raw;
@@ -122,13 +121,14 @@ __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
     Oct<T> g[GROUPS], u[GROUPS];
     uint32_t top[3] = {0, 0, 0};
     const auto look = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
+      raise(top[0], go);
+      raise(top[1], uo);
+      if (!H8 && !h) return;
       Oct<T> ho;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float gv = go.get(i), uv = uo.get(i), hv = product(gv, uv);
-        top[0] = max(top[0], magnitude(gv));
-        top[1] = max(top[1], magnitude(uv));
-        top[2] = max(top[2], magnitude(hv));
+        const float hv = product(go.get(i), uo.get(i));
+        if constexpr (H8) top[2] = max(top[2], magnitude(hv));
         ho.set(i, hv);
       }
       if (h) ho.store(h, c, a.width);
@@ -148,19 +148,21 @@ __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
       uo.load(up, c, a.width);
       look(go, uo, c);
     }
+    top[0] = widened<T>(top[0]);
+    top[1] = widened<T>(top[1]);
     block_max<WAVES>(top, lds[turn]);
     const Scale qg(top[0]), qu(top[1]), qh(top[2]);
     if (threadIdx.x == 0) {
       if (a.gate8.d_codes) a.gate8.d_scales[row] = qg.stored;
       if (a.up8.d_codes) a.up8.d_scales[row] = qu.stored;
-      if (a.h8.d_codes) a.h8.d_scales[row] = qh.stored;
+      if constexpr (H8) a.h8.d_scales[row] = qh.stored;
     }
     const auto write = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
       if (a.gate8.d_codes)
         *(uint2 *)(a.gate8.d_codes + row * a.gate8.stride + c) = codes8(qg, [&](int i) { return go.get(i); });
       if (a.up8.d_codes)
         *(uint2 *)(a.up8.d_codes + row * a.up8.stride + c) = codes8(qu, [&](int i) { return uo.get(i); });
-      if (a.h8.d_codes)
+      if constexpr (H8)
         *(uint2 *)(a.h8.d_codes + row * a.h8.stride + c) =
             codes8(qh, [&](int i) { return product(go.get(i), uo.get(i)); });
     };
@@ -208,9 +210,18 @@ __global__ void __launch_bounds__(256) swiglu_backward_kernel(SwigluBackArgs a, 
   }
 }
 
+unsigned row_blocks(int n) { return (unsigned)std::min(n, 65536); }
+template <class T, bool H8>
+hipError_t launch_swiglu(const SwigluArgs &a, hipStream_t s) {
+  const unsigned blocks = row_blocks(a.n);
+  if (a.width <= 1024) swiglu_kernel<T, 1, 2, H8><<<blocks, 64, 0, s>>>(a);
+  else if (a.width <= 4096) swiglu_kernel<T, 4, 2, H8><<<blocks, 256, 0, s>>>(a);
+  else if (a.width <= 12288) swiglu_kernel<T, 8, 3, H8><<<blocks, 512, 0, s>>>(a);
+  else swiglu_kernel<T, 16, 2, H8><<<blocks, 1024, 0, s>>>(a);
+  return hipGetLastError();
+}
 // Blocks of a kernel that walks `all` items 256 at a time.
 unsigned walk_blocks(int64_t all) { return (unsigned)std::min<int64_t>((all + 255) / 256, 65536); }
-unsigned row_blocks(int n) { return (unsigned)std::min(n, 65536); }
 
 }  // namespace
 
@@ -219,8 +230,11 @@ hipError_t launch_store(int32_t dtype, int32_t n, int32_t width, const void *x, 
   const StoreArgs a{x, x_stride, codes, codes_stride, scales, n, width};
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
+    // the block that holds the row in registers
     if (width <= 1024) store_kernel<T, 1, 2><<<row_blocks(n), 64, 0, s>>>(a);
+    else if (width <= 4096) store_kernel<T, 4, 2><<<row_blocks(n), 256, 0, s>>>(a);
     else if (width <= 8192) store_kernel<T, 4, 4><<<row_blocks(n), 256, 0, s>>>(a);
+    else if (width <= 12288) store_kernel<T, 4, 6><<<row_blocks(n), 256, 0, s>>>(a);
     else store_kernel<T, 16, 4><<<row_blocks(n), 1024, 0, s>>>(a);
     return hipGetLastError();
   });
@@ -293,10 +307,7 @@ welvet_status welvet_hip_rows8_swiglu(int32_t dtype, int32_t n, int32_t width, c
   WH_HIP(tok::with_type(dtype, [&](auto t) {
     using T = decltype(t);
     hipStream_t s = (hipStream_t)stream;
-    if (width <= 1024) r8::swiglu_kernel<T, 1, 2><<<r8::row_blocks(n), 64, 0, s>>>(a);
-    else if (width <= 8192) r8::swiglu_kernel<T, 8, 2><<<r8::row_blocks(n), 512, 0, s>>>(a);
-    else r8::swiglu_kernel<T, 16, 2><<<r8::row_blocks(n), 1024, 0, s>>>(a);
-    return hipGetLastError();
+    return h8 ? r8::launch_swiglu<T, true>(a, s) : r8::launch_swiglu<T, false>(a, s);
   }));
   return ok();
 }

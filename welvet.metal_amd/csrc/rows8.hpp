@@ -3,7 +3,7 @@
 // c in [-127, 127] and one scale s, value = s c.  Internal to the library.
 //   s = max |x| / 127, rounded to f32;  c = x / s, to nearest, ties to even
 // The code is that of the exact quotient: a product with 1 / s decides unless
-// it lies within 2^-13 of a half, where the remainder x - k s does, exactly.
+// it lies within 2e-5 of a half (it is off by at most 127 2^-23), where the remainder x - k s does, exactly.
 // A row of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and
 // codes 0, so whatever reads it is NaN.
 #pragma once
@@ -34,8 +34,8 @@ struct Scale {
   __device__ inline int code(float x) const {
     const float a = fabsf(x) * lift, q = a * inv;
     float t = rintf(q);
-    if (fabsf(q - t) > 0.4999f) {
-      // within 127 2^-22 of a half: k + 1/2 against the quotient by the remainder,
+    if (fabsf(q - t) > 0.49998f) {
+      // within 2e-5 of a half: k + 1/2 against the quotient by the remainder,
       // a multiple of a's or s's last place near s / 2, so the fma does not round
       const float k = floorf(q), d = fmaf(-k, s, a), half = 0.5f * s;
       t = d > half || (d == half && ((int)k & 1)) ? k + 1.0f : k;
@@ -84,12 +84,48 @@ struct Oct {
 };
 
 // Codes of eight values as two words (0 throughout in a row that is not finite).
+// fma(x, inv, 1.5 2^23) is x inv rounded to a whole number, as its last bits.
 template <class F>
 __device__ inline uint2 codes8(const Scale &q, F &&value) {
-  uint32_t w[2] = {0, 0};
+  constexpr float kWhole = 0x1.8p23f;
+  if (!q.finite) return make_uint2(0, 0);
+  uint32_t c[8];
+  float off = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(uint8_t)q.code(value(i)) << (8 * (i & 3));
-  return q.finite ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
+  for (int i = 0; i < 8; ++i) {
+    const float x = value(i), r = fmaf(x, q.inv, kWhole);
+    c[i] = f2u(r);
+    off = fmaxf(off, fabsf(fmaf(x, q.inv, kWhole - r)));
+  }
+  if (off > 0.49998f || q.lift != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = (uint32_t)q.code(value(i));
+  }
+  const auto four = [&](int i) {  // the last bytes of four words
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[i + 3], c[i + 2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(c[i + 1], c[i], 0x0c0c0400u), 0x05040100u);
+  };
+  return make_uint2(four(0), four(4));
+}
+// The largest magnitude's bits so far, in the type's own width.
+template <class T>
+__device__ inline void raise(uint32_t &top, const Oct<T> &o) {
+  if constexpr (sizeof(typename T::raw) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, o.w[i] & 0x7fffffffu);
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 t = __builtin_bit_cast(u16x2, top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, o.w[i] & 0x7fff7fffu));
+    top = __builtin_bit_cast(uint32_t, t);
+  }
+}
+// ... as an f32's.
+template <class T>
+__device__ inline uint32_t widened(uint32_t top) {
+  if constexpr (sizeof(typename T::raw) == 4) return top;
+  else return magnitude(T::get((typename T::raw)max(top & 0xffffu, top >> 16)));
 }
 __device__ inline float value_of(uint32_t word, int i) { return (float)(int8_t)(word >> (8 * i)); }
 
@@ -122,6 +158,38 @@ __device__ inline float act_f32(float x, int act) {
   case kGELU: return x * Sigmoid(gelu_arg(x)).z;
   }
   return x;
+}
+// Before a rounding to 16 bits: the exponential's argument rounded once, which
+// moves z by at most 0.4 2^-24 and x z, for x < 0, by |x| 2^-24 of itself.
+__device__ inline float quick_sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269502f * x));
+}
+// The activation of a value that becomes a T.
+template <class T>
+__device__ inline float act_of(float x, int act) {
+  if constexpr (sizeof(typename T::raw) == 2) {
+    if (act == kSilu) return x * quick_sigmoid(x);
+    if (act == kSigmoid) return quick_sigmoid(x);
+    if (act == kGELU) return x * quick_sigmoid(gelu_arg(x));
+  }
+  return act_f32(x, act);
+}
+// Eight values at a time, the activation looked at once.
+template <class T>
+__device__ inline void act8(float (&v)[8], int act) {
+  const auto each = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of<T>(v[i], decltype(a)::value);
+  };
+  switch (act) {
+  case kReLU: return each(std::integral_constant<int, kReLU>{});
+  case kReLU2: return each(std::integral_constant<int, kReLU2>{});
+  case kLeakyReLU: return each(std::integral_constant<int, kLeakyReLU>{});
+  case kSilu: return each(std::integral_constant<int, kSilu>{});
+  case kSigmoid: return each(std::integral_constant<int, kSigmoid>{});
+  case kTanh: return each(std::integral_constant<int, kTanh>{});
+  case kGELU: return each(std::integral_constant<int, kGELU>{});
+  }
 }
 __device__ inline float act_prime_f32(float x, int act) {
   switch (act) {

@@ -1,11 +1,18 @@
 // rows8_backward.hip — the backward of a layer from activations kept in 8 bits
 // (rows8.hpp): with pre = p_t c the pre-activations and x = s_t c the input,
 //   dpre = dy act'(pre);  dw = dpre^T x;  dx = dpre W
-// Both products run on the bf16 matrix cores: codes are exact in bf16, and
-// what is left of each term, dpre s_t (dw) or dpre v_o (dx, W = v_o w), is
-// split into bf16 parts.  One pass over dy forms dpre and writes those parts
-// with the sum along their rows (dw's transposed), a second one the codes'
-// images; the products then read nothing but whole stages of bf16.
+// Both products run on the f16 matrix cores: codes are exact in f16, and what
+// is left of each term, dpre s_t (dw) or dpre v_o (dx, W = v_o w), becomes f16
+// parts.  So that f16's range holds them, a channel's (dw) or token's (dx)
+// terms are multiplied by the power of two that brings a bound of theirs, max
+// |dy| s_t or |dy| v_o times what |act'| can be, to 2^14..2^15: two parts keep
+// 22 bits of a term, or 2^-39 of the bound where that is more; the product's
+// epilogue divides by it, exactly.  (Three bf16 parts need no bound and half as
+// many instructions again.)
+//
+// Three steps: the codes' images with the sum along their rows, and the
+// bounds; dpre and its parts from one pass over dy (dw's transposed); the
+// products, which read nothing but whole stages of f16.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -21,20 +28,19 @@ using namespace r8;
 using namespace tiles;
 
 constexpr int kMaxSize = 1 << 20;
-constexpr int kTile = 64;                                     // of the passes: rows and columns a block
-int64_t along(int64_t n) { return (n + 31) / 32 * 32; }       // a sum's length in whole stages of bf16
+constexpr int kTile = 64;                                 // of the passes: rows and columns a block
+constexpr int kBoundCols = 512;                           // of dy a block of the bounds
+// ... and rows: no more than 32 blocks of them.
+int bound_rows(int64_t n) { return (int)((n + 32 * kTile - 1) / (32 * kTile)) * kTile; }
+int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
+__host__ __device__ constexpr int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 
-// v as P bf16 parts, each the rest's nearest.  From the largest bf16 on the
-// first is infinite and the others nothing.
+__device__ inline uint16_t half_bits(float v) { return F16::put(v); }
+// v as P f16 parts, each the rest's nearest; what is not finite is its first part alone.
 template <int P>
 __device__ inline void split(float v, uint16_t (&part)[P]) {
-  part[0] = BF16::put(v);
-  const bool whole = fabsf(v) < 0x1.fep127f;
-#pragma unroll
-  for (int p = 1; p < P; ++p) {
-    v -= BF16::get(part[p - 1]);
-    part[p] = whole ? BF16::put(v) : (uint16_t)0;
-  }
+  part[0] = half_bits(v);
+  if constexpr (P == 2) part[1] = fabsf(v) < 65504.0f ? half_bits(v - F16::get(part[0])) : (uint16_t)0;
 }
 
 // A block's 64 x 64 values, two rows a word, so that columns can be read as rows.
@@ -42,38 +48,42 @@ struct Turn {
   uint32_t word[kTile][kTile / 2 + 1];
   __device__ inline void put(int col, int pair, uint32_t v) { word[col][pair] = v; }
   // Sixteen bytes (eight rows) of each column into the image [cols][pitch]:
-  // rows from `row` on, up to `pitch`, columns from `col` on, up to `cols`.
+  // rows from `row` on (an image's rows hold whole tiles), columns from `col` on.
   __device__ inline void write(uint16_t *image, int64_t pitch, int row, int col, int cols) const {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int c = (threadIdx.x >> 3) + 32 * k, at = (threadIdx.x & 7) * 4;
-      if (col + c < cols && row + 2 * at < pitch)
+      if (col + c < cols)
         *(uint4 *)(image + (int64_t)(col + c) * pitch + row + 2 * at) =
             make_uint4(word[c][at], word[c][at + 1], word[c][at + 2], word[c][at + 3]);
     }
   }
 };
 
-// Codes [rows][stride] -> bf16 [width][pitch], the rows' numbers along it.
-__global__ void __launch_bounds__(256) image_kernel(const int8_t *__restrict__ codes, int64_t stride, int rows,
-                                                    int width, int64_t pitch, int across, uint16_t *image) {
-  __shared__ Turn turn;
-  const int row = (int)(blockIdx.x / across) * kTile, col = (int)(blockIdx.x % across) * kTile;
-  const int pair = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
-  uint2 w[2];
+// Codes [rows][stride] -> f16 [width][pitch], the rows' numbers along it.
+struct Image {
+  const int8_t *codes;
+  int64_t stride, pitch;
+  int rows, width, across;
+  uint16_t *to;
+  int blocks;
+  __device__ inline void make(int block, Turn &turn) const {
+    const int row = block / across * kTile, col = block % across * kTile;
+    const int pair = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
+    uint2 w[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int r = row + 2 * pair + k;
-    w[k] = r < rows && col + c < width ? *(const uint2 *)(codes + (int64_t)r * stride + col + c) : make_uint2(0, 0);
-  }
+    for (int k = 0; k < 2; ++k) {
+      const int r = row + 2 * pair + k;
+      w[k] = r < rows && col + c < width ? *(const uint2 *)(codes + (int64_t)r * stride + col + c) : make_uint2(0, 0);
+    }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float lo = value_of(i < 4 ? w[0].x : w[0].y, i & 3), hi = value_of(i < 4 ? w[1].x : w[1].y, i & 3);
-    turn.put(c + i, pair, (f2u(lo) >> 16) | (f2u(hi) & 0xffff0000u));
+    for (int i = 0; i < 8; ++i)
+      turn.put(c + i, pair, half_bits(value_of(i < 4 ? w[0].x : w[0].y, i & 3)) |
+                                ((uint32_t)half_bits(value_of(i < 4 ? w[1].x : w[1].y, i & 3)) << 16));
+    __syncthreads();
+    turn.write(to, pitch, row, col, width);
   }
-  __syncthreads();
-  turn.write(image, pitch, row, col, width);
-}
+};
 
 struct GradArgs {
   const void *dy;
@@ -81,44 +91,164 @@ struct GradArgs {
   const int8_t *pre;  // null: Linear
   int64_t pre_stride;
   const float *pre_scales;
-  const float *x_scales, *w_scales;
+  const float *x_scales, *w_scales;  // null: no dw, no dx
   void *dpre;
   int64_t dpre_stride;
   uint16_t *along_n, *along_o;  // dw's parts [PW][out][n_pitch], dx's [PX][n][o_pitch]
   int64_t n_pitch, o_pitch;
+  uint32_t *col_bound, *row_bound;  // [row blocks][out] of |dy| s_t, [column blocks][n] of |dy| v_o
+  float *col_back, *row_back;       // the powers of two that the products are divided by, inverted
   int n, out, act, across;
+  int bound_rows, col_parts, row_parts;  // a block's rows, bounds a channel and a token
 };
+// What |act'| can be at a row's pre-activations.
+__device__ inline float steepest(const GradArgs &a, int row) {
+  return a.act == kReLU2 ? 256.0f * a.pre_scales[row] : a.act == kSilu || a.act == kGELU ? 1.25f : 1.0f;
+}
+__device__ inline uint32_t finite_bits(float v) { return magnitude(v) < 0x7f800000u ? magnitude(v) : 0; }
+// 2^k that brings a bound to 2^14..2^15.
+__device__ inline float lift_of(uint32_t bound) {
+  const int e = (int)(bound >> 23) - 127;
+  return bound == 0 ? 1.0f : u2f((uint32_t)(min(max(14 - e, -126), 126) + 127) << 23);
+}
+
+// Bounds of a block's rows and columns; a wave takes a quarter of the rows, a
+// lane eight of the columns.
+template <class T>
+__device__ inline void bounds(const GradArgs &a, int block, uint32_t *lds) {
+  constexpr int kAhead = sizeof(typename T::raw) == 4 ? 4 : 8;
+  const int bm = block / a.row_parts, bn = block % a.row_parts;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = bn * kBoundCols + lane * 8;
+  const int begin = bm * a.bound_rows + wave * (a.bound_rows / 4), end = min(begin + a.bound_rows / 4, a.n);
+  uint32_t top[8] = {};
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = a.w_scales && c + i < a.out ? a.w_scales[c + i] : 0.0f;
+  for (int r0 = begin; r0 < end; r0 += kAhead) {
+    Oct<T> o[kAhead];
+    float s[kAhead], steep[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int r = min(r0 + j, end - 1);  // the last row again changes nothing
+      o[j].load((const typename T::raw *)a.dy + (int64_t)r * a.dy_stride, min(c, a.out), a.out);
+      steep[j] = steepest(a, r);
+      s[j] = a.x_scales ? a.x_scales[r] * steep[j] : 0.0f;
+    }
+    uint32_t most[kAhead] = {};
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = o[j].get(i);
+        top[i] = max(top[i], finite_bits(d * s[j]));
+        most[j] = max(most[j], finite_bits(d * (v[i] * steep[j])));
+      }
+    if (a.w_scales) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) most[j] = max(most[j], (uint32_t)__shfl_xor((int)most[j], off));
+      uint32_t own = most[0];
+#pragma unroll
+      for (int j = 1; j < kAhead; ++j) own = lane == j ? most[j] : own;
+      if (lane < kAhead && r0 + lane < end) a.row_bound[(int64_t)bn * a.n + r0 + lane] = own;
+    }
+  }
+  if (!a.x_scales) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lds[wave * kBoundCols + lane * 8 + i] = top[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBoundCols && bn * kBoundCols + i < a.out; i += 256)
+    a.col_bound[(int64_t)bm * a.out + bn * kBoundCols + i] =
+        max(max(lds[i], lds[kBoundCols + i]), max(lds[2 * kBoundCols + i], lds[3 * kBoundCols + i]));
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) prepare_kernel(Image x, Image w, GradArgs a) {
+  __shared__ Turn turn;
+  static_assert(sizeof(Turn) >= 4 * kBoundCols * 4, "the bounds' place");
+  int block = blockIdx.x;
+  const int of_dy = a.col_parts * a.row_parts;
+  if (block < of_dy) return bounds<T>(a, block, &turn.word[0][0]);
+  block -= of_dy;
+  if (block < x.blocks) return x.make(block, turn);
+  w.make(block - x.blocks, turn);
+}
+
+// Many bounds a channel or token into their first.
+__global__ void __launch_bounds__(256) fold_kernel(GradArgs a) {
+  int i = (int)blockIdx.x * 256 + threadIdx.x;
+  const auto fold = [](uint32_t *bound, int parts, int all, int at) {
+    uint32_t top = 0;
+    for (int p = 0; p < parts; ++p) top = max(top, bound[(int64_t)p * all + at]);
+    bound[at] = top;
+  };
+  if (a.along_n) {
+    if (i < a.out) return fold(a.col_bound, a.col_parts, a.out, i);
+    i -= a.out;
+  }
+  if (a.along_o && i < a.n) fold(a.row_bound, a.row_parts, a.n, i);
+}
+
+// Powers of two of this block's 64 rows or columns into `lift`, from `parts` bounds each.
+__device__ inline void lifts(const uint32_t *bound, int parts, int first, int all, float *back, uint32_t *lds,
+                             float *lift) {
+  const int i = threadIdx.x & 63, part = threadIdx.x >> 6;
+  uint32_t top = 0;
+  if (first + i < all)
+    for (int p = part; p < parts; p += 4) top = max(top, bound[(int64_t)p * all + first + i]);
+  lds[threadIdx.x] = top;
+  __syncthreads();
+  if (part == 0) {
+    const float l = lift_of(max(max(lds[i], lds[64 + i]), max(lds[128 + i], lds[192 + i])));
+    lift[i] = l;
+    if (back && first + i < all) back[first + i] = 1.0f / l;
+  }
+  __syncthreads();
+}
+
 template <class T, int PW, int PX>
 __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   using raw = typename T::raw;
   __shared__ Turn turn[PW];
+  __shared__ float lift_n[kTile], lift_o[kTile];
   const int row = (int)(blockIdx.x / a.across) * kTile, col = (int)(blockIdx.x % a.across) * kTile;
   const int pair = threadIdx.x >> 3, c = col + (threadIdx.x & 7) * 8;
   float v[2][8], s[2] = {0, 0};
+  Oct<T> o[2];
+  uint2 w[2] = {};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = row + 2 * pair + k;
     const bool in = r < a.n && c < a.out;
-    Oct<T> o;
-    o.load((const raw *)a.dy + (in ? (int64_t)r * a.dy_stride : 0), in ? c : a.out, a.out);
+    o[k].load((const raw *)a.dy + (in ? (int64_t)r * a.dy_stride : 0), in ? c : a.out, a.out);
+    if (in && a.pre) w[k] = *(const uint2 *)(a.pre + (int64_t)r * a.pre_stride + c);
+  }
+  uint32_t *lds = &turn[0].word[0][0];
+  if (a.along_n)
+    lifts(a.col_bound, a.col_parts, col, a.out, row == 0 ? a.col_back : nullptr, lds, lift_o);
+  if (a.along_o)
+    lifts(a.row_bound, a.row_parts, row, a.n, col == 0 ? a.row_back : nullptr, lds, lift_n);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[k][i] = o.get(i);
-    if (!in) continue;
+  for (int k = 0; k < 2; ++k) {
+    const int r = row + 2 * pair + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[k][i] = o[k].get(i);
+    if (r >= a.n || c >= a.out) continue;
     if (a.x_scales) s[k] = a.x_scales[r];
     if (a.pre) {
-      const uint2 w = *(const uint2 *)(a.pre + (int64_t)r * a.pre_stride + c);
       const float p = a.pre_scales[r];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        v[k][i] = c + i < a.out ? v[k][i] * act_prime_f32(value_of(i < 4 ? w.x : w.y, i & 3) * p, a.act) : 0.0f;
+        v[k][i] = c + i < a.out ? v[k][i] * act_prime_f32(value_of(i < 4 ? w[k].x : w[k].y, i & 3) * p, a.act) : 0.0f;
     }
     if (a.dpre) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o.set(i, v[k][i]);
-      o.store((raw *)a.dpre + (int64_t)r * a.dpre_stride, c, a.out);
+      for (int i = 0; i < 8; ++i) o[k].set(i, v[k][i]);
+      o[k].store((raw *)a.dpre + (int64_t)r * a.dpre_stride, c, a.out);
     }
   }
-  if (a.along_o && c < a.o_pitch) {
+  if (a.along_o) {
     float scale[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) scale[i] = c + i < a.out ? a.w_scales[c + i] : 0.0f;
@@ -126,26 +256,29 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
     for (int k = 0; k < 2; ++k) {
       const int r = row + 2 * pair + k;
       if (r >= a.n) continue;
-      uint32_t w[PX][4] = {};
+      const float lift = lift_n[2 * pair + k];
+      uint32_t word[PX][4] = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint16_t part[PX];
-        split<PX>(c + i < a.out ? v[k][i] * scale[i] : 0.0f, part);
+        split<PX>(c + i < a.out ? v[k][i] * scale[i] * lift : 0.0f, part);
 #pragma unroll
-        for (int p = 0; p < PX; ++p) w[p][i >> 1] |= (uint32_t)part[p] << (16 * (i & 1));
+        for (int p = 0; p < PX; ++p) word[p][i >> 1] |= (uint32_t)part[p] << (16 * (i & 1));
       }
 #pragma unroll
       for (int p = 0; p < PX; ++p)
-        *(uint4 *)(a.along_o + ((int64_t)p * a.n + r) * a.o_pitch + c) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+        *(uint4 *)(a.along_o + ((int64_t)p * a.n + r) * a.o_pitch + c) =
+            make_uint4(word[p][0], word[p][1], word[p][2], word[p][3]);
     }
   }
   if (a.along_n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint16_t lo[PW], hi[PW];
+      const float lift = lift_o[c - col + i];
       // rows past the last are nothing, whatever 0 times their values would be
-      split<PW>(row + 2 * pair < a.n ? v[0][i] * s[0] : 0.0f, lo);
-      split<PW>(row + 2 * pair + 1 < a.n ? v[1][i] * s[1] : 0.0f, hi);
+      split<PW>(row + 2 * pair < a.n ? v[0][i] * s[0] * lift : 0.0f, lo);
+      split<PW>(row + 2 * pair + 1 < a.n ? v[1][i] * s[1] * lift : 0.0f, hi);
 #pragma unroll
       for (int p = 0; p < PW; ++p) turn[p].put(c - col + i, pair, lo[p] | ((uint32_t)hi[p] << 16));
     }
@@ -163,81 +296,79 @@ __global__ void __launch_bounds__(256) zero_kernel(float *to, int64_t all) {
 
 // ---------------------------------------------------------------- products
 template <class T, bool ADD, class Tile>
-__global__ void __launch_bounds__(Tile::kWaves * 64) bf16_tile_kernel(Operands g, typename T::raw *to, int64_t stride,
+__global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Operands g, const float *__restrict__ back,
+                                                                      typename T::raw *to, int64_t stride,
                                                                       int tiles_m, int tiles_n) {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
   const Place at = place(tiles_m, tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
+  float *backs = (float *)(lds + Tile::kResults);
   Tile::run(g, m0, n0, acc, lds);
-  Tile::results(m0, n0, acc, [&](int row, int c, float v) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = back[min(m0 + i, g.a_rows - 1)];
+  __syncthreads();
+  Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
     if (row >= g.a_rows || c >= g.b_rows) return;
-    typename T::raw *p = to + row * stride + c;
-    *p = T::put(ADD ? T::get(*p) + v : v);
+    const float b = backs[row - m0];
+    Oct<T> o;
+    if constexpr (ADD) o.load(to + row * stride, c, g.b_rows);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.set(i, ADD ? o.get(i) + v[i] * b : v[i] * b);
+    o.store(to + row * stride, c, g.b_rows);
   });
 }
 
-// 256 x 256 with as many stages in LDS as fit, and 128 x 128.
+// 256 x 256 and 128 x 128.
 template <int P>
-using Large = Tile<Bf16Op, P, 2, 4, 4, 2, P == 1 ? 4 : P == 2 ? 3 : 2>;
+using Large = Tile<HalfOp, P, 2, 4, 4, 2>;
 template <int P>
-using Medium = Tile<Bf16Op, P, 2, 2, 2, 2, P == 3 ? 3 : 4>;
+using Medium = Tile<HalfOp, P, 2, 2, 2, 2>;
 
 template <class T, bool ADD, class Tile>
-hipError_t launch_tiles(const Operands &g, void *to, int64_t stride, hipStream_t s) {
-  const int tm = (g.a_rows + Tile::kRows - 1) / Tile::kRows, tn = (g.b_rows + Tile::kCols - 1) / Tile::kCols;
-  bf16_tile_kernel<T, ADD, Tile><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, (typename T::raw *)to, stride, tm, tn);
+hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t stride, hipStream_t s) {
+  const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
+  half_tile_kernel<T, ADD, Tile><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, back, (typename T::raw *)to, stride, tm, tn);
   return hipGetLastError();
 }
-// to[a_rows][b_rows] (+)= A . B^T with A of P parts.
+// to[a_rows][b_rows] (+)= back . A . B^T with A of P parts.
 template <class T, bool ADD, int P>
-hipError_t launch_bf16(const Operands &g, void *to, int64_t stride, hipStream_t s) {
-  if ((int64_t)((g.a_rows + 255) / 256) * ((g.b_rows + 255) / 256) >= 128)
-    return launch_tiles<T, ADD, Large<P>>(g, to, stride, s);
-  return launch_tiles<T, ADD, Medium<P>>(g, to, stride, s);
+hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, hipStream_t s) {
+  if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 128)
+    return launch_tiles<T, ADD, Large<P>>(g, back, to, stride, s);
+  return launch_tiles<T, ADD, Medium<P>>(g, back, to, stride, s);
 }
 
+// Parts of dw's and dx's terms.  One part, rounded as a BFloat16 gradient was
+// (and to 3 bits more), is enough for a dx that is rounded to BFloat16 itself.
+constexpr int kPartsW = 2;
 template <class T>
-struct Parts;
-template <>
-struct Parts<F32> {
-  static constexpr int kW = 3, kX = 3;
-};
-template <>
-struct Parts<F16> {
-  static constexpr int kW = 2, kX = 2;
-};
-template <>
-struct Parts<BF16> {
-  static constexpr int kW = 2, kX = 1;
-};
+constexpr int kPartsX = std::is_same_v<T, BF16> ? 1 : 2;
+
+constexpr int kFewBounds = 4;
 
 struct Plan {
-  size_t grad_w, grad_x, codes_x, codes_w;  // offsets
+  size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back;  // offsets
   size_t bytes;
 };
 Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
-  const int pw = dtype == kFloat32 ? 3 : 2, px = dtype == kFloat32 ? 3 : dtype == kFloat16 ? 2 : 1;
   Plan p{};
   size_t at = 0;
-  const auto take = [&](int64_t values) {
+  const auto take = [&](int64_t bytes) {
     const size_t was = at;
-    at += pad256((size_t)values * 2);
+    at += pad256((size_t)bytes);
     return was;
   };
-  p.grad_w = take(pw * out * along(n));
-  p.codes_x = take(in * along(n));
-  p.grad_x = take(px * n * along(out));
-  p.codes_w = take(in * along(out));
+  p.grad_w = take(2 * kPartsW * out * along(n));
+  p.codes_x = take(2 * in * along(n));
+  p.grad_x = take(2 * (dtype == kBFloat16 ? kPartsX<BF16> : kPartsX<F32>) * n * along(out));
+  p.codes_w = take(2 * in * along(out));
+  p.col_bound = take(4 * std::min<int64_t>(32, tiles_of(n, kTile)) * out);  // not fewer than any smaller n needs
+  p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
+  p.col_back = take(4 * out);
+  p.row_back = take(4 * n);
   p.bytes = at;
   return p;
-}
-
-hipError_t launch_image(const int8_t *codes, int64_t stride, int rows, int width, int64_t pitch, uint16_t *image,
-                        hipStream_t s) {
-  const int across = (width + kTile - 1) / kTile;
-  image_kernel<<<(unsigned)((pitch + kTile - 1) / kTile) * across, 256, 0, s>>>(codes, stride, rows, width, pitch, across, image);
-  return hipGetLastError();
 }
 
 bool sizes_ok(int32_t n, int32_t in, int32_t out) {
@@ -245,9 +376,9 @@ bool sizes_ok(int32_t n, int32_t in, int32_t out) {
 }
 // A launch of fewer than 2^32 threads: 256 a 64 x 64 tile of the passes.
 bool launchable(int64_t n, int64_t in, int64_t out) {
-  const auto tiles = [](int64_t v) { return (v + kTile - 1) / kTile; };
-  constexpr int64_t most = (int64_t)1 << 24;
-  return tiles(along(n)) * tiles(along(out)) < most && tiles(along(n)) * tiles(in) < most && tiles(along(out)) * tiles(in) < most;
+  constexpr int64_t most = (int64_t)1 << 23;
+  const int64_t tn = tiles_of(n, kTile), ti = tiles_of(in, kTile), to = tiles_of(out, kTile);
+  return tn * to < most && ti * (tn + to) < most;
 }
 
 }  // namespace
@@ -307,6 +438,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   }
   char *ws = (char *)d_ws;
   GradArgs a{};
+  Image x{}, w{};
   a.dy = d_dy;
   a.dy_stride = dy_stride;
   if (act != kLinear) {
@@ -319,37 +451,54 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   a.n = n;
   a.out = out;
   a.act = act;
-  a.across = (int)((along(out) + kTile - 1) / kTile);
+  a.across = tiles_of(out, kTile);
+  a.bound_rows = bound_rows(n);
+  a.col_parts = tiles_of(n, a.bound_rows);
+  a.row_parts = tiles_of(out, kBoundCols);
   a.n_pitch = along(n);
   a.o_pitch = along(out);
+  a.col_bound = (uint32_t *)(ws + p.col_bound);
+  a.row_bound = (uint32_t *)(ws + p.row_bound);
+  a.col_back = (float *)(ws + p.col_back);
+  a.row_back = (float *)(ws + p.row_back);
+  const int in_tiles = tiles_of(in, kTile);
   if (d_dw) {
     a.x_scales = x8->d_scales;
     a.along_n = (uint16_t *)(ws + p.grad_w);
+    x = {x8->d_codes, x8->stride, a.n_pitch, n, in, in_tiles, (uint16_t *)(ws + p.codes_x), tiles_of(n, kTile) * in_tiles};
   }
   if (d_dx) {
     a.w_scales = layer->scales;
     a.along_o = (uint16_t *)(ws + p.grad_x);
+    w = {layer->codes, layer->pitch, a.o_pitch, out, in, in_tiles, (uint16_t *)(ws + p.codes_w), a.across * in_tiles};
   }
-  uint16_t *codes_x = (uint16_t *)(ws + p.codes_x), *codes_w = (uint16_t *)(ws + p.codes_w);
-  const unsigned blocks = (unsigned)((a.n_pitch + kTile - 1) / kTile) * a.across;
   WH_HIP(tok::with_type(dtype, [&](auto t) -> hipError_t {
     using T = decltype(t);
-    constexpr int PW = Parts<T>::kW, PX = Parts<T>::kX;
-    grad_kernel<T, PW, PX><<<blocks, 256, 0, s>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && d_dw) {
-      e = launch_image(x8->d_codes, x8->stride, n, in, a.n_pitch, codes_x, s);
-      if (e != hipSuccess) return e;
-      const Operands g{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
-                       (const char *)codes_x, 2 * a.n_pitch, in, (int)(a.n_pitch / 32)};
-      e = accumulate ? launch_bf16<F32, true, PW>(g, d_dw, in, s) : launch_bf16<F32, false, PW>(g, d_dw, in, s);
+    constexpr int PX = kPartsX<T>;
+    hipError_t e = hipSuccess;
+    if (products) {
+      prepare_kernel<T><<<x.blocks + w.blocks + a.col_parts * a.row_parts, 256, 0, s>>>(x, w, a);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      // every 64 x 64 tile of the next pass reads the bounds of its rows and columns
+      if ((d_dw && a.col_parts > kFewBounds) || (d_dx && a.row_parts > kFewBounds)) {
+        fold_kernel<<<tiles_of((d_dw ? out : 0) + (d_dx ? n : 0), 256), 256, 0, s>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        a.col_parts = a.row_parts = 1;
+      }
     }
-    if (e == hipSuccess && d_dx) {
-      e = launch_image(layer->codes, layer->pitch, out, in, a.o_pitch, codes_w, s);
+    grad_kernel<T, kPartsW, PX><<<(unsigned)tiles_of(n, kTile) * a.across, 256, 0, s>>>(a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (d_dw) {
+      const Operands g{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
+                       (const char *)x.to, 2 * a.n_pitch, in, tiles_of(2 * (int64_t)n, kStageBytes)};
+      e = accumulate ? launch_half<F32, true, kPartsW>(g, a.col_back, d_dw, in, s)
+                     : launch_half<F32, false, kPartsW>(g, a.col_back, d_dw, in, s);
       if (e != hipSuccess) return e;
+    }
+    if (d_dx) {
       const Operands g{(const char *)a.along_o, 2 * a.o_pitch, 2 * n * a.o_pitch, n, INT32_MAX,
-                       (const char *)codes_w, 2 * a.o_pitch, in, (int)(a.o_pitch / 32)};
-      e = launch_bf16<T, false, PX>(g, d_dx, dx_stride, s);
+                       (const char *)w.to, 2 * a.o_pitch, in, tiles_of(2 * (int64_t)out, kStageBytes)};
+      e = launch_half<T, false, PX>(g, a.row_back, d_dx, dx_stride, s);
     }
     return e;
   }));

@@ -1,17 +1,32 @@
 // tiles.hpp — one block's tile of C = A . B^T on the matrix cores, for operands
-// whose rows lie along the sum: bytes (Int8Op) or bf16 (Bf16Op, A as a sum of
-// P parts).  Internal to the library.
+// whose rows lie along the sum: bytes (Int8Op) or f16 (HalfOp, A as a sum of P
+// parts).  Internal to the library.
 //
-// A stage is 64 bytes of each of the tile's rows, copied from memory straight
-// into LDS, a 16-byte chunk a lane; NBUF stages are under way at a time and a
-// block has one barrier a stage.  Chunk c of row r lies at c ^ (r / 2 % 4): the
-// copies stay whole 64-byte pieces of a row, and eight lanes that read the
-// same chunk of neighbouring rows touch all of LDS's banks once.  Rows past an
-// operand's last are the last one again, and their results are not stored.
+// A stage is 128 bytes of each of the tile's rows, copied from memory straight
+// into LDS, a 16-byte chunk a lane; A's stages take turns in three places, B's
+// in two, so that a stage of A is still under way when a block meets at its one
+// barrier a stage.  A's P parts are stages of their own over one of B.  Chunk c
+// of row r lies at c ^ (r / 2 % 8): the copies stay whole 128-byte lines, and
+// sixteen lanes that read the same chunk of neighbouring rows touch all of LDS's
+// banks once.  A wave's chunks for one 32-byte slab of the sum are read while
+// the slab before is multiplied.  Rows past an operand's last are the last one
+// again, and their results are not stored.
+//
+// 256 x 256 is bound by the operands' way from the L2s (the copies alone, of
+// 8192 x 11008 x 4096 bytes, take 205 us of 367, the products alone 280), at
+// some 2.0 GHz.  Measured beside it (us; int8 8192 x 11008 x 4096, f16 8192 x
+// 4096 x 11008, f16 of two parts 11008 x 4096 x 8192): 367, 611, 1256; four
+// waves of 128 x 128 each 343, 630, 1284; 128 x 128 tiles, two blocks a CU, 369,
+// 734; stages of 64 bytes, four places, 397, 754, 1514; two parts as twice the
+// sum 1358; two places for both, loads issued after the barrier 367, 586, 1370
+// (128 x 256); the barrier ahead of the last slab's products 376, 612, 1238.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
+#include <utility>
 
 namespace wh {
 namespace tiles {
@@ -19,7 +34,7 @@ namespace tiles {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct Int8Op {
   using acc = i32x16;
@@ -27,15 +42,19 @@ struct Int8Op {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
   }
 };
-struct Bf16Op {
+struct HalfOp {
   using acc = f32x16;
   __device__ static inline acc mma(i32x4 a, i32x4 b, acc c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
   }
 };
 
-constexpr int kStageBytes = 64;
+constexpr int kStageBytes = 128;
+// Bytes between rows of at least `bytes`: an odd multiple of the 256 bytes after
+// which memory's channels change, so that a tile's rows, read at one place along
+// them, lie in all of an L2's 16.
+constexpr int64_t spread(int64_t bytes) { return ((bytes + 255) / 256 | 1) * 256; }
 
 struct Operands {
   const char *a;
@@ -49,99 +68,150 @@ struct Operands {
 };
 
 // WM x WN waves, each TM x TN products of 32 x 32.
-template <class Op, int P, int WM, int WN, int TM, int TN, int NBUF>
+template <class Op, int P, int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRows = WM * TM * 32, kCols = WN * TN * 32;
-  static constexpr int kStage = (P * kRows + kCols) * kStageBytes, kLds = NBUF * kStage;
-  static constexpr int kLoads = (P * kRows + kCols) / 16 / kWaves;
-  static_assert((P * kRows + kCols) % (16 * kWaves) == 0, "every wave copies whole pieces of 16 rows");
+  static constexpr int kA = kRows * kStageBytes, kB = kCols * kStageBytes, kLds = 3 * kA + 2 * kB;
+  static constexpr int kLoadsA = kRows / 8 / kWaves, kLoadsB = kCols / 8 / kWaves;
   static constexpr int kTM = TM, kTN = TN;
+  // of LDS after the products: the results' turning place, then the caller's
+  static constexpr int kResults = kWaves * 32 * (TN * 32 + 4) * 4;
+  static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kWaves % 2 == 0,
+                "every wave copies whole pieces of 8 rows, its chunks' places the same in all");
+  static_assert(P == 1 || P == 2, "parts");
+  static_assert(TM * TN >= TM + TN || TM * TN == 4, "products to hide the reads under");
   using Acc = typename Op::acc;
-
-  // at most `left` of this wave's loads still under way, and none of its LDS reads
+  // at most `left` of this wave's copies still under way, and none of its LDS reads
   template <int LEFT>
   __device__ static inline void wait() {
     static_assert(LEFT < 64, "the counter's range");
     __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4));
     asm volatile("" ::: "memory");
   }
-
+  // The tile at (m0, n0) into acc; B's rows are the instruction's first side, so a
+  // lane's results are four neighbouring columns each time.
   __device__ static inline void run(const Operands &o, int m0, int n0, Acc (&acc)[TM][TN], char *lds) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const char *from[kLoads];
-    int last[kLoads];
-    const int chunk = ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
+    const char *from_a[kLoadsA], *from_b[kLoadsB];
+    const int chunk = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;
+    // how far the last stage's chunk lies past A's last one
+    const int past = max((o.stages - 1) * kStageBytes + chunk - o.a_last, 0);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int piece = j * kWaves + wave;
-      if (piece < P * (kRows / 16)) {
-        const int part = piece / (kRows / 16), r = m0 + piece % (kRows / 16) * 16 + (lane >> 2);
-        from[j] = o.a + part * o.a_plane + (int64_t)min(r, o.a_rows - 1) * o.a_pitch;
-        last[j] = o.a_last;
-      } else {
-        const int r = n0 + (piece - P * (kRows / 16)) * 16 + (lane >> 2);
-        from[j] = o.b + (int64_t)min(r, o.b_rows - 1) * o.b_pitch;
-        last[j] = INT32_MAX;
+    for (int j = 0; j < kLoadsA; ++j)
+      from_a[j] = o.a + (int64_t)min(m0 + (j * kWaves + wave) * 8 + (lane >> 3), o.a_rows - 1) * o.a_pitch + chunk;
+#pragma unroll
+    for (int j = 0; j < kLoadsB; ++j)
+      from_b[j] = o.b + (int64_t)min(n0 + (j * kWaves + wave) * 8 + (lane >> 3), o.b_rows - 1) * o.b_pitch + chunk;
+    const int steps = o.stages * P;
+    const auto copy = [&](const char *p, char *to) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)p,
+                                       (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    const auto load_a = [&](int h, int part, char *to) {
+      if (h >= steps - P && o.a_last != INT32_MAX && (P == 1 || part == 0)) {
+#pragma unroll
+        for (int j = 0; j < kLoadsA; ++j) from_a[j] -= past;
       }
-    }
-    const auto load = [&](int stage, int buf) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int at = min(stage * kStageBytes + chunk, last[j]);
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)(from[j] + at),
-            (__attribute__((address_space(3))) void *)(lds + buf * kStage + (j * kWaves + wave) * 1024), 16, 0, 0);
+      for (int j = 0; j < kLoadsA; ++j) {
+        copy(P == 1 || part == 0 ? from_a[j] : from_a[j] + o.a_plane, to + (j * kWaves + wave) * 1024);
+        if (part == P - 1) from_a[j] += kStageBytes;
       }
     };
-    // this lane's chunk of its first row of A and of B; the second half of a stage lies at ^ 32
-    const int swz = (((lane >> 5) ^ ((lane >> 1) & 3)) * 16) + (lane & 31) * kStageBytes;
-    const int a_at = wm * TM * 32 * kStageBytes + swz, b_at = (P * kRows + wn * TN * 32) * kStageBytes + swz;
+    const auto load_b = [&](char *to) {
 #pragma unroll
-    for (int s = 0; s < NBUF - 1; ++s)
-      if (s < o.stages) load(s, s);
-    int buf = 0, into = NBUF - 1;
-    for (int s = 0; s < o.stages; ++s) {
-      if (s + NBUF - 2 < o.stages) wait<(NBUF - 2) * kLoads>();
-      else wait<0>();
+      for (int j = 0; j < kLoadsB; ++j) {
+        copy(from_b[j], to + (j * kWaves + wave) * 1024);
+        from_b[j] += kStageBytes;
+      }
+    };
+    // this lane's chunk of its first rows; slab s lies at ^ 32 s
+    const int swz = (((lane >> 5) ^ ((lane >> 1) & 7)) * 16) + (lane & 31) * kStageBytes;
+    const int a_at = wm * TM * 32 * kStageBytes + swz, b_at = wn * TN * 32 * kStageBytes + swz;
+    char *const lds_b = lds + 3 * kA;
+    i32x4 a[2][TM], b[2][TN];
+    const auto fetch = [&](const char *at, const char *bt, int slab, int into) {
+#pragma unroll
+      for (int u = 0; u < TN; ++u) b[into][u] = *(const i32x4 *)(bt + ((b_at ^ (slab * 32)) + u * 32 * kStageBytes));
+#pragma unroll
+      for (int t = 0; t < TM; ++t) a[into][t] = *(const i32x4 *)(at + ((a_at ^ (slab * 32)) + t * 32 * kStageBytes));
+    };
+    constexpr int kReads = TN + TM, kMul = TM * TN;
+    load_b(lds_b);
+    load_a(0, 0, lds);
+    if (steps > 1) load_a(1, 1 % P, lds + kA);
+    int ia = 0, ib = 0;  // slots of this step
+    const auto step = [&](int h, auto part_) {
+      constexpr int part = decltype(part_)::value;
+      if (h + P + 1 >= steps) wait<0>();
+      else wait<P == 2 && part == 1 ? kLoadsA + kLoadsB : kLoadsA>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s + NBUF - 1 < o.stages) load(s + NBUF - 1, into);
-      const char *at = lds + buf * kStage;
+      if (part == 0 && h + P < steps) load_b(lds_b + (ib ^ 1) * kB);
+      if (h + 2 < steps) load_a(h + 2, (part + 2) % P, lds + (ia == 0 ? 2 : ia - 1) * kA);
+      const char *at = lds + ia * kA, *bt = lds_b + ib * kB;
+      fetch(at, bt, 0, 0);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        i32x4 a[P][TM], b[TN];
+      for (int slab = 0; slab < 4; ++slab) {
+        if (slab < 3) fetch(at, bt, slab + 1, (slab + 1) & 1);
 #pragma unroll
-        for (int u = 0; u < TN; ++u) b[u] = *(const i32x4 *)(at + ((b_at ^ (half * 32)) + u * 32 * kStageBytes));
+        for (int t = 0; t < TM; ++t)
 #pragma unroll
-        for (int p = 0; p < P; ++p)
+          for (int u = 0; u < TN; ++u)
+            acc[t][u] = Op::mma(b[slab & 1][u], a[slab & 1][t], acc[t][u]);
+        // a read after each product, until they are all under way
+        if (slab < 3) {
 #pragma unroll
-          for (int t = 0; t < TM; ++t)
-            a[p][t] = *(const i32x4 *)(at + ((a_at ^ (half * 32)) + (p * kRows + t * 32) * kStageBytes));
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-          for (int t = 0; t < TM; ++t)
-#pragma unroll
-            for (int u = 0; u < TN; ++u) acc[t][u] = Op::mma(a[p][t], b[u], acc[t][u]);
+          for (int i = 0; i < kReads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
       }
-      buf = buf + 1 == NBUF ? 0 : buf + 1;
-      into = into + 1 == NBUF ? 0 : into + 1;
+      ia = ia == 2 ? 0 : ia + 1;
+      if (part == P - 1) ib ^= 1;
+    };
+    for (int h = 0; h < steps; h += P) {
+      step(h, std::integral_constant<int, 0>{});
+      if constexpr (P == 2) step(h + 1, std::integral_constant<int, 1>{});
     }
   }
-  // f(row, col, value) of this lane's results, row by row: 32 lanes take 32 neighbouring columns.
+  // The first of the eight columns that `results` gives a lane.
+  __device__ static inline int first_col(int n0) {
+    return n0 + (int)(threadIdx.x >> 6) % WN * TN * 32 + (int)(threadIdx.x & 63) % (TN * 4) * 8;
+  }
+  // f(row, col, values) with eight neighbouring columns of a row a lane, eight or
+  // more lanes a row: a wave turns its results 32 rows at a time in LDS, which
+  // has to be left by the block's products (a barrier).
+  using Value = std::remove_cv_t<std::remove_reference_t<decltype(std::declval<Acc>()[0])>>;
   template <class F>
-  __device__ static inline void results(int m0, int n0, const Acc (&acc)[TM][TN], F &&f) {
+  __device__ static inline void results(int m0, int n0, const Acc (&acc)[TM][TN], char *lds, F &&f) {
+    constexpr int kPitch = TN * 32 + 4, kAcross = TN * 4;  // values, lanes a row
+    static_assert(kWaves * 32 * kPitch * 4 <= kResults, "the results' place");
+    typedef Value quad __attribute__((ext_vector_type(4)));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
+    Value *mine = (Value *)lds + wave * 32 * kPitch;
+    const int m = m0 + wave / WN * TM * 32 + lane / kAcross, n = n0 + wave % WN * TN * 32 + lane % kAcross * 8;
 #pragma unroll
-    for (int t = 0; t < TM; ++t)
+    for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int u = 0; u < TN; ++u)
 #pragma unroll
-        for (int u = 0; u < TN; ++u)
-          f(m0 + (wm * TM + t) * 32 + (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3), n0 + (wn * TN + u) * 32 + (lane & 31),
-            acc[t][u][i]);
+        for (int i = 0; i < 16; i += 4)
+          *(quad *)(mine + (lane & 31) * kPitch + u * 32 + i * 2 + (lane >> 5) * 4) =
+              quad{acc[t][u][i], acc[t][u][i + 1], acc[t][u][i + 2], acc[t][u][i + 3]};
+      asm volatile("" ::: "memory");
+#pragma unroll 1
+      for (int r = 0; r < 32; r += 64 / kAcross) {
+        const quad *at = (const quad *)(mine + (r + lane / kAcross) * kPitch + lane % kAcross * 8);
+        const quad lo = at[0], hi = at[1];
+        const Value v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        f(m + t * 32 + r, n, v);
+      }
+      asm volatile("" ::: "memory");
+    }
   }
 };
 
