@@ -85,7 +85,7 @@ def test_backward_is_checked():
     refused(call(d_dw=128, x=ROWS, ws=24), "workspace")
     refused(call(dy_stride=59, d_dpre=128))
     for n, inn, out in ((-1, 50, 60), (3, 0, 60), (3, 50, 2 ** 20 + 1), (2 ** 20 + 1, 50, 60),
-                        (2 ** 20, 50, 2 ** 16 + 2)):  # the last: 2^24 tiles and more
+                        (2 ** 20, 50, 2 ** 15 + 2)):  # the last: 2^22 blocks and more
         refused(call(n=n, inn=inn, out=out, d_dpre=128))
         assert pywelvet.lib().welvet_hip_rows8_backward_bytes(1, n, inn, out, C.byref(C.c_size_t())).code == 1
     accepted(call(d_dpre=128, ws=None, ws_bytes=0))

@@ -30,30 +30,86 @@ struct Out {
 };
 __device__ inline float pre_of(int sum, float scale, float bias) { return fmaf((float)sum, scale, bias); }
 
-// ---------------------------------------------------------- up to 64 rows
+// Eight results of a row from channel c on.
+template <class T>
+__device__ inline void put8(const Out &o, int row, int c, const int (&sum)[8], float s, const float (&scale)[8],
+                            const float (&bias)[8]) {
+  float v[8];
+  Oct<T> out;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = pre_of(sum[i], s * scale[i], bias[i]);
+  if (o.pre) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.set(i, v[i]);
+    out.store((typename T::raw *)o.pre + row * o.pre_stride, c, o.out);
+  }
+  if (o.post) {
+    act8<T>(v, o.act);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.set(i, v[i]);
+    out.store((typename T::raw *)o.post + row * o.post_stride, c, o.out);
+  }
+}
+// A lane's eight channels: their scales and biases.
+__device__ inline void channels(const Out &o, int first, float (&scale)[8], float (&bias)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    scale[i] = o.w_scales[min(first + i, o.out - 1)];
+    bias[i] = o.bias[min(first + i, o.out - 1)];
+  }
+}
+
+// --------------------------------------------------------------- few rows
 // Weights are read once and bound the call: a block takes 16 channels, its
 // eight waves every eighth 64 bytes of their rows, and joins the waves' sums in
 // LDS.  Sixteen rows of x are the matrix instruction's other side, TILES times.
-template <class T, int TILES>
-__global__ void __launch_bounds__(512) int8_few_kernel(const int8_t *__restrict__ codes, int64_t pitch,
-                                                       const int8_t *__restrict__ x, int64_t x_stride, int last,
-                                                       int steps, Out o) {
-  constexpr int kWaves = 8, kAhead = TILES == 1 ? 8 : 4;
-  __shared__ i32x4 part[kWaves][TILES][64];
+struct Few {
+  const int8_t *codes;
+  int64_t pitch;
+  const int8_t *x;
+  int64_t x_stride;
+  int last, steps;
+};
+template <class T, int WAVES, int TILES>
+__device__ inline void few_join(const Out &o, int first, const i32x4 (&acc)[TILES], i32x4 *part, const float *x_scales) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) part[(wave * TILES + t) * 64 + lane] = acc[t];
+  __syncthreads();
+  if (wave >= TILES) return;
+  i32x4 sum = part[wave * 64 + lane];
+#pragma unroll
+  for (int k = 1; k < WAVES; ++k) sum += part[(k * TILES + wave) * 64 + lane];
+  const int row = wave * 16 + (lane & 15);
+  if (row >= o.n) return;
+  const float scale = x_scales[row];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = first + (lane >> 4) * 4 + i;
+    if (c >= o.out) break;
+    const float pre = pre_of(sum[i], scale * o.w_scales[c], o.bias[c]);
+    if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(pre);
+    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_of<T>(pre, o.act));
+  }
+}
+template <class T, int WAVES, int TILES>
+__global__ void __launch_bounds__(WAVES * 64) int8_few_kernel(Few f, Out o) {
+  constexpr int kAhead = TILES == 1 ? 8 : 4;
+  __shared__ i32x4 part[WAVES * TILES * 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int first = blockIdx.x * 16;
-  const int8_t *w = codes + (int64_t)min(first + r, o.out - 1) * pitch + q * 16;
+  const int8_t *w = f.codes + (int64_t)min(first + r, o.out - 1) * f.pitch + q * 16;
   const int8_t *xs[TILES];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) xs[t] = x + (int64_t)min(t * 16 + r, o.n - 1) * x_stride;
+  for (int t = 0; t < TILES; ++t) xs[t] = f.x + (int64_t)min(t * 16 + r, o.n - 1) * f.x_stride;
   i32x4 acc[TILES] = {};
   int s = wave;
-  for (; s + (kAhead - 1) * kWaves < steps; s += kAhead * kWaves) {
+  for (; s + (kAhead - 1) * WAVES < f.steps; s += kAhead * WAVES) {
     i32x4 a[kAhead], b[kAhead][TILES];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      a[k] = __builtin_nontemporal_load((const i32x4 *)(w + (int64_t)(s + k * kWaves) * 64));
-      const int at = min((s + k * kWaves) * 64 + q * 16, last);
+      a[k] = __builtin_nontemporal_load((const i32x4 *)(w + (int64_t)(s + k * WAVES) * 64));
+      const int at = min((s + k * WAVES) * 64 + q * 16, f.last);
 #pragma unroll
       for (int t = 0; t < TILES; ++t) b[k][t] = *(const i32x4 *)(xs[t] + at);
     }
@@ -62,105 +118,219 @@ __global__ void __launch_bounds__(512) int8_few_kernel(const int8_t *__restrict_
 #pragma unroll
       for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][t], acc[t], 0, 0, 0);
   }
-  for (; s < steps; s += kWaves) {
+  for (; s < f.steps; s += WAVES) {
     const i32x4 a = __builtin_nontemporal_load((const i32x4 *)(w + (int64_t)s * 64));
-    const int at = min(s * 64 + q * 16, last);
+    const int at = min(s * 64 + q * 16, f.last);
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
       acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const i32x4 *)(xs[t] + at), acc[t], 0, 0, 0);
   }
+  few_join<T, WAVES, TILES>(o, first, acc, part, o.x_scales);
+}
+
+// A few rows straight from x: every block stores them in 8 bits for itself, in
+// LDS, while its first weights are under way; one launch instead of two.  The
+// block's waves share the rows.
+constexpr int kOwnRows = 4, kOwnCodes = 32768, kOwnWaves = 8;
+template <class T>
+__global__ void __launch_bounds__(kOwnWaves * 64, 6) int8_own_kernel(Few f, const typename T::raw *x, int64_t x_stride,
+                                                                  int in, Out o) {
+  constexpr int kAhead = 8, kGroups = sizeof(typename T::raw) == 4 ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) uint2 codes[kOwnCodes / 8];
+  __shared__ i32x4 part[kOwnWaves * 64];
+  __shared__ uint32_t tops[kOwnWaves];
+  __shared__ float scales[kOwnRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int first = blockIdx.x * 16, padded_in = f.last + 16;
+  const int8_t *w = f.codes + (int64_t)min(first + r, o.out - 1) * f.pitch + q * 16;
+  const int waves = o.n == 1 ? kOwnWaves : o.n == 2 ? kOwnWaves / 2 : kOwnWaves / 4;  // of a row
+  const int row = min(wave / waves, o.n - 1), own = threadIdx.x % (waves * 64), step = waves * 64;
+  const typename T::raw *from = x + row * x_stride;
+  const Eights e(in);
+  Oct<T> held[kGroups], rest;
+  uint32_t top = 0;
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) part[wave][t][lane] = acc[t];
-  __syncthreads();
-  if (wave >= TILES) return;
-  i32x4 sum = part[0][wave][lane];
+  for (int g = 0; g < kGroups; ++g)
+    if (g * step < e.whole) e.load(held[g], from, g * step + own);
+  i32x4 a[kAhead];
 #pragma unroll
-  for (int k = 1; k < kWaves; ++k) sum += part[k][wave][lane];
-  const int row = wave * 16 + r;
-  if (row >= o.n) return;
-  const float scale = o.x_scales[row];
+  for (int k = 0; k < kAhead; ++k)  // past the row's end: its last bytes again, not used
+    a[k] = __builtin_nontemporal_load((const i32x4 *)(w + (int64_t)min(wave + k * kOwnWaves, f.steps - 1) * 64));
+  issued();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = first + q * 4 + i;
-    if (c >= o.out) break;
-    const float pre = pre_of(sum[i], scale * o.w_scales[c], o.bias[c]);
-    if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(pre);
-    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_of<T>(pre, o.act));
+  for (int g = 0; g < kGroups; ++g)
+    if (g * step < e.whole) raise(top, held[g]);
+  if (e.left && own == 0) {
+    rest.load(from, e.whole * 8, in);
+    raise(top, rest);
   }
+  for (int g = kGroups * step; g < e.whole; g += step) {
+    Oct<T> h;
+    e.load(h, from, g + own);
+    raise(top, h);
+  }
+  top = widened<T>(top);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  for (int k = wave / waves * waves; k < wave / waves * waves + waves; ++k) top = max(top, tops[k]);
+  const Scale s8(top);
+  int8_t *to = (int8_t *)codes + row * padded_in;
+  if (own == 0) {  // waves without a row of theirs have the last one's again
+    scales[row] = s8.stored;
+    e.finish(to, s8, rest);
+  }
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
+    if (g * step + own < e.whole) {
+      issued();
+      *(uint2 *)(to + (g * step + own) * 8) = codes8(s8, [&](int i) { return held[g].get(i); });
+    }
+  for (int g = kGroups * step + own; g < e.whole; g += step) {
+    Oct<T> h;
+    e.load(h, from, g);
+    *(uint2 *)(to + g * 8) = codes8(s8, [&](int i) { return h.get(i); });
+  }
+  __syncthreads();
+  const char *xs = (const char *)codes + min(r, o.n - 1) * padded_in;
+  i32x4 acc[1] = {};
+  for (int s = wave; s < f.steps; s += kAhead * kOwnWaves) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (s + k * kOwnWaves < f.steps)
+        acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+            a[k], *(const i32x4 *)(xs + min((s + k * kOwnWaves) * 64 + q * 16, f.last)), acc[0], 0, 0, 0);
+    if (s + kAhead * kOwnWaves < f.steps)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        a[k] = __builtin_nontemporal_load(
+            (const i32x4 *)(w + (int64_t)min(s + (kAhead + k) * kOwnWaves, f.steps - 1) * 64));
+  }
+  few_join<T, kOwnWaves, 1>(o, first, acc, part, scales);
 }
 
 // -------------------------------------------------------------- many rows
-template <class T, class Tile>
-__global__ void __launch_bounds__(Tile::kWaves * 64) int8_tile_kernel(Operands g, Out o, int tiles_m, int tiles_n) {
+template <class T, class Tile, bool PART>
+__global__ void __launch_bounds__(Tile::kWaves * 64) int8_tile_kernel(Operands g, Out o, Splits p, int tiles_m,
+                                                                      int tiles_n) {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  float *x_scales = (float *)(lds + Tile::kResults);
-  const Place at = place(tiles_m, tiles_n);
+  const int tile = PART ? (int)blockIdx.x / p.splits : blockIdx.x, split = PART ? (int)blockIdx.x % p.splits : 0;
+  const Place at = place(tile, tiles_m, tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
-  Tile::run(g, m0, n0, acc, lds);
+  Tile::run(PART ? g.part(split * p.each, min(p.each, g.stages - split * p.each)) : g, m0, n0, acc, lds);
   __syncthreads();
-  for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) x_scales[i] = o.x_scales[min(m0 + i, o.n - 1)];
-  // a lane's channels are the same in all its rows
-  const int first = Tile::first_col(n0);
-  float scale[8], bias[8];
+  if constexpr (PART) {
+    Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
+      if (row >= o.n || c >= o.out) return;
+      int *to = (int *)p.parts + split * p.parts_values + (int64_t)row * o.out;
+      Oct<F32> v;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    scale[i] = o.w_scales[min(first + i, o.out - 1)];
-    bias[i] = o.bias[min(first + i, o.out - 1)];
+      for (int i = 0; i < 8; ++i) v.w[i] = sum[i];
+      v.store((uint32_t *)to, c, o.out);
+    });
+  } else {
+    float *x_scales = (float *)(lds + Tile::kResults);
+    for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) x_scales[i] = o.x_scales[min(m0 + i, o.n - 1)];
+    float scale[8], bias[8];  // a lane's channels are the same in all its rows
+    channels(o, Tile::first_col(n0), scale, bias);
+    __syncthreads();
+    Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
+      if (row < o.n && c < o.out) put8<T>(o, row, c, sum, x_scales[row - m0], scale, bias);
+    });
   }
-  __syncthreads();
-  Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
-    if (row >= o.n || c >= o.out) return;
-    const float s = x_scales[row - m0];
-    float v[8];
-    Oct<T> out;
+}
+template <class T>
+__global__ void __launch_bounds__(256) int8_join_kernel(Splits p, Out o, int per_row) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
+  if (row >= o.n) return;
+  const uint32_t *at = (const uint32_t *)p.parts + (int64_t)row * o.out;
+  int sum[8] = {};
+  for (int k = 0; k < p.splits; k += 4) {
+    Oct<F32> v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = pre_of(sum[i], s * scale[i], bias[i]);
-    if (o.pre) {
+    for (int n = 0; n < 4; ++n) v[n].load(at + min(k + n, p.splits - 1) * p.parts_values, c, o.out);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out.set(i, v[i]);
-      out.store((typename T::raw *)o.pre + row * o.pre_stride, c, o.out);
-    }
-    if (o.post) {
-      act8<T>(v, o.act);
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out.set(i, v[i]);
-      out.store((typename T::raw *)o.post + row * o.post_stride, c, o.out);
-    }
-  });
+      for (int j = 0; j < 8; ++j) sum[j] += k + n < p.splits ? (int)v[n].w[j] : 0;
+  }
+  float scale[8], bias[8];
+  channels(o, c, scale, bias);
+  put8<T>(o, row, c, sum, o.x_scales[row], scale, bias);
 }
 
 using Large = Tile<Int8Op, 1, 2, 4, 4, 2>;   // 256 x 256, eight waves
 using Medium = Tile<Int8Op, 1, 2, 2, 2, 2>;  // 128 x 128, four
 
 template <class T, class Tile>
-hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_stride, const Out &o, hipStream_t s) {
+hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_stride, const Out &o, void *parts,
+                        hipStream_t s) {
   const int tm = (o.n + Tile::kRows - 1) / Tile::kRows, tn = (o.out + Tile::kCols - 1) / Tile::kCols;
   const Operands g{(const char *)x, x_stride, 0, o.n, (int)padded(l.in) - 16, (const char *)l.codes, l.pitch, l.out,
                    (l.in + kStageBytes - 1) / kStageBytes};
-  int8_tile_kernel<T, Tile><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, o, tm, tn);
+  const Splits p(tm, tn, g, Tile::kRows, parts);
+  if constexpr (Tile::kRows <= kSplitRows) {
+    if (p.splits > 1) {
+      int8_tile_kernel<T, Tile, true><<<tm * tn * p.splits, Tile::kWaves * 64, 0, s>>>(g, o, p, tm, tn);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      const int per_row = (o.out + 7) / 8;
+      int8_join_kernel<T><<<(unsigned)(((int64_t)o.n * per_row + 255) / 256), 256, 0, s>>>(p, o, per_row);
+      return hipGetLastError();
+    }
+  }
+  int8_tile_kernel<T, Tile, false><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, o, p, tm, tn);
   return hipGetLastError();
 }
 
 hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t *x, int64_t x_stride, const Out &o,
-                          hipStream_t s) {
+                          void *parts, hipStream_t s) {
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int last = (int)padded(l.in) - 16, steps = (l.in + 63) / 64;
+    const Few f{l.codes, l.pitch, x, x_stride, (int)padded(l.in) - 16, (l.in + 63) / 64};
     const unsigned blocks = (unsigned)((l.out + 15) / 16);
-    if (o.n <= 16) int8_few_kernel<T, 1><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
-    else if (o.n <= 32) int8_few_kernel<T, 2><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
-    else if (o.n <= 64) int8_few_kernel<T, 4><<<blocks, 512, 0, s>>>(l.codes, l.pitch, x, x_stride, last, steps, o);
-    else if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 128)
-      return launch_tiles<T, Large>(l, x, x_stride, o, s);
-    else return launch_tiles<T, Medium>(l, x, x_stride, o, s);
+    // 16 waves where eight a CU would be all there are
+    const bool wide = blocks <= 512 && f.steps >= 64;
+    if (o.n <= 16) {
+      if (wide) int8_few_kernel<T, 16, 1><<<blocks, 1024, 0, s>>>(f, o);
+      else int8_few_kernel<T, 8, 1><<<blocks, 512, 0, s>>>(f, o);
+      return hipGetLastError();
+    }
+    if (o.n <= 32) {
+      if (wide) int8_few_kernel<T, 16, 2><<<blocks, 1024, 0, s>>>(f, o);
+      else int8_few_kernel<T, 8, 2><<<blocks, 512, 0, s>>>(f, o);
+      return hipGetLastError();
+    }
+    if (o.n <= 64 && (int64_t)l.in * l.out <= 4 << 20) {
+      int8_few_kernel<T, 8, 4><<<blocks, 512, 0, s>>>(f, o);
+      return hipGetLastError();
+    }
+    // large tiles, a block a CU, where there is one for each (us, large and small
+    // tiles, bf16: 4096 -> 11008 of 2048 rows 146 / 142, of 4096 225 / 246; 11008 ->
+    // 4096 of 2048 rows, 128 large tiles, 175 / 125)
+    if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large>(l, x, x_stride, o, parts, s);
+    return launch_tiles<T, Medium>(l, x, x_stride, o, parts, s);
+  });
+}
+// One launch from x, for rows that the caller does not keep.
+bool own_rows(int32_t in, int32_t n) { return n <= kOwnRows && n * padded(in) <= kOwnCodes; }
+hipError_t launch_own(const welvet_hip_int8 &l, int32_t dtype, const void *x, int64_t x_stride, const Out &o,
+                      hipStream_t s) {
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const Few f{l.codes, l.pitch, nullptr, 0, (int)padded(l.in) - 16, (l.in + 63) / 64};
+    int8_own_kernel<T><<<(unsigned)((l.out + 15) / 16), 512, 0, s>>>(f, (const typename T::raw *)x, x_stride, l.in, o);
     return hipGetLastError();
   });
 }
 
-// The forward's own rows.
+// The forward's own rows, then the parts of a split sum.
 int64_t row_bytes(int32_t in) { return spread(in); }
-size_t forward_bytes(int32_t in, int64_t n) { return pad256((size_t)n * row_bytes(in)) + pad256((size_t)n * 4); }
+size_t parts_at(int32_t in, int64_t n) { return pad256((size_t)n * row_bytes(in)) + pad256((size_t)n * 4); }
+size_t forward_bytes(const welvet_hip_int8 &l, int64_t n) { return parts_at(l.in, n) + parts_bytes(n, l.out); }
 
 void free_layer(welvet_hip_int8 *l) {
   if (!l) return;
@@ -301,7 +471,7 @@ void welvet_hip_int8_release(welvet_hip_int8 *l) { free_layer(l); }
 
 welvet_status welvet_hip_int8_bytes(const welvet_hip_int8 *l, int32_t n, size_t *bytes) {
   if (!l || n < 0 || n > r8::kMaxRows || !bytes) return make_status(kInvalid, "int8: invalid argument");
-  *bytes = forward_bytes(l->in, n);
+  *bytes = forward_bytes(*l, n);
   return ok();
 }
 
@@ -314,7 +484,7 @@ welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *l, int32_t dtype, i
   if (!tok::aligned(d_x, tok::float_size(dtype)))
     return make_status(kInvalid, "int8: device pointers must be aligned to their elements");
   if (const char *why = rows ? r8::rows_fault(rows, n, l->in) : nullptr) return make_status(kInvalid, "int8: %s", why);
-  const size_t need = forward_bytes(l->in, n);
+  const size_t need = forward_bytes(*l, n);
   if (n > 0 && (!d_ws || ws_bytes < need || !tok::aligned(d_ws, 16)))
     return make_status(kInvalid, "int8: %zu bytes of 16-byte aligned workspace are needed", need);
   st = require_device();
@@ -322,8 +492,12 @@ welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *l, int32_t dtype, i
   welvet_hip_rows8 r{(int8_t *)d_ws, row_bytes(l->in), (float *)((char *)d_ws + tok::pad256(n * row_bytes(l->in)))};
   if (rows) r = *rows;
   const Out o{d_pre, d_post, pre_stride, post_stride, r.d_scales, l->scales, l->bias, n, l->out, l->act};
+  if (!rows && own_rows(l->in, n)) {
+    WH_HIP(launch_own(*l, dtype, d_x, x_stride, o, (hipStream_t)stream));
+    return ok();
+  }
   WH_HIP(r8::launch_store(dtype, n, l->in, d_x, x_stride, r.d_codes, r.stride, r.d_scales, (hipStream_t)stream));
-  WH_HIP(launch_product(*l, dtype, r.d_codes, r.stride, o, (hipStream_t)stream));
+  WH_HIP(launch_product(*l, dtype, r.d_codes, r.stride, o, (char *)d_ws + parts_at(l->in, n), (hipStream_t)stream));
   return ok();
 }
 
@@ -333,13 +507,13 @@ welvet_status welvet_hip_int8_product(const welvet_hip_int8 *l, int32_t dtype, i
   welvet_status st = checked_out(l, dtype, n, d_pre, pre_stride, d_post, post_stride);
   if (st.code) return st;
   if (const char *why = r8::rows_fault(rows, n, l->in)) return make_status(kInvalid, "int8: %s", why);
-  const size_t need = forward_bytes(l->in, n);
+  const size_t need = forward_bytes(*l, n);
   if (n > 0 && (!d_ws || ws_bytes < need || !tok::aligned(d_ws, 16)))
     return make_status(kInvalid, "int8: %zu bytes of 16-byte aligned workspace are needed", need);
   st = require_device();
   if (st.code || n == 0) return st;
   const Out o{d_pre, d_post, pre_stride, post_stride, rows->d_scales, l->scales, l->bias, n, l->out, l->act};
-  WH_HIP(launch_product(*l, dtype, rows->d_codes, rows->stride, o, (hipStream_t)stream));
+  WH_HIP(launch_product(*l, dtype, rows->d_codes, rows->stride, o, (char *)d_ws + parts_at(l->in, n), (hipStream_t)stream));
   return ok();
 }
 

@@ -22,7 +22,8 @@ namespace {
 using namespace r8;
 
 constexpr int kThreads = 512;
-constexpr int kStretch = 16384;       // tokens a block: 64 KB of counts, two blocks a CU
+constexpr int kStretch = 8192;        // tokens a block: with the biases 40 KB of LDS, four blocks a CU
+constexpr int kOcts = kStretch / 8 / kThreads;
 constexpr int kMaxHistory = (1 << 20) - 1, kMaxBiases = 1024;
 constexpr uint32_t kCount = kMaxHistory, kBias = 1u << 20, kBiases = 0x7ffu << 20, kPrompt = 1u << 31;
 
@@ -66,95 +67,151 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
   using raw = typename T::raw;
   __shared__ uint4 words[kStretch / 4];
   __shared__ int index[kMaxBiases];
-  __shared__ float bias[kMaxBiases];
+  __shared__ float biases[kMaxBiases];
   uint32_t *count = (uint32_t *)words;
   const int row = blockIdx.x / a.parts, begin = (int)(blockIdx.x % a.parts) * a.len;
   const int len = min(a.len, a.vocab - begin), tid = threadIdx.x;
   const raw *in = (const raw *)a.in + (int64_t)row * a.in_stride + begin;
   raw *out = (raw *)a.out + (int64_t)row * a.out_stride + begin;
+  // Loads go out in the order in which they are waited for, each as early as it
+  // can: the history's first tokens and the list, the mask, the logits that it
+  // leaves, and those that the list names.
+  constexpr int kFirst = 4, kList = kMaxBiases / kThreads;
+  const int32_t *said = a.r.d_history + (int64_t)row * a.r.history_stride;
+  int32_t first[kFirst], at[kList];
+  float bias[kList];
+  if (a.r.history > 0)
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) first[k] = said[min(k * kThreads + tid, a.r.history - 1)];
+  if (a.r.biases > 0)
+#pragma unroll
+    for (int k = 0; k < kList; ++k)
+      if (k * kThreads < a.r.biases) {
+        const int64_t i = (int64_t)row * a.r.biases + min(k * kThreads + tid, a.r.biases - 1);
+        at[k] = a.r.d_bias_index[i];
+        bias[k] = a.r.d_bias[i];
+      }
   const uint32_t *mask = nullptr;
   if (a.r.masks > 0) {
     const int id = a.r.d_mask_id ? a.r.d_mask_id[row] : row;
     if (id >= 0 && id < a.r.masks) mask = a.r.d_masks + id * a.r.mask_stride + begin / 32;
   }
-  const auto open8 = [&](int c) -> uint32_t { return mask ? mask[c >> 5] >> (c & 31) & 0xffu : 0xffu; };
   const int history = a.r.history > 0 && a.r.d_history_len ? min(max(a.r.d_history_len[row], 0), a.r.history) : a.r.history;
   const int prompt = a.r.d_prompt_len ? min(max(a.r.d_prompt_len[row], 0), history) : 0;
-  const int32_t *said = a.r.d_history + (int64_t)row * a.r.history_stride;
-  const bool sparse = history > 0 || a.r.biases > 0;
-  if (sparse) {
-    for (int i = tid; i < (len + 3) / 4; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    for (int i = tid; i < history; i += kThreads) {
-      const int64_t v = (int64_t)said[i] - begin;
-      if (v < 0 || v >= len) continue;
-      if (i < prompt) atomicOr(&count[v], kPrompt);
-      else atomicAdd(&count[v], 1u);
-    }
-    for (int i = tid; i < a.r.biases; i += kThreads) {
-      const int64_t v = (int64_t)a.r.d_bias_index[(int64_t)row * a.r.biases + i] - begin;
-      const bool here = v >= 0 && v < len;
-      index[i] = here ? (int)v : -1;
-      bias[i] = a.r.d_bias[(int64_t)row * a.r.biases + i];
-      if (here) atomicAdd(&count[v], kBias);
-    }
-    __syncthreads();
-  }
   const Row rules{a.r.d_repetition ? (double)a.r.d_repetition[row] : 1.0,
                   a.r.d_frequency ? (double)a.r.d_frequency[row] : 0.0,
                   a.r.d_presence ? (double)a.r.d_presence[row] : 0.0};
-  if (!INPLACE || mask) {
-    for (int c = tid * 8; c < len; c += kThreads * 8) {
-      const uint32_t open = open8(c);
-      Oct<T> o;
-      if constexpr (INPLACE) {
-        if (open == 0xffu) continue;
-        if (open == 0) {
+  const auto open8 = [&](int c) -> uint32_t { return mask ? mask[c >> 5] >> (c & 31) & 0xffu : 0xffu; };
+  uint32_t open[kOcts];
+  Oct<T> held[kOcts];
 #pragma unroll
-          for (int w = 0; w < Oct<T>::kWords; ++w)
-            o.w[w] = sizeof(raw) == 4 ? (uint32_t)kShut<T> : (uint32_t)kShut<T> * 0x10001u;
+  for (int k = 0; k < kOcts; ++k) open[k] = open8(min((k * kThreads + tid) * 8, (len - 1) & ~7));
+#pragma unroll
+  for (int k = 0; k < kOcts; ++k) {
+    const int c = (k * kThreads + tid) * 8;
+    if (c >= len) open[k] = 0;
+    if (!INPLACE && open[k]) held[k].load(in, c, len);
+  }
+  const bool sparse = history > 0 || a.r.biases > 0;
+  raw z[kList];  // the logits that the list names
+  if (sparse) {
+    for (int i = tid; i < (len + 3) / 4; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+    if (a.r.biases > 0)
+#pragma unroll
+      for (int k = 0; k < kList; ++k) {
+        const int i = k * kThreads + tid;
+        if (k * kThreads >= a.r.biases) break;
+        const int64_t v = (int64_t)at[k] - begin;
+        at[k] = i < a.r.biases && v >= 0 && v < len ? (int)v : -1;
+        if (at[k] >= 0) z[k] = in[at[k]];
+        if (i < a.r.biases) {
+          index[i] = at[k];
+          biases[i] = bias[k];
+        }
+      }
+    __syncthreads();
+    const auto count_one = [&](int i, int32_t token) {
+      const int64_t v = (int64_t)token - begin;
+      if (i >= history || v < 0 || v >= len) return;
+      if (i < prompt) atomicOr(&count[v], kPrompt);
+      else atomicAdd(&count[v], 1u);
+    };
+    if (history > 0)
+#pragma unroll
+      for (int k = 0; k < kFirst; ++k) count_one(k * kThreads + tid, first[k]);
+    for (int i = kFirst * kThreads + tid; i < history; i += kFirst * kThreads) {
+      int32_t more[kFirst];
+#pragma unroll
+      for (int k = 0; k < kFirst; ++k) more[k] = said[min(i + k * kThreads, history - 1)];
+#pragma unroll
+      for (int k = 0; k < kFirst; ++k) count_one(i + k * kThreads, more[k]);
+    }
+    if (a.r.biases > 0)
+#pragma unroll
+      for (int k = 0; k < kList; ++k) {
+        if (k * kThreads >= a.r.biases) break;
+        if (at[k] >= 0) atomicAdd(&count[at[k]], kBias);
+      }
+    __syncthreads();
+  }
+  if (!INPLACE || mask) {
+#pragma unroll
+    for (int k = 0; k < kOcts; ++k) {
+      const int c = (k * kThreads + tid) * 8;
+      if (c >= len) break;
+      Oct<T> &o = held[k];
+      if constexpr (INPLACE) {
+        if (open[k] == 0xffu) continue;
+        if (open[k] == 0) {
+          o.fill(kShut<T>);
           o.store(out, c, len);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (!(open >> i & 1) && c + i < len) out[c + i] = kShut<T>;
+            if (!(open[k] >> i & 1) && c + i < len) out[c + i] = kShut<T>;
         }
       } else {
-        raw r[8];
-        if (open) o.load(in, c, len);
+        if (open[k] == 0) {
+          o.fill(kShut<T>);
+        } else {
+          if (sparse) {
+            const uint4 w0 = words[c / 4], w1 = words[c / 4 + 1];
+            const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            if (w0.x | w0.y | w0.z | w0.w | w1.x | w1.y | w1.z | w1.w) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = open >> i & 1 ? o.raw_at(i) : kShut<T>;
-        if (sparse && open) {
-          const uint4 w0 = words[c / 4], w1 = words[c / 4 + 1 < kStretch / 4 ? c / 4 + 1 : c / 4];
-          const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-          if (w0.x | w0.y | w0.z | w0.w | w1.x | w1.y | w1.z | w1.w) {
+              for (int i = 0; i < 8; ++i)
+                if (c + i < len && (w[i] & (kCount | kPrompt)))
+                  o.set_raw(i, rounded<T>(rules.apply((double)o.get(i), w[i])));
+            }
+          }
+          if (open[k] != 0xffu) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (c + i < len && (open >> i & 1) && (w[i] & (kCount | kPrompt)) && !(w[i] & kBiases))
-                r[i] = rounded<T>(rules.apply((double)o.get(i), w[i]));
+              if (!(open[k] >> i & 1)) o.set_raw(i, kShut<T>);
           }
         }
-        __builtin_memcpy(o.w, r, sizeof(o.w));
         o.store(out, c, len);
       }
     }
   }
   if (!sparse) return;
   __syncthreads();  // what a token with a bias holds by now is written again
-  for (int i = tid; i < a.r.biases; i += kThreads) {
-    const int v = index[i];
+#pragma unroll
+  for (int k = 0; k < kList; ++k) {
+    if (k * kThreads >= a.r.biases) break;
+    const int i = k * kThreads + tid, v = at[k];
     if (v < 0 || !(open8(v & ~7) >> (v & 7) & 1)) continue;
     const uint32_t w = count[v];
-    bool first = true;
-    if ((w & kBiases) != kBias)
-      for (int j = 0; j < i; ++j) first = first && index[j] != v;
-    if (!first) continue;
-    double z = rules.apply((double)T::get(in[v]), w);
-    if ((w & kBiases) == kBias) z += (double)bias[i];
-    else
-      for (int j = i; j < a.r.biases; ++j)
-        if (index[j] == v) z += (double)bias[j];
-    out[v] = rounded<T>(z);
+    const bool alone = (w & kBiases) == kBias;
+    bool earlier = false;  // the first of a token's entries stands for all
+    if (!alone)
+      for (int j = 0; j < i; ++j) earlier = earlier || index[j] == v;
+    if (earlier) continue;
+    double sum = rules.apply((double)T::get(z[k]), w) + (double)bias[k];
+    if (!alone)
+      for (int j = i + 1; j < a.r.biases; ++j)
+        if (index[j] == v) sum += (double)biases[j];
+    out[v] = rounded<T>(sum);
   }
   if constexpr (INPLACE) {
     for (int i = tid; i < history; i += kThreads) {

@@ -44,38 +44,48 @@ struct StoreArgs {
 // GROUPS of eight values a thread stay in registers; a longer row is read again.
 template <class T, int WAVES, int GROUPS>
 __global__ void __launch_bounds__(WAVES * 64) store_kernel(StoreArgs a) {
-  constexpr int kThreads = WAVES * 64, kStep = kThreads * 8;
+  constexpr int kThreads = WAVES * 64;
   __shared__ uint32_t lds[2][WAVES];
-  const int end = (a.width + kPad - 1) / kPad * kPad, first = threadIdx.x * 8;
+  const Eights e(a.width);
+  const int tid = threadIdx.x;
   int turn = 0;
   for (int row = blockIdx.x; row < a.n; row += gridDim.x, turn ^= 1) {
     const typename T::raw *x = (const typename T::raw *)a.x + (int64_t)row * a.x_stride;
     int8_t *codes = a.codes + (int64_t)row * a.codes_stride;
-    Oct<T> held[GROUPS];
+    Oct<T> held[GROUPS], rest;
     uint32_t top[1] = {0};
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
-      if (g * kStep < a.width) held[g].load(x, min(first + g * kStep, a.width), a.width);
+      if (g * kThreads < e.whole) e.load(held[g], x, g * kThreads + tid);
+    if (e.left && tid == 0) {
+      rest.load(x, e.whole * 8, a.width);
+      raise(top[0], rest);
+    }
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
-      if (g * kStep < a.width) raise(top[0], held[g]);
-    for (int c = first + GROUPS * kStep; c < a.width; c += kStep) {
+      if (g * kThreads < e.whole) raise(top[0], held[g]);
+    for (int g = GROUPS * kThreads; g < e.whole; g += kThreads) {
       Oct<T> o;
-      o.load(x, c, a.width);
+      e.load(o, x, g + tid);
       raise(top[0], o);
     }
     top[0] = widened<T>(top[0]);
     block_max<WAVES>(top, lds[turn]);
     const Scale q(top[0]);
-    if (threadIdx.x == 0) a.scales[row] = q.stored;
+    if (tid == 0) {
+      a.scales[row] = q.stored;
+      e.finish(codes, q, rest);
+    }
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
-      if (first + g * kStep < end)
-        *(uint2 *)(codes + first + g * kStep) = codes8(q, [&](int i) { return held[g].get(i); });
-    for (int c = first + GROUPS * kStep; c < end; c += kStep) {
+      if (g * kThreads + tid < e.whole) {
+        issued();  // a group at a time: side by side their sums take twice the registers
+        *(uint2 *)(codes + (g * kThreads + tid) * 8) = codes8(q, [&](int i) { return held[g].get(i); });
+      }
+    for (int g = GROUPS * kThreads + tid; g < e.whole; g += kThreads) {
       Oct<T> o;
-      o.load(x, c, a.width);
-      *(uint2 *)(codes + c) = codes8(q, [&](int i) { return o.get(i); });
+      e.load(o, x, g);
+      *(uint2 *)(codes + g * 8) = codes8(q, [&](int i) { return o.get(i); });
     }
   }
 }
@@ -104,76 +114,104 @@ struct SwigluArgs {
   int64_t h_stride;
   int n, width;
 };
-__device__ inline float product(float gate, float up) { return gate * Sigmoid(gate).z * up; }
+template <class T>
+__device__ inline float product(float gate, float up) { return act_of<T>(gate, kSilu) * up; }
 
 // H8: h's own rows are asked for; its products are formed again for their codes.
 template <class T, int WAVES, int GROUPS, bool H8>
 __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
-  constexpr int kThreads = WAVES * 64, kStep = kThreads * 8;
+  constexpr int kThreads = WAVES * 64;
   using raw = typename T::raw;
   __shared__ uint32_t lds[2][3 * WAVES];
-  const int end = (a.width + kPad - 1) / kPad * kPad, first = threadIdx.x * 8;
+  const Eights e(a.width);
+  const int tid = threadIdx.x;
   int turn = 0;
   for (int row = blockIdx.x; row < a.n; row += gridDim.x, turn ^= 1) {
     const raw *gate = (const raw *)a.gate + (int64_t)row * a.gate_stride;
     const raw *up = (const raw *)a.up + (int64_t)row * a.up_stride;
     raw *h = a.h ? (raw *)a.h + (int64_t)row * a.h_stride : nullptr;
-    Oct<T> g[GROUPS], u[GROUPS];
+    Oct<T> g[GROUPS], u[GROUPS], grest, urest;
     uint32_t top[3] = {0, 0, 0};
-    const auto look = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
+    // at: the place of the eight, -1 where another thread has them
+    const auto look = [&](const Oct<T> &go, const Oct<T> &uo, int at, int width) {
       raise(top[0], go);
       raise(top[1], uo);
       if (!H8 && !h) return;
       Oct<T> ho;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float hv = product(go.get(i), uo.get(i));
+        const float hv = product<T>(go.get(i), uo.get(i));
         if constexpr (H8) top[2] = max(top[2], magnitude(hv));
         ho.set(i, hv);
       }
-      if (h) ho.store(h, c, a.width);
+      if (h && at >= 0) ho.store(h, at * 8, width);
     };
+    const auto place = [&](int at) { return at < e.whole ? at : -1; };
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k)
-      if (k * kStep < a.width) {
-        g[k].load(gate, min(first + k * kStep, a.width), a.width);
-        u[k].load(up, min(first + k * kStep, a.width), a.width);
+      if (k * kThreads < e.whole) {
+        e.load(g[k], gate, k * kThreads + tid);
+        e.load(u[k], up, k * kThreads + tid);
       }
+    if (e.left && tid == 0) {
+      grest.load(gate, e.whole * 8, a.width);
+      urest.load(up, e.whole * 8, a.width);
+      look(grest, urest, e.whole, a.width);
+    }
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k)
-      if (k * kStep < a.width) look(g[k], u[k], first + k * kStep);
-    for (int c = first + GROUPS * kStep; c < a.width; c += kStep) {
+      if (k * kThreads < e.whole) {
+        issued();
+        look(g[k], u[k], place(k * kThreads + tid), INT32_MAX);
+      }
+    for (int k = GROUPS * kThreads; k < e.whole; k += kThreads) {
       Oct<T> go, uo;
-      go.load(gate, c, a.width);
-      uo.load(up, c, a.width);
-      look(go, uo, c);
+      e.load(go, gate, k + tid);
+      e.load(uo, up, k + tid);
+      look(go, uo, place(k + tid), INT32_MAX);
     }
     top[0] = widened<T>(top[0]);
     top[1] = widened<T>(top[1]);
     block_max<WAVES>(top, lds[turn]);
     const Scale qg(top[0]), qu(top[1]), qh(top[2]);
-    if (threadIdx.x == 0) {
-      if (a.gate8.d_codes) a.gate8.d_scales[row] = qg.stored;
-      if (a.up8.d_codes) a.up8.d_scales[row] = qu.stored;
-      if constexpr (H8) a.h8.d_scales[row] = qh.stored;
+    int8_t *gc = a.gate8.d_codes ? a.gate8.d_codes + row * a.gate8.stride : nullptr;
+    int8_t *uc = a.up8.d_codes ? a.up8.d_codes + row * a.up8.stride : nullptr;
+    int8_t *hc = H8 ? a.h8.d_codes + row * a.h8.stride : nullptr;
+    if (tid == 0) {
+      if (gc) {
+        a.gate8.d_scales[row] = qg.stored;
+        e.finish(gc, qg, grest);
+      }
+      if (uc) {
+        a.up8.d_scales[row] = qu.stored;
+        e.finish(uc, qu, urest);
+      }
+      if constexpr (H8) {
+        a.h8.d_scales[row] = qh.stored;
+        Oct<F32> hrest;
+        if (e.left)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hrest.set(i, product<T>(grest.get(i), urest.get(i)));
+        e.finish(hc, qh, hrest);
+      }
     }
-    const auto write = [&](const Oct<T> &go, const Oct<T> &uo, int c) {
-      if (a.gate8.d_codes)
-        *(uint2 *)(a.gate8.d_codes + row * a.gate8.stride + c) = codes8(qg, [&](int i) { return go.get(i); });
-      if (a.up8.d_codes)
-        *(uint2 *)(a.up8.d_codes + row * a.up8.stride + c) = codes8(qu, [&](int i) { return uo.get(i); });
+    const auto write = [&](const Oct<T> &go, const Oct<T> &uo, int at) {
+      if (gc) *(uint2 *)(gc + at * 8) = codes8(qg, [&](int i) { return go.get(i); });
+      if (uc) *(uint2 *)(uc + at * 8) = codes8(qu, [&](int i) { return uo.get(i); });
       if constexpr (H8)
-        *(uint2 *)(a.h8.d_codes + row * a.h8.stride + c) =
-            codes8(qh, [&](int i) { return product(go.get(i), uo.get(i)); });
+        *(uint2 *)(hc + at * 8) = codes8(qh, [&](int i) { return product<T>(go.get(i), uo.get(i)); });
     };
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k)
-      if (first + k * kStep < end) write(g[k], u[k], first + k * kStep);
-    for (int c = first + GROUPS * kStep; c < end; c += kStep) {
+      if (k * kThreads + tid < e.whole) {
+        issued();  // a group at a time: side by side their sums take twice the registers
+        write(g[k], u[k], k * kThreads + tid);
+      }
+    for (int k = GROUPS * kThreads + tid; k < e.whole; k += kThreads) {
       Oct<T> go, uo;
-      go.load(gate, c, a.width);
-      uo.load(up, c, a.width);
-      write(go, uo, c);
+      e.load(go, gate, k);
+      e.load(uo, up, k);
+      write(go, uo, k);
     }
   }
 }
@@ -214,7 +252,7 @@ unsigned row_blocks(int n) { return (unsigned)std::min(n, 65536); }
 template <class T, bool H8>
 hipError_t launch_swiglu(const SwigluArgs &a, hipStream_t s) {
   const unsigned blocks = row_blocks(a.n);
-  if (a.width <= 1024) swiglu_kernel<T, 1, 2, H8><<<blocks, 64, 0, s>>>(a);
+  if (a.width <= 1024) swiglu_kernel<T, 2, 1, H8><<<blocks, 128, 0, s>>>(a);
   else if (a.width <= 4096) swiglu_kernel<T, 4, 2, H8><<<blocks, 256, 0, s>>>(a);
   else if (a.width <= 12288) swiglu_kernel<T, 8, 3, H8><<<blocks, 512, 0, s>>>(a);
   else swiglu_kernel<T, 16, 2, H8><<<blocks, 1024, 0, s>>>(a);
@@ -230,8 +268,9 @@ hipError_t launch_store(int32_t dtype, int32_t n, int32_t width, const void *x, 
   const StoreArgs a{x, x_stride, codes, codes_stride, scales, n, width};
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    // the block that holds the row in registers
-    if (width <= 1024) store_kernel<T, 1, 2><<<row_blocks(n), 64, 0, s>>>(a);
+    // the block that holds the row in registers; of few rows, more of it
+    if (width <= 1024) store_kernel<T, 2, 1><<<row_blocks(n), 128, 0, s>>>(a);
+    else if (width <= 16384 && n <= 256) store_kernel<T, 16, 2><<<row_blocks(n), 1024, 0, s>>>(a);
     else if (width <= 4096) store_kernel<T, 4, 2><<<row_blocks(n), 256, 0, s>>>(a);
     else if (width <= 8192) store_kernel<T, 4, 4><<<row_blocks(n), 256, 0, s>>>(a);
     else if (width <= 12288) store_kernel<T, 4, 6><<<row_blocks(n), 256, 0, s>>>(a);

@@ -52,11 +52,9 @@ struct Oct {
   using raw = typename T::raw;
   static constexpr int kWords = sizeof(raw) * 2;
   uint32_t w[kWords];
+  __device__ inline void load(const raw *p) { __builtin_memcpy(w, p, sizeof(w)); }
   __device__ inline void load(const raw *row, int64_t c, int64_t width) {
-    if (c + 8 <= width) {
-      __builtin_memcpy(w, row + c, sizeof(w));
-      return;
-    }
+    if (c + 8 <= width) return load(row + c);
     raw r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = c + i < width ? row[c + i] : (raw)0;
@@ -67,10 +65,15 @@ struct Oct {
     else return (raw)(w[i >> 1] >> (16 * (i & 1)));
   }
   __device__ inline float get(int i) const { return T::get(raw_at(i)); }
-  __device__ inline void set(int i, float v) {
-    if constexpr (sizeof(raw) == 4) w[i] = T::put(v);
-    else if (i & 1) w[i >> 1] = (w[i >> 1] & 0xffffu) | ((uint32_t)T::put(v) << 16);
-    else w[i >> 1] = (w[i >> 1] & 0xffff0000u) | T::put(v);
+  __device__ inline void set_raw(int i, raw v) {
+    if constexpr (sizeof(raw) == 4) w[i] = v;
+    else if (i & 1) w[i >> 1] = (w[i >> 1] & 0xffffu) | ((uint32_t)v << 16);
+    else w[i >> 1] = (w[i >> 1] & 0xffff0000u) | v;
+  }
+  __device__ inline void set(int i, float v) { set_raw(i, T::put(v)); }
+  __device__ inline void fill(raw v) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = sizeof(raw) == 4 ? (uint32_t)v : (uint32_t)v * 0x10001u;
   }
   __device__ inline void store(raw *row, int64_t c, int64_t width) const {
     if (c + 8 <= width) {
@@ -107,6 +110,25 @@ __device__ inline uint2 codes8(const Scale &q, F &&value) {
   };
   return make_uint2(four(0), four(4));
 }
+// A row by eights: `whole` of them in full, loaded without a condition (a branch
+// around each load would have it waited for before the next), a thread past
+// the last having that again; and what is left, one thread's.
+struct Eights {
+  int whole, left;
+  __device__ explicit Eights(int width) : whole(width / 8), left(width % 8) {}
+  template <class T>
+  __device__ inline void load(Oct<T> &o, const typename T::raw *row, int at) const {
+    o.load(row + (int64_t)min(at, whole - 1) * 8);
+  }
+  // The row's last codes: those of `o`, where something is left, and zeros up to
+  // the row's multiple of 16.
+  template <class T>
+  __device__ inline void finish(int8_t *codes, const Scale &q, const Oct<T> &o) const {
+    int at = whole;
+    if (left) *(uint2 *)(codes + 8 * at++) = codes8(q, [&](int i) { return o.get(i); });
+    if (at & 1) *(uint2 *)(codes + 8 * at) = make_uint2(0, 0);
+  }
+};
 // The largest magnitude's bits so far, in the type's own width.
 template <class T>
 __device__ inline void raise(uint32_t &top, const Oct<T> &o) {
@@ -212,6 +234,23 @@ __device__ inline float act_prime_f32(float x, int act) {
   }
   }
   return act_prime_piecewise(x, act);
+}
+
+__device__ inline void prime8(float (&v)[8], int act) {
+  const auto each = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_prime_f32(v[i], decltype(a)::value);
+  };
+  switch (act) {
+  case kReLU: return each(std::integral_constant<int, kReLU>{});
+  case kReLU2: return each(std::integral_constant<int, kReLU2>{});
+  case kLeakyReLU: return each(std::integral_constant<int, kLeakyReLU>{});
+  case kSilu: return each(std::integral_constant<int, kSilu>{});
+  case kSigmoid: return each(std::integral_constant<int, kSigmoid>{});
+  case kTanh: return each(std::integral_constant<int, kTanh>{});
+  case kGELU: return each(std::integral_constant<int, kGELU>{});
+  default: return each(std::integral_constant<int, kLinear>{});
+  }
 }
 
 // What the rows' operators take: widths whose columns an int holds with a

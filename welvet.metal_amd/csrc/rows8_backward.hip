@@ -28,10 +28,10 @@ using namespace r8;
 using namespace tiles;
 
 constexpr int kMaxSize = 1 << 20;
-constexpr int kTile = 64;                                 // of the passes: rows and columns a block
-constexpr int kBoundCols = 512;                           // of dy a block of the bounds
-// ... and rows: no more than 32 blocks of them.
-int bound_rows(int64_t n) { return (int)((n + 32 * kTile - 1) / (32 * kTile)) * kTile; }
+constexpr int kThreads = 512, kRows = 128, kCols = 64;    // of the passes' blocks: 128 x 64 values
+constexpr int kBoundCols = 512, kBoundRows = 32;          // of dy a block of the bounds
+// ... the rows in whole steps, so that no more than 32 blocks take them.
+int bound_rows(int64_t n) { return (int)((n + 32 * kBoundRows - 1) / (32 * kBoundRows)) * kBoundRows; }
 int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
 __host__ __device__ constexpr int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 
@@ -43,16 +43,16 @@ __device__ inline void split(float v, uint16_t (&part)[P]) {
   if constexpr (P == 2) part[1] = fabsf(v) < 65504.0f ? half_bits(v - F16::get(part[0])) : (uint16_t)0;
 }
 
-// A block's 64 x 64 values, two rows a word, so that columns can be read as rows.
+// A block's values, two rows a word, so that columns can be read as rows.
 struct Turn {
-  uint32_t word[kTile][kTile / 2 + 1];
+  uint32_t word[kCols][kRows / 2 + 1];
   __device__ inline void put(int col, int pair, uint32_t v) { word[col][pair] = v; }
-  // Sixteen bytes (eight rows) of each column into the image [cols][pitch]:
-  // rows from `row` on (an image's rows hold whole tiles), columns from `col` on.
+  // Sixteen bytes (eight rows) of a column a thread into the image [cols][pitch]:
+  // rows from `row` on (an image's rows hold whole blocks), columns from `col` on.
   __device__ inline void write(uint16_t *image, int64_t pitch, int row, int col, int cols) const {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int c = (threadIdx.x >> 3) + 32 * k, at = (threadIdx.x & 7) * 4;
+      const int c = (threadIdx.x >> 4) + kCols / 2 * k, at = (threadIdx.x & 15) * 4;
       if (col + c < cols)
         *(uint4 *)(image + (int64_t)(col + c) * pitch + row + 2 * at) =
             make_uint4(word[c][at], word[c][at + 1], word[c][at + 2], word[c][at + 3]);
@@ -68,7 +68,7 @@ struct Image {
   uint16_t *to;
   int blocks;
   __device__ inline void make(int block, Turn &turn) const {
-    const int row = block / across * kTile, col = block % across * kTile;
+    const int row = block / across * kRows, col = block % across * kCols;
     const int pair = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
     uint2 w[2];
 #pragma unroll
@@ -101,9 +101,10 @@ struct GradArgs {
   int n, out, act, across;
   int bound_rows, col_parts, row_parts;  // a block's rows, bounds a channel and a token
 };
-// What |act'| can be at a row's pre-activations.
+// What |act'| can be, of ReLU2 at a row's pre-activations.
+__device__ inline float steepest(const GradArgs &a) { return a.act == kSilu || a.act == kGELU ? 1.25f : 1.0f; }
 __device__ inline float steepest(const GradArgs &a, int row) {
-  return a.act == kReLU2 ? 256.0f * a.pre_scales[row] : a.act == kSilu || a.act == kGELU ? 1.25f : 1.0f;
+  return a.act == kReLU2 ? 256.0f * a.pre_scales[row] : steepest(a);
 }
 __device__ inline uint32_t finite_bits(float v) { return magnitude(v) < 0x7f800000u ? magnitude(v) : 0; }
 // 2^k that brings a bound to 2^14..2^15.
@@ -112,27 +113,38 @@ __device__ inline float lift_of(uint32_t bound) {
   return bound == 0 ? 1.0f : u2f((uint32_t)(min(max(14 - e, -126), 126) + 127) << 23);
 }
 
-// Bounds of a block's rows and columns; a wave takes a quarter of the rows, a
-// lane eight of the columns.
-template <class T>
+// Bounds of a block's rows and columns; a wave takes four rows of a step, a lane
+// eight of the columns.
+template <class T, bool EIGHTS>
 __device__ inline void bounds(const GradArgs &a, int block, uint32_t *lds) {
-  constexpr int kAhead = sizeof(typename T::raw) == 4 ? 4 : 8;
+  using raw = typename T::raw;
+  constexpr int kAhead = kBoundRows / (kThreads / 64);
   const int bm = block / a.row_parts, bn = block % a.row_parts;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = bn * kBoundCols + lane * 8;
-  const int begin = bm * a.bound_rows + wave * (a.bound_rows / 4), end = min(begin + a.bound_rows / 4, a.n);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = bn * kBoundCols + lane * 8, end = min((bm + 1) * a.bound_rows, a.n);
+  // loads without a condition: what there is no scale for reads another's and leaves it
+  const bool dw = a.x_scales, dx = a.w_scales, square = a.act == kReLU2;
+  const float *xs = dw ? a.x_scales : a.row_back, *ps = square ? a.pre_scales : a.row_back;
+  const float *ws = dx ? a.w_scales : a.col_back;
   uint32_t top[8] = {};
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = a.w_scales && c + i < a.out ? a.w_scales[c + i] : 0.0f;
-  for (int r0 = begin; r0 < end; r0 += kAhead) {
+  for (int i = 0; i < 8; ++i) {
+    const float w = ws[min(c + i, a.out - 1)];
+    v[i] = dx && c + i < a.out ? w : 0.0f;
+  }
+  for (int r0 = bm * a.bound_rows + wave * kAhead; r0 < end; r0 += kBoundRows) {
     Oct<T> o[kAhead];
     float s[kAhead], steep[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int r = min(r0 + j, end - 1);  // the last row again changes nothing
-      o[j].load((const typename T::raw *)a.dy + (int64_t)r * a.dy_stride, min(c, a.out), a.out);
-      steep[j] = steepest(a, r);
-      s[j] = a.x_scales ? a.x_scales[r] * steep[j] : 0.0f;
+      const raw *dy = (const raw *)a.dy + (int64_t)r * a.dy_stride;
+      // in whole eights a lane past the last column has the last ones again: they change nothing
+      if constexpr (EIGHTS) o[j].load(dy + min(c, a.out - 8));
+      else o[j].load(dy, min(c, a.out), a.out);
+      steep[j] = square ? 256.0f * ps[r] : steepest(a);
+      s[j] = dw ? xs[r] * steep[j] : 0.0f;
     }
     uint32_t most[kAhead] = {};
 #pragma unroll
@@ -143,7 +155,7 @@ __device__ inline void bounds(const GradArgs &a, int block, uint32_t *lds) {
         top[i] = max(top[i], finite_bits(d * s[j]));
         most[j] = max(most[j], finite_bits(d * (v[i] * steep[j])));
       }
-    if (a.w_scales) {
+    if (dx) {
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1)
 #pragma unroll
@@ -154,22 +166,28 @@ __device__ inline void bounds(const GradArgs &a, int block, uint32_t *lds) {
       if (lane < kAhead && r0 + lane < end) a.row_bound[(int64_t)bn * a.n + r0 + lane] = own;
     }
   }
-  if (!a.x_scales) return;
+  if (!dw) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) lds[wave * kBoundCols + lane * 8 + i] = top[i];
   __syncthreads();
-  for (int i = threadIdx.x; i < kBoundCols && bn * kBoundCols + i < a.out; i += 256)
-    a.col_bound[(int64_t)bm * a.out + bn * kBoundCols + i] =
-        max(max(lds[i], lds[kBoundCols + i]), max(lds[2 * kBoundCols + i], lds[3 * kBoundCols + i]));
+  const int i = threadIdx.x;
+  uint32_t most = lds[i];
+#pragma unroll
+  for (int k = 1; k < kThreads / 64; ++k) most = max(most, lds[k * kBoundCols + i]);
+  if (bn * kBoundCols + i < a.out) a.col_bound[(int64_t)bm * a.out + bn * kBoundCols + i] = most;
 }
+static_assert(kBoundCols == kThreads, "a thread a column at the end");
 
 template <class T>
-__global__ void __launch_bounds__(256) prepare_kernel(Image x, Image w, GradArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) prepare_kernel(Image x, Image w, GradArgs a) {
   __shared__ Turn turn;
-  static_assert(sizeof(Turn) >= 4 * kBoundCols * 4, "the bounds' place");
+  static_assert(sizeof(Turn) >= kThreads / 64 * kBoundCols * 4, "the bounds' place");
   int block = blockIdx.x;
   const int of_dy = a.col_parts * a.row_parts;
-  if (block < of_dy) return bounds<T>(a, block, &turn.word[0][0]);
+  if (block < of_dy) {
+    if (a.out % 8 == 0) return bounds<T, true>(a, block, &turn.word[0][0]);
+    return bounds<T, false>(a, block, &turn.word[0][0]);
+  }
   block -= of_dy;
   if (block < x.blocks) return x.make(block, turn);
   w.make(block - x.blocks, turn);
@@ -190,29 +208,73 @@ __global__ void __launch_bounds__(256) fold_kernel(GradArgs a) {
   if (a.along_o && i < a.n) fold(a.row_bound, a.row_parts, a.n, i);
 }
 
-// Powers of two of this block's 64 rows or columns into `lift`, from `parts` bounds each.
+// Powers of two of this block's COUNT rows or columns into `lift`, from `parts`
+// bounds each.
+template <int COUNT>
 __device__ inline void lifts(const uint32_t *bound, int parts, int first, int all, float *back, uint32_t *lds,
                              float *lift) {
-  const int i = threadIdx.x & 63, part = threadIdx.x >> 6;
+  constexpr int kSide = kThreads / COUNT;
+  const int i = threadIdx.x % COUNT, part = threadIdx.x / COUNT;
   uint32_t top = 0;
   if (first + i < all)
-    for (int p = part; p < parts; p += 4) top = max(top, bound[(int64_t)p * all + first + i]);
+    for (int p = part; p < parts; p += kSide) top = max(top, bound[(int64_t)p * all + first + i]);
   lds[threadIdx.x] = top;
   __syncthreads();
   if (part == 0) {
-    const float l = lift_of(max(max(lds[i], lds[64 + i]), max(lds[128 + i], lds[192 + i])));
+#pragma unroll
+    for (int k = 1; k < kSide; ++k) top = max(top, lds[k * COUNT + i]);
+    const float l = lift_of(top);
     lift[i] = l;
     if (back && first + i < all) back[first + i] = 1.0f / l;
   }
   __syncthreads();
 }
 
-template <class T, int PW, int PX>
-__global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
+// The same of one block of rows without dx, whose columns' bounds lie in the block
+// itself: the same products, so that dw has the same bits either way.
+template <class T>
+__device__ inline void own_lifts(const GradArgs &a, const Oct<T> (&o)[2], int pair, int c, int col, uint32_t *lds,
+                                 float *lift) {
+  uint32_t top[8] = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = 2 * pair + k;
+    const float s = r < a.n ? a.x_scales[r] * steepest(a, r) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[i] = max(top[i], finite_bits(o[k].get(i) * s));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int off = 8; off < 64; off <<= 1) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], off));
+  if ((threadIdx.x & 63) < 8)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[(threadIdx.x >> 6) * kCols + c - col + i] = top[i];
+  __syncthreads();
+  if (threadIdx.x < kCols) {
+    uint32_t most = lds[threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kThreads / 64; ++k) most = max(most, lds[k * kCols + threadIdx.x]);
+    const float l = lift_of(most);
+    lift[threadIdx.x] = l;
+    if (col + (int)threadIdx.x < a.out) a.col_back[col + threadIdx.x] = 1.0f / l;
+  }
+  __syncthreads();
+}
+
+// dpre and its parts.  ONE: a single block of rows without dx; the first blocks
+// make the image of the input's codes.
+template <class T, int PW, int PX, bool ONE>
+__global__ void __launch_bounds__(kThreads) grad_kernel(Image image, GradArgs a) {
   using raw = typename T::raw;
   __shared__ Turn turn[PW];
-  __shared__ float lift_n[kTile], lift_o[kTile];
-  const int row = (int)(blockIdx.x / a.across) * kTile, col = (int)(blockIdx.x % a.across) * kTile;
+  __shared__ float lift_n[kRows], lift_o[kCols];
+  int block = blockIdx.x;
+  if constexpr (ONE) {
+    if (block < image.blocks) return image.make(block, turn[0]);
+    block -= image.blocks;
+  }
+  const int row = block / a.across * kRows, col = block % a.across * kCols;
   const int pair = threadIdx.x >> 3, c = col + (threadIdx.x & 7) * 8;
   float v[2][8], s[2] = {0, 0};
   Oct<T> o[2];
@@ -220,15 +282,18 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = row + 2 * pair + k;
-    const bool in = r < a.n && c < a.out;
-    o[k].load((const raw *)a.dy + (in ? (int64_t)r * a.dy_stride : 0), in ? c : a.out, a.out);
-    if (in && a.pre) w[k] = *(const uint2 *)(a.pre + (int64_t)r * a.pre_stride + c);
+    if (a.out % 8 == 0)  // what lies past the last row or column is not used
+      o[k].load((const raw *)a.dy + (int64_t)min(r, a.n - 1) * a.dy_stride + min(c, a.out - 8));
+    else
+      o[k].load((const raw *)a.dy + (int64_t)min(r, a.n - 1) * a.dy_stride, min(c, a.out), a.out);
+    if (a.pre) w[k] = *(const uint2 *)(a.pre + (int64_t)min(r, a.n - 1) * a.pre_stride + min(c, (a.out - 1) / 8 * 8));
   }
   uint32_t *lds = &turn[0].word[0][0];
-  if (a.along_n)
-    lifts(a.col_bound, a.col_parts, col, a.out, row == 0 ? a.col_back : nullptr, lds, lift_o);
-  if (a.along_o)
-    lifts(a.row_bound, a.row_parts, row, a.n, col == 0 ? a.row_back : nullptr, lds, lift_n);
+  if constexpr (ONE) own_lifts(a, o, pair, c, col, lds, lift_o);
+  if (!ONE && a.along_n)
+    lifts<kCols>(a.col_bound, a.col_parts, col, a.out, row == 0 ? a.col_back : nullptr, lds, lift_o);
+  if (!ONE && a.along_o)
+    lifts<kRows>(a.row_bound, a.row_parts, row, a.n, col == 0 ? a.row_back : nullptr, lds, lift_n);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = row + 2 * pair + k;
@@ -238,9 +303,12 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
     if (a.x_scales) s[k] = a.x_scales[r];
     if (a.pre) {
       const float p = a.pre_scales[r];
+      float prime[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[k][i] = c + i < a.out ? v[k][i] * act_prime_f32(value_of(i < 4 ? w[k].x : w[k].y, i & 3) * p, a.act) : 0.0f;
+      for (int i = 0; i < 8; ++i) prime[i] = value_of(i < 4 ? w[k].x : w[k].y, i & 3) * p;
+      prime8(prime, a.act);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = c + i < a.out ? v[k][i] * prime[i] : 0.0f;
     }
     if (a.dpre) {
 #pragma unroll
@@ -248,7 +316,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
       o[k].store((raw *)a.dpre + (int64_t)r * a.dpre_stride, c, a.out);
     }
   }
-  if (a.along_o) {
+  if (!ONE && a.along_o) {
     float scale[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) scale[i] = c + i < a.out ? a.w_scales[c + i] : 0.0f;
@@ -295,48 +363,94 @@ __global__ void __launch_bounds__(256) zero_kernel(float *to, int64_t all) {
 }
 
 // ---------------------------------------------------------------- products
-template <class T, bool ADD, class Tile>
+// Eight results of a row from column c on.
+template <class T, bool ADD>
+__device__ inline void put8(typename T::raw *to, int c, int cols, const float (&v)[8], float back) {
+  Oct<T> o;
+  if constexpr (ADD) o.load(to, c, cols);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.set(i, ADD ? o.get(i) + v[i] * back : v[i] * back);
+  o.store(to, c, cols);
+}
+template <class T, bool ADD, class Tile, bool PART>
 __global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Operands g, const float *__restrict__ back,
-                                                                      typename T::raw *to, int64_t stride,
+                                                                      typename T::raw *to, int64_t stride, Splits p,
                                                                       int tiles_m, int tiles_n) {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  const Place at = place(tiles_m, tiles_n);
+  const int tile = PART ? (int)blockIdx.x / p.splits : blockIdx.x, split = PART ? (int)blockIdx.x % p.splits : 0;
+  const Place at = place(tile, tiles_m, tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
-  float *backs = (float *)(lds + Tile::kResults);
-  Tile::run(g, m0, n0, acc, lds);
+  Tile::run(PART ? g.part(split * p.each, min(p.each, g.stages - split * p.each)) : g, m0, n0, acc, lds);
   __syncthreads();
-  for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = back[min(m0 + i, g.a_rows - 1)];
-  __syncthreads();
-  Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
-    if (row >= g.a_rows || c >= g.b_rows) return;
-    const float b = backs[row - m0];
-    Oct<T> o;
-    if constexpr (ADD) o.load(to + row * stride, c, g.b_rows);
+  if constexpr (PART) {
+    Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
+      if (row < g.a_rows && c < g.b_rows)
+        put8<F32, false>((uint32_t *)p.parts + split * p.parts_values + (int64_t)row * g.b_rows, c, g.b_rows, v, 1.0f);
+    });
+  } else {
+    float *backs = (float *)(lds + Tile::kResults);
+    for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = back[min(m0 + i, g.a_rows - 1)];
+    __syncthreads();
+    Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
+      if (row < g.a_rows && c < g.b_rows) put8<T, ADD>(to + row * stride, c, g.b_rows, v, backs[row - m0]);
+    });
+  }
+}
+// The parts' results in their order.
+template <class T, bool ADD>
+__global__ void __launch_bounds__(256) half_join_kernel(Splits p, const float *__restrict__ back, typename T::raw *to,
+                                                        int64_t stride, int rows, int cols, int per_row) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
+  if (row >= rows) return;
+  const uint32_t *at = (const uint32_t *)p.parts + (int64_t)row * cols;
+  float sum[8] = {};
+  for (int k = 0; k < p.splits; k += 4) {
+    Oct<F32> v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.set(i, ADD ? o.get(i) + v[i] * b : v[i] * b);
-    o.store(to + row * stride, c, g.b_rows);
-  });
+    for (int n = 0; n < 4; ++n) v[n].load(at + min(k + n, p.splits - 1) * p.parts_values, c, cols);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] = k + n < p.splits ? sum[j] + v[n].get(j) : sum[j];
+  }
+  put8<T, ADD>(to + row * stride, c, cols, sum, back[row]);
 }
 
-// 256 x 256 and 128 x 128.
+// 256 x 256, a block a CU, where there is one for each; 128 x 128, two.  (dw and dx
+// of bf16 4096 x 4096, 2048 rows, 256 of the large tiles: 283 us against 304; of
+// 1024 x 1024, 4096 rows, 16 and 64: 111 with the small ones, 127 with the large.)
 template <int P>
 using Large = Tile<HalfOp, P, 2, 4, 4, 2>;
 template <int P>
 using Medium = Tile<HalfOp, P, 2, 2, 2, 2>;
 
 template <class T, bool ADD, class Tile>
-hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t stride, hipStream_t s) {
+hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
   const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
-  half_tile_kernel<T, ADD, Tile><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, back, (typename T::raw *)to, stride, tm, tn);
+  const Splits p(tm, tn, g, Tile::kRows, parts);
+  auto *out = (typename T::raw *)to;
+  if constexpr (Tile::kRows <= kSplitRows) {
+    if (p.splits > 1) {
+      half_tile_kernel<T, ADD, Tile, true><<<tm * tn * p.splits, Tile::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      const int per_row = tiles_of(g.b_rows, 8);
+      half_join_kernel<T, ADD><<<(unsigned)(((int64_t)g.a_rows * per_row + 255) / 256), 256, 0, s>>>(
+          p, back, out, stride, g.a_rows, g.b_rows, per_row);
+      return hipGetLastError();
+    }
+  }
+  half_tile_kernel<T, ADD, Tile, false><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
   return hipGetLastError();
 }
 // to[a_rows][b_rows] (+)= back . A . B^T with A of P parts.
 template <class T, bool ADD, int P>
-hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, hipStream_t s) {
-  if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 128)
-    return launch_tiles<T, ADD, Large<P>>(g, back, to, stride, s);
-  return launch_tiles<T, ADD, Medium<P>>(g, back, to, stride, s);
+hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
+  if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256)
+    return launch_tiles<T, ADD, Large<P>>(g, back, to, stride, parts, s);
+  return launch_tiles<T, ADD, Medium<P>>(g, back, to, stride, parts, s);
 }
 
 // Parts of dw's and dx's terms.  One part, rounded as a BFloat16 gradient was
@@ -345,10 +459,10 @@ constexpr int kPartsW = 2;
 template <class T>
 constexpr int kPartsX = std::is_same_v<T, BF16> ? 1 : 2;
 
-constexpr int kFewBounds = 4;
+constexpr int kFewBounds = 16;
 
 struct Plan {
-  size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back;  // offsets
+  size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back, parts;  // offsets
   size_t bytes;
 };
 Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
@@ -363,10 +477,11 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
   p.codes_x = take(2 * in * along(n));
   p.grad_x = take(2 * (dtype == kBFloat16 ? kPartsX<BF16> : kPartsX<F32>) * n * along(out));
   p.codes_w = take(2 * in * along(out));
-  p.col_bound = take(4 * std::min<int64_t>(32, tiles_of(n, kTile)) * out);  // not fewer than any smaller n needs
+  p.col_bound = take(4 * std::min<int64_t>(32, tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
   p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
   p.col_back = take(4 * out);
   p.row_back = take(4 * n);
+  p.parts = take(std::max(parts_bytes(out, in), parts_bytes(n, in)));  // dw's, then dx's
   p.bytes = at;
   return p;
 }
@@ -374,11 +489,11 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
 bool sizes_ok(int32_t n, int32_t in, int32_t out) {
   return n >= 0 && n <= kMaxSize && in > 0 && in <= kMaxSize && out > 0 && out <= kMaxSize;
 }
-// A launch of fewer than 2^32 threads: 256 a 64 x 64 tile of the passes.
+// A launch of fewer than 2^32 threads: 512 a 128 x 64 block of the passes.
 bool launchable(int64_t n, int64_t in, int64_t out) {
-  constexpr int64_t most = (int64_t)1 << 23;
-  const int64_t tn = tiles_of(n, kTile), ti = tiles_of(in, kTile), to = tiles_of(out, kTile);
-  return tn * to < most && ti * (tn + to) < most;
+  constexpr int64_t most = (int64_t)1 << 22;
+  const int64_t tn = tiles_of(n, kRows), to = tiles_of(out, kRows);
+  return tn * tiles_of(out, kCols) < most && tiles_of(in, kCols) * (tn + to) < most;
 }
 
 }  // namespace
@@ -451,7 +566,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   a.n = n;
   a.out = out;
   a.act = act;
-  a.across = tiles_of(out, kTile);
+  a.across = tiles_of(out, kCols);
   a.bound_rows = bound_rows(n);
   a.col_parts = tiles_of(n, a.bound_rows);
   a.row_parts = tiles_of(out, kBoundCols);
@@ -461,23 +576,25 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   a.row_bound = (uint32_t *)(ws + p.row_bound);
   a.col_back = (float *)(ws + p.col_back);
   a.row_back = (float *)(ws + p.row_back);
-  const int in_tiles = tiles_of(in, kTile);
+  void *parts = ws + p.parts;
+  const int in_tiles = tiles_of(in, kCols);
   if (d_dw) {
     a.x_scales = x8->d_scales;
     a.along_n = (uint16_t *)(ws + p.grad_w);
-    x = {x8->d_codes, x8->stride, a.n_pitch, n, in, in_tiles, (uint16_t *)(ws + p.codes_x), tiles_of(n, kTile) * in_tiles};
+    x = {x8->d_codes, x8->stride, a.n_pitch, n, in, in_tiles, (uint16_t *)(ws + p.codes_x), tiles_of(n, kRows) * in_tiles};
   }
   if (d_dx) {
     a.w_scales = layer->scales;
     a.along_o = (uint16_t *)(ws + p.grad_x);
-    w = {layer->codes, layer->pitch, a.o_pitch, out, in, in_tiles, (uint16_t *)(ws + p.codes_w), a.across * in_tiles};
+    w = {layer->codes, layer->pitch, a.o_pitch, out, in, in_tiles, (uint16_t *)(ws + p.codes_w), tiles_of(out, kRows) * in_tiles};
   }
   WH_HIP(tok::with_type(dtype, [&](auto t) -> hipError_t {
     using T = decltype(t);
     constexpr int PX = kPartsX<T>;
     hipError_t e = hipSuccess;
-    if (products) {
-      prepare_kernel<T><<<x.blocks + w.blocks + a.col_parts * a.row_parts, 256, 0, s>>>(x, w, a);
+    const bool one = d_dw && !d_dx && n <= kRows;
+    if (products && !one) {
+      prepare_kernel<T><<<x.blocks + w.blocks + a.col_parts * a.row_parts, kThreads, 0, s>>>(x, w, a);
       if ((e = hipGetLastError()) != hipSuccess) return e;
       // every 64 x 64 tile of the next pass reads the bounds of its rows and columns
       if ((d_dw && a.col_parts > kFewBounds) || (d_dx && a.row_parts > kFewBounds)) {
@@ -486,19 +603,21 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
         a.col_parts = a.row_parts = 1;
       }
     }
-    grad_kernel<T, kPartsW, PX><<<(unsigned)tiles_of(n, kTile) * a.across, 256, 0, s>>>(a);
+    // up to 128 rows without dx one launch does both (f16 1001 -> 777, 100 rows: 27 -> ONEUS us in all)
+    if (one) grad_kernel<T, kPartsW, PX, true><<<x.blocks + a.across, kThreads, 0, s>>>(x, a);
+    else grad_kernel<T, kPartsW, PX, false><<<(unsigned)tiles_of(n, kRows) * a.across, kThreads, 0, s>>>(x, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (d_dw) {
       const Operands g{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
                        (const char *)x.to, 2 * a.n_pitch, in, tiles_of(2 * (int64_t)n, kStageBytes)};
-      e = accumulate ? launch_half<F32, true, kPartsW>(g, a.col_back, d_dw, in, s)
-                     : launch_half<F32, false, kPartsW>(g, a.col_back, d_dw, in, s);
+      e = accumulate ? launch_half<F32, true, kPartsW>(g, a.col_back, d_dw, in, parts, s)
+                     : launch_half<F32, false, kPartsW>(g, a.col_back, d_dw, in, parts, s);
       if (e != hipSuccess) return e;
     }
     if (d_dx) {
       const Operands g{(const char *)a.along_o, 2 * a.o_pitch, 2 * n * a.o_pitch, n, INT32_MAX,
                        (const char *)w.to, 2 * a.o_pitch, in, tiles_of(2 * (int64_t)out, kStageBytes)};
-      e = launch_half<T, false, PX>(g, a.row_back, d_dx, dx_stride, s);
+      e = launch_half<T, false, PX>(g, a.row_back, d_dx, dx_stride, parts, s);
     }
     return e;
   }));

@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -57,6 +58,15 @@ constexpr int kStageBytes = 128;
 constexpr int64_t spread(int64_t bytes) { return ((bytes + 255) / 256 | 1) * 256; }
 
 struct Operands {
+  // the stages from `first` on, `count` of them
+  __host__ __device__ Operands part(int first, int count) const {
+    Operands o = *this;
+    o.a += (int64_t)first * kStageBytes;
+    o.b += (int64_t)first * kStageBytes;
+    if (o.a_last != INT32_MAX) o.a_last -= first * kStageBytes;
+    o.stages = count;
+    return o;
+  }
   const char *a;
   int64_t a_pitch, a_plane;  // bytes between rows, between parts
   int a_rows;
@@ -79,7 +89,6 @@ struct Tile {
   static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kWaves % 2 == 0,
                 "every wave copies whole pieces of 8 rows, its chunks' places the same in all");
   static_assert(P == 1 || P == 2, "parts");
-  static_assert(TM * TN >= TM + TN || TM * TN == 4, "products to hide the reads under");
   using Acc = typename Op::acc;
   // at most `left` of this wave's copies still under way, and none of its LDS reads
   template <int LEFT>
@@ -215,14 +224,38 @@ struct Tile {
   }
 };
 
+// Few tiles: the sum's stages in parts, a block each, whose results are joined
+// in a launch of their own.  As many as give every CU a block, of four stages and
+// more, at most 16.
+constexpr int kSplitRows = 128;  // of the largest tile that is split
+struct Splits {
+  int splits, each;      // parts, and the stages of one
+  int64_t parts_values;  // of one's [rows][cols] results
+  void *parts;
+  Splits(int tiles_m, int tiles_n, const Operands &o, int tile_rows, void *ws)
+      : splits(1), each(o.stages), parts_values((int64_t)o.a_rows * o.b_rows), parts(ws) {
+    const int64_t tiles = (int64_t)tiles_m * tiles_n;
+    if (tile_rows > kSplitRows) return;
+    const int most = (int)std::min<int64_t>(16, std::min<int64_t>(256 / tiles, o.stages / 4));
+    if (most < 2) return;
+    each = (o.stages + most - 1) / most;
+    splits = (o.stages + each - 1) / each;
+  }
+};
+// Their workspace for results of rows x cols: at most 256 tiles of 128 x 128; not
+// less for more rows.
+inline size_t parts_bytes(int64_t rows, int64_t cols) {
+  return (size_t)std::min<int64_t>((int64_t)256 * kSplitRows * kSplitRows, 16 * rows * cols) * 4;
+}
+
 // The tile of a block: blocks of one XCD (every eighth) take neighbouring
 // tiles, so that its L2 holds their rows: columns by columns of eight rows.
 struct Place {
   int m, n;
 };
-__device__ inline Place place(int tiles_m, int tiles_n) {
-  const int all = tiles_m * tiles_n, per = all / 8, more = all % 8, xcd = blockIdx.x % 8;
-  const int at = xcd * per + min(xcd, more) + (int)(blockIdx.x / 8);
+__device__ inline Place place(int block, int tiles_m, int tiles_n) {
+  const int all = tiles_m * tiles_n, per = all / 8, more = all % 8, xcd = block % 8;
+  const int at = xcd * per + min(xcd, more) + block / 8;
   const int band = at / (8 * tiles_n), rows = min(8, tiles_m - band * 8), in = at - band * 8 * tiles_n;
   return {band * 8 + in % rows, in / rows};
 }
