@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
   float bias[kList];
   if (a.r.history > 0)
 #pragma unroll
-    for (int k = 0; k < kFirst; ++k) first[k] = said[min(k * kThreads + tid, a.r.history - 1)];
+    for (int k = 0; k < kFirst; ++k)
+      if (k * kThreads < a.r.history) first[k] = said[min(k * kThreads + tid, a.r.history - 1)];
   if (a.r.biases > 0)
 #pragma unroll
     for (int k = 0; k < kList; ++k)
@@ -138,7 +139,8 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
     };
     if (history > 0)
 #pragma unroll
-      for (int k = 0; k < kFirst; ++k) count_one(k * kThreads + tid, first[k]);
+      for (int k = 0; k < kFirst; ++k)
+        if (k * kThreads < a.r.history) count_one(k * kThreads + tid, first[k]);
     for (int i = kFirst * kThreads + tid; i < history; i += kFirst * kThreads) {
       int32_t more[kFirst];
 #pragma unroll
@@ -177,11 +179,15 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
           if (sparse) {
             const uint4 w0 = words[c / 4], w1 = words[c / 4 + 1];
             const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-            if (w0.x | w0.y | w0.z | w0.w | w1.x | w1.y | w1.z | w1.w) {
+            uint32_t said_here = 0;
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (c + i < len && (w[i] & (kCount | kPrompt)))
-                  o.set_raw(i, rounded<T>(rules.apply((double)o.get(i), w[i])));
+            for (int i = 0; i < 8; ++i) said_here |= (w[i] & (kCount | kPrompt)) ? 1u << i : 0u;
+            said_here &= c + 8 <= len ? open[k] : open[k] & ((1u << (len - c)) - 1);
+            // a token a turn: most lanes have none or one, and a turn is what eight
+            // conditions in a row would cost each
+            for (; said_here; said_here &= said_here - 1) {
+              const int i = __ffs(said_here) - 1;
+              o.set_at(i, rounded<T>(rules.apply((double)T::get(o.at(i)), count[c + i])));
             }
           }
           if (open[k] != 0xffu) {

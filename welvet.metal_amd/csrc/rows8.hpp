@@ -70,6 +70,21 @@ struct Oct {
     else if (i & 1) w[i >> 1] = (w[i >> 1] & 0xffffu) | ((uint32_t)v << 16);
     else w[i >> 1] = (w[i >> 1] & 0xffff0000u) | v;
   }
+  // the same where i is not known to the compiler
+  __device__ inline raw at(int i) const {
+    constexpr int kPer = 4 / sizeof(raw);
+    uint32_t v = 0;  // by masks: of selects the compiler makes an array in memory
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) v |= w[k] & (0u - (uint32_t)(i / kPer == k));
+    return (raw)(v >> (8 * sizeof(raw) * (i % kPer)));
+  }
+  __device__ inline void set_at(int i, raw v) {
+    constexpr int kPer = 4 / sizeof(raw);
+    const int by = 8 * sizeof(raw) * (i % kPer);
+    const uint32_t mask = (sizeof(raw) == 4 ? 0xffffffffu : 0xffffu) << by;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] ^= (w[k] ^ (uint32_t)v << by) & mask & (0u - (uint32_t)(i / kPer == k));
+  }
   __device__ inline void set(int i, float v) { set_raw(i, T::put(v)); }
   __device__ inline void fill(raw v) {
 #pragma unroll
