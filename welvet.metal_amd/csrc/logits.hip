@@ -6,10 +6,9 @@
 //   z = -inf                 where the row's mask shuts v
 // A block takes a stretch of a row's vocabulary.  It counts the history's
 // tokens of that stretch in LDS (whole numbers: the order does not matter), a
-// word a token: how often it was said, whether the prompt names it, how many
-// biases do.  Then it passes over the stretch once: bound by HBM, as nothing of
-// what a mask shuts is read.  Tokens with a bias go last, a thread each.  In
-// place, only what changes is touched.
+// word a token: how often it was said, whether the prompt names it, which entry
+// of the list does.  Then it passes over the stretch once: bound by HBM, as
+// nothing of what a mask shuts is read.  In place, only what changes is touched.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -22,10 +21,13 @@ namespace {
 using namespace r8;
 
 constexpr int kThreads = 512;
-constexpr int kStretch = 8192;        // tokens a block: with the biases 40 KB of LDS, four blocks a CU
-constexpr int kOcts = kStretch / 8 / kThreads;
+constexpr int kStretch = 8128;        // tokens a block: with the list 40 KB of LDS, four blocks a CU
+constexpr int kOcts = 2;
+static_assert(kOcts * kThreads * 8 >= kStretch && kStretch % 32 == 0, "whole words of a mask, in one go");
 constexpr int kMaxHistory = (1 << 20) - 1, kMaxBiases = 1024;
-constexpr uint32_t kCount = kMaxHistory, kBias = 1u << 20, kBiases = 0x7ffu << 20, kPrompt = 1u << 31;
+constexpr uint32_t kCount = kMaxHistory, kPrompt = 1u << 31;
+constexpr int kEntry = 20;  // bits from here to 30: 1 + the number of a list's entry that names the token
+constexpr uint32_t kEntries = 0x7ffu << kEntry;
 
 struct Args {
   welvet_hip_logit_rules r;
@@ -68,6 +70,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
   __shared__ uint4 words[kStretch / 4];
   __shared__ int index[kMaxBiases];
   __shared__ float biases[kMaxBiases];
+  __shared__ int twice;  // a token of this stretch is named by two entries
   uint32_t *count = (uint32_t *)words;
   const int row = blockIdx.x / a.parts, begin = (int)(blockIdx.x % a.parts) * a.len;
   const int len = min(a.len, a.vocab - begin), tid = threadIdx.x;
@@ -116,6 +119,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
   const bool sparse = history > 0 || a.r.biases > 0;
   raw z[kList];  // the logits that the list names
   if (sparse) {
+    if (tid == 0) twice = 0;
     for (int i = tid; i < (len + 3) / 4; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
     if (a.r.biases > 0)
 #pragma unroll
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
         if (k * kThreads >= a.r.biases) break;
         const int64_t v = (int64_t)at[k] - begin;
         at[k] = i < a.r.biases && v >= 0 && v < len ? (int)v : -1;
-        if (at[k] >= 0) z[k] = in[at[k]];
+        if (INPLACE && at[k] >= 0) z[k] = in[at[k]];
         if (i < a.r.biases) {
           index[i] = at[k];
           biases[i] = bias[k];
@@ -152,10 +156,21 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
 #pragma unroll
       for (int k = 0; k < kList; ++k) {
         if (k * kThreads >= a.r.biases) break;
-        if (at[k] >= 0) atomicAdd(&count[at[k]], kBias);
+        if (at[k] >= 0 && (atomicOr(&count[at[k]], (uint32_t)(k * kThreads + tid + 1) << kEntry) & kEntries)) twice = 1;
       }
     __syncthreads();
   }
+  // token v of word w
+  const auto changed = [&](raw was, int v, uint32_t w) {
+    double sum = rules.apply((double)T::get(was), w);
+    if (w & kEntries) {
+      if (!twice) sum += (double)biases[(w >> kEntry & 0x7ffu) - 1];
+      else
+        for (int j = 0; j < a.r.biases; ++j)
+          if (index[j] == v) sum += (double)biases[j];
+    }
+    return rounded<T>(sum);
+  };
   if (!INPLACE || mask) {
 #pragma unroll
     for (int k = 0; k < kOcts; ++k) {
@@ -181,13 +196,13 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
             const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
             uint32_t said_here = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) said_here |= (w[i] & (kCount | kPrompt)) ? 1u << i : 0u;
+            for (int i = 0; i < 8; ++i) said_here |= w[i] ? 1u << i : 0u;
             said_here &= c + 8 <= len ? open[k] : open[k] & ((1u << (len - c)) - 1);
             // a token a turn: most lanes have none or one, and a turn is what eight
             // conditions in a row would cost each
             for (; said_here; said_here &= said_here - 1) {
               const int i = __ffs(said_here) - 1;
-              o.set_at(i, rounded<T>(rules.apply((double)T::get(o.at(i)), count[c + i])));
+              o.set_at(i, changed(o.at(i), c + i, count[c + i]));
             }
           }
           if (open[k] != 0xffu) {
@@ -200,30 +215,22 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
       }
     }
   }
-  if (!sparse) return;
-  __syncthreads();  // what a token with a bias holds by now is written again
+  if (!INPLACE || !sparse) return;
 #pragma unroll
   for (int k = 0; k < kList; ++k) {
     if (k * kThreads >= a.r.biases) break;
     const int i = k * kThreads + tid, v = at[k];
     if (v < 0 || !(open8(v & ~7) >> (v & 7) & 1)) continue;
-    const uint32_t w = count[v];
-    const bool alone = (w & kBiases) == kBias;
     bool earlier = false;  // the first of a token's entries stands for all
-    if (!alone)
+    if (twice)
       for (int j = 0; j < i; ++j) earlier = earlier || index[j] == v;
-    if (earlier) continue;
-    double sum = rules.apply((double)T::get(z[k]), w) + (double)bias[k];
-    if (!alone)
-      for (int j = i + 1; j < a.r.biases; ++j)
-        if (index[j] == v) sum += (double)biases[j];
-    out[v] = rounded<T>(sum);
+    if (!earlier) out[v] = changed(z[k], v, count[v]);
   }
   if constexpr (INPLACE) {
     for (int i = tid; i < history; i += kThreads) {
       const int64_t v = (int64_t)said[i] - begin;
       if (v < 0 || v >= len || !(open8((int)v & ~7) >> (v & 7) & 1)) continue;
-      if (count[v] & kBiases) continue;  // the words with a bias do not change here
+      if (count[v] & kEntries) continue;  // the words with a bias do not change here
       const uint32_t w = atomicExch(&count[v], 0u);
       if (w) out[v] = rounded<T>(rules.apply((double)T::get(in[v]), w));
     }
