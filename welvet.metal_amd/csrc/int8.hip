@@ -264,8 +264,10 @@ __global__ void __launch_bounds__(256) int8_join_kernel(Splits p, Out o, int per
 
 using Large = Tile<Int8Op, 1, 2, 4, 4, 2>;   // 256 x 256, eight waves
 using Medium = Tile<Int8Op, 1, 2, 2, 2, 2>;  // 128 x 128, four
+using Deep = Tile<Int8Op, 1, 2, 4, 2, 1, 4, 4>;  // 128 x 128, eight
 
-template <class T, class Tile>
+// Split: the tile of the parts.
+template <class T, class Tile, class Split>
 hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_stride, const Out &o, void *parts,
                         hipStream_t s) {
   const int tm = (o.n + Tile::kRows - 1) / Tile::kRows, tn = (o.out + Tile::kCols - 1) / Tile::kCols;
@@ -274,7 +276,7 @@ hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_str
   const Splits p(tm, tn, g, Tile::kRows, parts);
   if constexpr (Tile::kRows <= kSplitRows) {
     if (p.splits > 1) {
-      int8_tile_kernel<T, Tile, true><<<tm * tn * p.splits, Tile::kWaves * 64, 0, s>>>(g, o, p, tm, tn);
+      int8_tile_kernel<T, Split, true><<<tm * tn * p.splits, Split::kWaves * 64, 0, s>>>(g, o, p, tm, tn);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       const int per_row = (o.out + 7) / 8;
@@ -311,8 +313,8 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
     // large tiles, a block a CU, where there is one for each (us, large and small
     // tiles, bf16: 4096 -> 11008 of 2048 rows 146 / 142, of 4096 225 / 246; 11008 ->
     // 4096 of 2048 rows, 128 large tiles, 175 / 125)
-    if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large>(l, x, x_stride, o, parts, s);
-    return launch_tiles<T, Medium>(l, x, x_stride, o, parts, s);
+    if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large, Large>(l, x, x_stride, o, parts, s);
+    return launch_tiles<T, Medium, Deep>(l, x, x_stride, o, parts, s);
   });
 }
 // One launch from x, for rows that the caller does not keep.

@@ -425,15 +425,18 @@ template <int P>
 using Large = Tile<HalfOp, P, 2, 4, 4, 2>;
 template <int P>
 using Medium = Tile<HalfOp, P, 2, 2, 2, 2>;
+template <int P>
+using Deep = Tile<HalfOp, P, 2, 4, 2, 1, 4, 4>;
 
-template <class T, bool ADD, class Tile>
+// Split: the tile of the parts.
+template <class T, bool ADD, class Tile, class Split>
 hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
   const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
   const Splits p(tm, tn, g, Tile::kRows, parts);
   auto *out = (typename T::raw *)to;
   if constexpr (Tile::kRows <= kSplitRows) {
     if (p.splits > 1) {
-      half_tile_kernel<T, ADD, Tile, true><<<tm * tn * p.splits, Tile::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
+      half_tile_kernel<T, ADD, Split, true><<<tm * tn * p.splits, Split::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       const int per_row = tiles_of(g.b_rows, 8);
@@ -449,8 +452,8 @@ hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t 
 template <class T, bool ADD, int P>
 hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
   if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256)
-    return launch_tiles<T, ADD, Large<P>>(g, back, to, stride, parts, s);
-  return launch_tiles<T, ADD, Medium<P>>(g, back, to, stride, parts, s);
+    return launch_tiles<T, ADD, Large<P>, Large<P>>(g, back, to, stride, parts, s);
+  return launch_tiles<T, ADD, Medium<P>, Deep<P>>(g, back, to, stride, parts, s);
 }
 
 // Parts of dw's and dx's terms.  One part, rounded as a BFloat16 gradient was

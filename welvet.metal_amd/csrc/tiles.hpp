@@ -77,11 +77,13 @@ struct Operands {
   int stages;
 };
 
-// WM x WN waves, each TM x TN products of 32 x 32.
-template <class Op, int P, int WM, int WN, int TM, int TN>
+// WM x WN waves, each TM x TN products of 32 x 32.  SA and SB: the operands'
+// places in LDS.  Three and two leave 128 x 128 tiles two blocks a CU; four of
+// each keep three stages under way where there is one block a CU, or none.
+template <class Op, int P, int WM, int WN, int TM, int TN, int SA = 3, int SB = 2>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRows = WM * TM * 32, kCols = WN * TN * 32;
-  static constexpr int kA = kRows * kStageBytes, kB = kCols * kStageBytes, kLds = 3 * kA + 2 * kB;
+  static constexpr int kA = kRows * kStageBytes, kB = kCols * kStageBytes, kLds = SA * kA + SB * kB;
   static constexpr int kLoadsA = kRows / 8 / kWaves, kLoadsB = kCols / 8 / kWaves;
   static constexpr int kTM = TM, kTN = TN;
   // of LDS after the products: the results' turning place, then the caller's
@@ -89,6 +91,7 @@ struct Tile {
   static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kWaves % 2 == 0,
                 "every wave copies whole pieces of 8 rows, its chunks' places the same in all");
   static_assert(P == 1 || P == 2, "parts");
+  static_assert((SA == 3 && SB == 2) || (SA == SB && SA >= 3), "the copies that may be left under way at a step");
   using Acc = typename Op::acc;
   // at most `left` of this wave's copies still under way, and none of its LDS reads
   template <int LEFT>
@@ -138,7 +141,7 @@ struct Tile {
     // this lane's chunk of its first rows; slab s lies at ^ 32 s
     const int swz = (((lane >> 5) ^ ((lane >> 1) & 7)) * 16) + (lane & 31) * kStageBytes;
     const int a_at = wm * TM * 32 * kStageBytes + swz, b_at = wn * TN * 32 * kStageBytes + swz;
-    char *const lds_b = lds + 3 * kA;
+    char *const lds_b = lds + SA * kA;
     i32x4 a[2][TM], b[2][TN];
     const auto fetch = [&](const char *at, const char *bt, int slab, int into) {
 #pragma unroll
@@ -147,18 +150,28 @@ struct Tile {
       for (int t = 0; t < TM; ++t) a[into][t] = *(const i32x4 *)(at + ((a_at ^ (slab * 32)) + t * 32 * kStageBytes));
     };
     constexpr int kReads = TN + TM, kMul = TM * TN;
-    load_b(lds_b);
-    load_a(0, 0, lds);
-    if (steps > 1) load_a(1, 1 % P, lds + kA);
-    int ia = 0, ib = 0;  // slots of this step
+    // A's steps and B's stages go out in the order in which they are needed; at step
+    // h A has SA - 1 steps, B SB - 1 stages out ahead.
+#pragma unroll
+    for (int h = 0; h < SA - 1; ++h) {
+      if (h % P == 0 && h / P < SB - 1 && h / P < o.stages) load_b(lds_b + h / P * kB);
+      if (h < steps) load_a(h, h % P, lds + h * kA);
+    }
+#pragma unroll
+    for (int s = (SA - 2) / P + 1; s < SB - 1; ++s)
+      if (s < o.stages) load_b(lds_b + s * kB);
+    int ia = 0, ib = 0;  // places of this step
     const auto step = [&](int h, auto part_) {
       constexpr int part = decltype(part_)::value;
-      if (h + P + 1 >= steps) wait<0>();
-      else wait<P == 2 && part == 1 ? kLoadsA + kLoadsB : kLoadsA>();
+      // what was sent after this step's A and B: A's of the steps between, and B's
+      // that were sent with them
+      constexpr int kSteps = SA - 2, kStages = SB == 2 ? (P == 2 && part == 1) : P == 1 ? kSteps : (kSteps + part) / 2;
+      if (h + SA + P >= steps) wait<0>();
+      else wait<kSteps * kLoadsA + kStages * kLoadsB>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (part == 0 && h + P < steps) load_b(lds_b + (ib ^ 1) * kB);
-      if (h + 2 < steps) load_a(h + 2, (part + 2) % P, lds + (ia == 0 ? 2 : ia - 1) * kA);
+      if (part == 0 && h + (SB - 1) * P < steps) load_b(lds_b + (ib == 0 ? SB - 1 : ib - 1) * kB);
+      if (h + SA - 1 < steps) load_a(h + SA - 1, (part + SA - 1) % P, lds + (ia == 0 ? SA - 1 : ia - 1) * kA);
       const char *at = lds + ia * kA, *bt = lds_b + ib * kB;
       fetch(at, bt, 0, 0);
 #pragma unroll
@@ -179,8 +192,8 @@ struct Tile {
         }
         __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
       }
-      ia = ia == 2 ? 0 : ia + 1;
-      if (part == P - 1) ib ^= 1;
+      ia = ia == SA - 1 ? 0 : ia + 1;
+      if (part == P - 1) ib = ib == SB - 1 ? 0 : ib + 1;
     };
     for (int h = 0; h < steps; h += P) {
       step(h, std::integral_constant<int, 0>{});
