@@ -536,11 +536,14 @@ WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, i
  * stride).  A Dense layer of any dtype can keep its activations so: it takes
  * dpre and dw here, and dx from its own weights.
  * dpre enters the products before it is rounded to `dtype`, times its row's
- * scale (dw) or its channel's (dx), as bf16 parts: three for Float32 (24
- * bits), two for 16-bit types (16 bits or more), one for dx in BFloat16
- * (rounded as its dy was); sums are f32, in a fixed order.  Such products below
- * 2^-102 are held to an absolute 2^-126, and from 3.38e38 on count as
- * infinite.  in and out <= 2^20, n <= 2^20. */
+ * scale (dw) or its channel's (dx): two f16 parts a term, 22 bits, but no
+ * finer than 2^-39 of the largest |dy| scale of its channel (dw) or token (dx)
+ * times what |act'| can be (1.25; 256 scales of the row for act 6); one part,
+ * 11 bits, for a BFloat16 dx.  Sums are f32, in a fixed order: the same bits on
+ * every run, and whichever outputs are asked for.  Terms of 2^127 and more
+ * count as infinite, bits of a term below 2^-126 are lost.  in, out and n <=
+ * 2^20, and (n / 128) (out / 64) and (in / 64) (n / 128 + out / 128), rounded
+ * up, < 2^22: what one launch takes. */
 WELVET_API welvet_status welvet_hip_rows8_backward_bytes(int32_t dtype, int32_t n, int32_t in,
                                                          int32_t out, size_t *bytes);
 WELVET_API welvet_status welvet_hip_rows8_backward(
