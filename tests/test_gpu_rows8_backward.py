@@ -121,6 +121,52 @@ def test_backward(stream, dtype, n, inn, out):
     assert_bit_equal(placed, dpre, "dpre in dy's place")
 
 
+# up to eight rows go another way: columns past a block's 512 and 1024, channels past its 512, odd sizes
+FEW = [(1, 1025, 1600), (2, 513, 100), (3, 2051, 1031), (4, 1024, 520), (5, 7, 3000), (7, 515, 31), (8, 1000, 2049),
+       (9, 1000, 2049), (16, 515, 700), (17, 515, 700)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,inn,out", FEW)
+def test_few_rows(stream, dtype, n, inn, out):
+    case = Case(dtype, n, inn, out, ACTS[(n + inn) % len(ACTS)], 8, extra=out % 3, shift=inn % 4)
+    first = case.check(stream)
+    for k in range(3):
+        assert_bit_equal(case.run(stream, dpre=k == 0, dx=k == 1, dw=k == 2)[k], first[k], "alone")
+    base = np.random.default_rng(2).normal(0, 1, (out, inn)).astype(np.float32)
+    case.check(stream, base=base)
+    placed = case.run(stream, in_place=True)
+    assert_bit_equal(case.d.get()[inn % 4:].reshape(n, out + case.extra)[:, :out], first[0], "dpre in dy's place")
+    assert_bit_equal(placed[1], first[1], "dx, dpre in dy's place")
+    assert_bit_equal(placed[2], first[2], "dw, dpre in dy's place")
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n", [2, 70, 200])
+def test_dpre_in_the_place_of_dy_with_both_products(stream, dtype, n):
+    case = Case(dtype, n, 130, 140, "silu", 9)
+    first = case.run(stream)
+    placed = case.run(stream, in_place=True)
+    assert_bit_equal(case.d.get().reshape(n, 140), first[0], "dpre")
+    for k in (1, 2):
+        assert_bit_equal(placed[k], first[k], "products")
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_few_rows_that_are_not_finite(stream, dtype):
+    case = Case(dtype, 5, 50, 60, "linear", 5)
+    dy = case.dy.copy()
+    dy[2, 9] = np.inf
+    case.d, case.dy_ptr, case.dy = matrix(dy, dtype)
+    dpre, dx, dw = case.run(stream)
+    dx, dw = to_f64(dx, dtype), dw.astype(np.float64)
+    assert not np.isfinite(dx[2]).any() and np.isfinite(np.delete(dx, 2, 0)).all()
+    assert not np.isfinite(dw[9]).any() and np.isfinite(np.delete(dw, 9, 0)).all()
+    case.xs[3] = np.nan
+    case.x8 = Rows(5, 50, 1, case.xc, case.xs)
+    assert np.isnan(case.run(stream)[2]).all()
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("name", ACTS)
 def test_every_activation(stream, dtype, name):

@@ -28,12 +28,13 @@ using namespace r8;
 using namespace tiles;
 
 constexpr int kMaxSize = 1 << 20;
+__host__ __device__ constexpr int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 constexpr int kThreads = 512, kRows = 128, kCols = 64;    // of the passes' blocks: 128 x 64 values
 constexpr int kBoundCols = 512, kBoundRows = 32;          // of dy a block of the bounds
-// ... the rows in whole steps, so that no more than 32 blocks take them.
-int bound_rows(int64_t n) { return (int)((n + 32 * kBoundRows - 1) / (32 * kBoundRows)) * kBoundRows; }
+// ... the rows in whole steps, so that no more than 16 blocks take them.
+constexpr int kMostBounds = 16;
+int bound_rows(int64_t n) { return tiles_of(n, kMostBounds * kBoundRows) * kBoundRows; }
 int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
-__host__ __device__ constexpr int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 
 __device__ inline uint16_t half_bits(float v) { return F16::put(v); }
 // v as P f16 parts, each the rest's nearest; what is not finite is its first part alone.
@@ -198,7 +199,9 @@ __global__ void __launch_bounds__(256) fold_kernel(GradArgs a) {
   int i = (int)blockIdx.x * 256 + threadIdx.x;
   const auto fold = [](uint32_t *bound, int parts, int all, int at) {
     uint32_t top = 0;
-    for (int p = 0; p < parts; ++p) top = max(top, bound[(int64_t)p * all + at]);
+    for (int p = 0; p < parts; p += 8)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, bound[(int64_t)min(p + k, parts - 1) * all + at]);
     bound[at] = top;
   };
   if (a.along_n) {
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Operands g
     });
   }
 }
-// The parts' results in their order.
+// The parts' results in their order; back null: 1.
 template <class T, bool ADD>
 __global__ void __launch_bounds__(256) half_join_kernel(Splits p, const float *__restrict__ back, typename T::raw *to,
                                                         int64_t stride, int rows, int cols, int per_row) {
@@ -415,7 +418,165 @@ __global__ void __launch_bounds__(256) half_join_kernel(Splits p, const float *_
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] = k + n < p.splits ? sum[j] + v[n].get(j) : sum[j];
   }
-  put8<T, ADD>(to + row * stride, c, cols, sum, back[row]);
+  put8<T, ADD>(to + row * stride, c, cols, sum, back ? back[row] : 1.0f);
+}
+
+// --------------------------------------------------------------- few rows
+// Up to kFew rows: dw is as many outer products, bound by its own bytes, dx as
+// many rows times the codes as they lie, bound by those; both in f32, from dy
+// itself.  (The way above makes an image of the codes first, two bytes written and
+// read again a weight.  f16 8320 -> 8034, all outputs with the stores, 2 rows 185 us
+// that way and 86 this: dw 49, 5.5 TB/s, dx 21, 3.2 TB/s of codes, and its join 5;
+// 8 rows 180 and 108; bf16 2048 -> 2048, 8 rows 42 and 36, but 16 rows 42 and 56.)
+constexpr int kFew = 8;
+
+// dpre, unrounded.
+template <class T>
+__device__ inline float dpre_of(const GradArgs &a, int t, int o) {
+  const float dy = T::get(((const typename T::raw *)a.dy)[(int64_t)t * a.dy_stride + o]);
+  return a.pre ? dy * act_prime_f32((float)a.pre[(int64_t)t * a.pre_stride + o] * a.pre_scales[t], a.act) : dy;
+}
+
+// A block takes 1024 columns of 32 channels, a thread four columns of all rows.
+constexpr int kDwRows = 32, kDwCols = 1024;
+template <class T, int N, bool ADD, bool NT>
+__global__ void __launch_bounds__(256) dw_few_kernel(GradArgs a, const int8_t *__restrict__ x, int64_t x_stride, int in,
+                                                     int chunks, float *dw) {
+  __shared__ float g[kDwRows][N];
+  const int first = (int)(blockIdx.x / chunks) * kDwRows, c = (int)(blockIdx.x % chunks) * kDwCols + threadIdx.x * 4;
+  const int end = (in + kPad - 1) / kPad * kPad;
+  float v[N][4];
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    const int r = min(t, a.n - 1);
+    const uint32_t w = *(const uint32_t *)(x + r * x_stride + min(c, end - 4));
+    const float s = a.x_scales[r];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[t][j] = t < a.n ? value_of(w, j) * s : 0.0f;
+  }
+  for (int i = threadIdx.x; i < kDwRows * N; i += 256) {
+    const int o = first + i / N, t = i % N;
+    g[i / N][t] = o < a.out && t < a.n ? dpre_of<T>(a, t, o) : 0.0f;
+  }
+  __syncthreads();
+  if (c >= in) return;
+#pragma unroll 4
+  for (int r = 0; r < kDwRows; ++r) {
+    if (first + r >= a.out) break;
+    float *to = dw + (int64_t)(first + r) * in;
+    float4 was = ADD ? load4(to, c, in) : make_float4(0, 0, 0, 0), sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < N; ++t) sum = fma4(g[r][t], make_float4(v[t][0], v[t][1], v[t][2], v[t][3]), sum);
+    if (ADD) sum = add4(was, sum);
+    if (NT && c + 4 <= in) store4_nt(to + c, sum);
+    else store4(to, c, in, sum);
+  }
+}
+
+// A block takes 512 columns and a part of the channels, a lane eight columns, the
+// waves every eighth channel; they join in LDS, the parts in half_join_kernel.
+constexpr int kDxCols = 512, kDxWaves = 8, kDxRows = 512;
+template <class T, int N>
+__global__ void __launch_bounds__(kDxWaves * 64) dx_few_kernel(GradArgs a, const int8_t *__restrict__ w, int64_t pitch,
+                                                               int in, int chunks, int each, float *parts,
+                                                               typename T::raw *dx, int64_t dx_stride) {
+  constexpr int kAhead = 8;
+  __shared__ __attribute__((aligned(16))) float g[kDxRows][N];
+  __shared__ __attribute__((aligned(16))) float sums[kDxWaves][kDxCols];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int split = blockIdx.x / chunks, first = (int)(blockIdx.x % chunks) * kDxCols;
+  const int begin = split * each, end = min(begin + each, a.out);
+  const int8_t *at = w + min((int64_t)first + lane * 8, pitch - 8);
+  float acc[N][8] = {};
+  for (int o0 = begin; o0 < end; o0 += kDxRows) {
+    const int rows = min(kDxRows, end - o0);
+    uint2 next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = *(const uint2 *)(at + (int64_t)min(o0 + wave + k * kDxWaves, end - 1) * pitch);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * N; i += kDxWaves * 64) {
+      const int o = o0 + i / N, t = i % N;
+      g[i / N][t] = t < a.n ? dpre_of<T>(a, t, o) * a.w_scales[o] : 0.0f;
+    }
+    __syncthreads();
+    for (int r = wave; r < rows; r += kAhead * kDxWaves) {
+      uint2 now[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        now[k] = next[k];
+        next[k] = *(const uint2 *)(at + (int64_t)min(o0 + r + (kAhead + k) * kDxWaves, end - 1) * pitch);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (r + k * kDxWaves >= rows) break;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = value_of(j < 4 ? now[k].x : now[k].y, j & 3);
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[t][j] = fmaf(g[r + k * kDxWaves][t], v[j], acc[t][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    if (t >= a.n) break;
+    __syncthreads();
+    *(float4 *)&sums[wave][lane * 8] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    *(float4 *)&sums[wave][lane * 8 + 4] = make_float4(acc[t][4], acc[t][5], acc[t][6], acc[t][7]);
+    __syncthreads();
+    const int c = first + threadIdx.x;
+    float sum = sums[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kDxWaves; ++k) sum += sums[k][threadIdx.x];
+    if (c >= in) continue;
+    if (parts) parts[((int64_t)split * a.n + t) * in + c] = sum;
+    else dx[t * dx_stride + c] = T::put(sum);
+  }
+}
+
+// f(constant of at least n rows)
+template <class F>
+hipError_t with_rows(int n, F &&f) {
+  if (n == 1) return f(std::integral_constant<int, 1>{});
+  if (n == 2) return f(std::integral_constant<int, 2>{});
+  if (n <= 4) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, kFew>{});
+}
+template <class T>
+hipError_t launch_dw_few(const GradArgs &a, const welvet_hip_rows8 *x, int in, float *dw, bool add, hipStream_t s) {
+  const int chunks = tiles_of(in, kDwCols);
+  const unsigned blocks = (unsigned)tiles_of(a.out, kDwRows) * chunks;
+  with_rows(a.n, [&](auto rows) {
+    const auto go = [&](auto kernel) { kernel<<<blocks, 256, 0, s>>>(a, x->d_codes, x->stride, in, chunks, dw); };
+    if (add) go(dw_few_kernel<T, rows.value, true, false>);
+    else if ((int64_t)in * a.out * 4 > kKept) go(dw_few_kernel<T, rows.value, false, true>);
+    else go(dw_few_kernel<T, rows.value, false, false>);
+    return hipSuccess;
+  });
+  return hipGetLastError();
+}
+template <class T>
+hipError_t launch_dx_few(const GradArgs &a, const welvet_hip_int8 *layer, typename T::raw *dx, int64_t dx_stride,
+                         void *parts, hipStream_t s) {
+  // two blocks a CU, of 64 channels and more; the parts' workspace holds 2^22 values
+  const int in = layer->in, chunks = tiles_of(in, kDxCols);
+  const int64_t values = (int64_t)a.n * in, room = ((int64_t)1 << 22) / values;
+  int splits = (int)std::max<int64_t>(1, std::min<int64_t>({16, 512 / chunks, a.out / 64, room}));
+  const int each = tiles_of(a.out, splits);
+  splits = tiles_of(a.out, each);
+  with_rows(a.n, [&](auto rows) {
+    dx_few_kernel<T, rows.value><<<chunks * splits, kDxWaves * 64, 0, s>>>(
+        a, layer->codes, layer->pitch, in, chunks, each, splits > 1 ? (float *)parts : nullptr, dx, dx_stride);
+    return hipSuccess;
+  });
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || splits == 1) return e;
+  const int per_row = tiles_of(in, 8);
+  half_join_kernel<T, false><<<(unsigned)((a.n * per_row + 255) / 256), 256, 0, s>>>(
+      Splits(splits, values, parts), nullptr, dx, dx_stride, a.n, in, per_row);
+  return hipGetLastError();
 }
 
 // 256 x 256, a block a CU, where there is one for each; 128 x 128, two.  (dw and dx
@@ -462,7 +623,11 @@ constexpr int kPartsW = 2;
 template <class T>
 constexpr int kPartsX = std::is_same_v<T, BF16> ? 1 : 2;
 
-constexpr int kFewBounds = 16;
+// Bounds that the next pass's blocks read in all, each those of its rows and columns,
+// past which they are folded first (us of the fold and that pass: bf16 8192 rows,
+// 11008 channels, 418304 bounds, 213 and 240 without; f32 1000 rows, 2048 channels,
+// 5120 bounds, 13.4 without, and the fold's launch alone takes 5).
+constexpr int64_t kFoldFrom = 1 << 16;
 
 struct Plan {
   size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back, parts;  // offsets
@@ -480,7 +645,7 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
   p.codes_x = take(2 * in * along(n));
   p.grad_x = take(2 * (dtype == kBFloat16 ? kPartsX<BF16> : kPartsX<F32>) * n * along(out));
   p.codes_w = take(2 * in * along(out));
-  p.col_bound = take(4 * std::min<int64_t>(32, tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
+  p.col_bound = take(4 * std::min<int64_t>(kMostBounds, tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
   p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
   p.col_back = take(4 * out);
   p.row_back = take(4 * n);
@@ -595,18 +760,25 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
     using T = decltype(t);
     constexpr int PX = kPartsX<T>;
     hipError_t e = hipSuccess;
+    if (n <= kFew) {
+      if (d_dw && (e = launch_dw_few<T>(a, x8, in, d_dw, accumulate, s)) != hipSuccess) return e;
+      if (d_dx) e = launch_dx_few<T>(a, layer, (typename T::raw *)d_dx, dx_stride, parts, s);
+      if (e != hipSuccess || !d_dpre) return e;
+      a.along_n = a.along_o = nullptr;
+      grad_kernel<T, kPartsW, PX, false><<<a.across, kThreads, 0, s>>>(x, a);  // last: dpre may lie in the place of dy
+      return hipGetLastError();
+    }
     const bool one = d_dw && !d_dx && n <= kRows;
     if (products && !one) {
       prepare_kernel<T><<<x.blocks + w.blocks + a.col_parts * a.row_parts, kThreads, 0, s>>>(x, w, a);
       if ((e = hipGetLastError()) != hipSuccess) return e;
-      // every 64 x 64 tile of the next pass reads the bounds of its rows and columns
-      if ((d_dw && a.col_parts > kFewBounds) || (d_dx && a.row_parts > kFewBounds)) {
+      if (((d_dw ? a.col_parts : 0) + (d_dx ? a.row_parts : 0)) * (int64_t)tiles_of(n, kRows) * a.across > kFoldFrom) {
         fold_kernel<<<tiles_of((d_dw ? out : 0) + (d_dx ? n : 0), 256), 256, 0, s>>>(a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         a.col_parts = a.row_parts = 1;
       }
     }
-    // up to 128 rows without dx one launch does both (f16 1001 -> 777, 100 rows: 27 -> ONEUS us in all)
+    // up to 128 rows without dx one launch does both (f16 1001 -> 777, 100 rows: 27 -> 22 us in all)
     if (one) grad_kernel<T, kPartsW, PX, true><<<x.blocks + a.across, kThreads, 0, s>>>(x, a);
     else grad_kernel<T, kPartsW, PX, false><<<(unsigned)tiles_of(n, kRows) * a.across, kThreads, 0, s>>>(x, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;

@@ -245,6 +245,7 @@ struct Splits {
   int splits, each;      // parts, and the stages of one
   int64_t parts_values;  // of one's [rows][cols] results
   void *parts;
+  Splits(int splits_, int64_t values, void *ws) : splits(splits_), each(0), parts_values(values), parts(ws) {}
   Splits(int tiles_m, int tiles_n, const Operands &o, int tile_rows, void *ws)
       : splits(1), each(o.stages), parts_values((int64_t)o.a_rows * o.b_rows), parts(ws) {
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
