@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(256) int8_join_kernel(Splits p, Out o, int per
 using Large = Tile<Int8Op, 1, 2, 4, 4, 2>;   // 256 x 256, eight waves
 using Medium = Tile<Int8Op, 1, 2, 2, 2, 2>;  // 128 x 128, four
 using Deep = Tile<Int8Op, 1, 2, 4, 2, 1, 4, 4>;  // 128 x 128, eight
+using Slim = Tile<Int8Op, 1, 2, 4, 1, 1, 6, 6>;  // 64 x 128, eight: half the copies of x
 
 // Split: the tile of the parts.
 template <class T, class Tile, class Split>
@@ -294,28 +295,33 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
     using T = decltype(t);
     const Few f{l.codes, l.pitch, x, x_stride, (int)padded(l.in) - 16, (l.in + 63) / 64};
     const unsigned blocks = (unsigned)((l.out + 15) / 16);
-    // 16 waves where eight a CU would be all there are
+    // 16 waves where eight a CU would be all there are (us, up to 16 rows: the tiles'
+    // parts take 21 to 23 from 4096 -> 11008, this 17.5 to 21.7; 4096 -> 1024 13 / 10)
     const bool wide = blocks <= 512 && f.steps >= 64;
     if (o.n <= 16) {
       if (wide) int8_few_kernel<T, 16, 1><<<blocks, 1024, 0, s>>>(f, o);
       else int8_few_kernel<T, 8, 1><<<blocks, 512, 0, s>>>(f, o);
       return hipGetLastError();
     }
-    if (o.n <= 32) {
-      if (wide) int8_few_kernel<T, 16, 2><<<blocks, 1024, 0, s>>>(f, o);
-      else int8_few_kernel<T, 8, 2><<<blocks, 512, 0, s>>>(f, o);
-      return hipGetLastError();
-    }
-    // small weights: one launch, where the other way's parts take two (us, 64 rows
-    // bf16: 1024 -> 1024 8.9 / 13.6; 4096 -> 11008 38 / 28, 6201 -> 640 23 / 17)
-    if (o.n <= 64 && l.in <= 2048 && (int64_t)l.in * l.out <= 4 << 20) {
-      int8_few_kernel<T, 8, 4><<<blocks, 512, 0, s>>>(f, o);
-      return hipGetLastError();
+    // small weights: one launch, where the other way's parts take two (us, bf16:
+    // 17 to 32 rows 4096 -> 1024 12 to 13 / 14 to 15, 4096 -> 11008 28 / 22; 64 rows
+    // 1024 -> 1024 8.9 / 13.6, 6201 -> 640 23 / 16, 4096 -> 11008 38 / 27)
+    if ((int64_t)l.in * l.out <= 4 << 20) {
+      if (o.n <= 32) {
+        if (wide) int8_few_kernel<T, 16, 2><<<blocks, 1024, 0, s>>>(f, o);
+        else int8_few_kernel<T, 8, 2><<<blocks, 512, 0, s>>>(f, o);
+        return hipGetLastError();
+      }
+      if (o.n <= 64 && l.in <= 2048) {
+        int8_few_kernel<T, 8, 4><<<blocks, 512, 0, s>>>(f, o);
+        return hipGetLastError();
+      }
     }
     // large tiles, a block a CU, where there is one for each (us, large and small
     // tiles, bf16: 4096 -> 11008 of 2048 rows 146 / 142, of 4096 225 / 246; 11008 ->
     // 4096 of 2048 rows, 128 large tiles, 175 / 125)
     if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large, Large>(l, x, x_stride, o, parts, s);
+    if (o.n <= 64) return launch_tiles<T, Medium, Slim>(l, x, x_stride, o, parts, s);
     return launch_tiles<T, Medium, Deep>(l, x, x_stride, o, parts, s);
   });
 }

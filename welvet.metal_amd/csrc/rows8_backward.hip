@@ -588,6 +588,8 @@ template <int P>
 using Medium = Tile<HalfOp, P, 2, 2, 2, 2>;
 template <int P>
 using Deep = Tile<HalfOp, P, 2, 4, 2, 1, 4, 4>;
+template <int P>
+using Slim = Tile<HalfOp, P, 2, 4, 1, 1, 6, 6>;
 
 // Split: the tile of the parts.
 template <class T, bool ADD, class Tile, class Split>
@@ -614,6 +616,7 @@ template <class T, bool ADD, int P>
 hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
   if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256)
     return launch_tiles<T, ADD, Large<P>, Large<P>>(g, back, to, stride, parts, s);
+  if (g.a_rows <= 64) return launch_tiles<T, ADD, Medium<P>, Slim<P>>(g, back, to, stride, parts, s);
   return launch_tiles<T, ADD, Medium<P>, Deep<P>>(g, back, to, stride, parts, s);
 }
 
