@@ -215,20 +215,17 @@ template <class T, class Tile, bool PART>
 __global__ void __launch_bounds__(Tile::kWaves * 64) int8_tile_kernel(Operands g, Out o, Splits p, int tiles_m,
                                                                       int tiles_n) {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  const int tile = PART ? (int)blockIdx.x / p.splits : blockIdx.x, split = PART ? (int)blockIdx.x % p.splits : 0;
+  const int tiles = tiles_m * tiles_n, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;  // 0 of the whole
   const Place at = place(tile, tiles_m, tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
   Tile::run(PART ? g.part(split * p.each, min(p.each, g.stages - split * p.each)) : g, m0, n0, acc, lds);
   __syncthreads();
   if constexpr (PART) {
-    Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
+    Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[4]) {
       if (row >= o.n || c >= o.out) return;
-      int *to = (int *)p.parts + split * p.parts_values + (int64_t)row * o.out;
-      Oct<F32> v;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v.w[i] = sum[i];
-      v.store((uint32_t *)to, c, o.out);
+      float *to = (float *)p.parts + split * p.parts_values + (int64_t)row * o.out;
+      store4(to, c, o.out, make_float4(__int_as_float(sum[0]), __int_as_float(sum[1]), __int_as_float(sum[2]), __int_as_float(sum[3])));
     });
   } else {
     float *x_scales = (float *)(lds + Tile::kResults);
@@ -236,7 +233,7 @@ __global__ void __launch_bounds__(Tile::kWaves * 64) int8_tile_kernel(Operands g
     float scale[8], bias[8];  // a lane's channels are the same in all its rows
     channels(o, Tile::first_col(n0), scale, bias);
     __syncthreads();
-    Tile::results(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
+    Tile::template results<8>(m0, n0, acc, lds, [&](int row, int c, const int (&sum)[8]) {
       if (row < o.n && c < o.out) put8<T>(o, row, c, sum, x_scales[row - m0], scale, bias);
     });
   }
@@ -277,7 +274,9 @@ hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_str
   const Splits p(tm, tn, g, Tile::kRows, parts);
   if constexpr (Tile::kRows <= kSplitRows) {
     if (p.splits > 1) {
-      int8_tile_kernel<T, Split, true><<<tm * tn * p.splits, Split::kWaves * 64, 0, s>>>(g, o, p, tm, tn);
+      const auto go = [&](auto kernel, int waves) { kernel<<<tm * tn * p.splits, waves * 64, 0, s>>>(g, o, p, tm, tn); };
+      if (Splits::one_a_cu(tm * tn)) go(int8_tile_kernel<T, Split, true>, Split::kWaves);
+      else go(int8_tile_kernel<T, Tile, true>, Tile::kWaves);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       const int per_row = (o.out + 7) / 8;

@@ -31,9 +31,11 @@ constexpr int kMaxSize = 1 << 20;
 __host__ __device__ constexpr int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 constexpr int kThreads = 512, kRows = 128, kCols = 64;    // of the passes' blocks: 128 x 64 values
 constexpr int kBoundCols = 512, kBoundRows = 32;          // of dy a block of the bounds
-// ... the rows in whole steps, so that no more than 16 blocks take them.
-constexpr int kMostBounds = 16;
-int bound_rows(int64_t n) { return tiles_of(n, kMostBounds * kBoundRows) * kBoundRows; }
+// ... the rows in whole steps, so that no more than 16 blocks take them, or 128 with
+// the columns' together (us of the pass, bf16 5267 rows, 448 channels: 16 of them 34,
+// 83 BOUNDUS).
+int most_bounds(int64_t out) { return std::max(16, 128 / tiles_of(out, kBoundCols)); }
+int bound_rows(int64_t n, int64_t out) { return tiles_of(n, most_bounds(out) * kBoundRows) * kBoundRows; }
 int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
 
 __device__ inline uint16_t half_bits(float v) { return F16::put(v); }
@@ -387,17 +389,28 @@ __global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Operands g
   Tile::run(PART ? g.part(split * p.each, min(p.each, g.stages - split * p.each)) : g, m0, n0, acc, lds);
   __syncthreads();
   if constexpr (PART) {
-    Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
+    Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[4]) {
       if (row < g.a_rows && c < g.b_rows)
-        put8<F32, false>((uint32_t *)p.parts + split * p.parts_values + (int64_t)row * g.b_rows, c, g.b_rows, v, 1.0f);
+        store4((float *)p.parts + split * p.parts_values + (int64_t)row * g.b_rows, c, g.b_rows,
+               make_float4(v[0], v[1], v[2], v[3]));
     });
   } else {
     float *backs = (float *)(lds + Tile::kResults);
     for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = back[min(m0 + i, g.a_rows - 1)];
     __syncthreads();
-    Tile::results(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
-      if (row < g.a_rows && c < g.b_rows) put8<T, ADD>(to + row * stride, c, g.b_rows, v, backs[row - m0]);
-    });
+    if constexpr (std::is_same_v<T, F32>) {
+      Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[4]) {
+        if (row >= g.a_rows || c >= g.b_rows) return;
+        float *into = (float *)to + row * stride;
+        float4 sum = mul4(make_float4(v[0], v[1], v[2], v[3]), backs[row - m0]);
+        if (ADD) sum = add4(load4(into, c, g.b_rows), sum);
+        store4(into, c, g.b_rows, sum);
+      });
+    } else {
+      Tile::template results<8>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
+        if (row < g.a_rows && c < g.b_rows) put8<T, ADD>(to + row * stride, c, g.b_rows, v, backs[row - m0]);
+      });
+    }
   }
 }
 // The parts' results in their order; back null: 1.
@@ -581,7 +594,10 @@ hipError_t launch_dx_few(const GradArgs &a, const welvet_hip_int8 *layer, typena
 
 // 256 x 256, a block a CU, where there is one for each; 128 x 128, two.  (dw and dx
 // of bf16 4096 x 4096, 2048 rows, 256 of the large tiles: 283 us against 304; of
-// 1024 x 1024, 4096 rows, 16 and 64: 111 with the small ones, 127 with the large.)
+// 1024 x 1024, 4096 rows, 16 and 64: 111 with the small ones, 127 with the large.
+// Fewer than four stages are mostly results, which two blocks a CU write beside each
+// other's products: dw 9536 x 8512 f32 of 153 rows 101 us, large 125; 8192 x 2048 of
+// 256 rows, four stages, 31 and 28.)
 template <int P>
 using Large = Tile<HalfOp, P, 2, 4, 4, 2>;
 template <int P>
@@ -599,7 +615,11 @@ hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t 
   auto *out = (typename T::raw *)to;
   if constexpr (Tile::kRows <= kSplitRows) {
     if (p.splits > 1) {
-      half_tile_kernel<T, ADD, Split, true><<<tm * tn * p.splits, Split::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
+      const auto go = [&](auto kernel, int waves) {
+        kernel<<<tm * tn * p.splits, waves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
+      };
+      if (Splits::one_a_cu(tm * tn)) go(half_tile_kernel<T, ADD, Split, true>, Split::kWaves);
+      else go(half_tile_kernel<T, ADD, Tile, true>, Tile::kWaves);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       const int per_row = tiles_of(g.b_rows, 8);
@@ -614,7 +634,7 @@ hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t 
 // to[a_rows][b_rows] (+)= back . A . B^T with A of P parts.
 template <class T, bool ADD, int P>
 hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
-  if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256)
+  if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256 && g.stages >= 4)
     return launch_tiles<T, ADD, Large<P>, Large<P>>(g, back, to, stride, parts, s);
   if (g.a_rows <= 64) return launch_tiles<T, ADD, Medium<P>, Slim<P>>(g, back, to, stride, parts, s);
   return launch_tiles<T, ADD, Medium<P>, Deep<P>>(g, back, to, stride, parts, s);
@@ -648,7 +668,7 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
   p.codes_x = take(2 * in * along(n));
   p.grad_x = take(2 * (dtype == kBFloat16 ? kPartsX<BF16> : kPartsX<F32>) * n * along(out));
   p.codes_w = take(2 * in * along(out));
-  p.col_bound = take(4 * std::min<int64_t>(kMostBounds, tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
+  p.col_bound = take(4 * std::min<int64_t>(most_bounds(out), tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
   p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
   p.col_back = take(4 * out);
   p.row_back = take(4 * n);
@@ -738,7 +758,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   a.out = out;
   a.act = act;
   a.across = tiles_of(out, kCols);
-  a.bound_rows = bound_rows(n);
+  a.bound_rows = bound_rows(n, out);
   a.col_parts = tiles_of(n, a.bound_rows);
   a.row_parts = tiles_of(out, kBoundCols);
   a.n_pitch = along(n);

@@ -204,18 +204,19 @@ struct Tile {
   __device__ static inline int first_col(int n0) {
     return n0 + (int)(threadIdx.x >> 6) % WN * TN * 32 + (int)(threadIdx.x & 63) % (TN * 4) * 8;
   }
-  // f(row, col, values) with eight neighbouring columns of a row a lane, eight or
-  // more lanes a row: a wave turns its results 32 rows at a time in LDS, which
+  // f(row, col, values) with W neighbouring columns of a row a lane, so that a store
+  // of theirs is 16 bytes and a row's lie side by side: a wave turns its results 32 rows at a time in LDS, which
   // has to be left by the block's products (a barrier).
   using Value = std::remove_cv_t<std::remove_reference_t<decltype(std::declval<Acc>()[0])>>;
-  template <class F>
+  template <int W, class F>
   __device__ static inline void results(int m0, int n0, const Acc (&acc)[TM][TN], char *lds, F &&f) {
-    constexpr int kPitch = TN * 32 + 4, kAcross = TN * 4;  // values, lanes a row
+    constexpr int kPitch = TN * 32 + 4, kAcross = TN * 32 / W;  // values, lanes a row
+    static_assert(W == 4 || W == 8, "columns");
     static_assert(kWaves * 32 * kPitch * 4 <= kResults, "the results' place");
     typedef Value quad __attribute__((ext_vector_type(4)));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Value *mine = (Value *)lds + wave * 32 * kPitch;
-    const int m = m0 + wave / WN * TM * 32 + lane / kAcross, n = n0 + wave % WN * TN * 32 + lane % kAcross * 8;
+    const int m = m0 + wave / WN * TM * 32 + lane / kAcross, n = n0 + wave % WN * TN * 32 + lane % kAcross * W;
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
 #pragma unroll
@@ -227,9 +228,10 @@ struct Tile {
       asm volatile("" ::: "memory");
 #pragma unroll 1
       for (int r = 0; r < 32; r += 64 / kAcross) {
-        const quad *at = (const quad *)(mine + (r + lane / kAcross) * kPitch + lane % kAcross * 8);
-        const quad lo = at[0], hi = at[1];
-        const Value v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        const quad *at = (const quad *)(mine + (r + lane / kAcross) * kPitch + lane % kAcross * W);
+        Value v[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = at[i / 4][i % 4];
         f(m + t * 32 + r, n, v);
       }
       asm volatile("" ::: "memory");
@@ -238,8 +240,8 @@ struct Tile {
 };
 
 // Few tiles: the sum's stages in parts, a block each, whose results are joined
-// in a launch of their own.  As many as give every CU a block, of four stages and
-// more, at most 16.
+// in a launch of their own.  As many as give every CU a block (more than 128 tiles:
+// two), of four stages and more, at most 16.
 constexpr int kSplitRows = 128;  // of the largest tile that is split
 struct Splits {
   int splits, each;      // parts, and the stages of one
@@ -250,16 +252,17 @@ struct Splits {
       : splits(1), each(o.stages), parts_values((int64_t)o.a_rows * o.b_rows), parts(ws) {
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
     if (tile_rows > kSplitRows) return;
-    const int most = (int)std::min<int64_t>(16, std::min<int64_t>(256 / tiles, o.stages / 4));
+    const int most = (int)std::min<int64_t>(16, std::min<int64_t>((one_a_cu(tiles) ? 256 : 512) / tiles, o.stages / 4));
     if (most < 2) return;
     each = (o.stages + most - 1) / most;
     splits = (o.stages + each - 1) / each;
   }
+  static bool one_a_cu(int64_t tiles) { return tiles <= 128; }
 };
-// Their workspace for results of rows x cols: at most 256 tiles of 128 x 128; not
+// Their workspace for results of rows x cols: at most 512 tiles of 128 x 128; not
 // less for more rows.
 inline size_t parts_bytes(int64_t rows, int64_t cols) {
-  return (size_t)std::min<int64_t>((int64_t)256 * kSplitRows * kSplitRows, 16 * rows * cols) * 4;
+  return (size_t)std::min<int64_t>((int64_t)512 * kSplitRows * kSplitRows, 16 * rows * cols) * 4;
 }
 
 // The tile of a block: blocks of one XCD (every eighth) take neighbouring
