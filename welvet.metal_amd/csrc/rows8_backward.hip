@@ -450,85 +450,107 @@ __device__ inline float dpre_of(const GradArgs &a, int t, int o) {
   return a.pre ? dy * act_prime_f32((float)a.pre[(int64_t)t * a.pre_stride + o] * a.pre_scales[t], a.act) : dy;
 }
 
-// A block takes 1024 columns of 32 channels, a thread four columns of all rows.
-constexpr int kDwRows = 32, kDwCols = 1024;
+struct FewArgs {
+  const int8_t *x;  // the input's codes
+  int64_t x_stride;
+  float *dw;
+  const int8_t *w;  // the layer's
+  int64_t pitch;
+  void *dx;
+  int64_t dx_stride;
+  float *parts;  // of dx, null: whole
+  int in, dw_chunks, dx_chunks, dx_blocks, each;
+};
+constexpr int kDwRows = 32, kDwCols = 1024, kDxCols = 512, kDxRows = 512;
+template <int N>
+union FewLds {
+  float dpre[kDwRows][N];
+  struct {
+    float terms[kDxRows][N], sums[kThreads / 64][kDxCols];
+  } dx;
+};
+
+// A block takes 1024 columns of 32 channels, a thread four columns of sixteen, all
+// rows; the first columns' block has dpre stored.
 template <class T, int N, bool ADD, bool NT>
-__global__ void __launch_bounds__(256) dw_few_kernel(GradArgs a, const int8_t *__restrict__ x, int64_t x_stride, int in,
-                                                     int chunks, float *dw) {
-  __shared__ float g[kDwRows][N];
-  const int first = (int)(blockIdx.x / chunks) * kDwRows, c = (int)(blockIdx.x % chunks) * kDwCols + threadIdx.x * 4;
-  const int end = (in + kPad - 1) / kPad * kPad;
+__device__ inline void dw_few(const GradArgs &a, const FewArgs &f, int block, float (&g)[kDwRows][N]) {
+  const int first = block / f.dw_chunks * kDwRows, c = block % f.dw_chunks * kDwCols + (threadIdx.x & 255) * 4;
+  const int last = (f.in + kPad - 1) / kPad * kPad - 4;
   float v[N][4];
 #pragma unroll
   for (int t = 0; t < N; ++t) {
     const int r = min(t, a.n - 1);
-    const uint32_t w = *(const uint32_t *)(x + r * x_stride + min(c, end - 4));
+    const uint32_t w = *(const uint32_t *)(f.x + r * f.x_stride + min(c, last));
     const float s = a.x_scales[r];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[t][j] = t < a.n ? value_of(w, j) * s : 0.0f;
   }
-  for (int i = threadIdx.x; i < kDwRows * N; i += 256) {
-    const int o = first + i / N, t = i % N;
-    g[i / N][t] = o < a.out && t < a.n ? dpre_of<T>(a, t, o) : 0.0f;
+  if (threadIdx.x < kDwRows * N) {
+    const int o = first + (int)threadIdx.x % kDwRows, t = threadIdx.x / kDwRows;
+    const bool there = o < a.out && t < a.n;
+    const float d = there ? dpre_of<T>(a, t, o) : 0.0f;
+    g[threadIdx.x % kDwRows][t] = d;
+    if (a.dpre && there && block % f.dw_chunks == 0)
+      ((typename T::raw *)a.dpre)[t * a.dpre_stride + o] = T::put(d);
   }
   __syncthreads();
-  if (c >= in) return;
+  if (c >= f.in) return;
 #pragma unroll 4
-  for (int r = 0; r < kDwRows; ++r) {
+  for (int k = 0; k < kDwRows / 2; ++k) {
+    const int r = (threadIdx.x >> 8) * (kDwRows / 2) + k;
     if (first + r >= a.out) break;
-    float *to = dw + (int64_t)(first + r) * in;
-    float4 was = ADD ? load4(to, c, in) : make_float4(0, 0, 0, 0), sum = make_float4(0, 0, 0, 0);
+    float *to = f.dw + (int64_t)(first + r) * f.in;
+    const float4 was = ADD ? load4(to, c, f.in) : make_float4(0, 0, 0, 0);
+    float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int t = 0; t < N; ++t) sum = fma4(g[r][t], make_float4(v[t][0], v[t][1], v[t][2], v[t][3]), sum);
     if (ADD) sum = add4(was, sum);
-    if (NT && c + 4 <= in) store4_nt(to + c, sum);
-    else store4(to, c, in, sum);
+    if (NT && c + 4 <= f.in) store4_nt(to + c, sum);
+    else store4(to, c, f.in, sum);
   }
 }
+static_assert(kDwRows * 8 <= kThreads, "a thread a value of dpre");
 
 // A block takes 512 columns and a part of the channels, a lane eight columns, the
 // waves every eighth channel; they join in LDS, the parts in half_join_kernel.
-constexpr int kDxCols = 512, kDxWaves = 8, kDxRows = 512;
 template <class T, int N>
-__global__ void __launch_bounds__(kDxWaves * 64) dx_few_kernel(GradArgs a, const int8_t *__restrict__ w, int64_t pitch,
-                                                               int in, int chunks, int each, float *parts,
-                                                               typename T::raw *dx, int64_t dx_stride) {
-  constexpr int kAhead = 8;
-  __shared__ __attribute__((aligned(16))) float g[kDxRows][N];
-  __shared__ __attribute__((aligned(16))) float sums[kDxWaves][kDxCols];
+__device__ inline void dx_few(const GradArgs &a, const FewArgs &f, int block, float (&terms)[kDxRows][N],
+                              float (&sums)[kThreads / 64][kDxCols]) {
+  constexpr int kAhead = 8, kWaves = kThreads / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int split = blockIdx.x / chunks, first = (int)(blockIdx.x % chunks) * kDxCols;
-  const int begin = split * each, end = min(begin + each, a.out);
-  const int8_t *at = w + min((int64_t)first + lane * 8, pitch - 8);
+  const int split = block / f.dx_chunks, first = block % f.dx_chunks * kDxCols;
+  const int begin = split * f.each, end = min(begin + f.each, a.out);
+  const int8_t *at = f.w + min((int64_t)first + lane * 8, f.pitch - 8);
   float acc[N][8] = {};
   for (int o0 = begin; o0 < end; o0 += kDxRows) {
     const int rows = min(kDxRows, end - o0);
     uint2 next[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) next[k] = *(const uint2 *)(at + (int64_t)min(o0 + wave + k * kDxWaves, end - 1) * pitch);
+    for (int k = 0; k < kAhead; ++k)
+      next[k] = *(const uint2 *)(at + (int64_t)min(o0 + wave + k * kWaves, end - 1) * f.pitch);
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * N; i += kDxWaves * 64) {
+    for (int i = threadIdx.x; i < rows * N; i += kThreads) {
       const int o = o0 + i / N, t = i % N;
-      g[i / N][t] = t < a.n ? dpre_of<T>(a, t, o) * a.w_scales[o] : 0.0f;
+      terms[i / N][t] = t < a.n ? dpre_of<T>(a, t, o) * a.w_scales[o] : 0.0f;
     }
     __syncthreads();
-    for (int r = wave; r < rows; r += kAhead * kDxWaves) {
+    for (int r = wave; r < rows; r += kAhead * kWaves) {
       uint2 now[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         now[k] = next[k];
-        next[k] = *(const uint2 *)(at + (int64_t)min(o0 + r + (kAhead + k) * kDxWaves, end - 1) * pitch);
+        next[k] = *(const uint2 *)(at + (int64_t)min(o0 + r + (kAhead + k) * kWaves, end - 1) * f.pitch);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (r + k * kDxWaves >= rows) break;
+        if (r + k * kWaves >= rows) break;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = value_of(j < 4 ? now[k].x : now[k].y, j & 3);
 #pragma unroll
         for (int t = 0; t < N; ++t)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[t][j] = fmaf(g[r + k * kDxWaves][t], v[j], acc[t][j]);
+          for (int j = 0; j < 8; ++j) acc[t][j] = fmaf(terms[r + k * kWaves][t], v[j], acc[t][j]);
       }
     }
   }
@@ -542,53 +564,67 @@ __global__ void __launch_bounds__(kDxWaves * 64) dx_few_kernel(GradArgs a, const
     const int c = first + threadIdx.x;
     float sum = sums[0][threadIdx.x];
 #pragma unroll
-    for (int k = 1; k < kDxWaves; ++k) sum += sums[k][threadIdx.x];
-    if (c >= in) continue;
-    if (parts) parts[((int64_t)split * a.n + t) * in + c] = sum;
-    else dx[t * dx_stride + c] = T::put(sum);
+    for (int k = 1; k < kWaves; ++k) sum += sums[k][threadIdx.x];
+    if (c >= f.in) continue;
+    if (f.parts) f.parts[((int64_t)split * a.n + t) * f.in + c] = sum;
+    else ((typename T::raw *)f.dx)[t * f.dx_stride + c] = T::put(sum);
   }
 }
+static_assert(kDxCols == kThreads, "a thread a column at the end");
 
-// f(constant of at least n rows)
-template <class F>
-hipError_t with_rows(int n, F &&f) {
-  if (n == 1) return f(std::integral_constant<int, 1>{});
-  if (n == 2) return f(std::integral_constant<int, 2>{});
-  if (n <= 4) return f(std::integral_constant<int, 4>{});
-  return f(std::integral_constant<int, kFew>{});
+// dx's blocks, the longer ones, first.
+template <class T, int N, bool ADD, bool NT>
+__global__ void __launch_bounds__(kThreads) few_kernel(GradArgs a, FewArgs f) {
+  __shared__ __attribute__((aligned(16))) FewLds<N> lds;
+  if ((int)blockIdx.x < f.dx_blocks) return dx_few<T, N>(a, f, blockIdx.x, lds.dx.terms, lds.dx.sums);
+  dw_few<T, N, ADD, NT>(a, f, blockIdx.x - f.dx_blocks, lds.dpre);
 }
-template <class T>
-hipError_t launch_dw_few(const GradArgs &a, const welvet_hip_rows8 *x, int in, float *dw, bool add, hipStream_t s) {
-  const int chunks = tiles_of(in, kDwCols);
-  const unsigned blocks = (unsigned)tiles_of(a.out, kDwRows) * chunks;
-  with_rows(a.n, [&](auto rows) {
-    const auto go = [&](auto kernel) { kernel<<<blocks, 256, 0, s>>>(a, x->d_codes, x->stride, in, chunks, dw); };
-    if (add) go(dw_few_kernel<T, rows.value, true, false>);
-    else if ((int64_t)in * a.out * 4 > kKept) go(dw_few_kernel<T, rows.value, false, true>);
-    else go(dw_few_kernel<T, rows.value, false, false>);
-    return hipSuccess;
-  });
+
+template <class T, int N>
+hipError_t launch_few(const GradArgs &a, const FewArgs &f, bool add, unsigned blocks, hipStream_t s) {
+  const auto go = [&](auto kernel) { kernel<<<blocks, kThreads, 0, s>>>(a, f); };
+  if (add) go(few_kernel<T, N, true, false>);
+  else if ((int64_t)f.in * a.out * 4 > kKept) go(few_kernel<T, N, false, true>);
+  else go(few_kernel<T, N, false, false>);
   return hipGetLastError();
 }
 template <class T>
-hipError_t launch_dx_few(const GradArgs &a, const welvet_hip_int8 *layer, typename T::raw *dx, int64_t dx_stride,
-                         void *parts, hipStream_t s) {
-  // two blocks a CU, of 64 channels and more; the parts' workspace holds 2^22 values
-  const int in = layer->in, chunks = tiles_of(in, kDxCols);
-  const int64_t values = (int64_t)a.n * in, room = ((int64_t)1 << 22) / values;
-  int splits = (int)std::max<int64_t>(1, std::min<int64_t>({16, 512 / chunks, a.out / 64, room}));
-  const int each = tiles_of(a.out, splits);
-  splits = tiles_of(a.out, each);
-  with_rows(a.n, [&](auto rows) {
-    dx_few_kernel<T, rows.value><<<chunks * splits, kDxWaves * 64, 0, s>>>(
-        a, layer->codes, layer->pitch, in, chunks, each, splits > 1 ? (float *)parts : nullptr, dx, dx_stride);
-    return hipSuccess;
-  });
-  const hipError_t e = hipGetLastError();
+hipError_t launch_few(const GradArgs &a, const welvet_hip_rows8 *x, const welvet_hip_int8 *layer, int in, float *dw,
+                      bool add, void *dx, int64_t dx_stride, void *parts, hipStream_t s) {
+  FewArgs f{};
+  f.in = in;
+  unsigned blocks = 0;
+  int splits = 1;
+  const int64_t values = (int64_t)a.n * in;
+  if (dw) {
+    f.x = x->d_codes;
+    f.x_stride = x->stride;
+    f.dw = dw;
+    f.dw_chunks = tiles_of(in, kDwCols);
+    blocks = (unsigned)tiles_of(a.out, kDwRows) * f.dw_chunks;
+  }
+  if (dx) {
+    f.w = layer->codes;
+    f.pitch = layer->pitch;
+    f.dx = dx;
+    f.dx_stride = dx_stride;
+    f.dx_chunks = tiles_of(in, kDxCols);
+    // two blocks a CU, of 64 channels and more; the parts' workspace holds 2^22 values
+    splits = (int)std::max<int64_t>(1, std::min<int64_t>({16, 512 / f.dx_chunks, a.out / 64, ((int64_t)1 << 22) / values}));
+    f.each = tiles_of(a.out, splits);
+    splits = tiles_of(a.out, f.each);
+    f.parts = splits > 1 ? (float *)parts : nullptr;
+    f.dx_blocks = f.dx_chunks * splits;
+    blocks += f.dx_blocks;
+  }
+  hipError_t e = a.n == 1   ? launch_few<T, 1>(a, f, add, blocks, s)
+                 : a.n == 2 ? launch_few<T, 2>(a, f, add, blocks, s)
+                 : a.n <= 4 ? launch_few<T, 4>(a, f, add, blocks, s)
+                            : launch_few<T, kFew>(a, f, add, blocks, s);
   if (e != hipSuccess || splits == 1) return e;
   const int per_row = tiles_of(in, 8);
   half_join_kernel<T, false><<<(unsigned)((a.n * per_row + 255) / 256), 256, 0, s>>>(
-      Splits(splits, values, parts), nullptr, dx, dx_stride, a.n, in, per_row);
+      Splits(splits, values, parts), nullptr, (typename T::raw *)dx, dx_stride, a.n, in, per_row);
   return hipGetLastError();
 }
 
@@ -784,11 +820,16 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
     constexpr int PX = kPartsX<T>;
     hipError_t e = hipSuccess;
     if (n <= kFew) {
-      if (d_dw && (e = launch_dw_few<T>(a, x8, in, d_dw, accumulate, s)) != hipSuccess) return e;
-      if (d_dx) e = launch_dx_few<T>(a, layer, (typename T::raw *)d_dx, dx_stride, parts, s);
-      if (e != hipSuccess || !d_dpre) return e;
+      if (products) {
+        // dpre in the place of dy, or without dw, comes last, in a launch of its own
+        const bool with_dw = d_dw && d_dpre != d_dy;
+        a.dpre = with_dw ? d_dpre : nullptr;
+        e = launch_few<T>(a, x8, layer, in, d_dw, accumulate, d_dx, dx_stride, parts, s);
+        if (e != hipSuccess || !d_dpre || with_dw) return e;
+        a.dpre = d_dpre;
+      }
       a.along_n = a.along_o = nullptr;
-      grad_kernel<T, kPartsW, PX, false><<<a.across, kThreads, 0, s>>>(x, a);  // last: dpre may lie in the place of dy
+      grad_kernel<T, kPartsW, PX, false><<<a.across, kThreads, 0, s>>>(x, a);
       return hipGetLastError();
     }
     const bool one = d_dw && !d_dx && n <= kRows;
