@@ -55,7 +55,7 @@ def run(stream, layer, dtype, n, ptr, rows=None, x_stride=None, pre=True, post=T
 SHAPES = [(1, 1, 1), (1, 17, 5), (3, 1001, 777), (2, 64, 16), (16, 128, 100), (17, 500, 33), (33, 4096, 48),
           (64, 777, 129), (65, 100, 130), (100, 1001, 777), (129, 64, 257), (300, 2000, 300), (700, 130, 5000),
           (1, 11008, 64), (40, 20000, 32), (4200, 192, 2100), (20, 4200, 1040), (64, 4200, 1040), (19, 1000, 4500),
-          (50, 300, 20000)]
+          (50, 300, 20000), (130, 2000, 8300)]
 
 
 @pytest.mark.parametrize("dtype", DT)

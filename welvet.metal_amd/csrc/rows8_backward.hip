@@ -33,7 +33,7 @@ constexpr int kThreads = 512, kRows = 128, kCols = 64;    // of the passes' bloc
 constexpr int kBoundCols = 512, kBoundRows = 32;          // of dy a block of the bounds
 // ... the rows in whole steps, so that no more than 16 blocks take them, or 128 with
 // the columns' together (us of the pass, bf16 5267 rows, 448 channels: 16 of them 34,
-// 83 BOUNDUS).
+// 83 12).
 int most_bounds(int64_t out) { return std::max(16, 128 / tiles_of(out, kBoundCols)); }
 int bound_rows(int64_t n, int64_t out) { return tiles_of(n, most_bounds(out) * kBoundRows) * kBoundRows; }
 int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
@@ -377,41 +377,62 @@ __device__ inline void put8(typename T::raw *to, int c, int cols, const float (&
   for (int i = 0; i < 8; ++i) o.set(i, ADD ? o.get(i) + v[i] * back : v[i] * back);
   o.store(to, c, cols);
 }
-template <class T, bool ADD, class Tile, bool PART>
-__global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Operands g, const float *__restrict__ back,
-                                                                      typename T::raw *to, int64_t stride, Splits p,
-                                                                      int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  const int tile = PART ? (int)blockIdx.x / p.splits : blockIdx.x, split = PART ? (int)blockIdx.x % p.splits : 0;
-  const Place at = place(tile, tiles_m, tiles_n);
+template <class T>
+struct Product {  // to[a_rows][b_rows] = back . A . B^T
+  Operands g;
+  const float *back;
+  typename T::raw *to;
+  int64_t stride;
+  Splits p;
+  int tiles_m, tiles_n;
+  int blocks() const { return tiles_m * tiles_n * p.splits; }
+};
+template <class T, bool ADD, class Tile>
+__device__ inline void half_tile(const Product<T> &q, int block, bool part, char *lds) {
+  const Operands &g = q.g;
+  const int tile = part ? block / q.p.splits : block, split = part ? block % q.p.splits : 0;
+  const Place at = place(tile, q.tiles_m, q.tiles_n);
   const int m0 = at.m * Tile::kRows, n0 = at.n * Tile::kCols;
   typename Tile::Acc acc[Tile::kTM][Tile::kTN] = {};
-  Tile::run(PART ? g.part(split * p.each, min(p.each, g.stages - split * p.each)) : g, m0, n0, acc, lds);
+  Tile::run(part ? g.part(split * q.p.each, min(q.p.each, g.stages - split * q.p.each)) : g, m0, n0, acc, lds);
   __syncthreads();
-  if constexpr (PART) {
+  if (part) {
     Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[4]) {
       if (row < g.a_rows && c < g.b_rows)
-        store4((float *)p.parts + split * p.parts_values + (int64_t)row * g.b_rows, c, g.b_rows,
+        store4((float *)q.p.parts + split * q.p.parts_values + (int64_t)row * g.b_rows, c, g.b_rows,
                make_float4(v[0], v[1], v[2], v[3]));
     });
-  } else {
-    float *backs = (float *)(lds + Tile::kResults);
-    for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = back[min(m0 + i, g.a_rows - 1)];
-    __syncthreads();
-    if constexpr (std::is_same_v<T, F32>) {
-      Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[4]) {
-        if (row >= g.a_rows || c >= g.b_rows) return;
-        float *into = (float *)to + row * stride;
-        float4 sum = mul4(make_float4(v[0], v[1], v[2], v[3]), backs[row - m0]);
-        if (ADD) sum = add4(load4(into, c, g.b_rows), sum);
-        store4(into, c, g.b_rows, sum);
-      });
-    } else {
-      Tile::template results<8>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
-        if (row < g.a_rows && c < g.b_rows) put8<T, ADD>(to + row * stride, c, g.b_rows, v, backs[row - m0]);
-      });
-    }
+    return;
   }
+  float *backs = (float *)(lds + Tile::kResults);
+  for (int i = threadIdx.x; i < Tile::kRows; i += Tile::kWaves * 64) backs[i] = q.back[min(m0 + i, g.a_rows - 1)];
+  __syncthreads();
+  if constexpr (std::is_same_v<T, F32>) {
+    Tile::template results<4>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[4]) {
+      if (row >= g.a_rows || c >= g.b_rows) return;
+      float *into = (float *)q.to + row * q.stride;
+      float4 sum = mul4(make_float4(v[0], v[1], v[2], v[3]), backs[row - m0]);
+      if (ADD) sum = add4(load4(into, c, g.b_rows), sum);
+      store4(into, c, g.b_rows, sum);
+    });
+  } else {
+    Tile::template results<8>(m0, n0, acc, lds, [&](int row, int c, const float (&v)[8]) {
+      if (row < g.a_rows && c < g.b_rows) put8<T, ADD>(q.to + row * q.stride, c, g.b_rows, v, backs[row - m0]);
+    });
+  }
+}
+template <class T, bool ADD, class Tile, bool PART>
+__global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Product<T> q) {
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  half_tile<T, ADD, Tile>(q, blockIdx.x, PART, lds);
+}
+// dx's blocks, whose sums are long, then dw's.
+template <class T, bool ADD, class TileX, class TileW>
+__global__ void __launch_bounds__(TileW::kWaves * 64) half_pair_kernel(Product<T> x, Product<F32> w, int of_x) {
+  static_assert(TileX::kWaves == TileW::kWaves && TileX::kLds == TileW::kLds, "one kind of block");
+  __shared__ __attribute__((aligned(1024))) char lds[TileW::kLds];
+  if ((int)blockIdx.x < of_x) return half_tile<T, false, TileX>(x, blockIdx.x, x.p.splits > 1, lds);
+  half_tile<F32, ADD, TileW>(w, blockIdx.x - of_x, w.p.splits > 1, lds);
 }
 // The parts' results in their order; back null: 1.
 template <class T, bool ADD>
@@ -643,28 +664,33 @@ using Deep = Tile<HalfOp, P, 2, 4, 2, 1, 4, 4>;
 template <int P>
 using Slim = Tile<HalfOp, P, 2, 4, 1, 1, 6, 6>;
 
+template <class T, class Tile>
+Product<T> product_of(const Operands &g, const float *back, void *to, int64_t stride, void *parts) {
+  const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
+  return {g, back, (typename T::raw *)to, stride, Splits(tm, tn, g, Tile::kRows, parts), tm, tn};
+}
+template <class T, bool ADD>
+hipError_t launch_join(const Product<T> &q, hipStream_t s) {
+  if (q.p.splits == 1) return hipGetLastError();
+  const int per_row = tiles_of(q.g.b_rows, 8);
+  half_join_kernel<T, ADD><<<(unsigned)(((int64_t)q.g.a_rows * per_row + 255) / 256), 256, 0, s>>>(
+      q.p, q.back, q.to, q.stride, q.g.a_rows, q.g.b_rows, per_row);
+  return hipGetLastError();
+}
 // Split: the tile of the parts.
 template <class T, bool ADD, class Tile, class Split>
 hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
-  const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
-  const Splits p(tm, tn, g, Tile::kRows, parts);
-  auto *out = (typename T::raw *)to;
+  const auto q = product_of<T, Tile>(g, back, to, stride, parts);
+  const auto go = [&](auto kernel, int waves) { kernel<<<q.blocks(), waves * 64, 0, s>>>(q); };
   if constexpr (Tile::kRows <= kSplitRows) {
-    if (p.splits > 1) {
-      const auto go = [&](auto kernel, int waves) {
-        kernel<<<tm * tn * p.splits, waves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
-      };
-      if (Splits::one_a_cu(tm * tn)) go(half_tile_kernel<T, ADD, Split, true>, Split::kWaves);
+    if (q.p.splits > 1) {
+      if (Splits::one_a_cu(q.tiles_m * q.tiles_n)) go(half_tile_kernel<T, ADD, Split, true>, Split::kWaves);
       else go(half_tile_kernel<T, ADD, Tile, true>, Tile::kWaves);
       const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
-      const int per_row = tiles_of(g.b_rows, 8);
-      half_join_kernel<T, ADD><<<(unsigned)(((int64_t)g.a_rows * per_row + 255) / 256), 256, 0, s>>>(
-          p, back, out, stride, g.a_rows, g.b_rows, per_row);
-      return hipGetLastError();
+      return e == hipSuccess ? launch_join<T, ADD>(q, s) : e;
     }
   }
-  half_tile_kernel<T, ADD, Tile, false><<<tm * tn, Tile::kWaves * 64, 0, s>>>(g, back, out, stride, p, tm, tn);
+  go(half_tile_kernel<T, ADD, Tile, false>, Tile::kWaves);
   return hipGetLastError();
 }
 // to[a_rows][b_rows] (+)= back . A . B^T with A of P parts.
@@ -674,6 +700,21 @@ hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t s
     return launch_tiles<T, ADD, Large<P>, Large<P>>(g, back, to, stride, parts, s);
   if (g.a_rows <= 64) return launch_tiles<T, ADD, Medium<P>, Slim<P>>(g, back, to, stride, parts, s);
   return launch_tiles<T, ADD, Medium<P>, Deep<P>>(g, back, to, stride, parts, s);
+}
+
+// dx and dw in one launch of 128 x 128 tiles, two blocks a CU, where dx alone has no
+// more tiles than there are CUs (us, both with the stores, in two launches and in one:
+// f32 2048 -> 8192 of 256 rows, 32 tiles, 53 of the products' time and 46.5; bf16 4096
+// -> 4096 of 64 rows 62 and 56; f32 8512 -> 9536 of 153, 134 tiles, 325 and 307; bf16
+// 2048 -> 11008 of 2000, 256 tiles, 487 and 484).
+constexpr int kPairTiles = 256;
+template <class T, bool ADD, int PX, int PW>
+hipError_t launch_pair(const Product<T> &x, const Product<F32> &w, hipStream_t s) {
+  half_pair_kernel<T, ADD, Medium<PX>, Medium<PW>><<<x.blocks() + w.blocks(), Medium<PW>::kWaves * 64, 0, s>>>(
+      x, w, x.blocks());
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) e = launch_join<T, false>(x, s);
+  return e == hipSuccess ? launch_join<F32, ADD>(w, s) : e;
 }
 
 // Parts of dw's and dx's terms.  One part, rounded as a BFloat16 gradient was
@@ -689,7 +730,7 @@ constexpr int kPartsX = std::is_same_v<T, BF16> ? 1 : 2;
 constexpr int64_t kFoldFrom = 1 << 16;
 
 struct Plan {
-  size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back, parts;  // offsets
+  size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back, parts, parts_x;  // offsets
   size_t bytes;
 };
 Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
@@ -708,7 +749,8 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
   p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
   p.col_back = take(4 * out);
   p.row_back = take(4 * n);
-  p.parts = take(std::max(parts_bytes(out, in), parts_bytes(n, in)));  // dw's, then dx's
+  p.parts = take(parts_bytes(out, in));
+  p.parts_x = take(parts_bytes(n, in));
   p.bytes = at;
   return p;
 }
@@ -824,7 +866,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
         // dpre in the place of dy, or without dw, comes last, in a launch of its own
         const bool with_dw = d_dw && d_dpre != d_dy;
         a.dpre = with_dw ? d_dpre : nullptr;
-        e = launch_few<T>(a, x8, layer, in, d_dw, accumulate, d_dx, dx_stride, parts, s);
+        e = launch_few<T>(a, x8, layer, in, d_dw, accumulate, d_dx, dx_stride, ws + p.parts_x, s);
         if (e != hipSuccess || !d_dpre || with_dw) return e;
         a.dpre = d_dpre;
       }
@@ -846,18 +888,23 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
     if (one) grad_kernel<T, kPartsW, PX, true><<<x.blocks + a.across, kThreads, 0, s>>>(x, a);
     else grad_kernel<T, kPartsW, PX, false><<<(unsigned)tiles_of(n, kRows) * a.across, kThreads, 0, s>>>(x, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
+    const Operands gw{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
+                      (const char *)x.to, 2 * a.n_pitch, in, tiles_of(2 * (int64_t)n, kStageBytes)};
+    const Operands gx{(const char *)a.along_o, 2 * a.o_pitch, 2 * n * a.o_pitch, n, INT32_MAX,
+                      (const char *)w.to, 2 * a.o_pitch, in, tiles_of(2 * (int64_t)out, kStageBytes)};
+    if (d_dw && d_dx) {
+      const auto px = product_of<T, Medium<PX>>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x);
+      if (px.tiles_m * px.tiles_n <= kPairTiles) {
+        const auto pw = product_of<F32, Medium<kPartsW>>(gw, a.col_back, d_dw, in, parts);
+        return accumulate ? launch_pair<T, true, PX, kPartsW>(px, pw, s) : launch_pair<T, false, PX, kPartsW>(px, pw, s);
+      }
+    }
     if (d_dw) {
-      const Operands g{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
-                       (const char *)x.to, 2 * a.n_pitch, in, tiles_of(2 * (int64_t)n, kStageBytes)};
-      e = accumulate ? launch_half<F32, true, kPartsW>(g, a.col_back, d_dw, in, parts, s)
-                     : launch_half<F32, false, kPartsW>(g, a.col_back, d_dw, in, parts, s);
+      e = accumulate ? launch_half<F32, true, kPartsW>(gw, a.col_back, d_dw, in, parts, s)
+                     : launch_half<F32, false, kPartsW>(gw, a.col_back, d_dw, in, parts, s);
       if (e != hipSuccess) return e;
     }
-    if (d_dx) {
-      const Operands g{(const char *)a.along_o, 2 * a.o_pitch, 2 * n * a.o_pitch, n, INT32_MAX,
-                       (const char *)w.to, 2 * a.o_pitch, in, tiles_of(2 * (int64_t)out, kStageBytes)};
-      e = launch_half<T, false, PX>(g, a.row_back, d_dx, dx_stride, parts, s);
-    }
+    if (d_dx) e = launch_half<T, false, PX>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x, s);
     return e;
   }));
   return ok();
