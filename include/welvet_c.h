@@ -439,8 +439,8 @@ WELVET_API welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vo
  * row, value = scale * c: what an integer product takes, and what a training
  * step keeps of its activations, a quarter of f32's bytes, until its backward
  * pass.  The calls follow the rules above (device pointers, streams, types,
- * checks, workspaces); d_codes is 16-byte aligned, [n][stride]
- * with the stride a multiple of 16 and at least the width rounded up to 16.
+ * checks, workspaces); d_codes is 16-byte aligned, [n][stride] with the stride
+ * a multiple of 16 and at least the width rounded up to 16.
  *   scale = max |x| / 127, rounded to f32;  c = x / scale to nearest, ties to
  *   even, of the exact quotient (at most 127: a scale below 2^-126 is itself
  *   rounded to few bits, and below 2^-150 it is 0)
@@ -482,11 +482,12 @@ WELVET_API welvet_status welvet_hip_rows8_swiglu_backward(
 /* A layer in -> out whose product runs in 8-bit integers: weights as rows of
  * codes, a scale for each output channel, stored as rows8_store does; bias (held
  * in f32) and act as in welvet_dense_mount.  in <= 131072 (a sum of products fits
- * 32 bits), out <= 2^24, in out < 2^31.  Mounted from host values W [out*in], from device
- * values (16-byte aligned; read on the null stream), from codes [out][in]
- * in [-127, 127] and scales [out] on the host, or from a mounted Dense session
- * of any dtype (its decoded weights, bias and activation; the session stays as
- * it is).  A mounted layer does not change: calls on it may overlap. */
+ * 32 bits), out <= 2^24, in out < 2^31.  Mounted from host values W [out*in],
+ * from device values (16-byte aligned; read on the null stream), from codes
+ * [out][in] in [-127, 127] and scales [out] on the host, or from a mounted
+ * Dense session of any dtype (its decoded weights, bias and activation; the
+ * session stays as it is).  A mounted layer does not change: calls on it may
+ * overlap. */
 typedef struct welvet_hip_int8 welvet_hip_int8;
 WELVET_API welvet_status welvet_hip_int8_mount(int32_t in, int32_t out, int32_t act, const float *W,
                                                const double *bias, size_t bias_len,
@@ -539,11 +540,11 @@ WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, i
  * scale (dw) or its channel's (dx): two f16 parts a term, 22 bits, but no
  * finer than 2^-39 of the largest |dy| scale of its channel (dw) or token (dx)
  * times what |act'| can be (1.25; 256 scales of the row for act 6); one part,
- * 11 bits, for a BFloat16 dx.  Sums are f32, in a fixed order: the same bits on
- * every run, and whichever outputs are asked for.  Terms of 2^127 and more
- * count as infinite, bits of a term below 2^-126 are lost.  in, out and n <=
- * 2^20, and (n / 128) (out / 64) and (in / 64) (n / 128 + out / 128), rounded
- * up, < 2^22: what one launch takes. */
+ * 11 bits, for a BFloat16 dx; up to 8 rows terms are f32.  Sums are f32, in a
+ * fixed order: the same bits on every run, and whichever outputs are asked for.
+ * Terms of 2^127 and more count as infinite, bits of a term below 2^-126 are
+ * lost.  in, out and n <= 2^20, and (n / 128) (out / 64) and (in / 64) (n / 128
+ * + out / 128), rounded up, < 2^22: what one launch takes. */
 WELVET_API welvet_status welvet_hip_rows8_backward_bytes(int32_t dtype, int32_t n, int32_t in,
                                                          int32_t out, size_t *bytes);
 WELVET_API welvet_status welvet_hip_rows8_backward(
@@ -584,7 +585,7 @@ typedef struct welvet_hip_logit_rules {
   const int32_t *d_mask_id;
 } welvet_hip_logit_rules;
 /* d_out may be d_logits (the same stride): then only the logits that a rule
- * changes are read and written. */
+ * names are written. */
 WELVET_API welvet_status welvet_hip_logits_rules(int32_t dtype, int32_t n, int32_t vocab,
                                                  const void *d_logits, int64_t stride,
                                                  const welvet_hip_logit_rules *rules, void *d_out,
