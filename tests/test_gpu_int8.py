@@ -55,7 +55,8 @@ def run(stream, layer, dtype, n, ptr, rows=None, x_stride=None, pre=True, post=T
 SHAPES = [(1, 1, 1), (1, 17, 5), (3, 1001, 777), (2, 64, 16), (16, 128, 100), (17, 500, 33), (33, 4096, 48),
           (64, 777, 129), (65, 100, 130), (100, 1001, 777), (129, 64, 257), (300, 2000, 300), (700, 130, 5000),
           (1, 11008, 64), (40, 20000, 32), (4200, 192, 2100), (20, 4200, 1040), (64, 4200, 1040), (19, 1000, 4500),
-          (50, 300, 20000), (130, 2000, 8300)]
+          (50, 300, 20000), (130, 2000, 8300),
+          (5, 1600, 21000), (2, 1600, 21001), (128, 300, 66000), (3, 700, 9000)]
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -91,7 +92,7 @@ def test_forward(stream, dtype, n, inn, out):
         assert_bit_equal(again.get(), post, "from rows")
 
 
-@pytest.mark.parametrize("inn,out", [(777, 300), (4096, 520), (11008, 64), (11008, 400)])
+@pytest.mark.parametrize("inn,out", [(777, 300), (4096, 520), (11008, 64), (11008, 400), (1600, 21000)])
 def test_a_row_has_the_same_bits_in_every_batch(stream, inn, out):
     rng = np.random.default_rng([inn, out])
     x = rng.normal(0, 1, (1100, inn)).astype(np.float32)

@@ -129,8 +129,10 @@ __global__ void __launch_bounds__(WAVES * 64) int8_few_kernel(Few f, Out o) {
 }
 
 // A few rows straight from x: every block stores them in 8 bits for itself, in
-// LDS, while its first weights are under way; one launch instead of two.  The
-// block's waves share the rows.
+// LDS, while its first weights are under way; one launch instead of two (us, bf16,
+// this and the store with int8_few_kernel: 4096 -> 11008 one row 12.1 / 15.4, three
+// 16 / 16; 1024 -> 1024 6.1 / 7.2; 8192 -> 1000 one row 9.5 / 12.7).  One row of 4096
+// -> 11008 reads its 45 MB at 3.8 TB/s.  The block's waves share the rows.
 constexpr int kOwnRows = 4, kOwnCodes = 32768, kOwnWaves = 8;
 template <class T>
 __global__ void __launch_bounds__(kOwnWaves * 64, 6) int8_own_kernel(Few f, const typename T::raw *x, int64_t x_stride,
@@ -262,6 +264,7 @@ __global__ void __launch_bounds__(256) int8_join_kernel(Splits p, Out o, int per
 using Large = Tile<Int8Op, 1, 2, 4, 4, 2>;   // 256 x 256, eight waves
 using Medium = Tile<Int8Op, 1, 2, 2, 2, 2>;  // 128 x 128, four
 using Deep = Tile<Int8Op, 1, 2, 4, 2, 1, 4, 4>;  // 128 x 128, eight
+using Narrow = Tile<Int8Op, 1, 2, 4, 1, 1, 3, 3>;  // 64 x 128, eight waves, two blocks a CU
 using Slim = Tile<Int8Op, 1, 2, 4, 1, 1, 6, 6>;  // 64 x 128, eight: half the copies of x
 
 // Split: the tile of the parts.
@@ -271,7 +274,7 @@ hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_str
   const int tm = (o.n + Tile::kRows - 1) / Tile::kRows, tn = (o.out + Tile::kCols - 1) / Tile::kCols;
   const Operands g{(const char *)x, x_stride, 0, o.n, (int)padded(l.in) - 16, (const char *)l.codes, l.pitch, l.out,
                    (l.in + kStageBytes - 1) / kStageBytes};
-  const Splits p(tm, tn, g, Tile::kRows, parts);
+  const Splits p(tm, tn, g, Tile::kRows, 1, parts);
   if constexpr (Tile::kRows <= kSplitRows) {
     if (p.splits > 1) {
       const auto go = [&](auto kernel, int waves) { kernel<<<tm * tn * p.splits, waves * 64, 0, s>>>(g, o, p, tm, tn); };
@@ -288,6 +291,14 @@ hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_str
   return hipGetLastError();
 }
 
+// Channels for whole 64 x 128 tiles on half the CUs and more, and weights that outweigh
+// a few rows' ways above (us, bf16, n rows with the few-row kernels and with tiles: 4096
+// -> 131072 n 1 119 / 97, n 16 190 / 102, 5.3 TB/s; 1024 -> 32000 n 1 28 / 12, 1024 ->
+// 21504 n 8 11.5 / 14.6; 4096 -> 18432 n 16 31.5 / 23.5, 4096 -> 14336 n 16 25.7 / 22
+// but n 1 18.4 / 20.2).
+bool many_channels(const welvet_hip_int8 &l) {
+  return l.out > 128 * Narrow::kCols && (int64_t)l.in * l.out > 30 << 20;
+}
 hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t *x, int64_t x_stride, const Out &o,
                           void *parts, hipStream_t s) {
   return with_type(dtype, [&](auto t) {
@@ -297,6 +308,7 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
     // 16 waves where eight a CU would be all there are (us, up to 16 rows: the tiles'
     // parts take 21 to 23 from 4096 -> 11008, this 17.5 to 21.7; 4096 -> 1024 13 / 10)
     const bool wide = blocks <= 512 && f.steps >= 64;
+    if (o.n <= 64 && many_channels(l)) return launch_tiles<T, Narrow, Narrow>(l, x, x_stride, o, parts, s);
     if (o.n <= 16) {
       if (wide) int8_few_kernel<T, 16, 1><<<blocks, 1024, 0, s>>>(f, o);
       else int8_few_kernel<T, 8, 1><<<blocks, 512, 0, s>>>(f, o);
@@ -316,16 +328,21 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
         return hipGetLastError();
       }
     }
-    // large tiles, a block a CU, where there is one for each (us, large and small
-    // tiles, bf16: 4096 -> 11008 of 2048 rows 146 / 142, of 4096 225 / 246; 11008 ->
+    // large tiles, a block a CU, where there is one for each and more than half of it
+    // is rows (us, large and small tiles, bf16: 4096 -> 65536 of 128 rows 76 / 58; 4096 -> 11008 of 2048 rows 146 / 142, of 4096 225 / 246; 11008 ->
     // 4096 of 2048 rows, 128 large tiles, 175 / 125)
-    if ((int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large, Large>(l, x, x_stride, o, parts, s);
-    if (o.n <= 64) return launch_tiles<T, Medium, Slim>(l, x, x_stride, o, parts, s);
+    if (o.n > 128 && (int64_t)((o.n + 255) / 256) * ((l.out + 255) / 256) >= 256) return launch_tiles<T, Large, Large>(l, x, x_stride, o, parts, s);
+    if (o.n <= 64) return launch_tiles<T, Narrow, Slim>(l, x, x_stride, o, parts, s);
     return launch_tiles<T, Medium, Deep>(l, x, x_stride, o, parts, s);
   });
 }
-// One launch from x, for rows that the caller does not keep.
-bool own_rows(int32_t in, int32_t n) { return n <= kOwnRows && n * padded(in) <= kOwnCodes; }
+// One launch from x, for rows that the caller does not keep; not of short rows where
+// blocks come one after the other on a CU (us, bf16, one row, this and the other way:
+// 1024 -> 4096 6.2 / 8, 1024 -> 8192 9.1 / 8.5, 1024 -> 11008 11.7 / 9.2; 4096 -> 18432
+// 20.9 / 24).
+bool own_rows(const welvet_hip_int8 &l, int32_t n) {
+  return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in >= 4096) && !many_channels(l);
+}
 hipError_t launch_own(const welvet_hip_int8 &l, int32_t dtype, const void *x, int64_t x_stride, const Out &o,
                       hipStream_t s) {
   return with_type(dtype, [&](auto t) {
@@ -501,7 +518,7 @@ welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *l, int32_t dtype, i
   welvet_hip_rows8 r{(int8_t *)d_ws, row_bytes(l->in), (float *)((char *)d_ws + tok::pad256(n * row_bytes(l->in)))};
   if (rows) r = *rows;
   const Out o{d_pre, d_post, pre_stride, post_stride, r.d_scales, l->scales, l->bias, n, l->out, l->act};
-  if (!rows && own_rows(l->in, n)) {
+  if (!rows && own_rows(*l, n)) {
     WH_HIP(launch_own(*l, dtype, d_x, x_stride, o, (hipStream_t)stream));
     return ok();
   }

@@ -3,7 +3,10 @@
 //   s = max |x| / 127,  c_i = x_i / s to nearest even,  value s c_i
 //   h = silu(gate) up;  dgate = dh up silu'(gate),  dup = dh silu(gate)
 // Bound by HBM: a row a block, read once into registers, its largest magnitude
-// joined across the block, then its codes written.
+// joined across the block, then its codes written.  bf16 8192 x 11008: stored 66 us
+// (4.1 TB/s), read back 43, SwiGLU with both kept 147 (4.9 TB/s), its backward 127
+// (5.7); with h in 8 bits as well 228, as its products are formed twice.  A few rows
+// take 2.5 to 6 us, the launch and one row's loads, join and stores.
 #include <hip/hip_runtime.h>
 
 #include "rows8.hpp"
@@ -268,10 +271,12 @@ hipError_t launch_store(int32_t dtype, int32_t n, int32_t width, const void *x, 
   const StoreArgs a{x, x_stride, codes, codes_stride, scales, n, width};
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    // the block that holds the row in registers; of few rows, more of it
+    // the block that holds the row in registers; of few long rows, more waves (bf16
+    // 11008, us with four waves and sixteen: 64 rows 8.5 / 4.6, 512 9.6 / 8.1, 1024
+    // 12.2 / 14.4; 4096 the same up to 256 rows, 4.7 / 5.5 of 384)
     if (width <= 1024) store_kernel<T, 2, 1><<<row_blocks(n), 128, 0, s>>>(a);
-    else if (width <= 16384 && n <= 256) store_kernel<T, 16, 2><<<row_blocks(n), 1024, 0, s>>>(a);
     else if (width <= 4096) store_kernel<T, 4, 2><<<row_blocks(n), 256, 0, s>>>(a);
+    else if (width <= 16384 && n <= 512) store_kernel<T, 16, 2><<<row_blocks(n), 1024, 0, s>>>(a);
     else if (width <= 8192) store_kernel<T, 4, 4><<<row_blocks(n), 256, 0, s>>>(a);
     else if (width <= 12288) store_kernel<T, 4, 6><<<row_blocks(n), 256, 0, s>>>(a);
     else store_kernel<T, 16, 4><<<row_blocks(n), 1024, 0, s>>>(a);

@@ -667,7 +667,7 @@ using Slim = Tile<HalfOp, P, 2, 4, 1, 1, 6, 6>;
 template <class T, class Tile>
 Product<T> product_of(const Operands &g, const float *back, void *to, int64_t stride, void *parts) {
   const int tm = tiles_of(g.a_rows, Tile::kRows), tn = tiles_of(g.b_rows, Tile::kCols);
-  return {g, back, (typename T::raw *)to, stride, Splits(tm, tn, g, Tile::kRows, parts), tm, tn};
+  return {g, back, (typename T::raw *)to, stride, Splits(tm, tn, g, Tile::kRows, Tile::kParts, parts), tm, tn};
 }
 template <class T, bool ADD>
 hipError_t launch_join(const Product<T> &q, hipStream_t s) {

@@ -85,7 +85,7 @@ struct Tile {
   static constexpr int kWaves = WM * WN, kRows = WM * TM * 32, kCols = WN * TN * 32;
   static constexpr int kA = kRows * kStageBytes, kB = kCols * kStageBytes, kLds = SA * kA + SB * kB;
   static constexpr int kLoadsA = kRows / 8 / kWaves, kLoadsB = kCols / 8 / kWaves;
-  static constexpr int kTM = TM, kTN = TN;
+  static constexpr int kTM = TM, kTN = TN, kParts = P;
   // of LDS after the products: the results' turning place, then the caller's
   static constexpr int kResults = kWaves * 32 * (TN * 32 + 4) * 4;
   static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kWaves % 2 == 0,
@@ -240,23 +240,30 @@ struct Tile {
 };
 
 // Few tiles: the sum's stages in parts, a block each, whose results are joined
-// in a launch of their own.  As many as give every CU a block (more than 128 tiles:
-// two), of four stages and more, at most 16.
+// in a launch of their own.  As many as give every CU a block, from 129 tiles to 170
+// three each and two blocks a CU; of eight stages and more, at most 16.  In two parts
+// only sums of 40 steps and more: the parts' way through memory takes what they save
+// (int8, us, in parts and whole: 1024 -> 8192 of 256 rows, two of four stages, 29 / 15;
+// 2048 -> 8192 of 200, two of eight, 30 / 19; 4096 -> 4096 of 512, two of sixteen, 34 /
+// 31; 8192 -> 4096 45 / 50; 11008 -> 4096 53 / 64; 4096 -> 28672 of 128, 224 tiles in
+// two, 48 / 32).
 constexpr int kSplitRows = 128;  // of the largest tile that is split
 struct Splits {
   int splits, each;      // parts, and the stages of one
   int64_t parts_values;  // of one's [rows][cols] results
   void *parts;
   Splits(int splits_, int64_t values, void *ws) : splits(splits_), each(0), parts_values(values), parts(ws) {}
-  Splits(int tiles_m, int tiles_n, const Operands &o, int tile_rows, void *ws)
+  // steps: of the product a stage, A's parts
+  Splits(int tiles_m, int tiles_n, const Operands &o, int tile_rows, int steps, void *ws)
       : splits(1), each(o.stages), parts_values((int64_t)o.a_rows * o.b_rows), parts(ws) {
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
-    if (tile_rows > kSplitRows) return;
-    const int most = (int)std::min<int64_t>(16, std::min<int64_t>((one_a_cu(tiles) ? 256 : 512) / tiles, o.stages / 4));
-    if (most < 2) return;
+    if (tile_rows > kSplitRows || tiles > kMostSplit) return;
+    const int most = (int)std::min<int64_t>(16, std::min<int64_t>((one_a_cu(tiles) ? 256 : 512) / tiles, o.stages / 8));
+    if (most < 2 || (most == 2 && o.stages * steps < 40)) return;
     each = (o.stages + most - 1) / most;
     splits = (o.stages + each - 1) / each;
   }
+  static constexpr int64_t kMostSplit = 170;
   static bool one_a_cu(int64_t tiles) { return tiles <= 128; }
 };
 // Their workspace for results of rows x cols: at most 512 tiles of 128 x 128; not
