@@ -291,13 +291,13 @@ hipError_t launch_tiles(const welvet_hip_int8 &l, const int8_t *x, int64_t x_str
   return hipGetLastError();
 }
 
-// Channels for whole 64 x 128 tiles on half the CUs and more, and weights that outweigh
-// a few rows' ways above (us, bf16, n rows with the few-row kernels and with tiles: 4096
-// -> 131072 n 1 119 / 97, n 16 190 / 102, 5.3 TB/s; 1024 -> 32000 n 1 28 / 12, 1024 ->
-// 21504 n 8 11.5 / 14.6; 4096 -> 18432 n 16 31.5 / 23.5, 4096 -> 14336 n 16 25.7 / 22
-// but n 1 18.4 / 20.2).
-bool many_channels(const welvet_hip_int8 &l) {
-  return l.out > 128 * Narrow::kCols && (int64_t)l.in * l.out > 30 << 20;
+// Channels for whole 64 x 128 tiles on half the CUs and more (of more than eight rows a
+// third), and weights that outweigh a few rows' ways below (us, bf16, with the few-row
+// kernels and with tiles: 4096 -> 131072 one row 119 / 97, 16 rows 190 / 102, 5.3 TB/s;
+// 1024 -> 32000 one row 28 / 12, 1024 -> 21504 8 rows 11.5 / 14.6; 4096 -> 18432 one row
+// 20.9 / 20; 4096 -> 11008 16 rows 20.9 / 18.9, 8 rows 18.2 / 20.1).
+bool many_channels(const welvet_hip_int8 &l, int32_t n) {
+  return l.out > (n > 8 ? 80 : 128) * Narrow::kCols && (int64_t)l.in * l.out > 30 << 20;
 }
 hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t *x, int64_t x_stride, const Out &o,
                           void *parts, hipStream_t s) {
@@ -308,7 +308,7 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
     // 16 waves where eight a CU would be all there are (us, up to 16 rows: the tiles'
     // parts take 21 to 23 from 4096 -> 11008, this 17.5 to 21.7; 4096 -> 1024 13 / 10)
     const bool wide = blocks <= 512 && f.steps >= 64;
-    if (o.n <= 64 && many_channels(l)) return launch_tiles<T, Narrow, Narrow>(l, x, x_stride, o, parts, s);
+    if (o.n <= 64 && many_channels(l, o.n)) return launch_tiles<T, Narrow, Narrow>(l, x, x_stride, o, parts, s);
     if (o.n <= 16) {
       if (wide) int8_few_kernel<T, 16, 1><<<blocks, 1024, 0, s>>>(f, o);
       else int8_few_kernel<T, 8, 1><<<blocks, 512, 0, s>>>(f, o);
@@ -341,7 +341,7 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
 // 1024 -> 4096 6.2 / 8, 1024 -> 8192 9.1 / 8.5, 1024 -> 11008 11.7 / 9.2; 4096 -> 18432
 // 20.9 / 24).
 bool own_rows(const welvet_hip_int8 &l, int32_t n) {
-  return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in >= 4096) && !many_channels(l);
+  return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in >= 4096) && !many_channels(l, n);
 }
 hipError_t launch_own(const welvet_hip_int8 &l, int32_t dtype, const void *x, int64_t x_stride, const Out &o,
                       hipStream_t s) {

@@ -240,13 +240,14 @@ struct Tile {
 };
 
 // Few tiles: the sum's stages in parts, a block each, whose results are joined
-// in a launch of their own.  As many as give every CU a block, from 129 tiles to 170
-// three each and two blocks a CU; of eight stages and more, at most 16.  In two parts
-// only sums of 40 steps and more: the parts' way through memory takes what they save
-// (int8, us, in parts and whole: 1024 -> 8192 of 256 rows, two of four stages, 29 / 15;
-// 2048 -> 8192 of 200, two of eight, 30 / 19; 4096 -> 4096 of 512, two of sixteen, 34 /
-// 31; 8192 -> 4096 45 / 50; 11008 -> 4096 53 / 64; 4096 -> 28672 of 128, 224 tiles in
-// two, 48 / 32).
+// in a launch of their own.  As many as give every CU a block, of eight stages and
+// more, at most 16; in two parts sums of 40 steps and more, and those of 100 and more
+// in three from 129 tiles to 170, two blocks a CU: below, the parts' way through memory
+// takes more than they save (us, in parts and whole: int8 1024 -> 8192 of 256 rows, two
+// of four stages, 29 / 15; 2048 -> 8192 of 200, two of eight, 30 / 19; 4096 -> 4096 of
+// 512, two of sixteen, 34 / 31; 8192 -> 4096 45 / 50; 11008 -> 4096 53 / 64; 4096 ->
+// 18432 of 128, three of eleven, 39 / 30; dx f32 8512 <- 9536 of 153, three of 50
+// stages, 121 and 6 for the join / 182).
 constexpr int kSplitRows = 128;  // of the largest tile that is split
 struct Splits {
   int splits, each;      // parts, and the stages of one
@@ -257,13 +258,12 @@ struct Splits {
   Splits(int tiles_m, int tiles_n, const Operands &o, int tile_rows, int steps, void *ws)
       : splits(1), each(o.stages), parts_values((int64_t)o.a_rows * o.b_rows), parts(ws) {
     const int64_t tiles = (int64_t)tiles_m * tiles_n;
-    if (tile_rows > kSplitRows || tiles > kMostSplit) return;
+    if (tile_rows > kSplitRows || tiles > 170 || (!one_a_cu(tiles) && o.stages * steps < 100)) return;
     const int most = (int)std::min<int64_t>(16, std::min<int64_t>((one_a_cu(tiles) ? 256 : 512) / tiles, o.stages / 8));
     if (most < 2 || (most == 2 && o.stages * steps < 40)) return;
     each = (o.stages + most - 1) / most;
     splits = (o.stages + each - 1) / each;
   }
-  static constexpr int64_t kMostSplit = 170;
   static bool one_a_cu(int64_t tiles) { return tiles <= 128; }
 };
 // Their workspace for results of rows x cols: at most 512 tiles of 128 x 128; not
