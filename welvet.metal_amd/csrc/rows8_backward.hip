@@ -12,7 +12,10 @@
 //
 // Three steps: the codes' images with the sum along their rows, and the
 // bounds; dpre and its parts from one pass over dy (dw's transposed); the
-// products, which read nothing but whole stages of f16.
+// products, which read nothing but whole stages of f16.  bf16 4096 -> 11008 of 8192
+// rows: 94 and 208 us, at 4.4 and 4.8 TB/s, and 1340 + 670 to 710 for dw (two parts)
+// and dx (one), 1.1 PFLOP/s, where a library's f16 product reaches 1.5.  f32 2048 ->
+// 8192 of 256 rows: 14, 13.5 and 46 in one launch, with 5 to join dx's parts.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -46,10 +49,14 @@ __device__ inline void split(float v, uint16_t (&part)[P]) {
   if constexpr (P == 2) part[1] = fabsf(v) < 65504.0f ? half_bits(v - F16::get(part[0])) : (uint16_t)0;
 }
 
-// A block's values, two rows a word, so that columns can be read as rows.
+// A block's values, two rows a word, so that columns can be read as rows.  A column's
+// sixteen bytes k lie at k ^ 2 (column / 8): a wave's words, eight columns apart, and
+// sixteen lanes' reads of a column both touch all of LDS's banks once.
 struct Turn {
-  uint32_t word[kCols][kRows / 2 + 1];
-  __device__ inline void put(int col, int pair, uint32_t v) { word[col][pair] = v; }
+  static_assert(kRows == 128 && kCols == 64, "sixteen times sixteen bytes a column, eight eights of columns");
+  uint32_t word[kCols][kRows / 2];
+  __device__ static inline int place(int col, int pair) { return pair ^ (col >> 3) * 8; }
+  __device__ inline void put(int col, int pair, uint32_t v) { word[col][place(col, pair)] = v; }
   // Sixteen bytes (eight rows) of a column a thread into the image [cols][pitch]:
   // rows from `row` on (an image's rows hold whole blocks), columns from `col` on.
   __device__ inline void write(uint16_t *image, int64_t pitch, int row, int col, int cols) const {
@@ -57,8 +64,7 @@ struct Turn {
     for (int k = 0; k < 2; ++k) {
       const int c = (threadIdx.x >> 4) + kCols / 2 * k, at = (threadIdx.x & 15) * 4;
       if (col + c < cols)
-        *(uint4 *)(image + (int64_t)(col + c) * pitch + row + 2 * at) =
-            make_uint4(word[c][at], word[c][at + 1], word[c][at + 2], word[c][at + 3]);
+        *(uint4 *)(image + (int64_t)(col + c) * pitch + row + 2 * at) = *(const uint4 *)&word[c][place(c, at)];
     }
   }
 };
@@ -183,7 +189,7 @@ static_assert(kBoundCols == kThreads, "a thread a column at the end");
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, 6) prepare_kernel(Image x, Image w, GradArgs a) {
-  __shared__ Turn turn;
+  __shared__ __attribute__((aligned(16))) Turn turn;
   static_assert(sizeof(Turn) >= kThreads / 64 * kBoundCols * 4, "the bounds' place");
   int block = blockIdx.x;
   const int of_dy = a.col_parts * a.row_parts;
@@ -272,7 +278,7 @@ __device__ inline void own_lifts(const GradArgs &a, const Oct<T> (&o)[2], int pa
 template <class T, int PW, int PX, bool ONE>
 __global__ void __launch_bounds__(kThreads) grad_kernel(Image image, GradArgs a) {
   using raw = typename T::raw;
-  __shared__ Turn turn[PW];
+  __shared__ __attribute__((aligned(16))) Turn turn[PW];
   __shared__ float lift_n[kRows], lift_o[kCols];
   int block = blockIdx.x;
   if constexpr (ONE) {
@@ -458,10 +464,11 @@ __global__ void __launch_bounds__(256) half_join_kernel(Splits p, const float *_
 // --------------------------------------------------------------- few rows
 // Up to kFew rows: dw is as many outer products, bound by its own bytes, dx as
 // many rows times the codes as they lie, bound by those; both in f32, from dy
-// itself.  (The way above makes an image of the codes first, two bytes written and
-// read again a weight.  f16 8320 -> 8034, all outputs with the stores, 2 rows 185 us
-// that way and 86 this: dw 49, 5.5 TB/s, dx 21, 3.2 TB/s of codes, and its join 5;
-// 8 rows 180 and 108; bf16 2048 -> 2048, 8 rows 42 and 36, but 16 rows 42 and 56.)
+// itself, in one launch.  (The way above makes an image of the codes first, two bytes
+// written and read again a weight.  f16 8320 -> 8034, all outputs with the stores, 2
+// rows 185 us that way and 68 this, 56 of them dw's and the codes' 334 MB, 6 TB/s; 8
+// rows 180 and 76; bf16 2048 -> 2048, 8 rows 42 and 25.5.  Sixteen rows, dx in two
+// launches of eight: 42 that way and 56.)
 constexpr int kFew = 8;
 
 // dpre, unrounded.

@@ -555,6 +555,27 @@ DevStore wh::rt::session_store(welvet_dense_session *s, std::unique_lock<std::mu
   return s->W.dev();
 }
 
+welvet_status wh::rt::session_values(welvet_dense_session *s, DevBuf *w, std::vector<double> *bias, int *in, int *out,
+                                     int *act) {
+  WH_HIP(hipSetDevice(g_dev.id));
+  std::lock_guard<std::mutex> lock(s->mu);
+  w->stream = s->stream;
+  WH_HIP(w->alloc((size_t)s->W.n() * sizeof(float)));
+  WH_HIP(launch_decode(s->W.dtype, s->W.body, s->W.n(), s->W.dev().scale, s->W.minv, w->as<float>(), s->stream));
+  try {
+    bias->resize(s->W.bias_len);
+  } catch (...) {
+    return make_status(kInternal, "session values: out of memory");
+  }
+  if (!bias->empty())
+    WH_HIP(hipMemcpyAsync(bias->data(), s->W.bias, bias->size() * sizeof(double), hipMemcpyDeviceToHost, s->stream));
+  WH_HIP(hipStreamSynchronize(s->stream));
+  *in = s->W.cols;
+  *out = s->W.rows;
+  *act = s->act;
+  return ok();
+}
+
 extern "C" {
 
 const char *welvet_version(void) { return "0.71"; }
@@ -762,28 +783,6 @@ welvet_status welvet_hip_dense_export_f32(welvet_dense_session *s, float *W_out)
   WH_HIP(copy_to_host(W_out, d.p, bytes, s->stream));
   WH_HIP(hipStreamSynchronize(s->stream));
   return ok();
-}
-
-// The store's decoded weights, bias and activation as an int8 layer (int8.hip).
-welvet_status welvet_hip_int8_mount_dense(welvet_dense_session *s, welvet_hip_int8 **layer) {
-  if (!layer) return make_status(kInvalid, "int8: null layer");
-  *layer = nullptr;
-  if (!s) return make_status(kInvalid, "null session");
-  WH_HIP(hipSetDevice(g_dev.id));
-  std::lock_guard<std::mutex> lock(s->mu);
-  DevBuf w(s->stream);
-  WH_HIP(w.alloc((size_t)s->W.n() * sizeof(float)));
-  WH_HIP(launch_decode(s->W.dtype, s->W.body, s->W.n(), s->W.dev().scale, s->W.minv, w.as<float>(), s->stream));
-  std::vector<double> bias;
-  try {
-    bias.resize(s->W.bias_len);
-  } catch (...) {
-    return make_status(kInternal, "int8: out of memory");
-  }
-  if (!bias.empty())
-    WH_HIP(hipMemcpyAsync(bias.data(), s->W.bias, bias.size() * sizeof(double), hipMemcpyDeviceToHost, s->stream));
-  WH_HIP(hipStreamSynchronize(s->stream));
-  return welvet_hip_int8_mount_device(s->W.cols, s->W.rows, s->act, w.as<float>(), bias.data(), bias.size(), layer);
 }
 
 welvet_status welvet_hip_dense_backward(welvet_dense_session *s, const float *x, const float *pre,

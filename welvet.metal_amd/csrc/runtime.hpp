@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <vector>
 
 #include "../../include/welvet_c.h"
 #include "codec.hpp"
@@ -121,6 +122,9 @@ bool dims_ok(int32_t rows, int32_t cols);
 // A mounted session's store as the kernels take it; *lock holds the session
 // until the caller has enqueued what reads it.
 DevStore session_store(welvet_dense_session *s, std::unique_lock<std::mutex> *lock);
+// A mounted session's decoded weights [out][in], ready, its bias and activation.
+welvet_status session_values(welvet_dense_session *s, DevBuf *w, std::vector<double> *bias, int *in, int *out,
+                             int *act);
 
 // Volume hooks for the model sessions (volume.cpp): bind a ready store (taken
 // over), read a bound cell's store, change the batch, and
