@@ -119,6 +119,28 @@ def test_the_largest_sum(stream):
     assert e.value.code == 1
 
 
+def test_long_sums_of_many_channels(stream):
+    """129 tiles of channels, whose sums are long enough to be split in three all the same."""
+    inn, out, rng = 13000, 16500, np.random.default_rng(9)
+    w = rng.integers(-127, 128, (out, inn), dtype=np.int8)
+    c = np.zeros((100, 13008), np.int8)
+    c[:, :inn] = rng.integers(-127, 128, (100, inn))
+    scales, ws = rng.uniform(0.5, 1, 100).astype(np.float32), rng.uniform(0.5, 1, out).astype(np.float32)
+    # whole numbers below 2^53: exact in f64
+    sums = np.concatenate([c[:, :inn].astype(np.float64) @ w[o:o + 1500].T.astype(np.float64)
+                           for o in range(0, out, 1500)], 1)
+    want = sums * scales.astype(np.float64)[:, None] * ws.astype(np.float64)
+    codes, sc = Dev(c), Dev(scales)
+    with pywelvet.Int8Layer.from_codes(w, ws) as layer:
+        for n in (1, 60, 100):
+            pre = Dev(np.zeros((n, out), np.float32))
+            work = Dev(np.full(layer.workspace_bytes(n), 0xFF, np.uint8))
+            layer.product(1, n, pywelvet.rows8(codes.ptr, 13008, sc.ptr), d_pre=pre.ptr, ws=work.ptr,
+                          ws_bytes=work.nbytes, stream=stream)
+            work.get()
+            within(pre.get(), want[:n], 4 * U * np.abs(want[:n]), f"{n} rows")
+
+
 def test_codes_past_the_width_do_not_matter(stream):
     rng = np.random.default_rng(5)
     for n, inn, out in ((3, 33, 20), (40, 77, 20), (200, 100, 300)):

@@ -101,7 +101,7 @@ class Case:
 
 SHAPES = [(1, 1, 1), (1, 40, 70), (3, 17, 5), (31, 64, 64), (32, 65, 63), (33, 100, 129), (100, 1001, 777),
           (65, 300, 260), (256, 512, 1100), (700, 130, 33), (2100, 200, 128), (64, 600, 4100), (40, 130, 2050), (130, 8300, 1100),
-          (1100, 2100, 1000)]
+          (1100, 2100, 1000), (130, 8300, 3300), (3300, 2100, 1000)]
 
 
 @pytest.mark.parametrize("dtype", DT)
