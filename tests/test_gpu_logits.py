@@ -151,7 +151,8 @@ def apply(stream, z, dtype, r, extra=0, shift=0, in_place=False, mask_extra=0):
 
 SHAPES = [(1, 1, 1, 1, 1), (2, 31, 5, 3, 1), (3, 33, 40, 0, 2), (1, 1001, 500, 8, 0), (4, 32000, 300, 8, 3),
           (3, 50257, 2000, 100, 2), (2, 131072, 5000, 1024, 1), (600, 777, 64, 5, 4), (300, 2049, 1, 1, 0),
-          (1, 16384, 0, 20, 1), (2, 16385, 100, 0, 0), (5, 40000, 0, 0, 2), (64, 8192, 3000, 300, 64)]
+          (1, 16384, 0, 20, 1), (2, 16385, 100, 0, 0), (5, 40000, 0, 0, 2), (64, 8192, 3000, 300, 64),
+          (520, 8192, 60, 5, 3), (513, 8193, 60, 5, 3)]
 
 
 @pytest.mark.parametrize("dtype", DT)

@@ -25,9 +25,9 @@ namespace {
 using namespace r8;
 
 constexpr int kThreads = 512;
-// Tokens a block: with the list 40 KB of LDS, four blocks a CU (blocks of 1024 threads
+// Tokens a block: with the list 38 KB of LDS, four blocks a CU (blocks of 1024 threads
 // with twice the tokens, two a CU: 73 us against 71 for the 50257).
-constexpr int kStretch = 8128;
+constexpr int kStretch = 8192;
 constexpr int kOcts = 2;
 static_assert(kOcts * kThreads * 8 >= kStretch && kStretch % 32 == 0, "whole words of a mask, in one go");
 constexpr int kMaxHistory = (1 << 20) - 1, kMaxBiases = 1024;
@@ -74,7 +74,7 @@ template <class T, bool INPLACE>
 __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
   using raw = typename T::raw;
   __shared__ uint4 words[kStretch / 4];
-  __shared__ int index[kMaxBiases];
+  __shared__ int16_t index[kMaxBiases];  // of the stretch, -1 elsewhere
   __shared__ float biases[kMaxBiases];
   __shared__ int twice;  // a token of this stretch is named by two entries
   uint32_t *count = (uint32_t *)words;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(Args a) {
         const int64_t v = (int64_t)at[k] - begin;
         at[k] = i < a.r.biases && v >= 0 && v < len ? (int)v : -1;
         if (i < a.r.biases) {
-          index[i] = at[k];
+          index[i] = (int16_t)at[k];
           biases[i] = bias[k];
         }
       }

@@ -13,8 +13,8 @@
 // Three steps: the codes' images with the sum along their rows, and the
 // bounds; dpre and its parts from one pass over dy (dw's transposed); the
 // products, which read nothing but whole stages of f16.  bf16 4096 -> 11008 of 8192
-// rows: 94 and 208 us, at 4.4 and 4.8 TB/s, and 1340 + 670 to 710 for dw (two parts)
-// and dx (one), 1.1 PFLOP/s, where a library's f16 product reaches 1.5.  f32 2048 ->
+// rows: 94 and 208 us, at 4.4 and 4.8 TB/s, and 1328 + 672 for dw (two parts) and dx
+// (one), 1.1 PFLOP/s, where a library's f16 product reaches 1.5.  f32 2048 ->
 // 8192 of 256 rows: 14, 13.5 and 46 in one launch, with 5 to join dx's parts.
 #include <hip/hip_runtime.h>
 

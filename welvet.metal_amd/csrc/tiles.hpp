@@ -19,7 +19,10 @@
 // waves of 128 x 128 each 343, 630, 1284; 128 x 128 tiles, two blocks a CU, 369,
 // 734; stages of 64 bytes, four places, 397, 754, 1514; two parts as twice the
 // sum 1358; two places for both, loads issued after the barrier 367, 586, 1370
-// (128 x 256); the barrier ahead of the last slab's products 376, 612, 1238.
+// (128 x 256); the barrier ahead of the last slab's products 376, 612, 1238.  With
+// the waves' priority raised for a stage's products, in the layers' own calls (f16 int8
+// 4096 -> 11008, dw of two parts and dx of 8192 rows): 478 -> 466, 1372 -> 1328, 697 ->
+// 672; with the barrier ahead as well 470, 1301, 710.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -174,6 +177,7 @@ struct Tile {
       if (h + SA - 1 < steps) load_a(h + SA - 1, (part + SA - 1) % P, lds + (ia == 0 ? SA - 1 : ia - 1) * kA);
       const char *at = lds + ia * kA, *bt = lds_b + ib * kB;
       fetch(at, bt, 0, 0);
+      __builtin_amdgcn_s_setprio(1);  // ahead of a wave that still waits or copies
 #pragma unroll
       for (int slab = 0; slab < 4; ++slab) {
         if (slab < 3) fetch(at, bt, slab + 1, (slab + 1) & 1);
@@ -192,6 +196,7 @@ struct Tile {
         }
         __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
       }
+      __builtin_amdgcn_s_setprio(0);
       ia = ia == SA - 1 ? 0 : ia + 1;
       if (part == P - 1) ib = ib == SB - 1 ? 0 : ib + 1;
     };
