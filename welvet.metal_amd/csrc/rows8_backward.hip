@@ -177,12 +177,12 @@ __device__ inline void bounds(const GradArgs &a, int block, uint32_t *lds) {
   }
   if (!dw) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) lds[wave * kBoundCols + lane * 8 + i] = top[i];
+  for (int i = 0; i < 8; ++i) lds[wave * kBoundCols + i * 64 + (lane ^ i * 8)] = top[i];  // a bank a lane, below too
   __syncthreads();
-  const int i = threadIdx.x;
-  uint32_t most = lds[i];
+  const int i = threadIdx.x, at = (i & 7) * 64 + (i >> 3 ^ (i & 7) * 8);
+  uint32_t most = lds[at];
 #pragma unroll
-  for (int k = 1; k < kThreads / 64; ++k) most = max(most, lds[k * kBoundCols + i]);
+  for (int k = 1; k < kThreads / 64; ++k) most = max(most, lds[k * kBoundCols + at]);
   if (bn * kBoundCols + i < a.out) a.col_bound[(int64_t)bm * a.out + bn * kBoundCols + i] = most;
 }
 static_assert(kBoundCols == kThreads, "a thread a column at the end");
