@@ -120,7 +120,8 @@ struct SwigluArgs {
 template <class T>
 __device__ inline float product(float gate, float up) { return act_of<T>(gate, kSilu) * up; }
 
-// H8: h's own rows are asked for; its products are formed again for their codes.
+// H8: h's own rows are asked for; its products are formed again for their codes
+// (kept, they cost registers for one block a CU instead of two).
 template <class T, int WAVES, int GROUPS, bool H8>
 __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
   constexpr int kThreads = WAVES * 64;
