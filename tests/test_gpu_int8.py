@@ -9,7 +9,7 @@ from devmem import Stream
 from parity import assert_bit_equal
 from rows8ref import ACT_ERR, ACTS, TINY, Rows, act, codes_of
 from test_gpu_rows8 import HALF_ULP, LEAST, matrix
-from tokmem import DT, U, Dev, to_bits, to_f64, within
+from tokmem import DT, U, Big, Dev, to_bits, to_f64, within
 
 pytestmark = pytest.mark.gpu
 
@@ -139,6 +139,33 @@ def test_long_sums_of_many_channels(stream):
                           ws_bytes=work.nbytes, stream=stream)
             work.get()
             within(pre.get(), want[:n], 4 * U * np.abs(want[:n]), f"{n} rows")
+
+
+@pytest.mark.parametrize("n", [2, 9, 70])
+def test_rows_past_32_bits(stream, n):
+    """The last row of x, of post and of the rows left behind begins past 2^32 values
+    (of codes: bytes), and has the bits that it has beside the others."""
+    inn, out, rng = 100, 300, np.random.default_rng(n)
+    stride = (2 ** 32 // (n - 1) + 64) // 16 * 16
+    x = rng.normal(0, 1, (n, inn)).astype(np.float32)
+    with pywelvet.Int8Layer(rng.normal(0, 0.1, (out, inn)), pywelvet.ACT["gelu"]) as layer:
+        d = Dev(x)
+        want = run(stream, layer, "float32", n, d.ptr)[1]
+        rows, scales = Big(stride * n), Dev(np.zeros(n, np.float32))
+        far, post = Big(4 * (stride * (n - 1) + inn)), Big(4 * (stride * (n - 1) + out))
+        for r in range(n):
+            far.put(4 * stride * r, x[r])
+        ws = Dev(np.full(layer.workspace_bytes(n), 0xFF, np.uint8))
+        for kept in (None, pywelvet.rows8(rows.ptr, stride, scales.ptr)):
+            layer.forward(1, n, far.ptr, rows=kept, d_post=post.ptr, x_stride=stride, post_stride=stride, ws=ws.ptr,
+                          ws_bytes=ws.nbytes, stream=stream)
+            ws.get()
+            for r in range(n):
+                assert_bit_equal(post.get(4 * stride * r, out, np.float32), want[r], f"row {r}")
+        codes, _ = codes_of(x)
+        assert np.array_equal(rows.get(stride * (n - 1), inn, np.int8), codes[n - 1])
+        for b in (rows, far, post):
+            b.free()
 
 
 def test_codes_past_the_width_do_not_matter(stream):

@@ -6,7 +6,7 @@ import pytest
 import pywelvet
 from devmem import Stream
 from parity import assert_bit_equal
-from tokmem import DT, Dev, strided, to_bits, to_f64
+from tokmem import DT, Big, Dev, strided, to_bits, to_f64
 
 pytestmark = pytest.mark.gpu
 
@@ -252,3 +252,29 @@ def test_logits_past_32_bits(stream):
     for t in range(n):
         assert_bit_equal(big.get(4 * stride * t, vocab, np.float32), want[t], f"row {t}")
     big.free()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_past_32_bits(stream, in_place):
+    """The last row of the logits and of the history begins past 2^32 values."""
+    rng, n, vocab, stride = np.random.default_rng(6), 3, 9000, 2 ** 31 + 24
+    z = to_bits(rng.normal(0, 4, (n, vocab)), "bfloat16")
+    r = make(rng, n, vocab, 300, 0, 2)
+    want = apply(stream, z, "bfloat16", r)
+    logits, out, said = (Big(size * (stride * (n - 1) + w)) for size, w in ((2, vocab), (2, vocab), (4, 300)))
+    for t in range(n):
+        logits.put(2 * stride * t, z[t])
+        said.put(4 * stride * t, r["history"][t])
+    keep = {k: Dev(r[k]) for k in ("length", "prompt", "repetition", "frequency", "presence", "masks", "mask")}
+    rules = pywelvet.LogitRules(
+        history=300, d_history=said.ptr, history_stride=stride, d_history_len=keep["length"].ptr,
+        d_prompt_len=keep["prompt"].ptr, d_repetition=keep["repetition"].ptr, d_frequency=keep["frequency"].ptr,
+        d_presence=keep["presence"].ptr, masks=2, d_masks=keep["masks"].ptr, mask_stride=r["masks"].shape[1],
+        d_mask_id=keep["mask"].ptr)
+    to = logits if in_place else out
+    rules.apply(3, n, vocab, logits.ptr, to.ptr, stride=stride, out_stride=stride, stream=stream)
+    keep["mask"].get()
+    for t in range(n):
+        assert to.get(2 * stride * t, vocab, np.uint16).tobytes() == want[t].tobytes()
+    for b in (logits, out, said):
+        b.free()

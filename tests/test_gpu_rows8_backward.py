@@ -16,7 +16,7 @@ from devmem import Stream
 from parity import assert_bit_equal
 from rows8ref import ACTS, PRIME_ERR, Rows, act, act_prime, codes_of, values
 from test_gpu_rows8 import HALF_ULP, LEAST, matrix
-from tokmem import DT, U, Dev, to_bits, to_f64, within
+from tokmem import DT, U, Big, Dev, to_bits, to_f64, within
 
 pytestmark = pytest.mark.gpu
 PARTS = {"float32": (2, 2), "float16": (2, 2), "bfloat16": (2, 1)}
@@ -196,6 +196,34 @@ def test_gradients_against_differences(stream):
     within(dpre, d, 1e-5 * size, "dpre")
     within(dx, d @ W, 1e-5 * size @ np.abs(W) + 1e-6 * np.abs(d) @ np.abs(W), "dx")
     within(dw, d.T @ x, 1e-5 * size.T @ np.abs(x) + 1e-6 * np.abs(d).T @ np.abs(x), "dw")
+
+
+@pytest.mark.parametrize("n", [5, 17, 140])
+def test_rows_past_32_bits(stream, n):
+    """The last rows of dy, dpre, dx begin past 2^32 values and the activations' past
+    2^32 bytes; all have the bits that they have beside the others."""
+    case = Case("bfloat16", n, 100, 130, "silu", 10)
+    first = case.run(stream)
+    stride = (2 ** 32 // (n - 1) + 160) // 16 * 16
+    dy, dpre, dx = (Big(2 * (stride * (n - 1) + w)) for w in (130, 130, 100))
+    x8, pre8 = Big(stride * n), Big(stride * n)
+    bits = case.d.get().reshape(n, 130)
+    for r in range(n):
+        dy.put(2 * stride * r, bits[r])
+        for to, codes in ((x8, case.xc), (pre8, case.pc)):
+            to.put(stride * r, codes[r].astype(np.int8))
+    xs, ps, dw = Dev(case.xs), Dev(case.ps), Dev(np.zeros((130, 100), np.float32))
+    pywelvet.rows8_backward(
+        pywelvet.ACT["silu"], 3, n, 100, 130, dy.ptr, pre=pywelvet.rows8(pre8.ptr, stride, ps.ptr),
+        x=pywelvet.rows8(x8.ptr, stride, xs.ptr), layer=case.layer, d_dpre=dpre.ptr, d_dx=dx.ptr, d_dw=dw.ptr,
+        dy_stride=stride, dpre_stride=stride, dx_stride=stride, ws=case.ws.ptr, ws_bytes=case.ws.nbytes, stream=stream)
+    case.ws.get()
+    for r in range(n):
+        assert_bit_equal(dpre.get(2 * stride * r, 130, np.uint16), first[0][r], f"dpre {r}")
+        assert_bit_equal(dx.get(2 * stride * r, 100, np.uint16), first[1][r], f"dx {r}")
+    assert_bit_equal(dw.get(), first[2], "dw")
+    for b in (dy, dpre, dx, x8, pre8):
+        b.free()
 
 
 def test_no_rows(stream):
