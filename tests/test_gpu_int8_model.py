@@ -109,11 +109,12 @@ def test_example_gradients():
     model.close()
 
 
-def test_graph_of_a_step(stream):
+@pytest.mark.parametrize("n", [70, 5])
+def test_graph_of_a_step(stream, n):
     """A layer's step and an answer's rules in one graph: every replay, with other
     inputs and work between them, has the bits of the calls themselves."""
     rng = np.random.default_rng(4)
-    n, inn, inter, vocab = 70, 130, 300, 1000
+    inn, inter, vocab = 130, 300, 1000
     x, dy = Dev(np.zeros((n, inn), np.float32)), Dev(np.zeros((n, vocab), np.float32))
     gate, up, head = (pywelvet.Int8Layer(rng.normal(0, 0.1, s), a) for s, a in (((inter, inn), -1), ((inter, inn), -1),
                                                                              ((vocab, inter), 2)))
