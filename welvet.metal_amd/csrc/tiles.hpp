@@ -32,6 +32,8 @@
 #include <type_traits>
 #include <utility>
 
+#include "stages.hpp"
+
 namespace wh {
 namespace tiles {
 
@@ -119,6 +121,7 @@ struct Tile {
     for (int j = 0; j < kLoadsB; ++j)
       from_b[j] = o.b + (int64_t)min(n0 + (j * kWaves + wave) * 8 + (lane >> 3), o.b_rows - 1) * o.b_pitch + chunk;
     const int steps = o.stages * P;
+    constexpr Stages order{P, SA, SB};
     const auto copy = [&](const char *p, char *to) {
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)p,
                                        (__attribute__((address_space(3))) void *)to, 16, 0, 0);
@@ -166,15 +169,12 @@ struct Tile {
     int ia = 0, ib = 0;  // places of this step
     const auto step = [&](int h, auto part_) {
       constexpr int part = decltype(part_)::value;
-      // what was sent after this step's A and B: A's of the steps between, and B's
-      // that were sent with them
-      constexpr int kSteps = SA - 2, kStages = SB == 2 ? (P == 2 && part == 1) : P == 1 ? kSteps : (kSteps + part) / 2;
-      if (h + SA + P >= steps) wait<0>();
-      else wait<kSteps * kLoadsA + kStages * kLoadsB>();
+      if (order.drains(h, steps)) wait<0>();
+      else wait<order.left_a() * kLoadsA + order.left_b(part) * kLoadsB>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (part == 0 && h + (SB - 1) * P < steps) load_b(lds_b + (ib == 0 ? SB - 1 : ib - 1) * kB);
-      if (h + SA - 1 < steps) load_a(h + SA - 1, (part + SA - 1) % P, lds + (ia == 0 ? SA - 1 : ia - 1) * kA);
+      if (part == 0 && order.sends_b(h, steps)) load_b(lds_b + (ib == 0 ? SB - 1 : ib - 1) * kB);
+      if (order.sends_a(h, steps)) load_a(h + SA - 1, (part + SA - 1) % P, lds + (ia == 0 ? SA - 1 : ia - 1) * kA);
       const char *at = lds + ia * kA, *bt = lds_b + ib * kB;
       fetch(at, bt, 0, 0);
       __builtin_amdgcn_s_setprio(1);  // ahead of a wave that still waits or copies
