@@ -539,9 +539,9 @@ WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, i
  * dpre enters the products before it is rounded to `dtype`, times its row's
  * scale (dw) or its channel's (dx): two f16 parts a term, 22 bits, but no
  * finer than 2^-39 of the largest |dy| scale of its channel (dw) or token (dx)
- * times what |act'| can be (1.25; 256 scales of the row for act 6); one part,
- * 11 bits, for a BFloat16 dx; up to 8 rows terms are f32.  Sums are f32, in a
- * fixed order: the same bits on every run, and whichever outputs are asked for.
+ * times what |act'| can be (1.25; 256 scales of the row for act 6); up to 8
+ * rows terms are f32.  Sums are f32, in a fixed order: the same bits on every
+ * run, and whichever outputs are asked for.
  * Terms of 2^127 and more count as infinite, bits of a term below 2^-126 are
  * lost.  in, out and n <= 2^20, and (n / 128) (out / 64) and (in / 64) (n / 128
  * + out / 128), rounded up, < 2^22: what one launch takes. */

@@ -14,15 +14,15 @@ OUT = os.path.join(ROOT, "welvet.metal_amd", "_build", "stages")
 
 
 def tiles():
-    """(parts, WM, WN, TM, TN, SA, SB) of every Tile<> in the sources; one with the
-    parts as a template argument of its own counts with one and with two."""
+    """(parts, WM, WN, TM, TN, SA, SB) of every Tile<> in the sources; kParts is
+    rows8_backward.hip's number of parts."""
     found = set()
     for path in glob.glob(os.path.join(CSRC, "*.hip")):
         with open(path) as f:
             for args in re.findall(r"= Tile<\w+, ([^>]*)>", f.read()):
                 parts, *rest = [a.strip() for a in args.split(",")]
                 rest = [int(r) for r in rest] + [3, 2][len(rest) - 4:]
-                found |= {(p, *rest) for p in ((1, 2) if parts == "P" else (int(parts),))}
+                found.add((2 if parts == "kParts" else int(parts), *rest))
     return sorted(found)
 
 
@@ -36,8 +36,7 @@ def check():
 
 
 def test_the_sources_tiles_are_found():
-    """Five of one part, in int8.hip and four of them in rows8_backward.hip as well,
-    and those four of two."""
+    """Five of one part in int8.hip, four of two in rows8_backward.hip."""
     assert len(tiles()) == 9 and (2, 2, 4, 1, 1, 6, 6) in tiles()
 
 

@@ -13,8 +13,8 @@
 // Three steps: the codes' images with the sum along their rows, and the
 // bounds; dpre and its parts from one pass over dy (dw's transposed); the
 // products, which read nothing but whole stages of f16.  bf16 4096 -> 11008 of 8192
-// rows: 94 and 208 us, at 4.4 and 4.8 TB/s, and 1328 + 672 for dw (two parts) and dx
-// (one), 1.1 PFLOP/s, where a library's f16 product reaches 1.5.  f32 2048 ->
+// rows: 92 and 232 us, at 4.4 and 5 TB/s, and 1304 and 1203 for dw and dx, 1.1 and 1.2
+// PFLOP/s of parts, where a library's f16 product reaches 1.5.  f32 2048 ->
 // 8192 of 256 rows: 14, 13.5 and 46 in one launch, with 5 to join dx's parts.
 #include <hip/hip_runtime.h>
 
@@ -42,11 +42,13 @@ int bound_rows(int64_t n, int64_t out) { return tiles_of(n, most_bounds(out) * k
 int64_t along(int64_t n) { return spread(2 * n) / 2; }    // values between an image's rows
 
 __device__ inline uint16_t half_bits(float v) { return F16::put(v); }
-// v as P f16 parts, each the rest's nearest; what is not finite is its first part alone.
-template <int P>
-__device__ inline void split(float v, uint16_t (&part)[P]) {
+// v as f16 parts, each the rest's nearest; what is not finite is its first part alone.
+// One part, 11 bits, is not enough for any type: terms that cancel leave its rounding,
+// 2^-12 of the largest, in their sum.
+constexpr int kParts = 2;
+__device__ inline void split(float v, uint16_t (&part)[kParts]) {
   part[0] = half_bits(v);
-  if constexpr (P == 2) part[1] = fabsf(v) < 65504.0f ? half_bits(v - F16::get(part[0])) : (uint16_t)0;
+  part[1] = fabsf(v) < 65504.0f ? half_bits(v - F16::get(part[0])) : (uint16_t)0;
 }
 
 // A block's values, two rows a word, so that columns can be read as rows.  A column's
@@ -103,7 +105,7 @@ struct GradArgs {
   const float *x_scales, *w_scales;  // null: no dw, no dx
   void *dpre;
   int64_t dpre_stride;
-  uint16_t *along_n, *along_o;  // dw's parts [PW][out][n_pitch], dx's [PX][n][o_pitch]
+  uint16_t *along_n, *along_o;  // dw's parts [kParts][out][n_pitch], dx's [kParts][n][o_pitch]
   int64_t n_pitch, o_pitch;
   uint32_t *col_bound, *row_bound;  // [row blocks][out] of |dy| s_t, [column blocks][n] of |dy| v_o
   float *col_back, *row_back;       // the powers of two that the products are divided by, inverted
@@ -275,10 +277,10 @@ __device__ inline void own_lifts(const GradArgs &a, const Oct<T> (&o)[2], int pa
 
 // dpre and its parts.  ONE: a single block of rows without dx; the first blocks
 // make the image of the input's codes.
-template <class T, int PW, int PX, bool ONE>
+template <class T, bool ONE>
 __global__ void __launch_bounds__(kThreads) grad_kernel(Image image, GradArgs a) {
   using raw = typename T::raw;
-  __shared__ __attribute__((aligned(16))) Turn turn[PW];
+  __shared__ __attribute__((aligned(16))) Turn turn[kParts];
   __shared__ float lift_n[kRows], lift_o[kCols];
   int block = blockIdx.x;
   if constexpr (ONE) {
@@ -336,16 +338,16 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Image image, GradArgs a)
       const int r = row + 2 * pair + k;
       if (r >= a.n) continue;
       const float lift = lift_n[2 * pair + k];
-      uint32_t word[PX][4] = {};
+      uint32_t word[kParts][4] = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        uint16_t part[PX];
-        split<PX>(c + i < a.out ? v[k][i] * scale[i] * lift : 0.0f, part);
+        uint16_t part[kParts];
+        split(c + i < a.out ? v[k][i] * scale[i] * lift : 0.0f, part);
 #pragma unroll
-        for (int p = 0; p < PX; ++p) word[p][i >> 1] |= (uint32_t)part[p] << (16 * (i & 1));
+        for (int p = 0; p < kParts; ++p) word[p][i >> 1] |= (uint32_t)part[p] << (16 * (i & 1));
       }
 #pragma unroll
-      for (int p = 0; p < PX; ++p)
+      for (int p = 0; p < kParts; ++p)
         *(uint4 *)(a.along_o + ((int64_t)p * a.n + r) * a.o_pitch + c) =
             make_uint4(word[p][0], word[p][1], word[p][2], word[p][3]);
     }
@@ -353,17 +355,17 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Image image, GradArgs a)
   if (a.along_n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint16_t lo[PW], hi[PW];
+      uint16_t lo[kParts], hi[kParts];
       const float lift = lift_o[c - col + i];
       // rows past the last are nothing, whatever 0 times their values would be
-      split<PW>(row + 2 * pair < a.n ? v[0][i] * s[0] * lift : 0.0f, lo);
-      split<PW>(row + 2 * pair + 1 < a.n ? v[1][i] * s[1] * lift : 0.0f, hi);
+      split(row + 2 * pair < a.n ? v[0][i] * s[0] * lift : 0.0f, lo);
+      split(row + 2 * pair + 1 < a.n ? v[1][i] * s[1] * lift : 0.0f, hi);
 #pragma unroll
-      for (int p = 0; p < PW; ++p) turn[p].put(c - col + i, pair, lo[p] | ((uint32_t)hi[p] << 16));
+      for (int p = 0; p < kParts; ++p) turn[p].put(c - col + i, pair, lo[p] | ((uint32_t)hi[p] << 16));
     }
     __syncthreads();
 #pragma unroll
-    for (int p = 0; p < PW; ++p)
+    for (int p = 0; p < kParts; ++p)
       turn[p].write(a.along_n + (int64_t)p * a.out * a.n_pitch, a.n_pitch, row, col, a.out);
   }
 }
@@ -433,12 +435,11 @@ __global__ void __launch_bounds__(Tile::kWaves * 64) half_tile_kernel(Product<T>
   half_tile<T, ADD, Tile>(q, blockIdx.x, PART, lds);
 }
 // dx's blocks, whose sums are long, then dw's.
-template <class T, bool ADD, class TileX, class TileW>
-__global__ void __launch_bounds__(TileW::kWaves * 64) half_pair_kernel(Product<T> x, Product<F32> w, int of_x) {
-  static_assert(TileX::kWaves == TileW::kWaves && TileX::kLds == TileW::kLds, "one kind of block");
-  __shared__ __attribute__((aligned(1024))) char lds[TileW::kLds];
-  if ((int)blockIdx.x < of_x) return half_tile<T, false, TileX>(x, blockIdx.x, x.p.splits > 1, lds);
-  half_tile<F32, ADD, TileW>(w, blockIdx.x - of_x, w.p.splits > 1, lds);
+template <class T, bool ADD, class Tile>
+__global__ void __launch_bounds__(Tile::kWaves * 64) half_pair_kernel(Product<T> x, Product<F32> w, int of_x) {
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  if ((int)blockIdx.x < of_x) return half_tile<T, false, Tile>(x, blockIdx.x, x.p.splits > 1, lds);
+  half_tile<F32, ADD, Tile>(w, blockIdx.x - of_x, w.p.splits > 1, lds);
 }
 // The parts' results in their order; back null: 1.
 template <class T, bool ADD>
@@ -662,14 +663,10 @@ hipError_t launch_few(const GradArgs &a, const welvet_hip_rows8 *x, const welvet
 // Fewer than four stages are mostly results, which two blocks a CU write beside each
 // other's products: dw 9536 x 8512 f32 of 153 rows 101 us, large 125; 8192 x 2048 of
 // 256 rows, four stages, 31 and 28.)
-template <int P>
-using Large = Tile<HalfOp, P, 2, 4, 4, 2>;
-template <int P>
-using Medium = Tile<HalfOp, P, 2, 2, 2, 2>;
-template <int P>
-using Deep = Tile<HalfOp, P, 2, 4, 2, 1, 4, 4>;
-template <int P>
-using Slim = Tile<HalfOp, P, 2, 4, 1, 1, 6, 6>;
+using Large = Tile<HalfOp, kParts, 2, 4, 4, 2>;
+using Medium = Tile<HalfOp, kParts, 2, 2, 2, 2>;
+using Deep = Tile<HalfOp, kParts, 2, 4, 2, 1, 4, 4>;
+using Slim = Tile<HalfOp, kParts, 2, 4, 1, 1, 6, 6>;
 
 template <class T, class Tile>
 Product<T> product_of(const Operands &g, const float *back, void *to, int64_t stride, void *parts) {
@@ -700,13 +697,13 @@ hipError_t launch_tiles(const Operands &g, const float *back, void *to, int64_t 
   go(half_tile_kernel<T, ADD, Tile, false>, Tile::kWaves);
   return hipGetLastError();
 }
-// to[a_rows][b_rows] (+)= back . A . B^T with A of P parts.
-template <class T, bool ADD, int P>
+// to[a_rows][b_rows] (+)= back . A . B^T.
+template <class T, bool ADD>
 hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t stride, void *parts, hipStream_t s) {
   if ((int64_t)tiles_of(g.a_rows, 256) * tiles_of(g.b_rows, 256) >= 256 && g.stages >= 4)
-    return launch_tiles<T, ADD, Large<P>, Large<P>>(g, back, to, stride, parts, s);
-  if (g.a_rows <= 64) return launch_tiles<T, ADD, Medium<P>, Slim<P>>(g, back, to, stride, parts, s);
-  return launch_tiles<T, ADD, Medium<P>, Deep<P>>(g, back, to, stride, parts, s);
+    return launch_tiles<T, ADD, Large, Large>(g, back, to, stride, parts, s);
+  if (g.a_rows <= 64) return launch_tiles<T, ADD, Medium, Slim>(g, back, to, stride, parts, s);
+  return launch_tiles<T, ADD, Medium, Deep>(g, back, to, stride, parts, s);
 }
 
 // dx and dw in one launch of 128 x 128 tiles, two blocks a CU, where dx alone has no
@@ -715,20 +712,14 @@ hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t s
 // -> 4096 of 64 rows 62 and 56; f32 8512 -> 9536 of 153, 134 tiles, 325 and 307; bf16
 // 2048 -> 11008 of 2000, 256 tiles, 487 and 484).
 constexpr int kPairTiles = 256;
-template <class T, bool ADD, int PX, int PW>
+template <class T, bool ADD>
 hipError_t launch_pair(const Product<T> &x, const Product<F32> &w, hipStream_t s) {
-  half_pair_kernel<T, ADD, Medium<PX>, Medium<PW>><<<x.blocks() + w.blocks(), Medium<PW>::kWaves * 64, 0, s>>>(
+  half_pair_kernel<T, ADD, Medium><<<x.blocks() + w.blocks(), Medium::kWaves * 64, 0, s>>>(
       x, w, x.blocks());
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) e = launch_join<T, false>(x, s);
   return e == hipSuccess ? launch_join<F32, ADD>(w, s) : e;
 }
-
-// Parts of dw's and dx's terms.  One part, rounded as a BFloat16 gradient was
-// (and to 3 bits more), is enough for a dx that is rounded to BFloat16 itself.
-constexpr int kPartsW = 2;
-template <class T>
-constexpr int kPartsX = std::is_same_v<T, BF16> ? 1 : 2;
 
 // Bounds that the next pass's blocks read in all, each those of its rows and columns,
 // past which they are folded first (us of the fold and that pass: bf16 8192 rows,
@@ -740,7 +731,7 @@ struct Plan {
   size_t grad_w, grad_x, codes_x, codes_w, col_bound, row_bound, col_back, row_back, parts, parts_x;  // offsets
   size_t bytes;
 };
-Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
+Plan plan_of(int64_t n, int64_t in, int64_t out) {
   Plan p{};
   size_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -748,9 +739,9 @@ Plan plan_of(int32_t dtype, int64_t n, int64_t in, int64_t out) {
     at += pad256((size_t)bytes);
     return was;
   };
-  p.grad_w = take(2 * kPartsW * out * along(n));
+  p.grad_w = take(2 * kParts * out * along(n));
   p.codes_x = take(2 * in * along(n));
-  p.grad_x = take(2 * (dtype == kBFloat16 ? kPartsX<BF16> : kPartsX<F32>) * n * along(out));
+  p.grad_x = take(2 * kParts * n * along(out));
   p.codes_w = take(2 * in * along(out));
   p.col_bound = take(4 * std::min<int64_t>(most_bounds(out), tiles_of(n, kBoundRows)) * out);  // not fewer than any smaller n needs
   p.row_bound = take(4 * tiles_of(out, kBoundCols) * n);
@@ -784,7 +775,7 @@ welvet_status welvet_hip_rows8_backward_bytes(int32_t dtype, int32_t n, int32_t 
   if (!tok::float_type(dtype)) return make_status(kUnsupported, "rows8 backward: unsupported dtype %d", dtype);
   if (!sizes_ok(n, in, out) || !launchable(n, in, out) || !bytes)
     return make_status(kInvalid, "rows8 backward: invalid argument");
-  *bytes = plan_of(dtype, n, in, out).bytes;
+  *bytes = plan_of(n, in, out).bytes;
   return ok();
 }
 
@@ -812,7 +803,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   const int size = tok::float_size(dtype);
   if (!tok::aligned(d_dy, size) || !tok::aligned(d_dpre, size) || !tok::aligned(d_dx, size) || !tok::aligned(d_dw, 4))
     return make_status(kInvalid, "rows8 backward: device pointers must be aligned to their elements");
-  const Plan p = plan_of(dtype, n, in, out);
+  const Plan p = plan_of(n, in, out);
   const bool products = d_dw || d_dx;
   if (products && n > 0 && (!d_ws || ws_bytes < p.bytes || !tok::aligned(d_ws, 16)))
     return make_status(kInvalid, "rows8 backward: %zu bytes of 16-byte aligned workspace are needed", p.bytes);
@@ -866,7 +857,6 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
   }
   WH_HIP(tok::with_type(dtype, [&](auto t) -> hipError_t {
     using T = decltype(t);
-    constexpr int PX = kPartsX<T>;
     hipError_t e = hipSuccess;
     if (n <= kFew) {
       if (products) {
@@ -878,7 +868,7 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
         a.dpre = d_dpre;
       }
       a.along_n = a.along_o = nullptr;
-      grad_kernel<T, kPartsW, PX, false><<<a.across, kThreads, 0, s>>>(x, a);
+      grad_kernel<T, false><<<a.across, kThreads, 0, s>>>(x, a);
       return hipGetLastError();
     }
     const bool one = d_dw && !d_dx && n <= kRows;
@@ -892,26 +882,26 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
       }
     }
     // up to 128 rows without dx one launch does both (f16 1001 -> 777, 100 rows: 27 -> 22 us in all)
-    if (one) grad_kernel<T, kPartsW, PX, true><<<x.blocks + a.across, kThreads, 0, s>>>(x, a);
-    else grad_kernel<T, kPartsW, PX, false><<<(unsigned)tiles_of(n, kRows) * a.across, kThreads, 0, s>>>(x, a);
+    if (one) grad_kernel<T, true><<<x.blocks + a.across, kThreads, 0, s>>>(x, a);
+    else grad_kernel<T, false><<<(unsigned)tiles_of(n, kRows) * a.across, kThreads, 0, s>>>(x, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     const Operands gw{(const char *)a.along_n, 2 * a.n_pitch, 2 * out * a.n_pitch, out, INT32_MAX,
                       (const char *)x.to, 2 * a.n_pitch, in, tiles_of(2 * (int64_t)n, kStageBytes)};
     const Operands gx{(const char *)a.along_o, 2 * a.o_pitch, 2 * n * a.o_pitch, n, INT32_MAX,
                       (const char *)w.to, 2 * a.o_pitch, in, tiles_of(2 * (int64_t)out, kStageBytes)};
     if (d_dw && d_dx) {
-      const auto px = product_of<T, Medium<PX>>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x);
+      const auto px = product_of<T, Medium>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x);
       if (px.tiles_m * px.tiles_n <= kPairTiles) {
-        const auto pw = product_of<F32, Medium<kPartsW>>(gw, a.col_back, d_dw, in, parts);
-        return accumulate ? launch_pair<T, true, PX, kPartsW>(px, pw, s) : launch_pair<T, false, PX, kPartsW>(px, pw, s);
+        const auto pw = product_of<F32, Medium>(gw, a.col_back, d_dw, in, parts);
+        return accumulate ? launch_pair<T, true>(px, pw, s) : launch_pair<T, false>(px, pw, s);
       }
     }
     if (d_dw) {
-      e = accumulate ? launch_half<F32, true, kPartsW>(gw, a.col_back, d_dw, in, parts, s)
-                     : launch_half<F32, false, kPartsW>(gw, a.col_back, d_dw, in, parts, s);
+      e = accumulate ? launch_half<F32, true>(gw, a.col_back, d_dw, in, parts, s)
+                     : launch_half<F32, false>(gw, a.col_back, d_dw, in, parts, s);
       if (e != hipSuccess) return e;
     }
-    if (d_dx) e = launch_half<T, false, PX>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x, s);
+    if (d_dx) e = launch_half<T, false>(gx, a.row_back, d_dx, dx_stride, ws + p.parts_x, s);
     return e;
   }));
   return ok();
