@@ -445,7 +445,8 @@ WELVET_API welvet_status welvet_hip_distill(int32_t dtype, int32_t n, int32_t vo
  *   even, of the exact quotient (at most 127: a scale below 2^-126 is itself
  *   rounded to few bits, and below 2^-150 it is 0)
  * A row of zeros has scale 0.  A row that holds a NaN or an infinity has scale
- * NaN and codes 0: whatever reads it is NaN.  Codes between the width and its
+ * NaN and codes 0: whatever reads it is NaN, through every activation (of NaN a
+ * Dense layer's ReLU gives 0) and derivative.  Codes between the width and its
  * multiple of 16 are written as 0 and may hold anything where they are read.
  * n <= 2^24, widths <= 2^24. */
 typedef struct welvet_hip_rows8 {

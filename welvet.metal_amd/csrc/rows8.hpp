@@ -182,11 +182,12 @@ struct Sigmoid {
   }
 };
 // The activations and their derivatives in f32, by the formulas of act_value
-// and act_prime.
+// and act_prime, but of NaN, a row that is not finite, always NaN: those give
+// ReLU's answer and the piecewise derivatives whole values for it.
 __device__ inline float gelu_arg(float x) { return 1.59576912f * fmaf(0.044715f * x * x, x, x); }  // 2 u of 0.5 x (1 + tanh u)
 __device__ inline float act_f32(float x, int act) {
   switch (act) {
-  case kReLU: return x > 0.0f ? x : 0.0f;
+  case kReLU: return x <= 0.0f ? 0.0f : x;
   case kReLU2: return x < 0.0f ? 0.0f : x * x;
   case kLeakyReLU: return x < 0.0f ? (float)((double)x * 0.01) : x;
   case kSilu: return x * Sigmoid(x).z;
@@ -248,7 +249,7 @@ __device__ inline float act_prime_f32(float x, int act) {
     return fmaf(x * s.z * s.co, 1.59576912f * fmaf(0.134145f * x, x, 1.0f), s.z);
   }
   }
-  return act_prime_piecewise(x, act);
+  return x != x ? x : act_prime_piecewise(x, act);
 }
 
 __device__ inline void prime8(float (&v)[8], int act) {
