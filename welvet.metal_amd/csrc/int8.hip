@@ -50,7 +50,7 @@ __device__ inline void put8(const Out &o, int row, int c, const int (&sum)[8], f
     out.store((typename T::raw *)o.pre + row * o.pre_stride, c, o.out);
   }
   if (o.post) {
-    act8<T>(v, o.act);
+    acts<T>(v, o.act);
 #pragma unroll
     for (int i = 0; i < 8; ++i) out.set(i, v[i]);
     out.store((typename T::raw *)o.post + row * o.post_stride, c, o.out);
@@ -93,9 +93,11 @@ __device__ inline void few_join(const Out &o, int first, const i32x4 (&acc)[TILE
   for (int i = 0; i < 4; ++i) {
     const int c = first + (lane >> 4) * 4 + i;
     if (c >= o.out) break;
-    const float pre = pre_of(sum[i], scale * o.w_scales[c], o.bias[c]);
-    if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(pre);
-    if (o.post) ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(act_of<T>(pre, o.act));
+    float v[1] = {pre_of(sum[i], scale * o.w_scales[c], o.bias[c])};
+    if (o.pre) ((typename T::raw *)o.pre)[row * o.pre_stride + c] = T::put(v[0]);
+    if (!o.post) continue;
+    acts<T>(v, o.act);
+    ((typename T::raw *)o.post)[row * o.post_stride + c] = T::put(v[0]);
   }
 }
 template <class T, int WAVES, int TILES>

@@ -118,7 +118,13 @@ struct SwigluArgs {
   int n, width;
 };
 template <class T>
-__device__ inline float product(float gate, float up) { return act_of<T>(gate, kSilu) * up; }
+__device__ inline void products(const Oct<T> &gate, const Oct<T> &up, float (&h)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = gate.get(i);
+  acts<T, kSilu>(h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] *= up.get(i);
+}
 
 // H8: h's own rows are asked for; its products are formed again for their codes
 // (kept, they cost registers for one block a CU instead of two).
@@ -141,12 +147,13 @@ __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
       raise(top[0], go);
       raise(top[1], uo);
       if (!H8 && !h) return;
+      float p[8];
+      products(go, uo, p);
       Oct<T> ho;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float hv = product<T>(go.get(i), uo.get(i));
-        if constexpr (H8) top[2] = max(top[2], magnitude(hv));
-        ho.set(i, hv);
+        if constexpr (H8) top[2] = max(top[2], magnitude(p[i]));
+        ho.set(i, p[i]);
       }
       if (h && at >= 0) ho.store(h, at * 8, width);
     };
@@ -193,17 +200,23 @@ __global__ void __launch_bounds__(WAVES * 64) swiglu_kernel(SwigluArgs a) {
       if constexpr (H8) {
         a.h8.d_scales[row] = qh.stored;
         Oct<F32> hrest;
-        if (e.left)
+        if (e.left) {
+          float p[8];
+          products(grest, urest, p);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) hrest.set(i, product<T>(grest.get(i), urest.get(i)));
+          for (int i = 0; i < 8; ++i) hrest.set(i, p[i]);
+        }
         e.finish(hc, qh, hrest);
       }
     }
     const auto write = [&](const Oct<T> &go, const Oct<T> &uo, int at) {
       if (gc) *(uint2 *)(gc + at * 8) = codes8(qg, [&](int i) { return go.get(i); });
       if (uc) *(uint2 *)(uc + at * 8) = codes8(qu, [&](int i) { return uo.get(i); });
-      if constexpr (H8)
-        *(uint2 *)(hc + at * 8) = codes8(qh, [&](int i) { return product<T>(go.get(i), uo.get(i)); });
+      if constexpr (H8) {
+        float p[8];
+        products(go, uo, p);
+        *(uint2 *)(hc + at * 8) = codes8(qh, [&](int i) { return p[i]; });
+      }
     };
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k)
