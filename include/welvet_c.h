@@ -536,7 +536,8 @@ WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, i
  * Any of d_dpre, d_dw (with x8) and d_dx (with `layer`, of the same sizes) may
  * be NULL, not all; accumulate = 1 adds to dw.  d_dpre may be d_dy (the same
  * stride).  A Dense layer of any dtype can keep its activations so: it takes
- * dpre and dw here, and dx from its own weights.
+ * dpre and dw here, and dx from a forward of dpre through its transpose, mounted
+ * as a session of its own.
  * dpre enters the products before it is rounded to `dtype`, times its row's
  * scale (dw) or its channel's (dx): two f16 parts a term, 22 bits, but no
  * finer than 2^-39 of the largest |dy| scale of its channel (dw) or token (dx)
