@@ -900,11 +900,17 @@ class Int8Layer:
 
     @classmethod
     def from_codes(cls, codes, scales, act=-1, bias=None):
-        """From codes [out][inn] (int8) and scales [out]."""
+        """From codes [out][inn], whole numbers in [-127, 127] of any type, and scales [out]."""
         self = cls.__new__(cls)
-        codes, scales = np.ascontiguousarray(codes, np.int8), _f32(scales)
-        self.out, self.inn = codes.shape
-        assert scales.shape == (self.out,)
+        given, scales = np.asarray(codes), _f32(scales)
+        self.out, self.inn = given.shape
+        if given.size and not (given.min() >= -127 and given.max() <= 127):
+            raise WelvetError(1, "int8: codes outside [-127, 127]")
+        codes = np.ascontiguousarray(given, np.int8)
+        if given.dtype.kind not in "iub" and not np.array_equal(codes, given):
+            raise WelvetError(1, "int8: codes that are not whole numbers of [-127, 127]")
+        if scales.shape != (self.out,):
+            raise WelvetError(1, f"int8: scales of shape {scales.shape} for {self.out} channels")
         self._mount("welvet_hip_int8_mount_codes",
                     (self.inn, self.out, act, codes.ctypes.data_as(C.POINTER(C.c_int8)),
                      _fp(scales)), bias)
