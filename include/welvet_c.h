@@ -466,7 +466,8 @@ WELVET_API welvet_status welvet_hip_rows8_load(int32_t dtype, int32_t n, int32_t
  * from gate and up as given: into d_h (in `dtype`), into h8 in 8 bits (the
  * next integer product's rows; from h in f32), or both; gate8 and up8 keep
  * gate and up for the backward.  Any of gate8, up8, h8 and d_h may be NULL,
- * not all. */
+ * not all.  d_h may be d_gate or d_up (the same stride) where no rows are asked
+ * for. */
 WELVET_API welvet_status welvet_hip_rows8_swiglu(
     int32_t dtype, int32_t n, int32_t width, const void *d_gate, int64_t gate_stride,
     const void *d_up, int64_t up_stride, const welvet_hip_rows8 *gate8,

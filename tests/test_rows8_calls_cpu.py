@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import pywelvet
+from test_rows8_cpu import accepted, refused
 
 
 @pytest.mark.parametrize("codes", [np.array([[1, 200]]), np.array([[-128, 0]], np.int8), np.array([[0.5, 1.0]]),
@@ -18,3 +19,16 @@ def test_scales_of_another_count():
         with pytest.raises(pywelvet.WelvetError) as e:
             pywelvet.Int8Layer.from_codes(np.zeros((3, 5), np.int8), scales)
         assert e.value.code == 1 and "scales" in str(e.value)
+
+
+def test_swiglu_in_the_place_of_an_input_that_rows_keep():
+    """h in gate's or up's place: other threads look again at what is overwritten, so the
+    scales of rows that are asked for would be anything.  By itself h may lie there."""
+    rows = pywelvet.rows8(64, 64, 64)
+    call = lambda place, **kw: pywelvet.rows8_swiglu(1, 3, 60, 128, 192, d_h=place, status=True, **kw)  # noqa: E731
+    for place in (128, 192):
+        for asked in ("gate", "up", "h"):
+            refused(call(place, **{asked: rows}), "place")
+        refused(call(place, h_stride=61), "stride")
+        accepted(call(place))
+    accepted(call(place, gate_stride=61, h_stride=60))  # up's place, up's stride

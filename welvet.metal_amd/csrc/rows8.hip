@@ -354,6 +354,13 @@ welvet_status welvet_hip_rows8_swiglu(int32_t dtype, int32_t n, int32_t width, c
   for (const welvet_hip_rows8 *r : {gate8, up8, h8})
     if (const char *why = r ? r8::rows_fault(r, n, width) : nullptr)
       return make_status(kInvalid, "rows8 swiglu: %s", why);
+  // a row's last values are looked at by more than one thread, and in long rows twice:
+  // h in their place only where nothing but h depends on them
+  if (n > 0 && d_h && (d_h == d_gate || d_h == d_up)) {
+    if (gate8 || up8 || h8) return make_status(kInvalid, "rows8 swiglu: h in an input's place where rows are asked for");
+    if (n > 1 && h_stride != (d_h == d_gate ? gate_stride : up_stride))
+      return make_status(kInvalid, "rows8 swiglu: h in an input's place needs its row stride");
+  }
   const int size = tok::float_size(dtype);
   if (!tok::aligned(d_gate, size) || !tok::aligned(d_up, size) || !tok::aligned(d_h, size))
     return make_status(kInvalid, "rows8 swiglu: device pointers must be aligned to their elements");
