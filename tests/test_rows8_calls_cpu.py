@@ -32,3 +32,13 @@ def test_swiglu_in_the_place_of_an_input_that_rows_keep():
         refused(call(place, h_stride=61), "stride")
         accepted(call(place))
     accepted(call(place, gate_stride=61, h_stride=60))  # up's place, up's stride
+
+
+def test_backward_into_what_it_still_reads():
+    """dx in dy's or dpre's place: blocks of few rows write dx beside others that read dy."""
+    layer = type("Layer", (), {"h": None})()  # refused before a layer is looked into
+    call = lambda **kw: pywelvet.rows8_backward(-1, 1, 3, 60, 60, 64, layer=layer, ws=1 << 20, ws_bytes=1 << 62,  # noqa: E731
+                                                status=True, **kw)
+    refused(call(d_dx=64), "place")
+    refused(call(d_dx=128, d_dpre=128), "place")
+    refused(call(d_dx=128, d_dpre=192), "layer")

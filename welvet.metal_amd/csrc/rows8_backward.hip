@@ -791,6 +791,8 @@ welvet_status welvet_hip_rows8_backward(int32_t act, int32_t dtype, int32_t n, i
     return make_status(kInvalid, "rows8 backward: invalid argument");
   if (act < kLinear || act > kReLU2) return make_status(kInvalid, "rows8 backward: activation %d", act);
   if (!pre8 && act != kLinear) return make_status(kInvalid, "rows8 backward: the pre-activations are needed");
+  if (n > 0 && d_dx && (d_dx == d_dy || d_dx == d_dpre))
+    return make_status(kInvalid, "rows8 backward: dx in dy's or dpre's place");
   if (d_dw && !x8) return make_status(kInvalid, "rows8 backward: dw needs the input's rows");
   if (d_dx && (!layer || layer->in != in || layer->out != out))
     return make_status(kInvalid, "rows8 backward: dx needs a layer of %d -> %d", in, out);
