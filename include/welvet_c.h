@@ -515,7 +515,8 @@ WELVET_API welvet_status welvet_hip_int8_bytes(const welvet_hip_int8 *layer, int
  *   pre[t][o] = scale_t wscale_o sum_k c_tk w_ok + bias_o,  post = act(pre)
  * with the sum exact and the rest in f32, whatever n: a row's results have the
  * same bits in every batch.  Both are written in `dtype`, either may be NULL,
- * not both.  rows (nullable) receives x's rows, the backward's checkpoint. */
+ * not both, and either may lie where x does (all of x is read before).  rows
+ * (nullable) receives x's rows, the backward's checkpoint. */
 WELVET_API welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *layer, int32_t dtype,
                                                  int32_t n, const void *d_x, int64_t x_stride,
                                                  const welvet_hip_rows8 *rows, void *d_pre,
@@ -536,7 +537,7 @@ WELVET_API welvet_status welvet_hip_int8_product(const welvet_hip_int8 *layer, i
  *   dx = dpre . W                      [n][in], in `dtype`, W the int8 layer's
  * Any of d_dpre, d_dw (with x8) and d_dx (with `layer`, of the same sizes) may
  * be NULL, not all; accumulate = 1 adds to dw.  d_dpre may be d_dy (the same
- * stride).  A Dense layer of any dtype can keep its activations so: it takes
+ * stride), d_dx neither of them.  A Dense layer of any dtype can keep its activations so: it takes
  * dpre and dw here, and dx from a forward of dpre through its transpose, mounted
  * as a session of its own.
  * dpre enters the products before it is rounded to `dtype`, times its row's

@@ -351,6 +351,15 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
 bool own_rows(const welvet_hip_int8 &l, int32_t n) {
   return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in >= 4096) && !many_channels(l, n);
 }
+// Whether matrices of n rows share memory.  In one launch a block would read x beside
+// others that have written there.
+bool meet(const void *a, int64_t a_stride, int32_t a_cols, const void *b, int64_t b_stride, int32_t b_cols, int32_t n,
+          int size) {
+  const auto end = [&](const void *p, int64_t stride, int32_t cols) {
+    return (uintptr_t)p + (uintptr_t)(((n - 1) * stride + cols) * size);
+  };
+  return a && b && (uintptr_t)a < end(b, b_stride, b_cols) && (uintptr_t)b < end(a, a_stride, a_cols);
+}
 hipError_t launch_own(const welvet_hip_int8 &l, int32_t dtype, const void *x, int64_t x_stride, const Out &o,
                       hipStream_t s) {
   return with_type(dtype, [&](auto t) {
@@ -538,7 +547,9 @@ welvet_status welvet_hip_int8_forward(const welvet_hip_int8 *l, int32_t dtype, i
   welvet_hip_rows8 r{(int8_t *)d_ws, row_bytes(l->in), (float *)((char *)d_ws + tok::pad256(n * row_bytes(l->in)))};
   if (rows) r = *rows;
   const Out o{d_pre, d_post, pre_stride, post_stride, r.d_scales, l->scales, l->bias, n, l->out, l->act};
-  if (!rows && own_rows(*l, n)) {
+  const int size = tok::float_size(dtype);
+  if (!rows && own_rows(*l, n) && !meet(d_x, x_stride, l->in, d_pre, pre_stride, l->out, n, size) &&
+      !meet(d_x, x_stride, l->in, d_post, post_stride, l->out, n, size)) {
     WH_HIP(launch_own(*l, dtype, d_x, x_stride, o, (hipStream_t)stream));
     return ok();
   }
