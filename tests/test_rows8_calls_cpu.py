@@ -42,3 +42,12 @@ def test_backward_into_what_it_still_reads():
     refused(call(d_dx=64), "place")
     refused(call(d_dx=128, d_dpre=128), "place")
     refused(call(d_dx=128, d_dpre=192), "layer")
+
+
+def test_rules_are_not_changed_by_a_call():
+    """Rules may be applied from two threads, or to two vocabularies in turn."""
+    rules = pywelvet.LogitRules(masks=1, d_masks=64)
+    before = bytes(rules.desc)
+    for vocab in (100, 1000):
+        rules.apply(1, 2, vocab, 64, None, status=True)  # refused: nothing is launched
+        assert bytes(rules.desc) == before

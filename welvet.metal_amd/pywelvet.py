@@ -996,7 +996,7 @@ class LogitRules:
 
     def apply(self, dtype, n, vocab, d_logits, d_out, stride=None, out_stride=None, stream=None,
               status=False):
-        d = self.desc
+        d = LogitRulesDesc.from_buffer_copy(self.desc)  # calls on other threads have their own
         d.mask_stride = (vocab + 31) // 32 if self.mask_stride is None else self.mask_stride
         st = lib().welvet_hip_logits_rules(
             dtype, n, vocab, d_logits, vocab if stride is None else stride, C.byref(d), d_out,
