@@ -345,11 +345,14 @@ hipError_t launch_product(const welvet_hip_int8 &l, int32_t dtype, const int8_t 
   });
 }
 // One launch from x, for rows that the caller does not keep; not of short rows where
-// blocks come one after the other on a CU (us, bf16, one row, this and the other way:
-// 1024 -> 4096 6.2 / 8, 1024 -> 8192 9.1 / 8.5, 1024 -> 11008 11.7 / 9.2; 4096 -> 18432
-// 20.9 / 24).
+// blocks come one after the other on a CU.  us, bf16, weights from HBM, a pass among
+// others, this and the other way (whose two launches take 11 however small), one row and
+// four: out 8192, in 1024 9 / 11 and 9 / 11, 4096 10 / 13 and 12.5 / 13.4; out 9216, in
+// 1536 12 / 11 and 12.5 / 11.7, 2560 12.8 / 11.6 and 14.5 / 12.4, 3584 12.8 / 14 and 15.3 /
+// 15.3, 4096 12.7 / 15.9 and 15.6 / 16.6, 6144 21.5 / 21.1 and 25 / 22.4, 8192 22 / 26 and
+// 26.7 / 27.2; out 14336, in 2560 18 / 14 and 18 / 15, 3584 18.4 / 18.6 and 19.7 / 18.6.
 bool own_rows(const welvet_hip_int8 &l, int32_t n) {
-  return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in >= 4096) && !many_channels(l, n);
+  return n <= kOwnRows && n * padded(l.in) <= kOwnCodes && (l.out <= 8192 || l.in > 3200) && !many_channels(l, n);
 }
 // Whether matrices of n rows share memory.  In one launch a block would read x beside
 // others that have written there.
