@@ -4,8 +4,9 @@
 //   h = silu(gate) up;  dgate = dh up silu'(gate),  dup = dh silu(gate)
 // Bound by HBM: a row a block, read once into registers, its largest magnitude
 // joined across the block, then its codes written.  bf16 8192 x 11008: stored 66 us
-// (4.1 TB/s), read back 43, SwiGLU with both kept 147 (4.9 TB/s), its backward 127
-// (5.7); with h in 8 bits as well 228, as its products are formed twice.  A few rows
+// (4.1 TB/s), read back 43, SwiGLU with both kept 147 (4.9 TB/s), its backward 120
+// (6); with h in 8 bits beside both 171 to 195, by the values, as its products are formed
+// twice.  A few rows
 // take 2.5 to 6 us, the launch and one row's loads, join and stores.
 #include <hip/hip_runtime.h>
 

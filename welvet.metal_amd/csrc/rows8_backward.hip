@@ -13,8 +13,8 @@
 // Three steps: the codes' images with the sum along their rows, and the
 // bounds; dpre and its parts from one pass over dy (dw's transposed); the
 // products, which read nothing but whole stages of f16.  bf16 4096 -> 11008 of 8192
-// rows: 92 and 232 us, at 4.4 and 5 TB/s, and 1304 and 1203 for dw and dx, 1.1 and 1.2
-// PFLOP/s of parts, where a library's f16 product reaches 1.5.  f32 2048 ->
+// rows: 92 and 232 to 258 us, at 4.4 and 4.5 to 5 TB/s, and 1304 to 1340 and 1203 to 1216
+// for dw and dx, 1.1 and 1.2 PFLOP/s of parts, where a library's f16 product reaches 1.5.  f32 2048 ->
 // 8192 of 256 rows: 14, 13.5 and 46 in one launch, with 5 to join dx's parts.
 #include <hip/hip_runtime.h>
 
@@ -658,8 +658,9 @@ hipError_t launch_few(const GradArgs &a, const welvet_hip_rows8 *x, const welvet
 }
 
 // 256 x 256, a block a CU, where there is one for each; 128 x 128, two.  (dw and dx
-// of bf16 4096 x 4096, 2048 rows, 256 of the large tiles: 283 us against 304; of
-// 1024 x 1024, 4096 rows, 16 and 64: 111 with the small ones, 127 with the large.
+// of bf16 4096 x 4096, 2048 rows, 128 and 256 of the large tiles, with the stores: 324 us
+// against 341 without any; of 1024 x 1024, 4096 rows, 64 and 16: 256 with the large, 93
+// with the small ones.
 // Fewer than four stages are mostly results, which two blocks a CU write beside each
 // other's products: dw 9536 x 8512 f32 of 153 rows 101 us, large 125; 8192 x 2048 of
 // 256 rows, four stages, 31 and 28.)
@@ -708,9 +709,9 @@ hipError_t launch_half(const Operands &g, const float *back, void *to, int64_t s
 
 // dx and dw in one launch of 128 x 128 tiles, two blocks a CU, where dx alone has no
 // more tiles than there are CUs (us, both with the stores, in two launches and in one:
-// f32 2048 -> 8192 of 256 rows, 32 tiles, 53 of the products' time and 46.5; bf16 4096
-// -> 4096 of 64 rows 62 and 56; f32 8512 -> 9536 of 153, 134 tiles, 325 and 307; bf16
-// 2048 -> 11008 of 2000, 256 tiles, 487 and 484).
+// f32 2048 -> 8192 of 256 rows, 32 tiles, 93 and 88.5; bf16 4096 -> 4096 of 64 rows 63
+// and 59.5; f32 8512 -> 9536 of 153, 134 tiles, 285 and 258; bf16 2048 -> 11008 of 2000,
+// 256 tiles, 529 and 489).
 constexpr int kPairTiles = 256;
 template <class T, bool ADD>
 hipError_t launch_pair(const Product<T> &x, const Product<F32> &w, hipStream_t s) {
@@ -723,7 +724,7 @@ hipError_t launch_pair(const Product<T> &x, const Product<F32> &w, hipStream_t s
 
 // Bounds that the next pass's blocks read in all, each those of its rows and columns,
 // past which they are folded first (us of the fold and that pass: bf16 8192 rows,
-// 11008 channels, 418304 bounds, 213 and 240 without; f32 1000 rows, 2048 channels,
+// 11008 channels, 418304 bounds, 237 to 263 and 296 without; f32 1000 rows, 2048 channels,
 // 5120 bounds, 13.4 without, and the fold's launch alone takes 5).
 constexpr int64_t kFoldFrom = 1 << 16;
 

@@ -21,7 +21,7 @@
 // sum 1358; two places for both, loads issued after the barrier 367, 586, 1370
 // (128 x 256); the barrier ahead of the last slab's products 376, 612, 1238.  With
 // the waves' priority raised for a stage's products, in the layers' own calls (f16 int8
-// 4096 -> 11008, dw of two parts and dx of 8192 rows): 478 -> 466, 1372 -> 1328, 697 ->
+// 4096 -> 11008, dw of two parts and dx of one, 8192 rows): 478 -> 466, 1372 -> 1328, 697 ->
 // 672; with the barrier ahead as well 470, 1301, 710.
 #pragma once
 
