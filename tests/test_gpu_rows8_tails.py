@@ -69,6 +69,26 @@ def test_answers(stream, dtype, name, n):
     within(posts[dtype], want, err * 1.01 + HALF_ULP[dtype] * np.abs(want) + SMALL[dtype], name)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("name", ["silu", "sigmoid", "gelu"])
+def test_answers_do_not_depend_on_their_neighbours(stream, dtype, name):
+    """Values on both sides of what the 16-bit types' quick sigmoid takes, in rows that
+    one value a lane, eight a lane and a split sum's join answer: the same bits."""
+    x = np.random.default_rng(1).permutation(np.concatenate([tail(name), np.linspace(-3, 3, 40)]))
+    got = []
+    with pywelvet.Int8Layer.from_codes(np.repeat(np.ones((1041, 1), np.int8), 6000, 1), x / 6000,
+                                       pywelvet.ACT[name]) as layer:
+        for n in (1, 3, 20, 100, 3000):
+            d, post = Dev(to_bits(np.ones((n, 6000)), dtype)), Dev(np.zeros((n, 1041), to_bits(np.zeros(1), dtype).dtype))
+            ws = Dev(np.zeros(layer.workspace_bytes(n), np.uint8))
+            layer.forward(DT[dtype], n, d.ptr, d_post=post.ptr, ws=ws.ptr, ws_bytes=ws.nbytes, stream=stream)
+            rows = post.get()
+            assert np.array_equal(rows, np.tile(rows[:1], (n, 1)))
+            got.append(rows[0])
+    for g in got[1:]:
+        assert np.array_equal(g, got[0])
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])  # float16 holds nothing as large as these `up`
 def test_swiglu(stream, dtype):
     n, width = 3, 1001

@@ -207,9 +207,10 @@ __device__ inline float act_f32(float x, int act) {
   }
   return x;
 }
-// Before a rounding to 16 bits, from kQuick on: the exponential's argument rounded
-// once, which moves z by at most 0.4 2^-24 and x z, for x < 0, by |x| 2^-24 of itself.
-// Below, e^-x or its reciprocal leaves the instructions' range.
+// Before a rounding to 16 bits, or SwiGLU's product to 8, from kQuick on: the
+// exponential's argument rounded once, which moves z by at most 0.4 2^-24 and x z, for
+// x < 0, by |x| 2^-24 of itself.  Below, e^-x or its reciprocal leaves the instructions'
+// range.
 constexpr float kQuick = -87.0f;
 __device__ inline float quick_sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269502f * x));
