@@ -464,11 +464,11 @@ WELVET_API welvet_status welvet_hip_rows8_load(int32_t dtype, int32_t n, int32_t
                                                int64_t x_stride, void *stream);
 /* SwiGLU's product of its two projections, h = silu(gate) * up, formed in f32
  * from gate and up as given (within 10 2^-24 of itself and 2^-148 |gate up|, of
- * 16-bit types with gate < 0 within (10 + 2 |gate|) 2^-24): into d_h (in `dtype`), into h8 in 8 bits (the
- * next integer product's rows; from h in f32), or both; gate8 and up8 keep
- * gate and up for the backward.  Any of gate8, up8, h8 and d_h may be NULL,
- * not all.  d_h may be d_gate or d_up (the same stride) where no rows are asked
- * for. */
+ * 16-bit types with gate < 0 within (10 + 2 |gate|) 2^-24): into d_h (in
+ * `dtype`), into h8 in 8 bits (the next integer product's rows; from h in f32),
+ * or both; gate8 and up8 keep gate and up for the backward.  Any of gate8, up8,
+ * h8 and d_h may be NULL, not all.  d_h may be d_gate or d_up (the same stride)
+ * where no rows are asked for. */
 WELVET_API welvet_status welvet_hip_rows8_swiglu(
     int32_t dtype, int32_t n, int32_t width, const void *d_gate, int64_t gate_stride,
     const void *d_up, int64_t up_stride, const welvet_hip_rows8 *gate8,
